@@ -134,6 +134,25 @@ int mynn_quantized_matmul(void *out, int32_t *acc_out, const int8_t *lhs, const 
                           const int8_t *rhs, const void *rhs_scale,
                           int M, int N, int K, int dtype, mynn_stream s);
 
+/* Products with 4-bit weights.  No counterpart in the reference, whose quantised weights have 8 bits.
+ * wq: uint8 [N, K/2], 16-byte aligned: the code (0 .. 15) of an even column in the low four bits of its byte, of the
+ * odd column behind it in the high four.  Columns come in groups of `group` (32, 64 or a multiple of 128, dividing K);
+ * scale [N, K/group] in dtype, zero uint8 [N, K/group] (its low four bits) or NULL for 8 everywhere:
+ *   w[n,k] = scale[n, k/group] * (wq[n,k] - zero[n, k/group]).
+ * Sums are over the codes' differences, which are exact, and meet the scale once per group, in f32; one rounding at the
+ * store.  No scratch memory: both calls may be captured into a graph and overlap on any streams, and give the same bits
+ * from call to call.  An infinity or a NaN of act goes where the formula takes it: to its own row of out.
+ *
+ * act [M,K] (16-byte aligned), out [M,N], scale share dtype, MYNN_F16 or MYNN_BF16:
+ *   out[m,n] = T(sum_g scale[n,g] * sum_{k in g} act[m,k] * (wq[n,k] - zero[n,g])). */
+int mynn_dequant_matmul_int4(void *out, const void *act, const uint8_t *wq, const void *scale, const uint8_t *zero,
+                             int M, int N, int K, int group, int dtype, mynn_stream s);
+/* The same for int8 rows with a scale each (what mynn_dynamic_quantize_linear and mynn_add_rms_norm_quantize write):
+ * lhs [M,K] (16-byte aligned), lhs_scale [M]; a group's sum (of at most 128 columns) is exact in int32:
+ *   out[m,n] = T(lhs_scale[m] * sum_g scale[n,g] * sum_{k in g} lhs[m,k] * (wq[n,k] - zero[n,g])). */
+int mynn_quantized_matmul_int4(void *out, const int8_t *lhs, const void *lhs_scale, const uint8_t *wq, const void *scale,
+                               const uint8_t *zero, int M, int N, int K, int group, int dtype, mynn_stream s);
+
 /* DynamicQuantizeLinear -- dynamic_quantize_linear.cuh:39-153
  * `dynamic_quantize_linear_kernel(y,y_scale,y_zero_point,x,axis_dim,inner_size)`.
  * symmetric: int8, scale = amax/127 (1 for an all-zero slice), y = clamp(round_half_away(x*(1/s)),
@@ -297,6 +316,19 @@ int mynn_attention_streaming_ws(void *out, const void *Q, const void *K, const v
 /* RMSNormalization -- rms_norm.cuh:9-59: y = (x * (1/sqrt(mean(x^2)+eps))) * w per row. */
 int mynn_rms_norm(void *out, const void *x, const void *w, int rows, int dim, float eps,
                   int dtype, mynn_stream s);
+
+/* A residual's addition with the norm behind it (mynn_add, then mynn_rms_norm, in one pass over the rows):
+ *   sum = T(x + residual), out = T((sum * (1/sqrt(mean(sum^2)+eps))) * w) per row of dim values.
+ * residual NULL: sum = x.  sum NULL: not stored.  sum may be x or residual itself; out may be either of the two that sum
+ * is not. */
+int mynn_add_rms_norm(void *out, void *sum, const void *x, const void *residual, const void *w, int rows, int dim,
+                      float eps, int dtype, mynn_stream s);
+/* The same with the normalised rows in 8 bits, as mynn_quantized_matmul and mynn_quantized_matmul_int4 take them:
+ * y_scale[row] = amax/127 of the normalised row (1 for a row of zeros), y = clamp(round_half_away(value/scale),
+ * -127,127) as in mynn_dynamic_quantize_linear, from the 32-bit values (they are not rounded to T in between).  A row
+ * with a value that is not finite gets the scale NaN and codes of zero. */
+int mynn_add_rms_norm_quantize(int8_t *y, void *y_scale, void *sum, const void *x, const void *residual, const void *w,
+                               int rows, int dim, float eps, int dtype, mynn_stream s);
 
 /* Rope -- rope.cuh:18-46: half-split rotation, table row chosen by position[s] (device int64).
  * x,out [outer,S,D]; cos,sin [max_seq,D]. */
@@ -503,6 +535,13 @@ int mynn_model_profile(void *state, const int64_t *input_ids, const int64_t *pos
  * scale = amax/127 (1 for a zero row), q = clamp(round_half_away(w/scale), -128, 127). */
 int mynn_quantize_per_channel(int8_t *q, void *scale, const float *w, size_t rows, size_t cols,
                               int scale_dtype);
+/* 4-bit weights as mynn_dequant_matmul_int4 takes them, host memory: q uint8 [rows, cols/2], scale [rows, cols/group],
+ * zero uint8 [rows, cols/group] or NULL.  With zero NULL: scale = amax/7 of the group, code = 8 +
+ * clamp(round_half_away(w/scale), -8, 7).  With zero points: scale = (max(w,0) - min(w,0))/15, zero =
+ * round(-min(w,0)/scale), code = clamp(round_half_away(w/scale) + zero, 0, 15).  Codes go by the scale as it is stored
+ * (1 for a group whose scale would be 0).  A group with a value that is not finite, or too large for scale_dtype: MYNN_ERR_INVALID. */
+int mynn_quantize_int4_groups(uint8_t *q, void *scale, uint8_t *zero, const float *w, size_t rows, size_t cols,
+                              int group, int scale_dtype);
 /* RoPE tables (crates/llm/src/builder.rs:359-393), host memory [max_seq, head_dim]. */
 int mynn_rope_table(void *cos_t, void *sin_t, int max_seq, int head_dim, float base, int dtype);
 

@@ -80,6 +80,8 @@ SIGNATURES = {
     "mynn_dequant_weight_prepare": (_i, [_vp, _vp, _vp, _i, _i, _i, _vp]),
     "mynn_dequant_matmul_prepared": (_i, [_vp, _vp, _vp, _i, _i, _i, _i, _i, _vp]),
     "mynn_quantized_matmul": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _vp]),
+    "mynn_dequant_matmul_int4": (_i, [_vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _vp]),
+    "mynn_quantized_matmul_int4": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _vp]),
     "mynn_dynamic_quantize_linear": (_i, [_vp, _vp, _vp, _vp, _i, _i, _i, _i, _vp]),
     "mynn_attention": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _f, _i, _i, _i, _i, _vp, _i, _i, _i, _i, _i, _i, _i, _vp]),
     "mynn_attention_noalloc": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _f, _i, _i, _i, _i, _vp, _i, _i, _i, _i, _i, _i, _i, _vp]),
@@ -109,6 +111,8 @@ SIGNATURES = {
                                          _vp, _sz, _vp]),
     "mynn_quantizing_kvcache_update": (_i, [_vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _vp]),
     "mynn_rms_norm": (_i, [_vp, _vp, _vp, _i, _i, _f, _i, _vp]),
+    "mynn_add_rms_norm": (_i, [_vp, _vp, _vp, _vp, _vp, _i, _i, _f, _i, _vp]),
+    "mynn_add_rms_norm_quantize": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _f, _i, _vp]),
     "mynn_rope": (_i, [_vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _vp]),
     "mynn_gather_rows": (_i, [_vp, _vp, _vp, _i, _i, _sz, _vp]),
     "mynn_swiglu": (_i, [_vp, _vp, _vp, _sz, _i, _vp]),
@@ -151,6 +155,7 @@ SIGNATURES = {
     "mynn_device_weights_int8": (_i, [_vp]),
     "mynn_device_weights_free": (None, [_vp]),
     "mynn_quantize_per_channel": (_i, [_vp, _vp, _vp, _sz, _sz, _i]),
+    "mynn_quantize_int4_groups": (_i, [_vp, _vp, _vp, _vp, _sz, _sz, _i, _i]),
     "mynn_rope_table": (_i, [_vp, _vp, _i, _i, _f, _i]),
     "mynn_llm_create": (_vp, [_vp, _vp, _i, _i, _i64]),
     "mynn_llm_destroy": (None, [_vp]),
@@ -352,6 +357,42 @@ def quantized_matmul(lhs, lhs_scale, rhs, rhs_scale, want_acc=True):
     check(lib().mynn_quantized_matmul(_ptr(out), _ptr(acc), _ptr(lhs), _ptr(lhs_scale), _ptr(rhs), _ptr(rhs_scale),
                                       M, N, K, _dt(rhs_scale), _stream()))
     return out, acc
+
+
+def _int4_shape(wq, scale, zero):
+    """(N, K, group) of a 4-bit matrix: wq uint8 [N, K/2], scale [N, K/group], zero like scale in uint8 or None"""
+    N, half = wq.shape
+    groups = scale.shape[1]
+    if scale.shape[0] != N or groups < 1 or 2 * half % groups or wq.dtype != _torch.uint8 or (
+            zero is not None and (zero.shape != scale.shape or zero.dtype != _torch.uint8)):
+        raise MynnError("4-bit weights: wq %s %s, scale %s, zero %s do not fit together" % (
+            tuple(wq.shape), wq.dtype, tuple(scale.shape), None if zero is None else (tuple(zero.shape), zero.dtype)))
+    return N, 2 * half, 2 * half // groups
+
+
+def dequant_matmul_int4(act, wq, scale, zero=None):
+    """act [.., K] in 16 bits times 4-bit weights (wq uint8 [N, K/2], scale [N, groups], zero uint8 [N, groups] or None): [.., N]"""
+    _t()
+    N, K, group = _int4_shape(wq, scale, zero)
+    if act.shape[-1] != K or act.dtype != scale.dtype:
+        raise MynnError("dequant_matmul_int4: act %s %s, scale %s and K=%d do not fit together" % (tuple(act.shape), act.dtype, scale.dtype, K))
+    out = wq.new_empty(act.shape[:-1] + (N,), dtype=scale.dtype)
+    check(lib().mynn_dequant_matmul_int4(_ptr(out), _ptr(act), _ptr(wq), _ptr(scale), _ptr(zero), act.numel() // K, N, K, group, _dt(scale),
+                                         _stream()))
+    return out
+
+
+def quantized_matmul_int4(lhs, lhs_scale, wq, scale, zero=None):
+    """int8 rows lhs [M, K] with lhs_scale [M] times 4-bit weights (as dequant_matmul_int4): [M, N] in the scales' type"""
+    _t()
+    N, K, group = _int4_shape(wq, scale, zero)
+    if lhs.dim() != 2 or lhs.shape[1] != K or lhs.dtype != _torch.int8 or lhs_scale.numel() != lhs.shape[0] or lhs_scale.dtype != scale.dtype:
+        raise MynnError("quantized_matmul_int4: lhs %s %s, lhs_scale %s %s, scale %s and K=%d do not fit together" % (
+            tuple(lhs.shape), lhs.dtype, tuple(lhs_scale.shape), lhs_scale.dtype, scale.dtype, K))
+    out = wq.new_empty((lhs.shape[0], N), dtype=scale.dtype)
+    check(lib().mynn_quantized_matmul_int4(_ptr(out), _ptr(lhs), _ptr(lhs_scale), _ptr(wq), _ptr(scale), _ptr(zero), lhs.shape[0], N, K, group,
+                                           _dt(scale), _stream()))
+    return out
 
 
 def dynamic_quantize_linear(x, symmetric=True):
@@ -605,6 +646,35 @@ def rms_norm(x, w, eps):
     dim = x.shape[-1]
     check(lib().mynn_rms_norm(_ptr(out), _ptr(x), _ptr(w), x.numel() // dim, dim, float(eps), _dt(x), _stream()))
     return out
+
+
+def _add_norm_shape(name, x, residual, w):
+    dim = x.shape[-1]
+    if (residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype)) or w.numel() != dim or w.dtype != x.dtype:
+        raise MynnError("%s: x %s %s, residual %s, w %s %s do not fit together" % (
+            name, tuple(x.shape), x.dtype, None if residual is None else (tuple(residual.shape), residual.dtype), tuple(w.shape), w.dtype))
+    return x.numel() // max(dim, 1), dim
+
+
+def add_rms_norm(x, residual, w, eps):
+    """(RMSNorm of the stored sum x + residual, that sum); residual None: of x, and x itself"""
+    rows, dim = _add_norm_shape("add_rms_norm", x, residual, w)
+    out = x.new_empty(x.shape)
+    total = x if residual is None else x.new_empty(x.shape)
+    check(lib().mynn_add_rms_norm(_ptr(out), None if residual is None else _ptr(total), _ptr(x), _ptr(residual), _ptr(w), rows, dim, float(eps),
+                                  _dt(x), _stream()))
+    return out, total
+
+
+def add_rms_norm_quantize(x, residual, w, eps):
+    """(int8 codes like x, scales [rows], the sum x + residual) of the normalised rows; residual None: of x, and x itself"""
+    rows, dim = _add_norm_shape("add_rms_norm_quantize", x, residual, w)
+    y = x.new_empty(x.shape, dtype=_t().int8)
+    s = x.new_empty((rows,))
+    total = x if residual is None else x.new_empty(x.shape)
+    check(lib().mynn_add_rms_norm_quantize(_ptr(y), _ptr(s), None if residual is None else _ptr(total), _ptr(x), _ptr(residual), _ptr(w), rows, dim,
+                                           float(eps), _dt(x), _stream()))
+    return y, s, total
 
 
 def rope(x, cos_t, sin_t, position):
@@ -1029,6 +1099,21 @@ def quantize_per_channel(w_f32, scale_dt):
     check(lib().mynn_quantize_per_channel(q.ctypes.data_as(_vp), s.ctypes.data_as(_vp), w.ctypes.data_as(_vp), rows,
                                           w.size // rows, scale_dt))
     return q, s
+
+
+def quantize_int4_groups(w_f32, group, scale_dt, symmetric=True):
+    """4-bit weights of a float matrix [N, K] (numpy in, numpy out): (wq uint8 [N, K/2], scale bits uint16 [N, K/group], zero points uint8 like
+    scale, or None when symmetric)"""
+    import numpy as np
+
+    w = np.ascontiguousarray(np.asarray(w_f32, np.float32))
+    rows, cols = w.shape
+    q = np.empty((rows, cols // 2), np.uint8)
+    s = np.empty((rows, max(cols // max(int(group), 1), 1)), np.uint16)
+    z = None if symmetric else np.empty(s.shape, np.uint8)
+    check(lib().mynn_quantize_int4_groups(q.ctypes.data_as(_vp), s.ctypes.data_as(_vp), None if z is None else z.ctypes.data_as(_vp),
+                                          w.ctypes.data_as(_vp), rows, cols, int(group), scale_dt))
+    return q, s, z
 
 
 def rope_table(max_seq, head_dim, base, dt):

@@ -1,0 +1,77 @@
+// Products with 4-bit weights.  A matrix [N, K] is N rows of K / 2 bytes, the even column of a byte in its low four bits, in groups of
+// `group` columns with a scale and a zero point each: w[n, k] = scale[n, k / group] * (code[n, k] - zero[n, k / group]), zero 8 where
+// none are given.  The sum of a group runs over the bare differences (small integers, exact in every type) and meets its scale once:
+//   out[m, n] = T( sum over groups of scale[n, g] * sum over k in g of act[m, k] * (code[n, k] - zero[n, g]) )
+// in 32 bits, rounded at the store; with int8 activations the inner sum is exact in int32 and the row's scale is applied last.
+#include "mfma.h"
+#include "mynn_common.h"
+
+namespace mynn {
+
+// one wave per output value, eight columns a lane and step
+template <typename T, typename A>
+__global__ __launch_bounds__(256) void int4_plain_kernel(T *out, const A *act, const T *act_scale, const uint8_t *wq, const T *scale, const uint8_t *zero,
+                                                         int N, int K, int group) {
+    const int n = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const size_t m = blockIdx.y;
+    if (n >= N) return;  // whole wave
+    const int groups = K / group;
+    float sum = 0.f;
+    for (int k = lane * 8; k < K; k += 64 * 8) {
+        const uint32_t w = *(const uint32_t *)(wq + ((size_t)n * K + k) / 2);
+        const size_t g = (size_t)n * groups + k / group;
+        const int z = zero ? zero[g] & 15 : 8;
+        const A *a = act + m * K + k;
+        float part = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const float d = (float)((int)((w >> (4 * i)) & 15) - z);
+            if constexpr (std::is_same<A, int8_t>::value) part = fmaf((float)a[i], d, part);
+            else part = fmaf(Elem<A>::ld(a, i), d, part);
+        }
+        sum = fmaf(Elem<T>::ld(scale, g), part, sum);
+    }
+    sum = wave_sum(sum);
+    if (lane == 0) Elem<T>::st(out, m * N + n, act_scale ? sum * Elem<T>::ld(act_scale, m) : sum);
+}
+
+static int check_int4(const char *who, const void *out, const void *act, const void *wq, const void *scale, int M, int N, int K, int group) {
+    MYNN_REQUIRE(out && act && wq && scale && M > 0 && N > 0 && K > 0, MYNN_ERR_INVALID, "%s: bad operand (M=%d N=%d K=%d)", who, M, N, K);
+    MYNN_REQUIRE(group == 32 || group == 64 || (group > 0 && group % 128 == 0), MYNN_ERR_UNSUPPORTED, "%s: group=%d (32, 64 or a multiple of 128)", who, group);
+    MYNN_REQUIRE(K % group == 0, MYNN_ERR_INVALID, "%s: K=%d is no multiple of the group of %d", who, K, group);
+    MYNN_REQUIRE(aligned16(act) && aligned16(wq), MYNN_ERR_INVALID, "%s: activations and weights have to be 16-byte aligned", who);
+    return 0;
+}
+
+}  // namespace mynn
+
+using namespace mynn;
+
+extern "C" int mynn_dequant_matmul_int4(void *out, const void *act, const uint8_t *wq, const void *scale, const uint8_t *zero, int M, int N, int K,
+                                        int group, int dtype, mynn_stream s) {
+    if (int rc = check_int4("dequant_matmul_int4", out, act, wq, scale, M, N, K, group)) return rc;
+    return dispatch_dtype16(dtype, [&](auto *t) {
+        using T = std::remove_pointer_t<decltype(t)>;
+        for (int m0 = 0; m0 < M; m0 += 32768) {
+            const int rows = M - m0 < 32768 ? M - m0 : 32768;
+            MYNN_LAUNCH((int4_plain_kernel<T, T>), dim3((N + 3) / 4, rows), dim3(256), 0, as_stream(s), (T *)out + (size_t)m0 * N,
+                        (const T *)act + (size_t)m0 * K, (const T *)nullptr, wq, (const T *)scale, zero, N, K, group);
+        }
+        return launch_status("int4_plain_kernel");
+    });
+}
+
+extern "C" int mynn_quantized_matmul_int4(void *out, const int8_t *lhs, const void *lhs_scale, const uint8_t *wq, const void *scale, const uint8_t *zero,
+                                          int M, int N, int K, int group, int dtype, mynn_stream s) {
+    if (int rc = check_int4("quantized_matmul_int4", out, lhs, wq, scale, M, N, K, group)) return rc;
+    MYNN_REQUIRE(lhs_scale, MYNN_ERR_INVALID, "quantized_matmul_int4: lhs_scale is null");
+    return dispatch_dtype16(dtype, [&](auto *t) {
+        using T = std::remove_pointer_t<decltype(t)>;
+        for (int m0 = 0; m0 < M; m0 += 32768) {
+            const int rows = M - m0 < 32768 ? M - m0 : 32768;
+            MYNN_LAUNCH((int4_plain_kernel<T, int8_t>), dim3((N + 3) / 4, rows), dim3(256), 0, as_stream(s), (T *)out + (size_t)m0 * N,
+                        lhs + (size_t)m0 * K, (const T *)lhs_scale + m0, wq, (const T *)scale, zero, N, K, group);
+        }
+        return launch_status("int4_plain_kernel");
+    });
+}

@@ -39,6 +39,45 @@ extern "C" int mynn_quantize_per_channel(int8_t *q, void *scale, const float *w,
     return 0;
 }
 
+extern "C" int mynn_quantize_int4_groups(uint8_t *q, void *scale, uint8_t *zero, const float *w, size_t rows, size_t cols, int group,
+                                         int scale_dtype) {
+    MYNN_REQUIRE(q && scale && w && rows > 0 && cols > 0, MYNN_ERR_INVALID, "quantize_int4_groups: bad operand");
+    MYNN_REQUIRE(scale_dtype == MYNN_F16 || scale_dtype == MYNN_BF16, MYNN_ERR_UNSUPPORTED, "quantize_int4_groups: dtype %d", scale_dtype);
+    MYNN_REQUIRE(group == 32 || group == 64 || (group > 0 && group % 128 == 0), MYNN_ERR_UNSUPPORTED,
+                 "quantize_int4_groups: group=%d (32, 64 or a multiple of 128)", group);
+    MYNN_REQUIRE(cols % group == 0, MYNN_ERR_INVALID, "quantize_int4_groups: %zu columns are no multiple of the group of %d", cols, group);
+    const size_t groups = cols / group;
+    int bad = 0;
+#pragma omp parallel for schedule(static) reduction(| : bad)
+    for (long long r = 0; r < (long long)rows; r++)
+        for (size_t g = 0; g < groups; g++) {
+            const float *x = w + (size_t)r * cols + g * group;
+            float lo = 0.f, hi = 0.f;
+            bool finite = true;
+            for (int c = 0; c < group; c++) {
+                finite = finite && std::isfinite(x[c]);
+                lo = fminf(lo, x[c]);
+                hi = fmaxf(hi, x[c]);
+            }
+            float s = zero ? hi / 15.0f - lo / 15.0f : fmaxf(hi, -lo) / 7.0f;
+            s = scale_dtype == MYNN_F16 ? Elem<f16_t>::rnd(s) : Elem<bf16_t>::rnd(s);
+            if (s == 0.f) s = 1.f;
+            if (!finite || !std::isfinite(s)) {
+                bad |= 1;
+                continue;
+            }
+            const float z = zero ? fminf(roundf(-lo / s), 15.f) : 8.f;
+            for (int c = 0; c < group; c += 2) {
+                auto code = [&](float v) { return (uint8_t)fminf(fmaxf(roundf(v / s) + z, 0.f), 15.f); };
+                q[((size_t)r * cols + g * group + c) / 2] = (uint8_t)(code(x[c]) | code(x[c + 1]) << 4);
+            }
+            store_host(scale, (size_t)r * groups + g, s, scale_dtype);
+            if (zero) zero[(size_t)r * groups + g] = (uint8_t)z;
+        }
+    MYNN_REQUIRE(!bad, MYNN_ERR_INVALID, "quantize_int4_groups: a group holds a value that is not finite or that the scale's type does not reach");
+    return 0;
+}
+
 extern "C" int mynn_rope_table(void *cos_t, void *sin_t, int max_seq, int head_dim, float base, int dtype) {
     MYNN_REQUIRE(cos_t && sin_t && max_seq > 0 && head_dim > 0 && head_dim % 2 == 0, MYNN_ERR_INVALID,
                  "rope_table: bad operand");
