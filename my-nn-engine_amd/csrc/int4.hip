@@ -3,8 +3,7 @@
 // none are given.  The sum of a group runs over the bare differences (small integers, exact in every type) and meets its scale once:
 //   out[m, n] = T( sum over groups of scale[n, g] * sum over k in g of act[m, k] * (code[n, k] - zero[n, g]) )
 // in 32 bits, rounded at the store; with int8 activations the inner sum is exact in int32 and the row's scale is applied last.
-#include "mfma.h"
-#include "mynn_common.h"
+#include "int4_rows.h"
 
 namespace mynn {
 
@@ -35,10 +34,44 @@ __global__ __launch_bounds__(256) void int4_plain_kernel(T *out, const A *act, c
     if (lane == 0) Elem<T>::st(out, m * N + n, act_scale ? sum * Elem<T>::ld(act_scale, m) : sum);
 }
 
+constexpr int kCus = 256;
+
+// Up to 64 rows.  Two weight tiles a wave from 17 rows on: the activations, read from L2 by every workgroup, are then most of what a wave
+// loads.  Waves: as many as give each compute unit about 16, no more than there are pieces.
+template <typename T, bool I8, int FL> static int int4_rows(const Int4Args &a, hipStream_t s) {
+    auto go = [&](auto mt_, auto r_, auto nt_) {
+        constexpr int MT = decltype(mt_)::value, R = decltype(r_)::value, NT = decltype(nt_)::value;
+        const int blocks = (a.N + 16 * NT - 1) / (16 * NT), pieces = (a.K + 127) / 128;
+        const int most = MT == 1 ? 16 : 8, share = MT == 1 ? 2 : 1;
+        int waves = 1;
+        while (waves < most && blocks * waves < kCus * 16 && waves * 2 * share <= pieces) waves *= 2;
+        const size_t lds = (size_t)waves * MT * R * NT * 64 * sizeof(float);
+        MYNN_LAUNCH((int4_rows_kernel<T, I8, FL, MT, R, NT>), dim3(blocks), dim3(64 * waves), lds, s, a);
+        return launch_status("int4_rows_kernel");
+    };
+    using std::integral_constant;
+    if (a.M <= 4) return go(integral_constant<int, 1>{}, integral_constant<int, 1>{}, integral_constant<int, 1>{});
+    if (a.M <= 8) return go(integral_constant<int, 1>{}, integral_constant<int, 2>{}, integral_constant<int, 1>{});
+    if (a.M <= 16) return go(integral_constant<int, 1>{}, integral_constant<int, 4>{}, integral_constant<int, 1>{});
+    if (a.M <= 32) return go(integral_constant<int, 2>{}, integral_constant<int, 4>{}, integral_constant<int, 2>{});
+    if (a.M <= 48) return go(integral_constant<int, 3>{}, integral_constant<int, 4>{}, integral_constant<int, 2>{});
+    return go(integral_constant<int, 4>{}, integral_constant<int, 4>{}, integral_constant<int, 2>{});
+}
+
+template <typename T, bool I8> static int int4_few(const Int4Args &a, hipStream_t s) {
+    if (a.group == 32) return int4_rows<T, I8, 1>(a, s);
+    if (a.group == 64) return int4_rows<T, I8, 2>(a, s);
+    return int4_rows<T, I8, 4>(a, s);
+}
+
+// c / (pieces of a group) as the upper half of a product: exact while (pieces of a row) * (pieces of a group) < 2^32
+static uint32_t pieces_magic(int group) { return group <= 128 ? 0u : (uint32_t)((((uint64_t)1 << 32) + group / 128 - 1) / (group / 128)); }
+
 static int check_int4(const char *who, const void *out, const void *act, const void *wq, const void *scale, int M, int N, int K, int group) {
     MYNN_REQUIRE(out && act && wq && scale && M > 0 && N > 0 && K > 0, MYNN_ERR_INVALID, "%s: bad operand (M=%d N=%d K=%d)", who, M, N, K);
     MYNN_REQUIRE(group == 32 || group == 64 || (group > 0 && group % 128 == 0), MYNN_ERR_UNSUPPORTED, "%s: group=%d (32, 64 or a multiple of 128)", who, group);
     MYNN_REQUIRE(K % group == 0, MYNN_ERR_INVALID, "%s: K=%d is no multiple of the group of %d", who, K, group);
+    MYNN_REQUIRE(K <= 1 << 22, MYNN_ERR_UNSUPPORTED, "%s: K=%d", who, K);
     MYNN_REQUIRE(aligned16(act) && aligned16(wq), MYNN_ERR_INVALID, "%s: activations and weights have to be 16-byte aligned", who);
     return 0;
 }
@@ -50,8 +83,10 @@ using namespace mynn;
 extern "C" int mynn_dequant_matmul_int4(void *out, const void *act, const uint8_t *wq, const void *scale, const uint8_t *zero, int M, int N, int K,
                                         int group, int dtype, mynn_stream s) {
     if (int rc = check_int4("dequant_matmul_int4", out, act, wq, scale, M, N, K, group)) return rc;
+    const Int4Args args{out, act, nullptr, wq, scale, zero, M, N, K, group, pieces_magic(group)};
     return dispatch_dtype16(dtype, [&](auto *t) {
         using T = std::remove_pointer_t<decltype(t)>;
+        if (M <= 64) return int4_few<T, false>(args, as_stream(s));
         for (int m0 = 0; m0 < M; m0 += 32768) {
             const int rows = M - m0 < 32768 ? M - m0 : 32768;
             MYNN_LAUNCH((int4_plain_kernel<T, T>), dim3((N + 3) / 4, rows), dim3(256), 0, as_stream(s), (T *)out + (size_t)m0 * N,
@@ -65,8 +100,10 @@ extern "C" int mynn_quantized_matmul_int4(void *out, const int8_t *lhs, const vo
                                           int M, int N, int K, int group, int dtype, mynn_stream s) {
     if (int rc = check_int4("quantized_matmul_int4", out, lhs, wq, scale, M, N, K, group)) return rc;
     MYNN_REQUIRE(lhs_scale, MYNN_ERR_INVALID, "quantized_matmul_int4: lhs_scale is null");
+    const Int4Args args{out, lhs, lhs_scale, wq, scale, zero, M, N, K, group, pieces_magic(group)};
     return dispatch_dtype16(dtype, [&](auto *t) {
         using T = std::remove_pointer_t<decltype(t)>;
+        if (M <= 64) return int4_few<T, true>(args, as_stream(s));
         for (int m0 = 0; m0 < M; m0 += 32768) {
             const int rows = M - m0 < 32768 ? M - m0 : 32768;
             MYNN_LAUNCH((int4_plain_kernel<T, int8_t>), dim3((N + 3) / 4, rows), dim3(256), 0, as_stream(s), (T *)out + (size_t)m0 * N,
