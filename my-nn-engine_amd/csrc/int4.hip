@@ -3,36 +3,9 @@
 // none are given.  The sum of a group runs over the bare differences (small integers, exact in every type) and meets its scale once:
 //   out[m, n] = T( sum over groups of scale[n, g] * sum over k in g of act[m, k] * (code[n, k] - zero[n, g]) )
 // in 32 bits, rounded at the store; with int8 activations the inner sum is exact in int32 and the row's scale is applied last.
-#include "int4_rows.h"
+#include "int4_tile.h"
 
 namespace mynn {
-
-// one wave per output value, eight columns a lane and step
-template <typename T, typename A>
-__global__ __launch_bounds__(256) void int4_plain_kernel(T *out, const A *act, const T *act_scale, const uint8_t *wq, const T *scale, const uint8_t *zero,
-                                                         int N, int K, int group) {
-    const int n = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
-    const size_t m = blockIdx.y;
-    if (n >= N) return;  // whole wave
-    const int groups = K / group;
-    float sum = 0.f;
-    for (int k = lane * 8; k < K; k += 64 * 8) {
-        const uint32_t w = *(const uint32_t *)(wq + ((size_t)n * K + k) / 2);
-        const size_t g = (size_t)n * groups + k / group;
-        const int z = zero ? zero[g] & 15 : 8;
-        const A *a = act + m * K + k;
-        float part = 0.f;
-#pragma unroll
-        for (int i = 0; i < 8; i++) {
-            const float d = (float)((int)((w >> (4 * i)) & 15) - z);
-            if constexpr (std::is_same<A, int8_t>::value) part = fmaf((float)a[i], d, part);
-            else part = fmaf(Elem<A>::ld(a, i), d, part);
-        }
-        sum = fmaf(Elem<T>::ld(scale, g), part, sum);
-    }
-    sum = wave_sum(sum);
-    if (lane == 0) Elem<T>::st(out, m * N + n, act_scale ? sum * Elem<T>::ld(act_scale, m) : sum);
-}
 
 constexpr int kCus = 256;
 
@@ -64,6 +37,30 @@ template <typename T, bool I8> static int int4_few(const Int4Args &a, hipStream_
     return int4_rows<T, I8, 4>(a, s);
 }
 
+template <typename T, bool I8, int FL> static int int4_tiles(const Int4Args &a, hipStream_t s) {
+    auto go = [&](auto wm_) {
+        constexpr int WM = decltype(wm_)::value, WN = 8 / WM;
+        using G = Int4Tile<I8, FL, WM, WN>;
+        const long long tiles = (long long)((a.M + G::BM - 1) / G::BM) * ((a.N + G::BN - 1) / G::BN);
+        MYNN_REQUIRE(tiles < 1 << 30, MYNN_ERR_UNSUPPORTED, "4-bit product: M=%d N=%d", a.M, a.N);
+        constexpr int lds = G::NS * G::STAGE;
+        static bool lds_set = false;
+        if (!lds_set) {
+            MYNN_HIP(hipFuncSetAttribute((const void *)int4_tile_kernel<T, I8, FL, WM, WN>, hipFuncAttributeMaxDynamicSharedMemorySize, lds));
+            lds_set = true;
+        }
+        MYNN_LAUNCH((int4_tile_kernel<T, I8, FL, WM, WN>), dim3((unsigned)tiles), dim3(512), lds, s, a);
+        return launch_status("int4_tile_kernel");
+    };
+    const char *tm = getenv("I4TM");
+    return tm && atoi(tm) == 1 ? go(std::integral_constant<int, 1>{}) : go(std::integral_constant<int, 2>{});
+}
+template <typename T, bool I8> static int int4_many(const Int4Args &a, hipStream_t s) {
+    if (a.group == 32) return int4_tiles<T, I8, 1>(a, s);
+    if (a.group == 64) return int4_tiles<T, I8, 2>(a, s);
+    return int4_tiles<T, I8, 4>(a, s);
+}
+
 // c / (pieces of a group) as the upper half of a product: exact while (pieces of a row) * (pieces of a group) < 2^32
 static uint32_t pieces_magic(int group) { return group <= 128 ? 0u : (uint32_t)((((uint64_t)1 << 32) + group / 128 - 1) / (group / 128)); }
 
@@ -86,13 +83,7 @@ extern "C" int mynn_dequant_matmul_int4(void *out, const void *act, const uint8_
     const Int4Args args{out, act, nullptr, wq, scale, zero, M, N, K, group, pieces_magic(group)};
     return dispatch_dtype16(dtype, [&](auto *t) {
         using T = std::remove_pointer_t<decltype(t)>;
-        if (M <= 64) return int4_few<T, false>(args, as_stream(s));
-        for (int m0 = 0; m0 < M; m0 += 32768) {
-            const int rows = M - m0 < 32768 ? M - m0 : 32768;
-            MYNN_LAUNCH((int4_plain_kernel<T, T>), dim3((N + 3) / 4, rows), dim3(256), 0, as_stream(s), (T *)out + (size_t)m0 * N,
-                        (const T *)act + (size_t)m0 * K, (const T *)nullptr, wq, (const T *)scale, zero, N, K, group);
-        }
-        return launch_status("int4_plain_kernel");
+        return M <= 64 ? int4_few<T, false>(args, as_stream(s)) : int4_many<T, false>(args, as_stream(s));
     });
 }
 
@@ -103,12 +94,6 @@ extern "C" int mynn_quantized_matmul_int4(void *out, const int8_t *lhs, const vo
     const Int4Args args{out, lhs, lhs_scale, wq, scale, zero, M, N, K, group, pieces_magic(group)};
     return dispatch_dtype16(dtype, [&](auto *t) {
         using T = std::remove_pointer_t<decltype(t)>;
-        if (M <= 64) return int4_few<T, true>(args, as_stream(s));
-        for (int m0 = 0; m0 < M; m0 += 32768) {
-            const int rows = M - m0 < 32768 ? M - m0 : 32768;
-            MYNN_LAUNCH((int4_plain_kernel<T, int8_t>), dim3((N + 3) / 4, rows), dim3(256), 0, as_stream(s), (T *)out + (size_t)m0 * N,
-                        lhs + (size_t)m0 * K, (const T *)lhs_scale + m0, wq, (const T *)scale, zero, N, K, group);
-        }
-        return launch_status("int4_plain_kernel");
+        return M <= 64 ? int4_few<T, true>(args, as_stream(s)) : int4_many<T, true>(args, as_stream(s));
     });
 }
