@@ -190,7 +190,7 @@ def check(rc):
 
 
 # ------------------------------------------------------------------ torch plumbing
-# The host path of an operator call is most of the time of a small one (a 5632 x 2048 GEMV takes 3.9 us on the device).  The four
+# The host path of an operator call is most of the time of a small one (a 5632 x 2048 GEMV takes 3.9 us on the device).  The
 # operators a program calls most go through a module of their own (csrc/host_ops.cpp), which takes plain tensors and answers None
 # to everything else; the rest, and what it does not take, through ctypes: the current stream is asked for as a raw handle where torch has that (0.1 us; torch.cuda.current_stream() builds a Stream
 # object, 2.7 us), outputs come from new_empty of the tensor whose device they share (1.1 us; torch.empty with a device 1.5),
@@ -255,6 +255,9 @@ def _load_host_ops():
         raise ImportError("%s was built against torch %s, this is %s" % (path, module.torch_version, _torch.__version__))
     module.bind(MynnError, *(C.cast(getattr(l, n), _vp).value for n in (
         "mynn_last_error", "mynn_dequant_matmul", "mynn_quantized_matmul", "mynn_dynamic_quantize_linear", "mynn_attention")))
+    module.bind_int4(*(C.cast(getattr(l, n), _vp).value for n in (
+        "mynn_dequant_matmul_int4", "mynn_quantized_matmul_int4", "mynn_add_rms_norm", "mynn_add_rms_norm_quantize",
+        "mynn_dequantize_linear")))
     return module
 
 
@@ -282,6 +285,10 @@ def device_info():
 
 
 def dequantize_linear(x_i8, scale):
+    if x_i8.is_cuda:
+        out = (_ops or _host_ops()).dequantize_linear(x_i8, scale)
+        if out is not None:
+            return out
     import torch
 
     out = torch.empty(x_i8.shape, dtype=scale.dtype, device=x_i8.device)
@@ -372,6 +379,10 @@ def _int4_shape(wq, scale, zero):
 
 def dequant_matmul_int4(act, wq, scale, zero=None):
     """act [.., K] in 16 bits times 4-bit weights (wq uint8 [N, K/2], scale [N, groups], zero uint8 [N, groups] or None): [.., N]"""
+    if wq.is_cuda:
+        out = (_ops or _host_ops()).dequant_matmul_int4(act, wq, scale, zero)
+        if out is not None:
+            return out
     _t()
     N, K, group = _int4_shape(wq, scale, zero)
     if act.shape[-1] != K or act.dtype != scale.dtype:
@@ -384,6 +395,10 @@ def dequant_matmul_int4(act, wq, scale, zero=None):
 
 def quantized_matmul_int4(lhs, lhs_scale, wq, scale, zero=None):
     """int8 rows lhs [M, K] with lhs_scale [M] times 4-bit weights (as dequant_matmul_int4): [M, N] in the scales' type"""
+    if wq.is_cuda:
+        out = (_ops or _host_ops()).quantized_matmul_int4(lhs, lhs_scale, wq, scale, zero)
+        if out is not None:
+            return out
     _t()
     N, K, group = _int4_shape(wq, scale, zero)
     if lhs.dim() != 2 or lhs.shape[1] != K or lhs.dtype != _torch.int8 or lhs_scale.numel() != lhs.shape[0] or lhs_scale.dtype != scale.dtype:
@@ -658,6 +673,10 @@ def _add_norm_shape(name, x, residual, w):
 
 def add_rms_norm(x, residual, w, eps):
     """(RMSNorm of the stored sum x + residual, that sum); residual None: of x, and x itself"""
+    if x.is_cuda:
+        out = (_ops or _host_ops()).add_rms_norm(x, residual, w, eps)
+        if out is not None:
+            return out
     rows, dim = _add_norm_shape("add_rms_norm", x, residual, w)
     out = x.new_empty(x.shape)
     total = x if residual is None else x.new_empty(x.shape)
@@ -668,6 +687,10 @@ def add_rms_norm(x, residual, w, eps):
 
 def add_rms_norm_quantize(x, residual, w, eps):
     """(int8 codes like x, scales [rows], the sum x + residual) of the normalised rows; residual None: of x, and x itself"""
+    if x.is_cuda:
+        out = (_ops or _host_ops()).add_rms_norm_quantize(x, residual, w, eps)
+        if out is not None:
+            return out
     rows, dim = _add_norm_shape("add_rms_norm_quantize", x, residual, w)
     y = x.new_empty(x.shape, dtype=_t().int8)
     s = x.new_empty((rows,))

@@ -73,11 +73,138 @@ __global__ __launch_bounds__(kAnThreads) void add_norm_kernel(void *out_, T *y_s
     }
 }
 
+// sum / largest bits over the W waves of a row, in every thread
+template <int W> __device__ inline float an_row_sum(float v, float *red) {
+    v = wave_sum(v);
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = red[0];
+#pragma unroll
+    for (int i = 1; i < W; i++) v += red[i];
+    return v;
+}
+template <int W> __device__ inline float an_row_max(uint32_t v, uint32_t *red) {
+    auto dpp = [](uint32_t x, auto ctrl, auto rows) {
+        return (uint32_t)__builtin_amdgcn_update_dpp((int)x, (int)x, decltype(ctrl)::value, decltype(rows)::value, 0xF, false);
+    };
+    using std::integral_constant;
+    v = max(v, dpp(v, integral_constant<int, kDppXor1>{}, integral_constant<int, 0xF>{}));
+    v = max(v, dpp(v, integral_constant<int, kDppXor2>{}, integral_constant<int, 0xF>{}));
+    v = max(v, dpp(v, integral_constant<int, kDppHalfMirror>{}, integral_constant<int, 0xF>{}));
+    v = max(v, dpp(v, integral_constant<int, kDppMirror>{}, integral_constant<int, 0xF>{}));
+    v = max(v, dpp(v, integral_constant<int, kDppBcast15>{}, integral_constant<int, 0xA>{}));
+    v = max(v, dpp(v, integral_constant<int, kDppBcast31>{}, integral_constant<int, 0xC>{}));
+    v = (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < W; i++) v = max(v, red[i]);
+    return __builtin_bit_cast(float, v);
+}
+
+// Rows of 16-bit values, whole 16-byte pieces: read once, 128 bits a load, and kept in registers; a workgroup of W waves a row, NCH pieces a
+// thread.  Bound by memory (8192 x 4096 bf16 to 16 bits 46 us, to 8 bits 44: 5.8 TB/s and, the inputs partly in the caches, 6.9), few rows by
+// one round trip (one row of 4096 2.3 us; in four waves 2.5).  A wave a row was slower everywhere (8192 x 4096 83 and 48 us, 300 x 2048 4.6 against 3.4).  All
+// loads, the weights' too, are asked for first and without a test around them (pieces past the row repeat its last one and count as zero): the
+// launch is one round trip to memory, a reduction (for 8 bits two) and the stores.  The sum's 32-bit values are packed to the storage type
+// at once, which is what is stored, normalised and kept.
+template <typename T, bool Q8, int NCH, int W>
+__global__ __launch_bounds__(64 * W) void add_norm_vec_kernel(void *out_, const T *x, const T *residual, const T *w, T *sum, int dim, float eps, T *y_scale) {
+    __shared__ float red[W];
+    __shared__ uint32_t peak[W];
+    const int lane = threadIdx.x, row = blockIdx.x;
+    const size_t base = (size_t)row * dim;
+    const int chunks = dim >> 3;
+    U4 v[NCH], r[NCH], nw[NCH];
+#pragma unroll
+    for (int q = 0; q < NCH; q++) {
+        const size_t c = base + (size_t)min(lane + q * 64 * W, chunks - 1) * 8;
+        v[q] = *(const U4 *)(x + c);
+        if (residual) r[q] = *(const U4 *)(residual + c);
+    }
+#pragma unroll
+    for (int q = 0; q < NCH; q++) nw[q] = *(const U4 *)(w + (size_t)min(lane + q * 64 * W, chunks - 1) * 8);
+    float ss = 0.f;
+#pragma unroll
+    for (int q = 0; q < NCH; q++) {
+        const int c = lane + q * 64 * W;
+        float f[8];
+        widen8<T>(v[q], f);
+        if (residual) {
+            float g[8];
+            widen8<T>(r[q], g);
+            v[q] = U4{pack2<T>(f[0] + g[0], f[1] + g[1]), pack2<T>(f[2] + g[2], f[3] + g[3]), pack2<T>(f[4] + g[4], f[5] + g[5]), pack2<T>(f[6] + g[6], f[7] + g[7])};
+        }
+        if (c >= chunks) v[q] = U4{0u, 0u, 0u, 0u};
+        else if (sum) *(U4 *)(sum + base + (size_t)c * 8) = v[q];
+        widen8<T>(v[q], f);
+#pragma unroll
+        for (int i = 0; i < 8; i++) ss += f[i] * f[i];
+    }
+    const float inv = 1.0f / sqrtf(an_row_sum<W>(ss, red) / (float)dim + eps);
+    if constexpr (!Q8) {
+#pragma unroll
+        for (int q = 0; q < NCH; q++) {
+            const int c = lane + q * 64 * W;
+            float f[8], g[8];
+            widen8<T>(v[q], f);
+            widen8<T>(nw[q], g);
+            const U4 o = U4{pack2<T>((f[0] * inv) * g[0], (f[1] * inv) * g[1]), pack2<T>((f[2] * inv) * g[2], (f[3] * inv) * g[3]),
+                            pack2<T>((f[4] * inv) * g[4], (f[5] * inv) * g[5]), pack2<T>((f[6] * inv) * g[6], (f[7] * inv) * g[7])};
+            if (c < chunks) *(U4 *)((T *)out_ + base + (size_t)c * 8) = o;
+        }
+    } else {
+        // (the normalised values are made twice rather than kept: 16 registers a piece)
+        uint32_t amax = 0;
+#pragma unroll
+        for (int q = 0; q < NCH; q++) {
+            float f[8], g[8];
+            widen8<T>(v[q], f);
+            widen8<T>(nw[q], g);
+#pragma unroll
+            for (int i = 0; i < 8; i++) amax = max(amax, lane + q * 64 * W < chunks ? an_bits((f[i] * inv) * g[i]) : 0u);
+        }
+        const AnStep step(an_row_max<W>(amax, peak));
+#pragma unroll
+        for (int q = 0; q < NCH; q++) {
+            const int c = lane + q * 64 * W;
+            float f[8], g[8];
+            widen8<T>(v[q], f);
+            widen8<T>(nw[q], g);
+            uint32_t b[2] = {0u, 0u};
+#pragma unroll
+            for (int i = 0; i < 8; i++) b[i >> 2] |= ((uint32_t)(int)step.code((f[i] * inv) * g[i]) & 0xFFu) << (8 * (i & 3));
+            if (c < chunks) *(uint2 *)((int8_t *)out_ + base + (size_t)c * 8) = uint2{b[0], b[1]};
+        }
+        if (lane == 0) Elem<T>::st(y_scale, row, step.step);
+    }
+}
+
 template <bool Q8>
 static int add_norm(void *out, void *y_scale, void *sum, const void *x, const void *residual, const void *w, int rows, int dim, float eps, int dtype,
                     hipStream_t s) {
     return dispatch_dtype(dtype, [&](auto *t) {
         using T = std::remove_pointer_t<decltype(t)>;
+        if constexpr (sizeof(T) == 2) {
+            const bool whole = dim % 8 == 0 && aligned16(x) && aligned16(w) && (!residual || aligned16(residual)) && (!sum || aligned16(sum)) &&
+                               ((uintptr_t)out & (Q8 ? 7 : 15)) == 0;
+            auto go = [&](auto nch, auto w_) {
+                constexpr int NCH = decltype(nch)::value, W = decltype(w_)::value;
+                MYNN_LAUNCH((add_norm_vec_kernel<T, Q8, NCH, W>), dim3(rows), dim3(64 * W), 0, s, out, (const T *)x, (const T *)residual, (const T *)w,
+                            (T *)sum, dim, eps, (T *)y_scale);
+                return launch_status("add_norm_vec_kernel");
+            };
+            using std::integral_constant;
+            const int chunks = dim / 8;
+            if (whole) {
+                if (chunks <= 256) return go(integral_constant<int, 1>{}, integral_constant<int, 4>{});
+                if (chunks <= 512 && rows >= 256) return go(integral_constant<int, 2>{}, integral_constant<int, 4>{});
+                if (chunks <= 512) return go(integral_constant<int, 1>{}, integral_constant<int, 8>{});
+                if (chunks <= 1024) return go(integral_constant<int, 2>{}, integral_constant<int, 8>{});
+                if (chunks <= 2048) return go(integral_constant<int, 2>{}, integral_constant<int, 16>{});
+                if (chunks <= 4096) return go(integral_constant<int, 4>{}, integral_constant<int, 16>{});
+            }
+        }
         MYNN_LAUNCH((add_norm_kernel<T, Q8>), dim3(rows), dim3(kAnThreads), 0, s, out, (T *)y_scale, (T *)sum, (const T *)x, (const T *)residual,
                     (const T *)w, dim, eps);
         return launch_status("add_norm_kernel");

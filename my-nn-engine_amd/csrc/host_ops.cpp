@@ -20,6 +20,11 @@ decltype(&mynn_dequant_matmul) g_dequant_matmul;
 decltype(&mynn_quantized_matmul) g_quantized_matmul;
 decltype(&mynn_dynamic_quantize_linear) g_dynamic_quantize_linear;
 decltype(&mynn_attention) g_attention;
+decltype(&mynn_dequant_matmul_int4) g_dequant_matmul_int4;
+decltype(&mynn_quantized_matmul_int4) g_quantized_matmul_int4;
+decltype(&mynn_add_rms_norm) g_add_rms_norm;
+decltype(&mynn_add_rms_norm_quantize) g_add_rms_norm_quantize;
+decltype(&mynn_dequantize_linear) g_dequantize_linear;
 PyObject *g_error;
 
 int code_of(at::ScalarType t) {
@@ -160,6 +165,150 @@ PyObject *attention(PyObject *, PyObject *const *args, Py_ssize_t n) {
     });
 }
 
+// a 4-bit matrix: wq uint8 [N, K / 2], scale [N, groups], zero uint8 like scale or None
+struct Int4 {
+    const at::Tensor *wq, *scale, *zero = nullptr;
+    int64_t N = 0, K = 0, groups = 0;
+    int code = -1;
+    Int4(PyObject *w, PyObject *s, PyObject *z) : wq(plain(w)), scale(plain(s)) {
+        if (!wq || !scale || wq->dim() != 2 || scale->dim() != 2 || wq->scalar_type() != at::kByte || (z != Py_None && !(zero = plain(z)))) return;
+        N = wq->size(0), groups = scale->size(1);
+        const int64_t cols = 2 * wq->size(1);
+        if (scale->size(0) != N || groups < 1 || cols % groups || (zero && (zero->scalar_type() != at::kByte || zero->sizes() != scale->sizes()))) return;
+        K = cols;
+        code = code_of(scale->scalar_type());
+    }
+    explicit operator bool() const { return K > 0 && code >= 0; }
+};
+
+// (act [.., K], wq, scale, zero or None) -> [.., N]
+PyObject *dequant_matmul_int4(PyObject *, PyObject *const *args, Py_ssize_t n) {
+    if (n != 4) return none();
+    return guarded([&]() -> PyObject * {
+        const at::Tensor *act = plain(args[0]);
+        const Int4 w(args[1], args[2], args[3]);
+        if (!act || !w || act->dim() < 1 || act->size(-1) != w.K || act->scalar_type() != w.scale->scalar_type()) return none();
+        const int64_t M = act->numel() / w.K;
+        c10::SmallVector<int64_t, 4> sizes(act->sizes().begin(), act->sizes().end());
+        sizes.back() = w.N;
+        const at::Tensor out = make(sizes, *w.wq, w.scale->scalar_type());
+        void *o = data(out), *a = data(*act), *q = data(*w.wq), *s = data(*w.scale), *z = w.zero ? data(*w.zero) : nullptr;
+        const mynn_stream st = current_stream();
+        const int rc = without_gil([&] {
+            return g_dequant_matmul_int4(o, a, (const uint8_t *)q, s, (const uint8_t *)z, (int)M, (int)w.N, (int)w.K, (int)(w.K / w.groups), w.code, st);
+        });
+        return rc ? failed(rc) : THPVariable_Wrap(out);
+    });
+}
+
+// (lhs [M, K], lhs_scale [M], wq, scale, zero or None) -> [M, N]
+PyObject *quantized_matmul_int4(PyObject *, PyObject *const *args, Py_ssize_t n) {
+    if (n != 5) return none();
+    return guarded([&]() -> PyObject * {
+        const at::Tensor *lhs = plain(args[0]), *ls = plain(args[1]);
+        const Int4 w(args[2], args[3], args[4]);
+        if (!lhs || !ls || !w || lhs->dim() != 2 || lhs->size(1) != w.K || lhs->scalar_type() != at::kChar || ls->numel() != lhs->size(0) ||
+            ls->scalar_type() != w.scale->scalar_type())
+            return none();
+        const int64_t M = lhs->size(0);
+        const at::Tensor out = make({M, w.N}, *w.wq, w.scale->scalar_type());
+        void *o = data(out), *l = data(*lhs), *lsp = data(*ls), *q = data(*w.wq), *s = data(*w.scale), *z = w.zero ? data(*w.zero) : nullptr;
+        const mynn_stream st = current_stream();
+        const int rc = without_gil([&] {
+            return g_quantized_matmul_int4(o, (const int8_t *)l, lsp, (const uint8_t *)q, s, (const uint8_t *)z, (int)M, (int)w.N, (int)w.K, (int)(w.K / w.groups),
+                                           w.code, st);
+        });
+        return rc ? failed(rc) : THPVariable_Wrap(out);
+    });
+}
+
+// (x [.., dim], residual like x or None, w [dim], eps): the rows and what the sum is, or nullptr where this way does not take them
+struct NormArgs {
+    const at::Tensor *x, *residual = nullptr, *w;
+    int64_t rows = 0, dim = 0;
+    int code = -1;
+    float eps = 0.f;
+    explicit NormArgs(PyObject *const *args) : x(plain(args[0])), w(plain(args[2])) {
+        if (!x || !w || x->dim() < 1 || (args[1] != Py_None && !(residual = plain(args[1]))) || !PyFloat_CheckExact(args[3])) return;
+        if (x->size(-1) < 1 || w->numel() != x->size(-1) || w->scalar_type() != x->scalar_type() ||
+            (residual && (residual->sizes() != x->sizes() || residual->scalar_type() != x->scalar_type())))
+            return;
+        dim = x->size(-1);
+        rows = x->numel() / dim;
+        eps = (float)PyFloat_AS_DOUBLE(args[3]);
+        code = code_of(x->scalar_type());
+    }
+    explicit operator bool() const { return code >= 0; }
+};
+
+// -> (the normalised rows, the sum)
+PyObject *add_rms_norm(PyObject *, PyObject *const *args, Py_ssize_t n) {
+    if (n != 4) return none();
+    return guarded([&]() -> PyObject * {
+        const NormArgs a(args);
+        if (!a) return none();
+        const at::Tensor out = make(a.x->sizes(), *a.x, a.x->scalar_type()), sum = a.residual ? make(a.x->sizes(), *a.x, a.x->scalar_type()) : *a.x;
+        void *o = data(out), *t = a.residual ? data(sum) : nullptr, *x = data(*a.x), *r = a.residual ? data(*a.residual) : nullptr, *w = data(*a.w);
+        const mynn_stream st = current_stream();
+        const int rc = without_gil([&] { return g_add_rms_norm(o, t, x, r, w, (int)a.rows, (int)a.dim, a.eps, a.code, st); });
+        if (rc) return failed(rc);
+        PyObject *tuple = PyTuple_New(2);
+        if (!tuple) return nullptr;
+        PyTuple_SET_ITEM(tuple, 0, THPVariable_Wrap(out));
+        PyTuple_SET_ITEM(tuple, 1, THPVariable_Wrap(sum));
+        return tuple;
+    });
+}
+
+// -> (int8 codes, scales [rows], the sum)
+PyObject *add_rms_norm_quantize(PyObject *, PyObject *const *args, Py_ssize_t n) {
+    if (n != 4) return none();
+    return guarded([&]() -> PyObject * {
+        const NormArgs a(args);
+        if (!a) return none();
+        const at::Tensor y = make(a.x->sizes(), *a.x, at::kChar), s = make({a.rows}, *a.x, a.x->scalar_type()),
+                         sum = a.residual ? make(a.x->sizes(), *a.x, a.x->scalar_type()) : *a.x;
+        void *yp = data(y), *sp = data(s), *t = a.residual ? data(sum) : nullptr, *x = data(*a.x), *r = a.residual ? data(*a.residual) : nullptr, *w = data(*a.w);
+        const mynn_stream st = current_stream();
+        const int rc = without_gil([&] { return g_add_rms_norm_quantize((int8_t *)yp, sp, t, x, r, w, (int)a.rows, (int)a.dim, a.eps, a.code, st); });
+        if (rc) return failed(rc);
+        PyObject *tuple = PyTuple_New(3);
+        if (!tuple) return nullptr;
+        PyTuple_SET_ITEM(tuple, 0, THPVariable_Wrap(y));
+        PyTuple_SET_ITEM(tuple, 1, THPVariable_Wrap(s));
+        PyTuple_SET_ITEM(tuple, 2, THPVariable_Wrap(sum));
+        return tuple;
+    });
+}
+
+// (codes [rows, ..], scale [rows]) -> what the codes stand for, in the scale's type
+PyObject *dequantize_linear(PyObject *, PyObject *const *args, Py_ssize_t n) {
+    if (n != 2) return none();
+    return guarded([&]() -> PyObject * {
+        const at::Tensor *x = plain(args[0]), *scale = plain(args[1]);
+        if (!x || !scale || x->dim() < 1 || x->size(0) < 1 || x->scalar_type() != at::kChar || code_of(scale->scalar_type()) < 0) return none();
+        const int64_t rows = x->size(0), inner = x->numel() / rows;
+        const at::Tensor out = make(x->sizes(), *x, scale->scalar_type());
+        void *o = data(out), *xp = data(*x), *sp = data(*scale);
+        const int code = code_of(scale->scalar_type());
+        const mynn_stream st = current_stream();
+        const int rc = without_gil([&] { return g_dequantize_linear(o, (const int8_t *)xp, sp, (size_t)rows, (size_t)inner, code, st); });
+        return rc ? failed(rc) : THPVariable_Wrap(out);
+    });
+}
+
+// the addresses of a call's arguments, or false with an exception set
+bool addresses(PyObject *const *args, int count, void **p) {
+    for (int i = 0; i < count; i++) {
+        p[i] = PyLong_AsVoidPtr(args[i]);
+        if (!p[i]) {
+            if (!PyErr_Occurred()) PyErr_SetString(PyExc_ValueError, "bind: null address");
+            return false;
+        }
+    }
+    return true;
+}
+
 // (exception class, addresses of mynn_last_error and of the four operators)
 PyObject *bind(PyObject *, PyObject *const *args, Py_ssize_t n) {
     if (n != 6) {
@@ -167,13 +316,7 @@ PyObject *bind(PyObject *, PyObject *const *args, Py_ssize_t n) {
         return nullptr;
     }
     void *p[5];
-    for (int i = 0; i < 5; i++) {
-        p[i] = PyLong_AsVoidPtr(args[i + 1]);
-        if (!p[i]) {
-            if (!PyErr_Occurred()) PyErr_SetString(PyExc_ValueError, "bind: null address");
-            return nullptr;
-        }
-    }
+    if (!addresses(args + 1, 5, p)) return nullptr;
     Py_INCREF(args[0]);
     Py_XSETREF(g_error, args[0]);
     g_last_error = (decltype(g_last_error))p[0];
@@ -184,8 +327,26 @@ PyObject *bind(PyObject *, PyObject *const *args, Py_ssize_t n) {
     Py_RETURN_NONE;
 }
 
+// (addresses of the operators of 4-bit weights and of dequantize_linear, behind bind)
+PyObject *bind_int4(PyObject *, PyObject *const *args, Py_ssize_t n) {
+    if (n != 5) {
+        PyErr_SetString(PyExc_TypeError, "bind_int4: five arguments");
+        return nullptr;
+    }
+    void *p[5];
+    if (!addresses(args, 5, p)) return nullptr;
+    g_dequant_matmul_int4 = (decltype(g_dequant_matmul_int4))p[0];
+    g_quantized_matmul_int4 = (decltype(g_quantized_matmul_int4))p[1];
+    g_add_rms_norm = (decltype(g_add_rms_norm))p[2];
+    g_add_rms_norm_quantize = (decltype(g_add_rms_norm_quantize))p[3];
+    g_dequantize_linear = (decltype(g_dequantize_linear))p[4];
+    Py_RETURN_NONE;
+}
+
 #define MYNN_METHOD(f) {#f, (PyCFunction)(void (*)(void))f, METH_FASTCALL, nullptr}
 PyMethodDef g_methods[] = {MYNN_METHOD(bind), MYNN_METHOD(dequant_matmul), MYNN_METHOD(quantized_matmul), MYNN_METHOD(dynamic_quantize_linear), MYNN_METHOD(attention),
+                           MYNN_METHOD(bind_int4), MYNN_METHOD(dequant_matmul_int4), MYNN_METHOD(quantized_matmul_int4), MYNN_METHOD(add_rms_norm),
+                           MYNN_METHOD(add_rms_norm_quantize), MYNN_METHOD(dequantize_linear),
                            {nullptr, nullptr, 0, nullptr}};
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_host_ops", nullptr, -1, g_methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -14,12 +14,12 @@ constexpr int kCus = 256;
 template <typename T, bool I8, int FL> static int int4_rows(const Int4Args &a, hipStream_t s) {
     auto go = [&](auto mt_, auto r_, auto nt_) {
         constexpr int MT = decltype(mt_)::value, R = decltype(r_)::value, NT = decltype(nt_)::value;
-        const int blocks = (a.N + 16 * NT - 1) / (16 * NT), pieces = (a.K + 127) / 128;
+        const int blocks = (a.N + 16 * NT - 1) / (16 * NT) * ((a.M + 63) / 64), pieces = (a.K + 127) / 128;
         const int most = MT == 1 ? 16 : 8, share = MT == 1 ? 2 : 1;
         int waves = 1;
         while (waves < most && blocks * waves < kCus * 16 && waves * 2 * share <= pieces) waves *= 2;
         const size_t lds = (size_t)waves * MT * R * NT * 64 * sizeof(float);
-        MYNN_LAUNCH((int4_rows_kernel<T, I8, FL, MT, R, NT>), dim3(blocks), dim3(64 * waves), lds, s, a);
+        MYNN_LAUNCH((int4_rows_kernel<T, I8, FL, MT, R, NT>), dim3((a.N + 16 * NT - 1) / (16 * NT), (a.M + 63) / 64), dim3(64 * waves), lds, s, a);
         return launch_status("int4_rows_kernel");
     };
     using std::integral_constant;
@@ -37,23 +37,42 @@ template <typename T, bool I8> static int int4_few(const Int4Args &a, hipStream_
     return int4_rows<T, I8, 4>(a, s);
 }
 
-template <typename T, bool I8, int FL> static int int4_tiles(const Int4Args &a, hipStream_t s) {
-    auto go = [&](auto wm_) {
-        constexpr int WM = decltype(wm_)::value, WN = 8 / WM;
-        using G = Int4Tile<I8, FL, WM, WN>;
-        const long long tiles = (long long)((a.M + G::BM - 1) / G::BM) * ((a.N + G::BN - 1) / G::BN);
-        MYNN_REQUIRE(tiles < 1 << 30, MYNN_ERR_UNSUPPORTED, "4-bit product: M=%d N=%d", a.M, a.N);
-        constexpr int lds = G::NS * G::STAGE;
-        static bool lds_set = false;
-        if (!lds_set) {
-            MYNN_HIP(hipFuncSetAttribute((const void *)int4_tile_kernel<T, I8, FL, WM, WN>, hipFuncAttributeMaxDynamicSharedMemorySize, lds));
-            lds_set = true;
-        }
-        MYNN_LAUNCH((int4_tile_kernel<T, I8, FL, WM, WN>), dim3((unsigned)tiles), dim3(512), lds, s, a);
-        return launch_status("int4_tile_kernel");
+// Heights of the row tiles, in blocks of 32 rows: four as often as they go and the rest in a short tile, or all (but for one block) alike, by
+// how long the last compute unit is busy.  A tile of h blocks takes h + 1.5 units, of int8 h + 2.2 (one round of K = 4096, us: 46, 58,
+// 80, 104 for one to four blocks of fp16, 40, 48, 60, 75 of int8).
+static Int4Rows int4_row_tiles(int M, int columns, double fixed) {
+    const int blocks = (M + 31) / 32;
+    auto busy = [&](const Int4Rows &r) {
+        const double high = r.high + fixed, low = r.low ? r.low + fixed : 0.0;
+        const long long tall = (long long)r.tall * columns, others = (long long)(r.tiles - r.tall) * columns, over = tall % kCus;
+        // (the short tiles go beside the tall ones of the last round, and on from there)
+        const long long beside = over && others ? (kCus - over) * (long long)(high / low) : 0;
+        return (double)((tall + kCus - 1) / kCus) * high + (others > beside ? (double)((others - beside + kCus - 1) / kCus) * low : 0.0);
     };
-    const char *tm = getenv("I4TM");
-    return tm && atoi(tm) == 1 ? go(std::integral_constant<int, 1>{}) : go(std::integral_constant<int, 2>{});
+    Int4Rows best{blocks / 4, 4, blocks % 4, (blocks + 3) / 4};
+    if (!best.tall) best = {1, blocks, 0, 1};
+    for (int tiles = (blocks + 3) / 4; tiles <= blocks; tiles++) {
+        const int low = blocks / tiles, over = blocks % tiles;
+        const Int4Rows even = over ? Int4Rows{over, low + 1, low, tiles} : Int4Rows{tiles, low, 0, tiles};
+        if (busy(even) < busy(best)) best = even;
+        if (low == 1) break;
+    }
+    return best;
+}
+
+template <typename T, bool I8, int FL> static int int4_tiles(const Int4Args &a, hipStream_t s) {
+    using G = Int4Tile<I8, FL>;
+    const int columns = (a.N + G::BN - 1) / G::BN;
+    const Int4Rows rows = int4_row_tiles(a.M, columns, I8 ? 2.2 : 1.5);
+    MYNN_REQUIRE((long long)rows.tiles * columns < 1 << 30, MYNN_ERR_UNSUPPORTED, "4-bit product: M=%d N=%d", a.M, a.N);
+    constexpr int lds = G::NS * G::STAGE;
+    static bool lds_set = false;
+    if (!lds_set) {
+        MYNN_HIP(hipFuncSetAttribute((const void *)int4_tile_kernel<T, I8, FL>, hipFuncAttributeMaxDynamicSharedMemorySize, lds));
+        lds_set = true;
+    }
+    MYNN_LAUNCH((int4_tile_kernel<T, I8, FL>), dim3(rows.tiles * columns), dim3(512), lds, s, a, rows);
+    return launch_status("int4_tile_kernel");
 }
 template <typename T, bool I8> static int int4_many(const Int4Args &a, hipStream_t s) {
     if (a.group == 32) return int4_tiles<T, I8, 1>(a, s);
@@ -83,7 +102,8 @@ extern "C" int mynn_dequant_matmul_int4(void *out, const void *act, const uint8_
     const Int4Args args{out, act, nullptr, wq, scale, zero, M, N, K, group, pieces_magic(group)};
     return dispatch_dtype16(dtype, [&](auto *t) {
         using T = std::remove_pointer_t<decltype(t)>;
-        return M <= 64 ? int4_few<T, false>(args, as_stream(s)) : int4_many<T, false>(args, as_stream(s));
+        static const int most_few = getenv("I4FEW") ? atoi(getenv("I4FEW")) : 64;
+        return M <= most_few ? int4_few<T, false>(args, as_stream(s)) : int4_many<T, false>(args, as_stream(s));
     });
 }
 
@@ -94,6 +114,7 @@ extern "C" int mynn_quantized_matmul_int4(void *out, const int8_t *lhs, const vo
     const Int4Args args{out, lhs, lhs_scale, wq, scale, zero, M, N, K, group, pieces_magic(group)};
     return dispatch_dtype16(dtype, [&](auto *t) {
         using T = std::remove_pointer_t<decltype(t)>;
-        return M <= 64 ? int4_few<T, true>(args, as_stream(s)) : int4_many<T, true>(args, as_stream(s));
+        static const int most_few = getenv("I4FEW") ? atoi(getenv("I4FEW")) : 64;
+        return M <= most_few ? int4_few<T, true>(args, as_stream(s)) : int4_many<T, true>(args, as_stream(s));
     });
 }

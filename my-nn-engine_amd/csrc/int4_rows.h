@@ -94,7 +94,7 @@ __global__ __launch_bounds__(MT == 1 ? 1024 : 512) void int4_rows_kernel(Int4Arg
     extern __shared__ __align__(16) float red[];
     const int lane = threadIdx.x & 63, col = lane & 15, kg = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
-    const int n0 = blockIdx.x * (16 * NT);
+    const int n0 = blockIdx.x * (16 * NT), m0 = blockIdx.y * 64;
     const int groups = p.K / p.group, full = p.K >> 7;
     constexpr int EB = I8 ? 1 : 2;
 
@@ -111,7 +111,7 @@ __global__ __launch_bounds__(MT == 1 ? 1024 : 512) void int4_rows_kernel(Int4Arg
     const char *arow[MT];
 #pragma unroll
     for (int t = 0; t < MT; t++) {
-        const size_t m = min(16 * t + (col & 3) * 4 + (col >> 2), p.M - 1);
+        const size_t m = min(m0 + 16 * t + (col & 3) * 4 + (col >> 2), p.M - 1);
         arow[t] = (const char *)p.act + (m * p.K + (FL == 4 ? 32 : 8) * kg) * EB;
     }
 
@@ -294,7 +294,7 @@ __global__ __launch_bounds__(MT == 1 ? 1024 : 512) void int4_rows_kernel(Int4Arg
     __syncthreads();
     for (int v = wave; v < V; v += waves) {
         const int t = v / (MT * R), m = v / R % MT, i = v % R;
-        const int row = 16 * m + 4 * i + kg, n = n0 + 16 * t + col;
+        const int row = m0 + 16 * m + 4 * i + kg, n = n0 + 16 * t + col;
         float sum = red[v * 64 + lane];
         for (int w = 1; w < waves; w++) sum += red[(w * V + v) * 64 + lane];
         if (row < p.M && n < p.N) {

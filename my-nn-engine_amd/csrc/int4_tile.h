@@ -57,14 +57,14 @@ struct Int4ZeroI8 {
 };
 
 // LDS of a stage: activations, codes, then a dword for each column's scale and one for its zero point, for each group of a piece
-template <bool I8, int FL, int WM, int WN> struct Int4Tile {
-    static constexpr int BM = 64 * WM, BN = 64 * WN, PARTS = 4 / FL;
+template <bool I8, int FL> struct Int4Tile {
+    static constexpr int TI = 4, BM = 32 * TI, BN = 256, PARTS = 4 / FL;
     static constexpr int ROW = I8 ? 128 : 256;  // bytes of a piece of an activation row
     static constexpr int A = BM * ROW, W = BN * 64, S = BN * 4 * PARTS;
     static constexpr int STAGE = A + W + 2 * S;
     static constexpr int NS = 3 * STAGE <= 160 * 1024 ? 3 : 2;
-    static constexpr int LA = A / 8192, LW = W / 8192, LS = PARTS * WN * 2 / 8;  // load instructions of a wave and stage
-    static_assert(WM * WN == 8 && NS * STAGE <= 160 * 1024, "");
+    static constexpr int LW = W / 8192, LS = PARTS;  // load instructions of a wave and stage, codes and scales
+    static_assert(NS * STAGE <= 160 * 1024, "");
 };
 
 // 4 or 1 or 2 bytes a lane to LDS dword lds + 4 * lane
@@ -80,26 +80,39 @@ __device__ inline void load_u8_to_lds(const void *p, uint32_t lds) {
 }
 #pragma clang diagnostic pop
 
-template <typename T, bool I8, int FL, int WM, int WN>
-__global__ __launch_bounds__(512, 2) void int4_tile_kernel(Int4Args p) {
-    using G = Int4Tile<I8, FL, WM, WN>;
+// The row tiles of a column: `tall` of `high` blocks of 32 rows, then short ones of `low`.
+struct Int4Rows {
+    int tall, high, low, tiles;
+};
+
+template <typename T, bool I8, int FL>
+__global__ __launch_bounds__(512, 2) void int4_tile_kernel(Int4Args p, Int4Rows rows) {
+    using G = Int4Tile<I8, FL>;
     constexpr int EB = I8 ? 1 : 2, ROW = G::ROW, PARTS = G::PARTS, NS = G::NS;
     constexpr int SP = (I8 ? 1 : 2) * FL;  // instructions to a scale
     constexpr int CPR = ROW / 16;          // 16-byte chunks of a row
     extern __shared__ __align__(16) char lds[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int wm = wave / WN, wn = wave % WN;
-    const int tiles_m = (p.M + G::BM - 1) / G::BM;
     // Consecutive workgroups go round-robin over the 8 XCDs: an id becomes an index that is contiguous inside an XCD, where the row
-    // tiles that share weights follow one another.
+    // tiles that share weights follow one another.  All tall tiles come before the short ones, which fill the gaps of the last round.
     int tm, tn;
     {
-        const int nb = gridDim.x, x = blockIdx.x & 7, per = nb >> 3, rem = nb & 7;
-        const int l = x * per + min(x, rem) + (blockIdx.x >> 3);
-        tn = l / tiles_m;
-        tm = l - tn * tiles_m;
+        const int x = blockIdx.x & 7, i = blockIdx.x >> 3;
+        const int columns = (p.N + G::BN - 1) / G::BN, tall = rows.tall * columns, others = rows.tiles - rows.tall, low = others * columns;
+        const int mine = (tall >> 3) + (x < (tall & 7)), y = (x - tall) & 7;  // (the XCDs that got one tall tile less come first for the short ones)
+        if (i < mine) {
+            const int l = x * (tall >> 3) + min(x, tall & 7) + i;
+            tn = l / rows.tall;
+            tm = l - tn * rows.tall;
+        } else {
+            const int l = y * (low >> 3) + min(y, low & 7) + i - mine;
+            tn = l / others;
+            tm = rows.tall + l - tn * others;
+        }
     }
-    const int m0 = __builtin_amdgcn_readfirstlane(tm * G::BM), n0 = __builtin_amdgcn_readfirstlane(tn * G::BN);
+    const bool is_tall = tm < rows.tall;
+    const int height = __builtin_amdgcn_readfirstlane(is_tall ? rows.high : rows.low);
+    const int m0 = 32 * __builtin_amdgcn_readfirstlane(is_tall ? tm * rows.high : rows.tall * rows.high + (tm - rows.tall) * rows.low), n0 = __builtin_amdgcn_readfirstlane(tn * G::BN);
     const int groups = p.K / p.group, pieces = (p.K + 127) >> 7;
     const int c32 = lane & 31, kh = lane >> 5;
 
@@ -107,12 +120,7 @@ __global__ __launch_bounds__(512, 2) void int4_tile_kernel(Int4Args p) {
     // neighbouring rows fall into different banks.  Offsets are from 4096 bytes in front of the tile's first row, less what load_group_to_lds adds.
     auto akey = [](int r) { return I8 ? (r >> 1) & 7 : r & 15; };
     auto wkey = [](int r) { return (r >> 2) & 3; };
-    uint32_t aoff[G::LA], woff[G::LW];
-#pragma unroll
-    for (int i = 0; i < G::LA; i++) {
-        const int at = (wave * G::LA + i) * 64 + lane, r = at / CPR;
-        aoff[i] = (uint32_t)min(r, p.M - 1 - m0) * (uint32_t)(p.K * EB) + 16u * (uint32_t)((at % CPR) ^ akey(r)) + 4096u - 1024u * (i % 4);
-    }
+    uint32_t woff[G::LW];
 #pragma unroll
     for (int i = 0; i < G::LW; i++) {
         const int at = (wave * G::LW + i) * 64 + lane, r = at / 4;
@@ -120,39 +128,30 @@ __global__ __launch_bounds__(512, 2) void int4_tile_kernel(Int4Args p) {
     }
     const char *abase = (const char *)p.act + (size_t)m0 * p.K * EB - 4096;
     const char *wbase = (const char *)p.wq + (size_t)n0 * (p.K >> 1) - 4096;
-    // scales by the first half of the loads of this kind, zero points by the second (scales again where there are none: all waves have the
-    // same number in flight)
     const uint32_t at0 = lds_offset(lds);
-    auto stage = [&](int c, int slot) {
-        const uint32_t to = at0 + slot * G::STAGE;
-        uint32_t ao[G::LA], wo[G::LW];
+    auto stage_codes = [&](int c, int slot) {
+        uint32_t off[G::LW];
 #pragma unroll
-        for (int i = 0; i < G::LA; i++) ao[i] = aoff[i];
-#pragma unroll
-        for (int i = 0; i < G::LW; i++) wo[i] = woff[i];
-        if (FL < 4 && 128 * c + 128 > p.K) {  // (chunks behind the row are not multiplied: its last one in their place)
-            const int alast = (p.K - 128 * c) * EB / 16 - 1, wlast = (p.K - 128 * c) / 32 - 1;
-#pragma unroll
-            for (int i = 0; i < G::LA; i++) {
-                const int at = (wave * G::LA + i) * 64 + lane;
-                ao[i] -= 16u * (uint32_t)max(((at % CPR) ^ akey(at / CPR)) - alast, 0);
-            }
+        for (int i = 0; i < G::LW; i++) off[i] = woff[i];
+        if (FL < 4 && 128 * c + 128 > p.K) {
+            const int last = (p.K - 128 * c) / 32 - 1;
 #pragma unroll
             for (int i = 0; i < G::LW; i++) {
                 const int at = (wave * G::LW + i) * 64 + lane;
-                wo[i] -= 16u * (uint32_t)max(((at % 4) ^ wkey(at / 4)) - wlast, 0);
+                off[i] -= 16u * (uint32_t)max(((at % 4) ^ wkey(at / 4)) - last, 0);
             }
         }
-        const char *a = abase + (size_t)c * ROW, *w = wbase + (size_t)c * 64;
-#pragma unroll
-        for (int i = 0; i + 4 <= G::LA; i += 4) load_group_to_lds<4>(a, ao + i, to + (wave * G::LA + i) * 1024);
-        if constexpr (G::LA % 4) load_group_to_lds<G::LA % 4>(a, ao + G::LA / 4 * 4, to + (wave * G::LA + G::LA / 4 * 4) * 1024);
-        load_group_to_lds<G::LW>(w, wo, to + G::A + wave * G::LW * 1024);
+        load_group_to_lds<G::LW>(wbase + (size_t)c * 64, off, at0 + slot * G::STAGE + G::A + wave * G::LW * 1024);
+    };
+    // scales by the first half of the loads of this kind, zero points by the second (scales again where there are none: all waves have the
+    // same number in flight)
+    auto stage_scales = [&](int c, int slot) {
+        const uint32_t to = at0 + slot * G::STAGE;
 #pragma unroll
         for (int i = 0; i < G::LS; i++) {
-            const int v = wave * G::LS + i, half = PARTS * WN;          // (of the wave alike)
+            const int v = wave * G::LS + i, half = PARTS * 4;  // (of the wave alike)
             const bool zeros = v >= half;
-            const int u = zeros ? v - half : v, part = u / WN, block = u % WN;
+            const int u = zeros ? v - half : v, part = u / 4, block = u % 4;
             const size_t n = min(n0 + 64 * block + lane, p.N - 1);
             const int g = FL == 4 ? (p.pieces_magic ? (int)__umulhi((uint32_t)c, p.pieces_magic) : c) : min(c * PARTS + part, groups - 1);
             const uint32_t slot_at = to + G::A + G::W + v * 256;
@@ -160,111 +159,139 @@ __global__ __launch_bounds__(512, 2) void int4_tile_kernel(Int4Args p) {
             else load_u16_to_lds((const uint16_t *)p.scale + n * groups + g, slot_at);
         }
     };
-    constexpr int INFLIGHT = G::LA + G::LW + G::LS;
-
-    f16x_t tot[2][2];
+    auto run = [&](auto ti_) {
+        constexpr int TI = decltype(ti_)::value;
+        constexpr int LA = (32 * TI * ROW + 8191) / 8192, INFLIGHT = LA + G::LW + G::LS;
+        uint32_t aoff[LA];
 #pragma unroll
-    for (int i = 0; i < 2; i++)
-#pragma unroll
-        for (int t = 0; t < 2; t++)
-#pragma unroll
-            for (int e = 0; e < 16; e++) tot[i][t][e] = 0.f;
-
-    stage(0, 0);
-    if (NS == 3 && pieces > 1) stage(1, 1);
-    int slot = 0;
-    for (int c = 0; c < pieces; c++) {
-        // this piece has arrived (the next one may be on its way), and nobody reads the stage that is filled next any more
-        if (NS == 3 && c + 1 < pieces) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(INFLIGHT) : "memory");
-        else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        __syncthreads();
-        if (c + NS - 1 < pieces) stage(c + NS - 1, slot == 0 ? NS - 1 : slot - 1);
-        const char *at = lds + slot * G::STAGE;
-        slot = slot == NS - 1 ? 0 : slot + 1;
-
-        uint32_t w[2][8];
-#pragma unroll
-        for (int t = 0; t < 2; t++) {
-            const int r = 64 * wn + 32 * t + c32;
-            const char *row = at + G::A + r * 64;
-            if constexpr (FL == 1) {
-#pragma unroll
-                for (int h = 0; h < 4; h++) {
-                    const uint2 v = *(const uint2 *)(row + (h ^ wkey(r)) * 16 + 8 * kh);
-                    w[t][2 * h] = v.x;
-                    w[t][2 * h + 1] = v.y;
-                }
-            } else {
-#pragma unroll
-                for (int h = 0; h < 2; h++) {
-                    const U4 v = *(const U4 *)(row + ((2 * h + kh) ^ wkey(r)) * 16);
-#pragma unroll
-                    for (int j = 0; j < 4; j++) w[t][4 * h + j] = v[j];
-                }
-            }
+        for (int i = 0; i < LA; i++) {
+            const int at = (wave * LA + i) * 64 + lane, r = at / CPR;
+            aoff[i] = (uint32_t)min(r, p.M - 1 - m0) * (uint32_t)(p.K * EB) + 16u * (uint32_t)((at % CPR) ^ akey(r)) + 4096u - 1024u * (i % 4);
         }
+        auto stage_act = [&](int c, int slot) {
+            uint32_t off[LA];
 #pragma unroll
-        for (int part = 0; part < PARTS; part++) {
-            if (FL < 4 && 128 * c + 32 * FL * part >= p.K) break;
-            float s[2];
-            uint32_t z[2];
+            for (int i = 0; i < LA; i++) off[i] = aoff[i];
+            if (FL < 4 && 128 * c + 128 > p.K) {  // (chunks behind the row are not multiplied: its last one in their place)
+                const int last = (p.K - 128 * c) * EB / 16 - 1;
 #pragma unroll
-            for (int t = 0; t < 2; t++) {
-                const char *sz = at + G::A + G::W + ((part * WN + wn) * 64 + 32 * t + c32) * 4;
-                const uint16_t half = *(const uint16_t *)sz;
-                s[t] = Elem<T>::ld((const T *)&half, 0);
-                z[t] = p.zero ? *(const uint32_t *)(sz + G::S) & 15u : 8u;
+                for (int i = 0; i < LA; i++) {
+                    const int at = (wave * LA + i) * 64 + lane;
+                    off[i] -= 16u * (uint32_t)max(((at % CPR) ^ akey(at / CPR)) - last, 0);
+                }
             }
-            std::conditional_t<I8, i16v_t, f16x_t> acc[2][2] = {{{}, {}}, {{}, {}}};
-            const std::conditional_t<I8, Int4ZeroI8, Int4Zero<T>> conv[2] = {std::conditional_t<I8, Int4ZeroI8, Int4Zero<T>>(z[0]), std::conditional_t<I8, Int4ZeroI8, Int4Zero<T>>(z[1])};
+            const char *a = abase + (size_t)c * ROW;
+            const uint32_t to = at0 + slot * G::STAGE + wave * LA * 1024;
 #pragma unroll
-            for (int k = 0; k < SP; k++) {
-                const int st = part * SP + k;  // instruction of the piece
+            for (int i = 0; i + 4 <= LA; i += 4) load_group_to_lds<4>(a, off + i, to + i * 1024);
+            if constexpr (LA % 4) load_group_to_lds<LA % 4>(a, off + LA / 4 * 4, to + LA / 4 * 4096);
+        };
+        auto stage = [&](int c, int slot) {
+            stage_act(c, slot);
+            stage_codes(c, slot);
+            stage_scales(c, slot);
+        };
+        f16x_t tot[TI];
+#pragma unroll
+        for (int i = 0; i < TI; i++)
+#pragma unroll
+            for (int e = 0; e < 16; e++) tot[i][e] = 0.f;
+
+        stage(0, 0);
+        if (NS == 3 && pieces > 1) stage(1, 1);
+        int slot = 0;
+        for (int c = 0; c < pieces; c++) {
+            // this piece has arrived (the next one may be on its way), and nobody reads the stage that is filled next any more
+            if (NS == 3 && c + 1 < pieces) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(INFLIGHT) : "memory");
+            else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            __syncthreads();
+            const int to = slot == 0 ? NS - 1 : slot - 1;
+            const char *at = lds + slot * G::STAGE;
+            slot = slot == NS - 1 ? 0 : slot + 1;
+
+            uint32_t w[8];
+            {
+                const int r = 32 * wave + c32;
+                const char *row = at + G::A + r * 64;
+                if constexpr (FL == 1) {
+#pragma unroll
+                    for (int h = 0; h < 4; h++) {
+                        const uint2 v = *(const uint2 *)(row + (h ^ wkey(r)) * 16 + 8 * kh);
+                        w[2 * h] = v.x;
+                        w[2 * h + 1] = v.y;
+                    }
+                } else {
+#pragma unroll
+                    for (int h = 0; h < 2; h++) {
+                        const U4 v = *(const U4 *)(row + ((2 * h + kh) ^ wkey(r)) * 16);
+#pragma unroll
+                        for (int j = 0; j < 4; j++) w[4 * h + j] = v[j];
+                    }
+                }
+            }
+            // (fragments are read an instruction ahead, and the loads of a later piece asked for between the first products)
+            U4 a[2][TI];
+            auto fragments = [&](int st) {
                 int chunk;
                 if constexpr (I8) chunk = FL == 1 ? 2 * st + kh : 4 * (st >> 1) + 2 * kh + (st & 1);
                 else chunk = FL == 1 ? 4 * (st >> 1) + 2 * kh + (st & 1) : 8 * (st >> 2) + 4 * kh + (st & 3);
-                U4 a[2], b[2];
 #pragma unroll
-                for (int i = 0; i < 2; i++) {
-                    const int r = 64 * wm + 32 * i + c32;
-                    a[i] = *(const U4 *)(at + r * ROW + (chunk ^ akey(r)) * 16);
+                for (int i = 0; i < TI; i++) {
+                    const int r = 32 * i + c32;
+                    a[st & 1][i] = *(const U4 *)(at + r * ROW + (chunk ^ akey(r)) * 16);
                 }
+            };
+            fragments(0);
+            const bool more = c + NS - 1 < pieces;
 #pragma unroll
-                for (int t = 0; t < 2; t++) {
-                    if constexpr (I8) b[t] = conv[t](w[t][2 * st], w[t][2 * st + 1]);
-                    else b[t] = conv[t](w[t][st]);
-                }
+            for (int part = 0; part < PARTS; part++) {
+                if (FL < 4 && 128 * c + 32 * FL * part >= p.K) break;
+                const char *sz = at + G::A + G::W + (part * 256 + 32 * wave + c32) * 4;
+                const uint16_t half = *(const uint16_t *)sz;
+                const float s = Elem<T>::ld((const T *)&half, 0);
+                const std::conditional_t<I8, Int4ZeroI8, Int4Zero<T>> conv(p.zero ? *(const uint32_t *)(sz + G::S) & 15u : 8u);
+                std::conditional_t<I8, i16v_t, f16x_t> acc[TI] = {};
 #pragma unroll
-                for (int i = 0; i < 2; i++)
-#pragma unroll
-                    for (int t = 0; t < 2; t++) {
-                        if constexpr (I8)
-                            acc[i][t] = __builtin_amdgcn_mfma_i32_32x32x32_i8(__builtin_bit_cast(i4_t, a[i]), __builtin_bit_cast(i4_t, b[t]), acc[i][t], 0, 0, 0);
-                        else acc[i][t] = Mfma<T>::run(a[i], b[t], acc[i][t]);
+                for (int k = 0; k < SP; k++) {
+                    const int st = part * SP + k;  // instruction of the piece
+                    if (st + 1 < PARTS * SP) fragments(st + 1);
+                    if (more && part == 0) {
+                        if (k == 0) stage_act(c + NS - 1, to);
+                        if (k == (SP > 1 ? 1 : 0)) stage_codes(c + NS - 1, to);
+                        if (k == (SP > 2 ? 2 : SP - 1)) stage_scales(c + NS - 1, to);
                     }
+                    U4 b;
+                    if constexpr (I8) b = conv(w[2 * st], w[2 * st + 1]);
+                    else b = conv(w[st]);
+#pragma unroll
+                    for (int i = 0; i < TI; i++) {
+                        if constexpr (I8) acc[i] = __builtin_amdgcn_mfma_i32_32x32x32_i8(__builtin_bit_cast(i4_t, a[st & 1][i]), __builtin_bit_cast(i4_t, b), acc[i], 0, 0, 0);
+                        else acc[i] = Mfma<T>::run(a[st & 1][i], b, acc[i]);
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+#pragma unroll
+                for (int i = 0; i < TI; i++)
+#pragma unroll
+                    for (int e = 0; e < 16; e++) tot[i][e] = fmaf(s, (float)acc[i][e], tot[i][e]);
             }
-#pragma unroll
-            for (int i = 0; i < 2; i++)
-#pragma unroll
-                for (int t = 0; t < 2; t++)
-#pragma unroll
-                    for (int e = 0; e < 16; e++) tot[i][t][e] = fmaf(s[t], (float)acc[i][t][e], tot[i][t][e]);
         }
-    }
 
+        const int n = n0 + 32 * wave + c32;
 #pragma unroll
-    for (int i = 0; i < 2; i++)
+        for (int i = 0; i < TI; i++)
 #pragma unroll
-        for (int e = 0; e < 16; e++) {
-            const int row = m0 + 64 * wm + 32 * i + 8 * (e >> 2) + 4 * kh + (e & 3);
-            if (row >= p.M) continue;
-            const float as = I8 ? Elem<T>::ld((const T *)p.act_scale, row) : 1.f;
-#pragma unroll
-            for (int t = 0; t < 2; t++) {
-                const int n = n0 + 64 * wn + 32 * t + c32;
-                if (n < p.N) Elem<T>::st((T *)p.out, (size_t)row * p.N + n, I8 ? tot[i][t][e] * as : tot[i][t][e]);
+            for (int e = 0; e < 16; e++) {
+                const int row = m0 + 32 * i + 8 * (e >> 2) + 4 * kh + (e & 3);
+                if (row < p.M && n < p.N)
+                    Elem<T>::st((T *)p.out, (size_t)row * p.N + n, I8 ? tot[i][e] * Elem<T>::ld((const T *)p.act_scale, row) : tot[i][e]);
             }
-        }
+    };
+    // (a loop for each height: the sums and fragments are registers)
+    if (height == 4) run(std::integral_constant<int, 4>{});
+    else if (height == 3) run(std::integral_constant<int, 3>{});
+    else if (height == 2) run(std::integral_constant<int, 2>{});
+    else run(std::integral_constant<int, 1>{});
 }
 
 }  // namespace mynn
