@@ -3,6 +3,9 @@
 // none are given.  The sum of a group runs over the bare differences (small integers, exact in every type) and meets its scale once:
 //   out[m, n] = T( sum over groups of scale[n, g] * sum over k in g of act[m, k] * (code[n, k] - zero[n, g]) )
 // in 32 bits, rounded at the store; with int8 activations the inner sum is exact in int32 and the row's scale is applied last.
+#include <algorithm>
+
+#include "int4_stream.h"
 #include "int4_tile.h"
 
 namespace mynn {
@@ -31,7 +34,44 @@ template <typename T, bool I8, int FL> static int int4_rows(const Int4Args &a, h
     return go(integral_constant<int, 4>{}, integral_constant<int, 4>{}, integral_constant<int, 2>{});
 }
 
+// Up to 8 rows.  Rows of whole slices, at least a tile of them.
+static bool int4_streams(const Int4Args &a) { return a.M <= 8 && a.K % 128 == 0 && a.N >= 8 && (size_t)8 * a.K < 1u << 31; }
+
+template <typename T, bool I8, int FL> static int int4_stream(const Int4Args &a, hipStream_t s) {
+    auto go = [&](auto mp_, auto p_, auto d_) {
+        constexpr int MP = decltype(mp_)::value, P = decltype(p_)::value, D = decltype(d_)::value;
+        const int units = (a.K / 128 + 16 / MP * P - 1) / (16 / MP * P), tiles = (a.N + MP - 1) / MP;
+        Int4Stream plan;
+        plan.slabs = (units + 7) / 8;
+        plan.over_k = (units + plan.slabs - 1) / plan.slabs;
+        // eight waves a compute unit: each loads its activations once (twelve, 28672 x 4096, one row: 14.1 -> 15.6 us; six: 16.4)
+        const int turns = std::max(1, 4 / plan.over_k), slots = kCus * 8 / plan.over_k;
+        const int most = std::max(1, 32768 / (plan.over_k * MP * MP * (int)sizeof(float)) / turns);
+        plan.per_wave = std::min(std::min(most, 64), (tiles + slots - 1) / slots);
+        plan.tiles = turns * plan.per_wave;
+        const size_t lds = (size_t)plan.tiles * plan.over_k * MP * MP * sizeof(float);
+        MYNN_LAUNCH((int4_stream_kernel<T, I8, FL, MP, P, D>), dim3((tiles + plan.tiles - 1) / plan.tiles), dim3(64 * turns * plan.over_k), lds, s, a, plan);
+        return launch_status("int4_stream_kernel");
+    };
+    using std::integral_constant;
+    // (P, D): units of 128 S columns of a wave's share, tiles in flight.  Larger shares where eight waves do not cover K otherwise (4096 x 14336, us,
+    // four rows: 14.4 -> 12.5, eight 19.7 -> 18.1; elsewhere slower: 28672 x 4096, one row 14.1 -> 20.6).
+    auto shares = [&](auto mp) {
+        constexpr int MP = decltype(mp)::value;
+        if constexpr (FL > 1) {
+            if (a.K > 128 * (16 / MP) * 2 * 8) return go(mp, integral_constant<int, 4>{}, integral_constant<int, 2>{});
+        }
+        if (MP == 1 && a.K <= 2048) return go(mp, integral_constant<int, 1>{}, integral_constant<int, 4>{});
+        return go(mp, integral_constant<int, 2>{}, integral_constant<int, 3>{});
+    };
+    if (a.M == 1) return shares(integral_constant<int, 1>{});
+    if (a.M == 2) return shares(integral_constant<int, 2>{});
+    if (a.M <= 4) return shares(integral_constant<int, 4>{});
+    return shares(integral_constant<int, 8>{});
+}
+
 template <typename T, bool I8> static int int4_few(const Int4Args &a, hipStream_t s) {
+    if (int4_streams(a)) return a.group == 32 ? int4_stream<T, I8, 1>(a, s) : a.group == 64 ? int4_stream<T, I8, 2>(a, s) : int4_stream<T, I8, 4>(a, s);
     if (a.group == 32) return int4_rows<T, I8, 1>(a, s);
     if (a.group == 64) return int4_rows<T, I8, 2>(a, s);
     return int4_rows<T, I8, 4>(a, s);

@@ -106,7 +106,7 @@ __global__ __launch_bounds__(MT == 1 ? 1024 : 512) void int4_rows_kernel(Int4Arg
         const size_t n = min(n0 + 16 * t + col, p.N - 1);
         wrow[t] = p.wq + n * (size_t)(p.K >> 1) + kg * 16;
         srow[t] = (const T *)p.scale + n * groups;
-        zrow[t] = p.zero ? p.zero + n * groups : nullptr;
+        zrow[t] = p.zero ? p.zero + n * groups : (const uint8_t *)srow[t];  // (any that may be read: no test around the loads)
     }
     const char *arow[MT];
 #pragma unroll
@@ -144,27 +144,22 @@ __global__ __launch_bounds__(MT == 1 ? 1024 : 512) void int4_rows_kernel(Int4Arg
             if constexpr (FL == 4) {
                 const int g = p.pieces_magic ? (int)__umulhi((uint32_t)c, p.pieces_magic) : c;
                 q.s[t].x = ((const uint16_t *)srow[t])[g];
-                q.z[t] = zrow[t] ? zrow[t][g] : 8u;
+                q.z[t] = zrow[t][g];
             } else {
                 constexpr int P = 4 / FL;  // groups of a piece
                 const int g = c * P, have = FL == 1 ? steps : (steps + 1) / 2;
-                uint32_t s[4] = {0, 0, 0, 0}, z = 0x08080808u;
+                uint32_t s[4] = {0, 0, 0, 0}, z = 0;
                 if (have == P) {  // (of the wave alike)
                     if constexpr (P == 4) __builtin_memcpy(&q.s[t], srow[t] + g, 8);
                     else __builtin_memcpy(&q.s[t].x, srow[t] + g, 4);
-                    if (zrow[t]) {
-                        z = 0;
-                        __builtin_memcpy(&z, zrow[t] + g, P);
-                    }
+                    __builtin_memcpy(&z, zrow[t] + g, P);
                 } else {
-                    uint32_t zz = 0;
                     for (int i = 0; i < P; i++) {
                         const int at = g + min(i, have - 1);
                         s[i] = ((const uint16_t *)srow[t])[at];
-                        zz |= (zrow[t] ? (uint32_t)zrow[t][at] : 8u) << (8 * i);
+                        z |= (uint32_t)zrow[t][at] << (8 * i);
                     }
                     q.s[t] = uint2{s[0] | s[1] << 16, s[2] | s[3] << 16};
-                    z = zz;
                 }
                 q.z[t] = z;
             }
@@ -181,6 +176,10 @@ __global__ __launch_bounds__(MT == 1 ? 1024 : 512) void int4_rows_kernel(Int4Arg
         if constexpr (FL < 4) {
 #pragma unroll
             for (int t = 0; t < NT; t++) int4_transpose(q.w[t]);
+        }
+        if (!p.zero) {
+#pragma unroll
+            for (int t = 0; t < NT; t++) q.z[t] = 0x08080808u;
         }
 #pragma unroll
         for (int part = 0; part < 4 / FL; part++) {
