@@ -18,8 +18,8 @@
  * next `model_init` (the reference ABI has no other way to say it; `mynn_model_create` takes the
  * configuration as an argument and touches nothing global); (b) the scratch memory of the entry
  * points that need some and are not given any: `mynn_dequant_matmul` (M >= 2), `mynn_quantized_matmul`
- * (M >= 3), `mynn_attention` (a cache split over workgroups) and `mynn_attention_streaming`.  Each of
- * these three groups keeps one grown-on-demand block PER STREAM, locked until the call's launches are
+ * (M >= 3), `mynn_attention` (a cache split over workgroups), `mynn_attention_streaming` and the products with 4-bit weights
+ * (more than 8 rows).  Each of these groups keeps one grown-on-demand block PER STREAM, locked until the call's launches are
  * made, so calls on different streams never share one and several host threads may call on one stream.
  * Growing synchronises that stream and cannot happen while the stream is being captured: a captured call
  * that needs a larger block than there is fails with MYNN_ERR_STATE (make it once before the capture).
@@ -140,18 +140,28 @@ int mynn_quantized_matmul(void *out, int32_t *acc_out, const int8_t *lhs, const 
  * scale [N, K/group] in dtype, zero uint8 [N, K/group] (its low four bits) or NULL for 8 everywhere:
  *   w[n,k] = scale[n, k/group] * (wq[n,k] - zero[n, k/group]).
  * Sums are over the codes' differences, which are exact, and meet the scale once per group, in f32; one rounding at the
- * store.  No scratch memory: both calls may be captured into a graph and overlap on any streams, and give the same bits
- * from call to call.  An infinity or a NaN of act goes where the formula takes it: to its own row of out.
+ * store.  An infinity or a NaN of act goes where the formula takes it: to its own row of out.  K up to 2^22.
+ * Where the tiles of more than 8 rows leave the device idle, the f32 sums run over several ranges of K, added in their order; their
+ * number is a function of M, N, K and the group alone, and every form of a call gives the same bits.  The ranges' sums need
+ * mynn_matmul_int4_workspace_bytes(...) bytes (0: no ranges): the _ws forms take them from the caller (16-byte aligned;
+ * nothing global is touched, and calls whose workspaces differ may overlap), the others from a block of the stream's; while being
+ * captured those use no memory at all and take the ranges one after the other (48 rows of 4096 x 14336: 89 us for 25).
  *
  * act [M,K] (16-byte aligned), out [M,N], scale share dtype, MYNN_F16 or MYNN_BF16:
  *   out[m,n] = T(sum_g scale[n,g] * sum_{k in g} act[m,k] * (wq[n,k] - zero[n,g])). */
 int mynn_dequant_matmul_int4(void *out, const void *act, const uint8_t *wq, const void *scale, const uint8_t *zero,
                              int M, int N, int K, int group, int dtype, mynn_stream s);
+size_t mynn_matmul_int4_workspace_bytes(int M, int N, int K, int group);
+int mynn_dequant_matmul_int4_ws(void *out, const void *act, const uint8_t *wq, const void *scale, const uint8_t *zero,
+                                int M, int N, int K, int group, int dtype, void *workspace, size_t workspace_bytes, mynn_stream s);
 /* The same for int8 rows with a scale each (what mynn_dynamic_quantize_linear and mynn_add_rms_norm_quantize write):
  * lhs [M,K] (16-byte aligned), lhs_scale [M]; a group's sum (of at most 128 columns) is exact in int32:
  *   out[m,n] = T(lhs_scale[m] * sum_g scale[n,g] * sum_{k in g} lhs[m,k] * (wq[n,k] - zero[n,g])). */
 int mynn_quantized_matmul_int4(void *out, const int8_t *lhs, const void *lhs_scale, const uint8_t *wq, const void *scale,
                                const uint8_t *zero, int M, int N, int K, int group, int dtype, mynn_stream s);
+int mynn_quantized_matmul_int4_ws(void *out, const int8_t *lhs, const void *lhs_scale, const uint8_t *wq, const void *scale,
+                                  const uint8_t *zero, int M, int N, int K, int group, int dtype, void *workspace,
+                                  size_t workspace_bytes, mynn_stream s);
 
 /* DynamicQuantizeLinear -- dynamic_quantize_linear.cuh:39-153
  * `dynamic_quantize_linear_kernel(y,y_scale,y_zero_point,x,axis_dim,inner_size)`.

@@ -81,6 +81,9 @@ SIGNATURES = {
     "mynn_dequant_matmul_prepared": (_i, [_vp, _vp, _vp, _i, _i, _i, _i, _i, _vp]),
     "mynn_quantized_matmul": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _vp]),
     "mynn_dequant_matmul_int4": (_i, [_vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _vp]),
+    "mynn_matmul_int4_workspace_bytes": (_sz, [_i, _i, _i, _i]),
+    "mynn_dequant_matmul_int4_ws": (_i, [_vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _vp, _sz, _vp]),
+    "mynn_quantized_matmul_int4_ws": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _vp, _sz, _vp]),
     "mynn_quantized_matmul_int4": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _vp]),
     "mynn_dynamic_quantize_linear": (_i, [_vp, _vp, _vp, _vp, _i, _i, _i, _i, _vp]),
     "mynn_attention": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _f, _i, _i, _i, _i, _vp, _i, _i, _i, _i, _i, _i, _i, _vp]),
@@ -256,8 +259,8 @@ def _load_host_ops():
     module.bind(MynnError, *(C.cast(getattr(l, n), _vp).value for n in (
         "mynn_last_error", "mynn_dequant_matmul", "mynn_quantized_matmul", "mynn_dynamic_quantize_linear", "mynn_attention")))
     module.bind_int4(*(C.cast(getattr(l, n), _vp).value for n in (
-        "mynn_dequant_matmul_int4", "mynn_quantized_matmul_int4", "mynn_add_rms_norm", "mynn_add_rms_norm_quantize",
-        "mynn_dequantize_linear")))
+        "mynn_dequant_matmul_int4_ws", "mynn_quantized_matmul_int4_ws", "mynn_add_rms_norm", "mynn_add_rms_norm_quantize",
+        "mynn_dequantize_linear", "mynn_matmul_int4_workspace_bytes")))
     return module
 
 
@@ -377,6 +380,12 @@ def _int4_shape(wq, scale, zero):
     return N, 2 * half, 2 * half // groups
 
 
+def _int4_workspace(wq, M, N, K, group):
+    """the product's memory from torch (a captured call's is the graph's own), None where it needs none"""
+    need = lib().mynn_matmul_int4_workspace_bytes(M, N, K, group)
+    return wq.new_empty((need,)) if need else None
+
+
 def dequant_matmul_int4(act, wq, scale, zero=None):
     """act [.., K] in 16 bits times 4-bit weights (wq uint8 [N, K/2], scale [N, groups], zero uint8 [N, groups] or None): [.., N]"""
     if wq.is_cuda:
@@ -388,8 +397,10 @@ def dequant_matmul_int4(act, wq, scale, zero=None):
     if act.shape[-1] != K or act.dtype != scale.dtype:
         raise MynnError("dequant_matmul_int4: act %s %s, scale %s and K=%d do not fit together" % (tuple(act.shape), act.dtype, scale.dtype, K))
     out = wq.new_empty(act.shape[:-1] + (N,), dtype=scale.dtype)
-    check(lib().mynn_dequant_matmul_int4(_ptr(out), _ptr(act), _ptr(wq), _ptr(scale), _ptr(zero), act.numel() // K, N, K, group, _dt(scale),
-                                         _stream()))
+    M = act.numel() // K
+    ws = _int4_workspace(wq, M, N, K, group)
+    check(lib().mynn_dequant_matmul_int4_ws(_ptr(out), _ptr(act), _ptr(wq), _ptr(scale), _ptr(zero), M, N, K, group, _dt(scale), _ptr(ws),
+                                            0 if ws is None else ws.numel(), _stream()))
     return out
 
 
@@ -404,9 +415,11 @@ def quantized_matmul_int4(lhs, lhs_scale, wq, scale, zero=None):
     if lhs.dim() != 2 or lhs.shape[1] != K or lhs.dtype != _torch.int8 or lhs_scale.numel() != lhs.shape[0] or lhs_scale.dtype != scale.dtype:
         raise MynnError("quantized_matmul_int4: lhs %s %s, lhs_scale %s %s, scale %s and K=%d do not fit together" % (
             tuple(lhs.shape), lhs.dtype, tuple(lhs_scale.shape), lhs_scale.dtype, scale.dtype, K))
-    out = wq.new_empty((lhs.shape[0], N), dtype=scale.dtype)
-    check(lib().mynn_quantized_matmul_int4(_ptr(out), _ptr(lhs), _ptr(lhs_scale), _ptr(wq), _ptr(scale), _ptr(zero), lhs.shape[0], N, K, group,
-                                           _dt(scale), _stream()))
+    M = lhs.shape[0]
+    out = wq.new_empty((M, N), dtype=scale.dtype)
+    ws = _int4_workspace(wq, M, N, K, group)
+    check(lib().mynn_quantized_matmul_int4_ws(_ptr(out), _ptr(lhs), _ptr(lhs_scale), _ptr(wq), _ptr(scale), _ptr(zero), M, N, K, group, _dt(scale),
+                                              _ptr(ws), 0 if ws is None else ws.numel(), _stream()))
     return out
 
 

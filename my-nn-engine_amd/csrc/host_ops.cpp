@@ -20,8 +20,9 @@ decltype(&mynn_dequant_matmul) g_dequant_matmul;
 decltype(&mynn_quantized_matmul) g_quantized_matmul;
 decltype(&mynn_dynamic_quantize_linear) g_dynamic_quantize_linear;
 decltype(&mynn_attention) g_attention;
-decltype(&mynn_dequant_matmul_int4) g_dequant_matmul_int4;
-decltype(&mynn_quantized_matmul_int4) g_quantized_matmul_int4;
+decltype(&mynn_matmul_int4_workspace_bytes) g_int4_bytes;
+decltype(&mynn_dequant_matmul_int4_ws) g_dequant_matmul_int4;
+decltype(&mynn_quantized_matmul_int4_ws) g_quantized_matmul_int4;
 decltype(&mynn_add_rms_norm) g_add_rms_norm;
 decltype(&mynn_add_rms_norm_quantize) g_add_rms_norm_quantize;
 decltype(&mynn_dequantize_linear) g_dequantize_linear;
@@ -179,6 +180,11 @@ struct Int4 {
         code = code_of(scale->scalar_type());
     }
     explicit operator bool() const { return K > 0 && code >= 0; }
+    // memory for a product of M rows (torch's: a captured call's is the graph's own); undefined where it needs none
+    at::Tensor workspace(int64_t M) const {
+        const size_t bytes = g_int4_bytes((int)M, (int)N, (int)K, (int)(K / groups));
+        return bytes ? make({(int64_t)bytes}, *wq, at::kByte) : at::Tensor();
+    }
 };
 
 // (act [.., K], wq, scale, zero or None) -> [.., N]
@@ -193,9 +199,12 @@ PyObject *dequant_matmul_int4(PyObject *, PyObject *const *args, Py_ssize_t n) {
         sizes.back() = w.N;
         const at::Tensor out = make(sizes, *w.wq, w.scale->scalar_type());
         void *o = data(out), *a = data(*act), *q = data(*w.wq), *s = data(*w.scale), *z = w.zero ? data(*w.zero) : nullptr;
+        const at::Tensor ws = w.workspace(M);
+        void *wsp = ws.defined() ? data(ws) : nullptr;
+        const size_t bytes = ws.defined() ? (size_t)ws.numel() : 0;
         const mynn_stream st = current_stream();
         const int rc = without_gil([&] {
-            return g_dequant_matmul_int4(o, a, (const uint8_t *)q, s, (const uint8_t *)z, (int)M, (int)w.N, (int)w.K, (int)(w.K / w.groups), w.code, st);
+            return g_dequant_matmul_int4(o, a, (const uint8_t *)q, s, (const uint8_t *)z, (int)M, (int)w.N, (int)w.K, (int)(w.K / w.groups), w.code, wsp, bytes, st);
         });
         return rc ? failed(rc) : THPVariable_Wrap(out);
     });
@@ -213,10 +222,13 @@ PyObject *quantized_matmul_int4(PyObject *, PyObject *const *args, Py_ssize_t n)
         const int64_t M = lhs->size(0);
         const at::Tensor out = make({M, w.N}, *w.wq, w.scale->scalar_type());
         void *o = data(out), *l = data(*lhs), *lsp = data(*ls), *q = data(*w.wq), *s = data(*w.scale), *z = w.zero ? data(*w.zero) : nullptr;
+        const at::Tensor ws = w.workspace(M);
+        void *wsp = ws.defined() ? data(ws) : nullptr;
+        const size_t bytes = ws.defined() ? (size_t)ws.numel() : 0;
         const mynn_stream st = current_stream();
         const int rc = without_gil([&] {
             return g_quantized_matmul_int4(o, (const int8_t *)l, lsp, (const uint8_t *)q, s, (const uint8_t *)z, (int)M, (int)w.N, (int)w.K, (int)(w.K / w.groups),
-                                           w.code, st);
+                                           w.code, wsp, bytes, st);
         });
         return rc ? failed(rc) : THPVariable_Wrap(out);
     });
@@ -329,17 +341,18 @@ PyObject *bind(PyObject *, PyObject *const *args, Py_ssize_t n) {
 
 // (addresses of the operators of 4-bit weights and of dequantize_linear, behind bind)
 PyObject *bind_int4(PyObject *, PyObject *const *args, Py_ssize_t n) {
-    if (n != 5) {
-        PyErr_SetString(PyExc_TypeError, "bind_int4: five arguments");
+    if (n != 6) {
+        PyErr_SetString(PyExc_TypeError, "bind_int4: six arguments");
         return nullptr;
     }
-    void *p[5];
-    if (!addresses(args, 5, p)) return nullptr;
+    void *p[6];
+    if (!addresses(args, 6, p)) return nullptr;
     g_dequant_matmul_int4 = (decltype(g_dequant_matmul_int4))p[0];
     g_quantized_matmul_int4 = (decltype(g_quantized_matmul_int4))p[1];
     g_add_rms_norm = (decltype(g_add_rms_norm))p[2];
     g_add_rms_norm_quantize = (decltype(g_add_rms_norm_quantize))p[3];
     g_dequantize_linear = (decltype(g_dequantize_linear))p[4];
+    g_int4_bytes = (decltype(g_int4_bytes))p[5];
     Py_RETURN_NONE;
 }
 

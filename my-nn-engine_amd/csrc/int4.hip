@@ -7,50 +7,43 @@
 
 #include "int4_stream.h"
 #include "int4_tile.h"
+#include "stream_block.h"
 
 namespace mynn {
 
 constexpr int kCus = 256;
 
-// Up to 64 rows.  Two weight tiles a wave from 17 rows on: the activations, read from L2 by every workgroup, are then most of what a wave
-// loads.  Waves: as many as give each compute unit about 16, no more than there are pieces.
-template <typename T, bool I8, int FL> static int int4_rows(const Int4Args &a, hipStream_t s) {
-    auto go = [&](auto mt_, auto r_, auto nt_) {
-        constexpr int MT = decltype(mt_)::value, R = decltype(r_)::value, NT = decltype(nt_)::value;
-        const int blocks = (a.N + 16 * NT - 1) / (16 * NT) * ((a.M + 63) / 64), pieces = (a.K + 127) / 128;
-        const int most = MT == 1 ? 16 : 8, share = MT == 1 ? 2 : 1;
-        int waves = 1;
-        while (waves < most && blocks * waves < kCus * 16 && waves * 2 * share <= pieces) waves *= 2;
-        const size_t lds = (size_t)waves * MT * R * NT * 64 * sizeof(float);
-        MYNN_LAUNCH((int4_rows_kernel<T, I8, FL, MT, R, NT>), dim3((a.N + 16 * NT - 1) / (16 * NT), (a.M + 63) / 64), dim3(64 * waves), lds, s, a);
-        return launch_status("int4_rows_kernel");
-    };
-    using std::integral_constant;
-    if (a.M <= 4) return go(integral_constant<int, 1>{}, integral_constant<int, 1>{}, integral_constant<int, 1>{});
-    if (a.M <= 8) return go(integral_constant<int, 1>{}, integral_constant<int, 2>{}, integral_constant<int, 1>{});
-    if (a.M <= 16) return go(integral_constant<int, 1>{}, integral_constant<int, 4>{}, integral_constant<int, 1>{});
-    if (a.M <= 32) return go(integral_constant<int, 2>{}, integral_constant<int, 4>{}, integral_constant<int, 2>{});
-    if (a.M <= 48) return go(integral_constant<int, 3>{}, integral_constant<int, 4>{}, integral_constant<int, 2>{});
-    return go(integral_constant<int, 4>{}, integral_constant<int, 4>{}, integral_constant<int, 2>{});
+// Few rows, of whole slices of 128 columns, for which eight waves hold the activations of all of K: more rows would be read several times over
+// (4096 x 14336, 16 rows, us: 40 this way, 20 as tiles; 4096 x 4096 12.8 against 14.9, 28672 x 4096 27.6 and 26.8, 24 rows of 11264 x 2048
+// 12.3 and 17).  Up to eight rows are always streamed (8 rows of 4096 x 14336 18).
+static bool int4_streams(const Int4Args &a) {
+    const int rows = a.M <= 8 ? 1 : a.M <= 16 ? 4096 : a.M <= 32 ? 2048 : 0;
+    return (rows == 1 || a.K <= (a.group == 32 ? rows / 2 : rows)) && a.K % 128 == 0 && a.N >= 16 && (size_t)8 * a.K < 1u << 31;
 }
 
-// Up to 8 rows.  Rows of whole slices, at least a tile of them.
-static bool int4_streams(const Int4Args &a) { return a.M <= 8 && a.K % 128 == 0 && a.N >= 8 && (size_t)8 * a.K < 1u << 31; }
-
 template <typename T, bool I8, int FL> static int int4_stream(const Int4Args &a, hipStream_t s) {
-    auto go = [&](auto mp_, auto p_, auto d_) {
-        constexpr int MP = decltype(mp_)::value, P = decltype(p_)::value, D = decltype(d_)::value;
+    auto go = [&](auto mp_, auto p_, auto d_, auto mt_) {
+        constexpr int MP = decltype(mp_)::value, P = decltype(p_)::value, D = decltype(d_)::value, MT = decltype(mt_)::value;
+        constexpr int OUT = MP * MP * MT;
         const int units = (a.K / 128 + 16 / MP * P - 1) / (16 / MP * P), tiles = (a.N + MP - 1) / MP;
         Int4Stream plan;
         plan.slabs = (units + 7) / 8;
         plan.over_k = (units + plan.slabs - 1) / plan.slabs;
         // eight waves a compute unit: each loads its activations once (twelve, 28672 x 4096, one row: 14.1 -> 15.6 us; six: 16.4)
         const int turns = std::max(1, 4 / plan.over_k), slots = kCus * 8 / plan.over_k;
-        const int most = std::max(1, 32768 / (plan.over_k * MP * MP * (int)sizeof(float)) / turns);
+        // (a workgroup's results of all its tiles lie in LDS)
+        const int most = std::max(1, (MP < 16 ? 32 : 128) * 1024 / (plan.over_k * OUT * (int)sizeof(float)) / turns);
         plan.per_wave = std::min(std::min(most, 64), (tiles + slots - 1) / slots);
         plan.tiles = turns * plan.per_wave;
-        const size_t lds = (size_t)plan.tiles * plan.over_k * MP * MP * sizeof(float);
-        MYNN_LAUNCH((int4_stream_kernel<T, I8, FL, MP, P, D>), dim3((tiles + plan.tiles - 1) / plan.tiles), dim3(64 * turns * plan.over_k), lds, s, a, plan);
+        const size_t lds = (size_t)plan.tiles * plan.over_k * OUT * sizeof(float);
+        if (MP == 16) {
+            static bool lds_set = false;
+            if (!lds_set) {
+                MYNN_HIP(hipFuncSetAttribute((const void *)int4_stream_kernel<T, I8, FL, MP, P, D, MT>, hipFuncAttributeMaxDynamicSharedMemorySize, 128 * 1024));
+                lds_set = true;
+            }
+        }
+        MYNN_LAUNCH((int4_stream_kernel<T, I8, FL, MP, P, D, MT>), dim3((tiles + plan.tiles - 1) / plan.tiles), dim3(64 * turns * plan.over_k), lds, s, a, plan);
         return launch_status("int4_stream_kernel");
     };
     using std::integral_constant;
@@ -59,28 +52,24 @@ template <typename T, bool I8, int FL> static int int4_stream(const Int4Args &a,
     auto shares = [&](auto mp) {
         constexpr int MP = decltype(mp)::value;
         if constexpr (FL > 1) {
-            if (a.K > 128 * (16 / MP) * 2 * 8) return go(mp, integral_constant<int, 4>{}, integral_constant<int, 2>{});
+            if (a.K > 128 * (16 / MP) * 2 * 8) return go(mp, integral_constant<int, 4>{}, integral_constant<int, 2>{}, integral_constant<int, 1>{});
         }
-        if (MP == 1 && a.K <= 2048) return go(mp, integral_constant<int, 1>{}, integral_constant<int, 4>{});
-        return go(mp, integral_constant<int, 2>{}, integral_constant<int, 3>{});
+        if (MP == 1 && a.K <= 2048) return go(mp, integral_constant<int, 1>{}, integral_constant<int, 4>{}, integral_constant<int, 1>{});
+        return go(mp, integral_constant<int, 2>{}, integral_constant<int, 3>{}, integral_constant<int, 1>{});
     };
     if (a.M == 1) return shares(integral_constant<int, 1>{});
     if (a.M == 2) return shares(integral_constant<int, 2>{});
     if (a.M <= 4) return shares(integral_constant<int, 4>{});
-    return shares(integral_constant<int, 8>{});
-}
-
-template <typename T, bool I8> static int int4_few(const Int4Args &a, hipStream_t s) {
-    if (int4_streams(a)) return a.group == 32 ? int4_stream<T, I8, 1>(a, s) : a.group == 64 ? int4_stream<T, I8, 2>(a, s) : int4_stream<T, I8, 4>(a, s);
-    if (a.group == 32) return int4_rows<T, I8, 1>(a, s);
-    if (a.group == 64) return int4_rows<T, I8, 2>(a, s);
-    return int4_rows<T, I8, 4>(a, s);
+    if (a.M <= 8) return shares(integral_constant<int, 8>{});
+    constexpr integral_constant<int, 16> full{};
+    if (a.M <= 16) return go(full, integral_constant<int, FL == 1 ? 2 : 4>{}, integral_constant<int, 2>{}, integral_constant<int, 1>{});
+    return go(full, integral_constant<int, FL == 1 ? 1 : 2>{}, integral_constant<int, 2>{}, integral_constant<int, 2>{});
 }
 
 // Heights of the row tiles, in blocks of 32 rows: four as often as they go and the rest in a short tile, or all (but for one block) alike, by
 // how long the last compute unit is busy.  A tile of h blocks takes h + 1.5 units, of int8 h + 2.2 (one round of K = 4096, us: 46, 58,
 // 80, 104 for one to four blocks of fp16, 40, 48, 60, 75 of int8).
-static Int4Rows int4_row_tiles(int M, int columns, double fixed) {
+static Int4Rows int4_row_tiles(int M, int columns, double fixed, int most) {
     const int blocks = (M + 31) / 32;
     auto busy = [&](const Int4Rows &r) {
         const double high = r.high + fixed, low = r.low ? r.low + fixed : 0.0;
@@ -89,35 +78,76 @@ static Int4Rows int4_row_tiles(int M, int columns, double fixed) {
         const long long beside = over && others ? (kCus - over) * (long long)(high / low) : 0;
         return (double)((tall + kCus - 1) / kCus) * high + (others > beside ? (double)((others - beside + kCus - 1) / kCus) * low : 0.0);
     };
-    Int4Rows best{blocks / 4, 4, blocks % 4, (blocks + 3) / 4};
+    Int4Rows best{blocks / most, most, blocks % most, (blocks + most - 1) / most};
     if (!best.tall) best = {1, blocks, 0, 1};
-    for (int tiles = (blocks + 3) / 4; tiles <= blocks; tiles++) {
+    for (int tiles = (blocks + most - 1) / most; tiles <= blocks; tiles++) {
         const int low = blocks / tiles, over = blocks % tiles;
         const Int4Rows even = over ? Int4Rows{over, low + 1, low, tiles} : Int4Rows{tiles, low, 0, tiles};
         if (busy(even) < busy(best)) best = even;
-        if (low == 1) break;
+        if (low == 1 || (long long)tiles * columns > 8 * kCus) break;  // (in many rounds the last one matters little)
     }
     return best;
 }
 
-template <typename T, bool I8, int FL> static int int4_tiles(const Int4Args &a, hipStream_t s) {
-    using G = Int4Tile<I8, FL>;
-    const int columns = (a.N + G::BN - 1) / G::BN;
-    const Int4Rows rows = int4_row_tiles(a.M, columns, I8 ? 2.2 : 1.5);
+// K ranges of a product whose tiles leave compute units idle: as many as fill them, of eight pieces at least -- a workgroup takes some 3 us to start
+// and to leave its sums, a piece 0.9, and the join reads what the ranges wrote (48 rows, us with 1 / 2 / 4 / 8 / 16 ranges: 4096 x 4096 30 / 22 /
+// 16.8 / 16.7 / 22, 4096 x 14336 89 / 51 / 32 / 24.6 / 24.3, 11264 x 2048 18.4 / 17.1 / 19.2 / 27, 28672 x 4096 36 / 34 / 43).
+static int int4_ranges(int M, int N, int K) {
+    const long long tiles = ((long long)M + 63) / 64 * ((N + 255ll) / 256);
+    return std::max(1, (int)std::min((long long)kCus / tiles, (K + 127ll) / 128 / 8));
+}
+static size_t int4_workspace(const Int4Args &a) {
+    const int ranges = int4_streams(a) ? 1 : int4_ranges(a.M, a.N, a.K);
+    return ranges > 1 ? (size_t)ranges * a.M * a.N * sizeof(float) : 0;
+}
+
+static StreamBlocks g_int4_blocks;  // the ranges' sums
+
+// Memory for the ranges' sums: the caller's, the stream's block, or none: a captured call that was given none takes the ranges one after the
+// other (the same bits), so that its graph may be replayed anywhere.
+struct Int4Memory {
+    bool given;
+    void *ptr;
+    size_t bytes;
+};
+
+template <typename T, bool I8, int FL> static int int4_tiles(const Int4Args &a, const Int4Memory &memory, hipStream_t s) {
+    const int columns = (a.N + Int4Tile<I8, FL>::BN - 1) / Int4Tile<I8, FL>::BN;
+    Int4Ranges ranges{int4_ranges(a.M, a.N, a.K), nullptr};
+    const Int4Rows rows = int4_row_tiles(a.M, columns * ranges.count, I8 ? 2.2 : 1.5, ranges.count > 1 ? 2 : 4);
     MYNN_REQUIRE((long long)rows.tiles * columns < 1 << 30, MYNN_ERR_UNSUPPORTED, "4-bit product: M=%d N=%d", a.M, a.N);
-    constexpr int lds = G::NS * G::STAGE;
     static bool lds_set = false;
     if (!lds_set) {
-        MYNN_HIP(hipFuncSetAttribute((const void *)int4_tile_kernel<T, I8, FL>, hipFuncAttributeMaxDynamicSharedMemorySize, lds));
+        MYNN_HIP(hipFuncSetAttribute((const void *)int4_tile_kernel<T, I8, FL>, hipFuncAttributeMaxDynamicSharedMemorySize, kI4Lds));
         lds_set = true;
     }
-    MYNN_LAUNCH((int4_tile_kernel<T, I8, FL>), dim3(rows.tiles * columns), dim3(512), lds, s, a, rows);
+    const size_t total = (size_t)a.M * a.N;
+    StreamBlocks::Lease block;
+    if (ranges.count > 1 && memory.given) ranges.part = (float *)memory.ptr;
+    else if (ranges.count > 1 && !stream_capturing(s)) {
+        if (const int rc = g_int4_blocks.lease(s, false, int4_workspace(a), 0, "4-bit product", &block)) return rc;
+        ranges.part = (float *)block.ptr;
+    }
+    MYNN_LAUNCH((int4_tile_kernel<T, I8, FL>), dim3(rows.tiles * columns * (ranges.part ? ranges.count : 1)), dim3(512), kI4Lds, s, a, rows, ranges);
+    if (ranges.part)
+        MYNN_LAUNCH((int4_join_kernel<T, I8>), dim3((unsigned)((total + 255) / 256)), dim3(256), 0, s, (T *)a.out, (const float *)ranges.part,
+                    (const T *)a.act_scale, ranges.count, (uint32_t)a.N, (uint32_t)total);
     return launch_status("int4_tile_kernel");
 }
-template <typename T, bool I8> static int int4_many(const Int4Args &a, hipStream_t s) {
-    if (a.group == 32) return int4_tiles<T, I8, 1>(a, s);
-    if (a.group == 64) return int4_tiles<T, I8, 2>(a, s);
-    return int4_tiles<T, I8, 4>(a, s);
+
+template <typename T, bool I8, int FL> static int int4_product_of(const Int4Args &a, const Int4Memory &memory, hipStream_t s) {
+    return int4_streams(a) ? int4_stream<T, I8, FL>(a, s) : int4_tiles<T, I8, FL>(a, memory, s);
+}
+template <bool I8> static int int4_product(const Int4Args &a, const Int4Memory &memory, int dtype, hipStream_t s) {
+    if (memory.given) {
+        const size_t need = int4_workspace(a);
+        MYNN_REQUIRE(!need || (memory.ptr && memory.bytes >= need && aligned16(memory.ptr)), MYNN_ERR_INVALID,
+                     "4-bit product: %zu bytes of workspace, 16-byte aligned, are needed", need);
+    }
+    return dispatch_dtype16(dtype, [&](auto *t) {
+        using T = std::remove_pointer_t<decltype(t)>;
+        return a.group == 32 ? int4_product_of<T, I8, 1>(a, memory, s) : a.group == 64 ? int4_product_of<T, I8, 2>(a, memory, s) : int4_product_of<T, I8, 4>(a, memory, s);
+    });
 }
 
 // c / (pieces of a group) as the upper half of a product: exact while (pieces of a row) * (pieces of a group) < 2^32
@@ -136,25 +166,39 @@ static int check_int4(const char *who, const void *out, const void *act, const v
 
 using namespace mynn;
 
+static int dequant_matmul_int4(void *out, const void *act, const uint8_t *wq, const void *scale, const uint8_t *zero, int M, int N, int K, int group, int dtype,
+                               const Int4Memory &memory, mynn_stream s) {
+    if (int rc = check_int4("dequant_matmul_int4", out, act, wq, scale, M, N, K, group)) return rc;
+    return int4_product<false>(Int4Args{out, act, nullptr, wq, scale, zero, M, N, K, group, pieces_magic(group)}, memory, dtype, as_stream(s));
+}
+static int quantized_matmul_int4(void *out, const int8_t *lhs, const void *lhs_scale, const uint8_t *wq, const void *scale, const uint8_t *zero, int M, int N,
+                                 int K, int group, int dtype, const Int4Memory &memory, mynn_stream s) {
+    if (int rc = check_int4("quantized_matmul_int4", out, lhs, wq, scale, M, N, K, group)) return rc;
+    MYNN_REQUIRE(lhs_scale, MYNN_ERR_INVALID, "quantized_matmul_int4: lhs_scale is null");
+    return int4_product<true>(Int4Args{out, lhs, lhs_scale, wq, scale, zero, M, N, K, group, pieces_magic(group)}, memory, dtype, as_stream(s));
+}
+
+extern "C" size_t mynn_matmul_int4_workspace_bytes(int M, int N, int K, int group) {
+    if (M < 1 || N < 1 || K < 1 || group < 1) return 0;
+    Int4Args a{};
+    a.M = M, a.N = N, a.K = K, a.group = group;
+    return int4_workspace(a);
+}
+
 extern "C" int mynn_dequant_matmul_int4(void *out, const void *act, const uint8_t *wq, const void *scale, const uint8_t *zero, int M, int N, int K,
                                         int group, int dtype, mynn_stream s) {
-    if (int rc = check_int4("dequant_matmul_int4", out, act, wq, scale, M, N, K, group)) return rc;
-    const Int4Args args{out, act, nullptr, wq, scale, zero, M, N, K, group, pieces_magic(group)};
-    return dispatch_dtype16(dtype, [&](auto *t) {
-        using T = std::remove_pointer_t<decltype(t)>;
-        static const int most_few = getenv("I4FEW") ? atoi(getenv("I4FEW")) : 64;
-        return M <= most_few ? int4_few<T, false>(args, as_stream(s)) : int4_many<T, false>(args, as_stream(s));
-    });
+    return dequant_matmul_int4(out, act, wq, scale, zero, M, N, K, group, dtype, Int4Memory{}, s);
+}
+extern "C" int mynn_dequant_matmul_int4_ws(void *out, const void *act, const uint8_t *wq, const void *scale, const uint8_t *zero, int M, int N, int K,
+                                           int group, int dtype, void *workspace, size_t workspace_bytes, mynn_stream s) {
+    return dequant_matmul_int4(out, act, wq, scale, zero, M, N, K, group, dtype, Int4Memory{true, workspace, workspace_bytes}, s);
 }
 
 extern "C" int mynn_quantized_matmul_int4(void *out, const int8_t *lhs, const void *lhs_scale, const uint8_t *wq, const void *scale, const uint8_t *zero,
                                           int M, int N, int K, int group, int dtype, mynn_stream s) {
-    if (int rc = check_int4("quantized_matmul_int4", out, lhs, wq, scale, M, N, K, group)) return rc;
-    MYNN_REQUIRE(lhs_scale, MYNN_ERR_INVALID, "quantized_matmul_int4: lhs_scale is null");
-    const Int4Args args{out, lhs, lhs_scale, wq, scale, zero, M, N, K, group, pieces_magic(group)};
-    return dispatch_dtype16(dtype, [&](auto *t) {
-        using T = std::remove_pointer_t<decltype(t)>;
-        static const int most_few = getenv("I4FEW") ? atoi(getenv("I4FEW")) : 64;
-        return M <= most_few ? int4_few<T, true>(args, as_stream(s)) : int4_many<T, true>(args, as_stream(s));
-    });
+    return quantized_matmul_int4(out, lhs, lhs_scale, wq, scale, zero, M, N, K, group, dtype, Int4Memory{}, s);
+}
+extern "C" int mynn_quantized_matmul_int4_ws(void *out, const int8_t *lhs, const void *lhs_scale, const uint8_t *wq, const void *scale, const uint8_t *zero,
+                                             int M, int N, int K, int group, int dtype, void *workspace, size_t workspace_bytes, mynn_stream s) {
+    return quantized_matmul_int4(out, lhs, lhs_scale, wq, scale, zero, M, N, K, group, dtype, Int4Memory{true, workspace, workspace_bytes}, s);
 }

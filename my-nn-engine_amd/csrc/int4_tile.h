@@ -11,7 +11,7 @@
 // What bounds it: MFMAs against the vector operations of two waves a SIMD -- for 32 MFMAs (int8: 16) of a wave and piece, 16 dwords of codes
 // (12 operations each in fp16, 19 in bf16, 9 to int8) and 64 sums to scale (int8: a conversion more).
 #pragma once
-#include "int4_rows.h"
+#include "int4_codes.h"
 
 namespace mynn {
 
@@ -56,27 +56,27 @@ struct Int4ZeroI8 {
     }
 };
 
-// LDS of a stage: activations, codes, then a dword for each column's scale and one for its zero point, for each group of a piece
+// LDS of a stage: codes, then a dword for each column's scale and one for its zero point, for each group of a piece, then activations of
+// 32 TI rows; as many stages as there is room for, up to six: short tiles wait for memory, not for the matrix cores.
+constexpr int kI4Lds = 160 * 1024;
 template <bool I8, int FL> struct Int4Tile {
-    static constexpr int TI = 4, BM = 32 * TI, BN = 256, PARTS = 4 / FL;
+    static constexpr int BN = 256, PARTS = 4 / FL;
     static constexpr int ROW = I8 ? 128 : 256;  // bytes of a piece of an activation row
-    static constexpr int A = BM * ROW, W = BN * 64, S = BN * 4 * PARTS;
-    static constexpr int STAGE = A + W + 2 * S;
-    static constexpr int NS = 3 * STAGE <= 160 * 1024 ? 3 : 2;
+    static constexpr int W = BN * 64, S = BN * 4 * PARTS, HEAD = W + 2 * S;
     static constexpr int LW = W / 8192, LS = PARTS;  // load instructions of a wave and stage, codes and scales
-    static_assert(NS * STAGE <= 160 * 1024, "");
+    static constexpr int loads(int ti) { return (32 * ti * ROW + 8191) / 8192; }
+    static constexpr int stage(int ti) { return HEAD + 8192 * loads(ti); }
+    static constexpr int stages(int ti) { return kI4Lds / stage(ti) < 6 ? kI4Lds / stage(ti) : 6; }
 };
 
-// 4 or 1 or 2 bytes a lane to LDS dword lds + 4 * lane
+// 2 bytes or one a lane to LDS dword lds + 4 * lane, from base + off (base wave-uniform)
 #pragma clang diagnostic push
 #pragma clang diagnostic ignored "-Winline-asm"
-__device__ inline void load_u16_to_lds(const void *p, uint32_t lds) {
+template <int BYTES> __device__ inline void load_small_to_lds(const char *base, uint32_t off, uint32_t lds) {
     lds = __builtin_amdgcn_readfirstlane(lds);
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_ushort %1, off" ::"s"(lds), "v"(p) : "memory", "m0");
-}
-__device__ inline void load_u8_to_lds(const void *p, uint32_t lds) {
-    lds = __builtin_amdgcn_readfirstlane(lds);
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_ubyte %1, off" ::"s"(lds), "v"(p) : "memory", "m0");
+    base = scalar_pointer(base);
+    if constexpr (BYTES == 2) asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_ushort %1, %2" ::"s"(lds), "v"(off), "s"(base) : "memory", "m0");
+    else asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_ubyte %1, %2" ::"s"(lds), "v"(off), "s"(base) : "memory", "m0");
 }
 #pragma clang diagnostic pop
 
@@ -84,11 +84,26 @@ __device__ inline void load_u8_to_lds(const void *p, uint32_t lds) {
 struct Int4Rows {
     int tall, high, low, tiles;
 };
+// K in ranges whose sums are added up in their order: by workgroups of their own that leave them in `part` ([range][M][N], for
+// int4_join_kernel), or without it one after the other in one workgroup -- the same bits.
+struct Int4Ranges {
+    int count;
+    float *part;
+};
+
+// the waiting part of a step: all but the `ahead` youngest stages of LOADS instructions have arrived
+template <int LOADS, int MOST> __device__ inline void wait_stages(int ahead) {
+    static_assert(LOADS * MOST < 64, "the counter has six bits");
+    if constexpr (MOST > 0) {
+        if (ahead >= MOST) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(LOADS * MOST) : "memory");
+        else wait_stages<LOADS, MOST - 1>(ahead);
+    } else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+}
 
 template <typename T, bool I8, int FL>
-__global__ __launch_bounds__(512, 2) void int4_tile_kernel(Int4Args p, Int4Rows rows) {
+__global__ __launch_bounds__(512, 2) void int4_tile_kernel(Int4Args p, Int4Rows rows, Int4Ranges ranges) {
     using G = Int4Tile<I8, FL>;
-    constexpr int EB = I8 ? 1 : 2, ROW = G::ROW, PARTS = G::PARTS, NS = G::NS;
+    constexpr int EB = I8 ? 1 : 2, ROW = G::ROW, PARTS = G::PARTS;
     constexpr int SP = (I8 ? 1 : 2) * FL;  // instructions to a scale
     constexpr int CPR = ROW / 16;          // 16-byte chunks of a row
     extern __shared__ __align__(16) char lds[];
@@ -98,7 +113,7 @@ __global__ __launch_bounds__(512, 2) void int4_tile_kernel(Int4Args p, Int4Rows 
     int tm, tn;
     {
         const int x = blockIdx.x & 7, i = blockIdx.x >> 3;
-        const int columns = (p.N + G::BN - 1) / G::BN, tall = rows.tall * columns, others = rows.tiles - rows.tall, low = others * columns;
+        const int columns = (p.N + G::BN - 1) / G::BN * (ranges.part ? ranges.count : 1), tall = rows.tall * columns, others = rows.tiles - rows.tall, low = others * columns;
         const int mine = (tall >> 3) + (x < (tall & 7)), y = (x - tall) & 7;  // (the XCDs that got one tall tile less come first for the short ones)
         if (i < mine) {
             const int l = x * (tall >> 3) + min(x, tall & 7) + i;
@@ -110,6 +125,13 @@ __global__ __launch_bounds__(512, 2) void int4_tile_kernel(Int4Args p, Int4Rows 
             tm = rows.tall + l - tn * others;
         }
     }
+    // (ranges of their own: the column tile's, side by side)
+    int z0 = 0, z1 = ranges.count;
+    if (ranges.part) {
+        z0 = tn % ranges.count;
+        z1 = z0 + 1;
+        tn /= ranges.count;
+    }
     const bool is_tall = tm < rows.tall;
     const int height = __builtin_amdgcn_readfirstlane(is_tall ? rows.high : rows.low);
     const int m0 = 32 * __builtin_amdgcn_readfirstlane(is_tall ? tm * rows.high : rows.tall * rows.high + (tm - rows.tall) * rows.low), n0 = __builtin_amdgcn_readfirstlane(tn * G::BN);
@@ -117,163 +139,161 @@ __global__ __launch_bounds__(512, 2) void int4_tile_kernel(Int4Args p, Int4Rows 
     const int c32 = lane & 31, kh = lane >> 5;
 
     // Staging: an instruction fills a kilobyte of whole rows.  The chunk at position q of row r is q ^ key(r), so that the reads of
-    // neighbouring rows fall into different banks.  Offsets are from 4096 bytes in front of the tile's first row, less what load_group_to_lds adds.
+    // neighbouring rows fall into different banks.
     auto akey = [](int r) { return I8 ? (r >> 1) & 7 : r & 15; };
     auto wkey = [](int r) { return (r >> 2) & 3; };
-    uint32_t woff[G::LW];
-#pragma unroll
-    for (int i = 0; i < G::LW; i++) {
-        const int at = (wave * G::LW + i) * 64 + lane, r = at / 4;
-        woff[i] = (uint32_t)min(r, p.N - 1 - n0) * (uint32_t)(p.K >> 1) + 16u * (uint32_t)((at % 4) ^ wkey(r)) + 4096u - 1024u * (i % 4);
-    }
-    const char *abase = (const char *)p.act + (size_t)m0 * p.K * EB - 4096;
-    const char *wbase = (const char *)p.wq + (size_t)n0 * (p.K >> 1) - 4096;
+    const char *abase = (const char *)p.act + (size_t)m0 * p.K * EB, *wbase = (const char *)p.wq + (size_t)n0 * (p.K >> 1);
     const uint32_t at0 = lds_offset(lds);
-    auto stage_codes = [&](int c, int slot) {
-        uint32_t off[G::LW];
-#pragma unroll
-        for (int i = 0; i < G::LW; i++) off[i] = woff[i];
-        if (FL < 4 && 128 * c + 128 > p.K) {
-            const int last = (p.K - 128 * c) / 32 - 1;
-#pragma unroll
-            for (int i = 0; i < G::LW; i++) {
-                const int at = (wave * G::LW + i) * 64 + lane;
-                off[i] -= 16u * (uint32_t)max(((at % 4) ^ wkey(at / 4)) - last, 0);
-            }
-        }
-        load_group_to_lds<G::LW>(wbase + (size_t)c * 64, off, at0 + slot * G::STAGE + G::A + wave * G::LW * 1024);
-    };
-    // scales by the first half of the loads of this kind, zero points by the second (scales again where there are none: all waves have the
-    // same number in flight)
-    auto stage_scales = [&](int c, int slot) {
-        const uint32_t to = at0 + slot * G::STAGE;
-#pragma unroll
-        for (int i = 0; i < G::LS; i++) {
-            const int v = wave * G::LS + i, half = PARTS * 4;  // (of the wave alike)
-            const bool zeros = v >= half;
-            const int u = zeros ? v - half : v, part = u / 4, block = u % 4;
-            const size_t n = min(n0 + 64 * block + lane, p.N - 1);
-            const int g = FL == 4 ? (p.pieces_magic ? (int)__umulhi((uint32_t)c, p.pieces_magic) : c) : min(c * PARTS + part, groups - 1);
-            const uint32_t slot_at = to + G::A + G::W + v * 256;
-            if (zeros && p.zero) load_u8_to_lds(p.zero + n * groups + g, slot_at);
-            else load_u16_to_lds((const uint16_t *)p.scale + n * groups + g, slot_at);
-        }
-    };
     auto run = [&](auto ti_) {
         constexpr int TI = decltype(ti_)::value;
-        constexpr int LA = (32 * TI * ROW + 8191) / 8192, INFLIGHT = LA + G::LW + G::LS;
-        uint32_t aoff[LA];
+        constexpr int LA = G::loads(TI), STAGE = G::stage(TI), NS = G::stages(TI), INFLIGHT = LA + G::LW + G::LS;
+        // This wave's loads of a stage, one instruction each: LA of activations, LW of codes, LS of scales (the first half of the waves) or zero
+        // points (the second; one scale for all its lanes where there are none: all waves have the same number in flight).
+        uint32_t aoff[LA], woff[G::LW], soff[G::LS];
 #pragma unroll
         for (int i = 0; i < LA; i++) {
             const int at = (wave * LA + i) * 64 + lane, r = at / CPR;
-            aoff[i] = (uint32_t)min(r, p.M - 1 - m0) * (uint32_t)(p.K * EB) + 16u * (uint32_t)((at % CPR) ^ akey(r)) + 4096u - 1024u * (i % 4);
+            aoff[i] = (uint32_t)min(r, p.M - 1 - m0) * (uint32_t)(p.K * EB) + 16u * (uint32_t)((at % CPR) ^ akey(r));
         }
-        auto stage_act = [&](int c, int slot) {
-            uint32_t off[LA];
 #pragma unroll
-            for (int i = 0; i < LA; i++) off[i] = aoff[i];
-            if (FL < 4 && 128 * c + 128 > p.K) {  // (chunks behind the row are not multiplied: its last one in their place)
-                const int last = (p.K - 128 * c) * EB / 16 - 1;
+        for (int i = 0; i < G::LW; i++) {
+            const int at = (wave * G::LW + i) * 64 + lane, r = at / 4;
+            woff[i] = (uint32_t)min(r, p.N - 1 - n0) * (uint32_t)(p.K >> 1) + 16u * (uint32_t)((at % 4) ^ wkey(r));
+        }
 #pragma unroll
-                for (int i = 0; i < LA; i++) {
+        for (int i = 0; i < G::LS; i++) {
+            const int v = wave * G::LS + i, row = min(64 * (v & 3) + lane, p.N - 1 - n0);
+            soff[i] = (uint32_t)row * (uint32_t)groups * (v < 4 * PARTS ? 2u : p.zero ? 1u : 0u);
+        }
+        auto load = [&](int i, int c, int slot) {
+            const uint32_t to = at0 + slot * STAGE;
+            // (of a broken piece: chunks behind the row are not multiplied, its last one in their place)
+            const bool broken = FL < 4 && 128 * c + 128 > p.K;
+            if (i < LA) {
+                uint32_t off = aoff[i];
+                if (broken) {
                     const int at = (wave * LA + i) * 64 + lane;
-                    off[i] -= 16u * (uint32_t)max(((at % CPR) ^ akey(at / CPR)) - last, 0);
+                    off -= 16u * (uint32_t)max(((at % CPR) ^ akey(at / CPR)) - ((p.K - 128 * c) * EB / 16 - 1), 0);
                 }
+                load_to_lds(abase + (size_t)c * ROW, off, to + G::HEAD + (wave * LA + i) * 1024);
+            } else if (i < LA + G::LW) {
+                i -= LA;
+                uint32_t off = woff[i];
+                if (broken) {
+                    const int at = (wave * G::LW + i) * 64 + lane;
+                    off -= 16u * (uint32_t)max(((at % 4) ^ wkey(at / 4)) - ((p.K - 128 * c) / 32 - 1), 0);
+                }
+                load_to_lds(wbase + (size_t)c * 64, off, to + (wave * G::LW + i) * 1024);
+            } else {
+                i -= LA + G::LW;
+                const int v = wave * G::LS + i, part = (v >> 2) % PARTS;  // (of the wave alike)
+                const int g = FL == 4 ? (p.pieces_magic ? (int)__umulhi((uint32_t)c, p.pieces_magic) : c) : min(c * PARTS + part, groups - 1);
+                const size_t first = (size_t)n0 * groups + g;
+                if (v >= 4 * PARTS && p.zero) load_small_to_lds<1>((const char *)p.zero + first, soff[i], to + G::W + v * 256);
+                else load_small_to_lds<2>((const char *)p.scale + first * 2, soff[i], to + G::W + v * 256);
             }
-            const char *a = abase + (size_t)c * ROW;
-            const uint32_t to = at0 + slot * G::STAGE + wave * LA * 1024;
-#pragma unroll
-            for (int i = 0; i + 4 <= LA; i += 4) load_group_to_lds<4>(a, off + i, to + i * 1024);
-            if constexpr (LA % 4) load_group_to_lds<LA % 4>(a, off + LA / 4 * 4, to + LA / 4 * 4096);
         };
         auto stage = [&](int c, int slot) {
-            stage_act(c, slot);
-            stage_codes(c, slot);
-            stage_scales(c, slot);
+#pragma unroll
+            for (int i = 0; i < INFLIGHT; i++) load(i, c, slot);
         };
-        f16x_t tot[TI];
+        constexpr bool SEQ = TI <= 2;  // (K is in ranges for short tiles only)
+        f16x_t tot[TI], sum[SEQ ? TI : 1];
+        for (int z = z0; z < z1; z++) {
+            const int c0 = (int)((unsigned)(pieces * z) / (unsigned)ranges.count), c1 = (int)((unsigned)(pieces * (z + 1)) / (unsigned)ranges.count);
+            if (z > z0) __syncthreads();
 #pragma unroll
-        for (int i = 0; i < TI; i++)
+            for (int i = 0; i < TI; i++)
 #pragma unroll
-            for (int e = 0; e < 16; e++) tot[i][e] = 0.f;
+                for (int e = 0; e < 16; e++) tot[i][e] = 0.f;
+#pragma unroll
+            for (int i = 0; i < NS - 1; i++)
+                if (c0 + i < c1) stage(c0 + i, i);
+            int slot = 0;
+            for (int c = c0; c < c1; c++) {
+                // this piece has arrived (later ones may be on their way), and nobody reads the stage that is filled next any more
+                wait_stages<INFLIGHT, NS - 2>(c1 - 1 - c);
+                __syncthreads();
+                const int to = slot == 0 ? NS - 1 : slot - 1;
+                const char *at = lds + slot * STAGE;
+                slot = slot == NS - 1 ? 0 : slot + 1;
 
-        stage(0, 0);
-        if (NS == 3 && pieces > 1) stage(1, 1);
-        int slot = 0;
-        for (int c = 0; c < pieces; c++) {
-            // this piece has arrived (the next one may be on its way), and nobody reads the stage that is filled next any more
-            if (NS == 3 && c + 1 < pieces) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(INFLIGHT) : "memory");
-            else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-            __syncthreads();
-            const int to = slot == 0 ? NS - 1 : slot - 1;
-            const char *at = lds + slot * G::STAGE;
-            slot = slot == NS - 1 ? 0 : slot + 1;
-
-            uint32_t w[8];
-            {
-                const int r = 32 * wave + c32;
-                const char *row = at + G::A + r * 64;
-                if constexpr (FL == 1) {
+                uint32_t w[8];
+                {
+                    const int r = 32 * wave + c32;
+                    const char *row = at + r * 64;
+                    if constexpr (FL == 1) {
 #pragma unroll
-                    for (int h = 0; h < 4; h++) {
-                        const uint2 v = *(const uint2 *)(row + (h ^ wkey(r)) * 16 + 8 * kh);
-                        w[2 * h] = v.x;
-                        w[2 * h + 1] = v.y;
-                    }
-                } else {
+                        for (int h = 0; h < 4; h++) {
+                            const uint2 v = *(const uint2 *)(row + (h ^ wkey(r)) * 16 + 8 * kh);
+                            w[2 * h] = v.x;
+                            w[2 * h + 1] = v.y;
+                        }
+                    } else {
 #pragma unroll
-                    for (int h = 0; h < 2; h++) {
-                        const U4 v = *(const U4 *)(row + ((2 * h + kh) ^ wkey(r)) * 16);
+                        for (int h = 0; h < 2; h++) {
+                            const U4 v = *(const U4 *)(row + ((2 * h + kh) ^ wkey(r)) * 16);
 #pragma unroll
-                        for (int j = 0; j < 4; j++) w[4 * h + j] = v[j];
+                            for (int j = 0; j < 4; j++) w[4 * h + j] = v[j];
+                        }
                     }
                 }
-            }
-            // (fragments are read an instruction ahead, and the loads of a later piece asked for between the first products)
-            U4 a[2][TI];
-            auto fragments = [&](int st) {
-                int chunk;
-                if constexpr (I8) chunk = FL == 1 ? 2 * st + kh : 4 * (st >> 1) + 2 * kh + (st & 1);
-                else chunk = FL == 1 ? 4 * (st >> 1) + 2 * kh + (st & 1) : 8 * (st >> 2) + 4 * kh + (st & 3);
-#pragma unroll
-                for (int i = 0; i < TI; i++) {
-                    const int r = 32 * i + c32;
-                    a[st & 1][i] = *(const U4 *)(at + r * ROW + (chunk ^ akey(r)) * 16);
-                }
-            };
-            fragments(0);
-            const bool more = c + NS - 1 < pieces;
-#pragma unroll
-            for (int part = 0; part < PARTS; part++) {
-                if (FL < 4 && 128 * c + 32 * FL * part >= p.K) break;
-                const char *sz = at + G::A + G::W + (part * 256 + 32 * wave + c32) * 4;
-                const uint16_t half = *(const uint16_t *)sz;
-                const float s = Elem<T>::ld((const T *)&half, 0);
-                const std::conditional_t<I8, Int4ZeroI8, Int4Zero<T>> conv(p.zero ? *(const uint32_t *)(sz + G::S) & 15u : 8u);
-                std::conditional_t<I8, i16v_t, f16x_t> acc[TI] = {};
-#pragma unroll
-                for (int k = 0; k < SP; k++) {
-                    const int st = part * SP + k;  // instruction of the piece
-                    if (st + 1 < PARTS * SP) fragments(st + 1);
-                    if (more && part == 0) {
-                        if (k == 0) stage_act(c + NS - 1, to);
-                        if (k == (SP > 1 ? 1 : 0)) stage_codes(c + NS - 1, to);
-                        if (k == (SP > 2 ? 2 : SP - 1)) stage_scales(c + NS - 1, to);
-                    }
-                    U4 b;
-                    if constexpr (I8) b = conv(w[2 * st], w[2 * st + 1]);
-                    else b = conv(w[st]);
+                // Fragments are read an instruction ahead, in short tiles, whose products do not cover the way to LDS, all of a piece at once; the
+                // loads of a later piece are asked for between the products, one here and there: the eight waves' together keep the memory pipe busy for
+                // most of a piece, and a wave that waits to hand it the next one does nothing else.
+                constexpr int STEPS = PARTS * SP, KEPT = TI <= 2 ? STEPS : 2;
+                U4 a[KEPT][TI];
+                auto fragments = [&](int st) {
+                    int chunk;
+                    if constexpr (I8) chunk = FL == 1 ? 2 * st + kh : 4 * (st >> 1) + 2 * kh + (st & 1);
+                    else chunk = FL == 1 ? 4 * (st >> 1) + 2 * kh + (st & 1) : 8 * (st >> 2) + 4 * kh + (st & 3);
 #pragma unroll
                     for (int i = 0; i < TI; i++) {
-                        if constexpr (I8) acc[i] = __builtin_amdgcn_mfma_i32_32x32x32_i8(__builtin_bit_cast(i4_t, a[st & 1][i]), __builtin_bit_cast(i4_t, b), acc[i], 0, 0, 0);
-                        else acc[i] = Mfma<T>::run(a[st & 1][i], b, acc[i]);
+                        const int r = 32 * i + c32;
+                        a[st % KEPT][i] = *(const U4 *)(at + G::HEAD + r * ROW + (chunk ^ akey(r)) * 16);
                     }
-                    __builtin_amdgcn_sched_barrier(0);
+                };
+#pragma unroll
+                for (int st = 0; st < KEPT - 1; st++) fragments(st);
+                const bool more = c + NS - 1 < c1;
+#pragma unroll
+                for (int part = 0; part < PARTS; part++) {
+                    if (FL < 4 && 128 * c + 32 * FL * part >= p.K) break;
+                    const char *sz = at + G::W + (part * 256 + 32 * wave + c32) * 4;
+                    const uint16_t half = *(const uint16_t *)sz;
+                    const float s = Elem<T>::ld((const T *)&half, 0);
+                    const std::conditional_t<I8, Int4ZeroI8, Int4Zero<T>> conv(p.zero ? *(const uint32_t *)(sz + G::S) & 15u : 8u);
+                    std::conditional_t<I8, i16v_t, f16x_t> acc[TI] = {};
+#pragma unroll
+                    for (int k = 0; k < SP; k++) {
+                        const int st = part * SP + k;  // instruction of the piece
+                        if (st + KEPT - 1 < STEPS) fragments(st + KEPT - 1);
+                        if (more) {
+#pragma unroll
+                            for (int i = 0; i < INFLIGHT; i++)
+                                if (i * STEPS / INFLIGHT == st) load(i, c + NS - 1, to);
+                        }
+                        U4 b;
+                        if constexpr (I8) b = conv(w[2 * st], w[2 * st + 1]);
+                        else b = conv(w[st]);
+#pragma unroll
+                        for (int i = 0; i < TI; i++) {
+                            if constexpr (I8) acc[i] = __builtin_amdgcn_mfma_i32_32x32x32_i8(__builtin_bit_cast(i4_t, a[st % KEPT][i]), __builtin_bit_cast(i4_t, b), acc[i], 0, 0, 0);
+                            else acc[i] = Mfma<T>::run(a[st % KEPT][i], b, acc[i]);
+                        }
+                        if constexpr (KEPT < STEPS) __builtin_amdgcn_sched_barrier(0);
+                    }
+#pragma unroll
+                    for (int i = 0; i < TI; i++)
+#pragma unroll
+                        for (int e = 0; e < 16; e++) tot[i][e] = fmaf(s, (float)acc[i][e], tot[i][e]);
                 }
+            }
+            if constexpr (SEQ) {
 #pragma unroll
                 for (int i = 0; i < TI; i++)
 #pragma unroll
-                    for (int e = 0; e < 16; e++) tot[i][e] = fmaf(s, (float)acc[i][e], tot[i][e]);
+                    for (int e = 0; e < 16; e++) sum[i][e] = z == z0 ? tot[i][e] : sum[i][e] + tot[i][e];
             }
         }
 
@@ -283,8 +303,10 @@ __global__ __launch_bounds__(512, 2) void int4_tile_kernel(Int4Args p, Int4Rows 
 #pragma unroll
             for (int e = 0; e < 16; e++) {
                 const int row = m0 + 32 * i + 8 * (e >> 2) + 4 * kh + (e & 3);
-                if (row < p.M && n < p.N)
-                    Elem<T>::st((T *)p.out, (size_t)row * p.N + n, I8 ? tot[i][e] * Elem<T>::ld((const T *)p.act_scale, row) : tot[i][e]);
+                if (row >= p.M || n >= p.N) continue;
+                const float v = SEQ ? sum[SEQ ? i : 0][e] : tot[i][e];
+                if (SEQ && ranges.part) ranges.part[((size_t)z0 * p.M + row) * p.N + n] = v;
+                else Elem<T>::st((T *)p.out, (size_t)row * p.N + n, I8 ? v * Elem<T>::ld((const T *)p.act_scale, row) : v);
             }
     };
     // (a loop for each height: the sums and fragments are registers)
@@ -292,6 +314,17 @@ __global__ __launch_bounds__(512, 2) void int4_tile_kernel(Int4Args p, Int4Rows 
     else if (height == 3) run(std::integral_constant<int, 3>{});
     else if (height == 2) run(std::integral_constant<int, 2>{});
     else run(std::integral_constant<int, 1>{});
+}
+
+// the ranges' sums added up in their order
+template <typename T, bool I8>
+__global__ __launch_bounds__(256) void int4_join_kernel(T *out, const float *part, const T *act_scale, int ranges, uint32_t N, uint32_t total) {
+    const uint32_t i = blockIdx.x * 256u + threadIdx.x;
+    if (i >= total) return;
+    float sum = part[i];
+    for (int z = 1; z < ranges; z++) sum += part[(size_t)z * total + i];
+    if constexpr (I8) sum *= Elem<T>::ld(act_scale, i / N);
+    Elem<T>::st(out, i, sum);
 }
 
 }  // namespace mynn

@@ -197,6 +197,30 @@ def test_captured_calls(rows, dim):
         assert torch.equal(o, out) and torch.equal(t, total) and torch.equal(c, codes) and torch.equal(s, scale)
 
 
+def test_the_way_without_the_module(monkeypatch):
+    x, r, w = operands(6, 640, F16)
+    expected = [mynn.add_rms_norm(x, r, w, EPS), mynn.add_rms_norm_quantize(x, r, w, EPS), mynn.add_rms_norm(x, None, w, EPS), mynn.add_rms_norm_quantize(x, None, w, EPS)]
+    codes, scale = expected[1][:2]
+    values = mynn.dequantize_linear(codes, scale)
+    monkeypatch.setattr(mynn, "_ops", mynn._NoHostOps())
+    again = [mynn.add_rms_norm(x, r, w, EPS), mynn.add_rms_norm_quantize(x, r, w, EPS), mynn.add_rms_norm(x, None, w, EPS), mynn.add_rms_norm_quantize(x, None, w, EPS)]
+    for a, b in zip(expected, again):
+        assert len(a) == len(b) and all(torch.equal(u, v) for u, v in zip(a, b))
+    assert expected[2][1] is not None and again[2][1] is x and torch.equal(mynn.dequantize_linear(codes, scale), values)
+
+
+# dequantize_linear of whole pieces of eight and of others, at any address: code times scale, rounded once
+@pytest.mark.parametrize("dtype", [F16, BF16, F32])
+@pytest.mark.parametrize("rows,cols,shift", [(1, 8, 0), (7, 4096, 0), (300, 200, 0), (5, 33, 0), (9, 64, 1), (3, 4096, 4)])
+def test_dequantize_linear(dtype, rows, cols, shift):
+    g = torch.Generator(device="cuda")
+    g.manual_seed(5)
+    buf = torch.randint(-128, 128, (rows * cols + 8,), generator=g, dtype=torch.int8, device="cuda")
+    x = buf[shift : shift + rows * cols].view(rows, cols)
+    scale = torch.rand((rows,), generator=g, device="cuda").to(dtype)
+    assert torch.equal(mynn.dequantize_linear(x, scale), (x.float() * scale.float()[:, None]).to(dtype))
+
+
 def test_wrapper_refuses_what_does_not_fit():
     x, r, w = operands(4, 64, F16)
     for f in (mynn.add_rms_norm, mynn.add_rms_norm_quantize):

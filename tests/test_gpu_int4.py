@@ -251,6 +251,96 @@ def test_same_bits_everywhere(kind, M, N, K, group):
         assert torch.equal(out, expected) and torch.equal(out_other, expected_other) and torch.equal(beside, expected_other) and torch.equal(eager, expected)
 
 
+def raw(kind, ops, out, workspace=None):
+    """the library's own call: without a workspace, or with one of so many bytes at so many bytes behind the start of a tensor"""
+    M, K = ops[0].shape
+    N, groups = ops[-2].shape
+    name = "mynn_dequant_matmul_int4" if kind == "linear" else "mynn_quantized_matmul_int4"
+    args = [out.data_ptr()] + [t.data_ptr() if t is not None else None for t in ops] + [M, N, K, K // groups, mynn.F16]
+    stream = torch.cuda.current_stream().cuda_stream
+    if workspace is None:
+        return getattr(mynn.lib(), name)(*args, stream)
+    return getattr(mynn.lib(), name + "_ws")(*args, *workspace, stream)
+
+
+# K in ranges (2, 4, 8 and 16 of them, one and two tiles of rows) and not: every form of a call has the same bits, eager and captured
+@KINDS
+@pytest.mark.parametrize("M,N,K,group,ranges", [(12, 300, 4096, 32, 4), (33, 1000, 4096, 64, 4), (100, 520, 16384, 128, 16), (40, 256, 2080, 32, 2),
+                                                (200, 256, 8192, 128, 8), (16, 512, 4096, 128, 1), (500, 4096, 512, 128, 1)])
+def test_every_form_of_a_call(kind, M, N, K, group, ranges):
+    ops = operands(kind, M, N, K, group, F16, True)
+    need = mynn.lib().mynn_matmul_int4_workspace_bytes(M, N, K, group)
+    assert need == (ranges * M * N * 4 if ranges > 1 else 0)
+    expected = call(kind, ops)
+    ref.assert_close(expected, *want(kind, ops))
+    out = torch.empty_like(expected)
+    assert raw(kind, ops, out.zero_()) == 0 and torch.equal(out, expected)
+    ws = torch.full((need + 4096,), 77, dtype=torch.uint8, device="cuda")
+    assert raw(kind, ops, out.zero_(), (ws.data_ptr() + 2048, need)) == 0 and torch.equal(out, expected)
+    assert bool((ws[:2048] == 77).all()) and bool((ws[2048 + need :] == 77).all())
+    if need:
+        assert raw(kind, ops, out, (ws.data_ptr(), need - 1)) == -1 and b"workspace" in mynn.lib().mynn_last_error()
+        assert raw(kind, ops, out, (None, need)) == -1 and raw(kind, ops, out, (ws.data_ptr() + 8, need)) == -1
+    else:
+        assert raw(kind, ops, out.zero_(), (None, 0)) == 0 and torch.equal(out, expected)
+    # three graphs: the plain call (no memory of the library's), the caller's workspace, the wrapper's; replayed side by side
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graphs, outs = [], [torch.empty_like(out) for _ in range(2)]
+    for f in (lambda: (raw(kind, ops, outs[0]), outs[0])[1], lambda: (raw(kind, ops, outs[1], (ws.data_ptr(), need)), outs[1])[1], lambda: call(kind, ops)):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=side):
+            o = f()
+        graphs.append((g, o))
+    streams = [torch.cuda.Stream() for _ in graphs]
+    for _ in range(3):
+        for _, o in graphs:
+            o.zero_()
+        torch.cuda.synchronize()
+        for s, (g, _) in zip(streams, graphs):
+            with torch.cuda.stream(s):
+                g.replay()
+        eager = call(kind, ops)
+        torch.cuda.synchronize()
+        assert torch.equal(eager, expected) and all(torch.equal(o, expected) for _, o in graphs)
+
+
+def test_threads_on_streams_of_their_own():
+    import threading
+
+    shapes = [(12, 300, 2048, 32), (40, 1024, 4096, 64), (3, 4096, 4096, 128), (200, 256, 8192, 128)]
+    sets = [operands("linear", *s, F16, True, seed=i) for i, s in enumerate(shapes)]
+    expected = [call("linear", o) for o in sets]
+    torch.cuda.synchronize()
+    failures = []
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(20):
+                out = torch.empty_like(expected[i])
+                if raw("linear", sets[i], out) != 0 or not torch.equal(out, expected[i]) or not torch.equal(call("linear", sets[i]), expected[i]):
+                    failures.append(i)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(len(sets))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failures
+
+
+@KINDS
+@pytest.mark.parametrize("M", [1, 40])
+def test_the_way_without_the_module(kind, M, monkeypatch):
+    """through ctypes: the same results and the same refusals as through the module of C++"""
+    ops = operands(kind, M, 300, 4096, 64, F16, True)
+    expected = call(kind, ops)
+    monkeypatch.setattr(mynn, "_ops", mynn._NoHostOps())
+    assert torch.equal(call(kind, ops), expected)
+    with pytest.raises(mynn.MynnError, match="fit together"):
+        call(kind, (ops[0][:, :64].contiguous(),) + ops[1:])
+
+
 @KINDS
 def test_wrapper_refuses_what_does_not_fit(kind):
     ops = operands(kind, 4, 32, 256, 64, F16, True)
