@@ -89,12 +89,22 @@ static Int4Rows int4_row_tiles(int M, int columns, double fixed, int most) {
     return best;
 }
 
-// K ranges of a product whose tiles leave compute units idle: as many as fill them, of eight pieces at least -- a workgroup takes some 3 us to start
-// and to leave its sums, a piece 0.9, and the join reads what the ranges wrote (48 rows, us with 1 / 2 / 4 / 8 / 16 ranges: 4096 x 4096 30 / 22 /
-// 16.8 / 16.7 / 22, 4096 x 14336 89 / 51 / 32 / 24.6 / 24.3, 11264 x 2048 18.4 / 17.1 / 19.2 / 27, 28672 x 4096 36 / 34 / 43).
+// K ranges of a product whose tiles leave compute units idle, by what they take: a piece 0.9 us, the sums that are left and added up 0.8 us a megabyte
+// and a launch of 2.5 us (us with 1 / 2 / 4 / 8 / 16 ranges: 48 x 4096 x 4096 30 / 20 / 15.7 / 13.9 / 20, 48 x 4096 x 14336 89 / 50 / 31 / 24.2 / 24,
+// 64 x 11264 x 2048 18.5 / 18.2 / 20.8, 48 x 28672 x 4096 36 / 34 / 42).
 static int int4_ranges(int M, int N, int K) {
-    const long long tiles = ((long long)M + 63) / 64 * ((N + 255ll) / 256);
-    return std::max(1, (int)std::min((long long)kCus / tiles, (K + 127ll) / 128 / 8));
+    const long long tiles = ((long long)M + 63) / 64 * ((N + 255ll) / 256), pieces = (K + 127ll) / 128;
+    const double sums = 0.8e-6 * M * N * sizeof(float);
+    int best = 1;
+    double least = 0.9 * pieces;
+    for (int r = 2; r <= 32 && r <= kCus / tiles && r <= pieces / 2; r++) {
+        const double us = 0.9 * ((pieces + r - 1) / r) + sums * r + 2.5;
+        if (us < least) {
+            least = us;
+            best = r;
+        }
+    }
+    return best;
 }
 static size_t int4_workspace(const Int4Args &a) {
     const int ranges = int4_streams(a) ? 1 : int4_ranges(a.M, a.N, a.K);
@@ -129,9 +139,16 @@ template <typename T, bool I8, int FL> static int int4_tiles(const Int4Args &a, 
         ranges.part = (float *)block.ptr;
     }
     MYNN_LAUNCH((int4_tile_kernel<T, I8, FL>), dim3(rows.tiles * columns * (ranges.part ? ranges.count : 1)), dim3(512), kI4Lds, s, a, rows, ranges);
-    if (ranges.part)
-        MYNN_LAUNCH((int4_join_kernel<T, I8>), dim3((unsigned)((total + 255) / 256)), dim3(256), 0, s, (T *)a.out, (const float *)ranges.part,
-                    (const T *)a.act_scale, ranges.count, (uint32_t)a.N, (uint32_t)total);
+    if (ranges.part) {
+        // (two values a thread where rows are whole pairs)
+        auto join = [&](auto v) {
+            constexpr int V = decltype(v)::value;
+            MYNN_LAUNCH((int4_join_kernel<T, I8, V>), dim3((unsigned)((total / V + 255) / 256)), dim3(256), 0, s, (T *)a.out, (const float *)ranges.part,
+                        (const T *)a.act_scale, ranges.count, (uint32_t)a.N, (uint32_t)total);
+        };
+        if (a.N % 2 == 0) join(std::integral_constant<int, 2>{});
+        else join(std::integral_constant<int, 1>{});
+    }
     return launch_status("int4_tile_kernel");
 }
 

@@ -316,15 +316,18 @@ __global__ __launch_bounds__(512, 2) void int4_tile_kernel(Int4Args p, Int4Rows 
     else run(std::integral_constant<int, 1>{});
 }
 
-// the ranges' sums added up in their order
-template <typename T, bool I8>
+// the ranges' sums added up in their order, V values a thread
+template <typename T, bool I8, int V>
 __global__ __launch_bounds__(256) void int4_join_kernel(T *out, const float *part, const T *act_scale, int ranges, uint32_t N, uint32_t total) {
-    const uint32_t i = blockIdx.x * 256u + threadIdx.x;
+    typedef float vec __attribute__((ext_vector_type(V)));
+    const uint32_t i = (blockIdx.x * 256u + threadIdx.x) * V;
     if (i >= total) return;
-    float sum = part[i];
-    for (int z = 1; z < ranges; z++) sum += part[(size_t)z * total + i];
+    vec sum = *(const vec *)(part + i);
+#pragma unroll 8
+    for (int z = 1; z < ranges; z++) sum += *(const vec *)(part + (size_t)z * total + i);
     if constexpr (I8) sum *= Elem<T>::ld(act_scale, i / N);
-    Elem<T>::st(out, i, sum);
+#pragma unroll
+    for (int v = 0; v < V; v++) Elem<T>::st(out, i + v, sum[v]);
 }
 
 }  // namespace mynn
