@@ -89,16 +89,16 @@ static Int4Rows int4_row_tiles(int M, int columns, double fixed, int most) {
     return best;
 }
 
-// K ranges of a product whose tiles leave compute units idle, by what they take: a piece 0.9 us, the sums that are left and added up 0.8 us a megabyte
-// and a launch of 2.5 us (us with 1 / 2 / 4 / 8 / 16 ranges: 48 x 4096 x 4096 30 / 20 / 15.7 / 13.9 / 20, 48 x 4096 x 14336 89 / 50 / 31 / 24.2 / 24,
-// 64 x 11264 x 2048 18.5 / 18.2 / 20.8, 48 x 28672 x 4096 36 / 34 / 42).
+// K ranges of a product whose tiles leave compute units idle, by what they take: a piece 0.85 us, the sums that are left and added up 0.8 us a
+// megabyte and a launch of 2.5 us (us with 1 / 2 / 4 / 8 / 16 ranges: 48 x 4096 x 4096 23.8 / 17.7 / 12.3 / 12.7 / 14, 48 x 4096 x 14336 87 / 48 / 29 / 25.6 /
+// 23.3, 256 x 2048 x 2048 18.5 / 17.1 / 16.8 / 22, 64 x 11264 x 2048 14.3 / 16.7 / 19.9 / 24, 64 x 28672 x 4096 35.1 / 35.2 / 43).
 static int int4_ranges(int M, int N, int K) {
     const long long tiles = ((long long)M + 63) / 64 * ((N + 255ll) / 256), pieces = (K + 127ll) / 128;
     const double sums = 0.8e-6 * M * N * sizeof(float);
     int best = 1;
-    double least = 0.9 * pieces;
+    double least = 0.85 * pieces;
     for (int r = 2; r <= 32 && r <= kCus / tiles && r <= pieces / 2; r++) {
-        const double us = 0.9 * ((pieces + r - 1) / r) + sums * r + 2.5;
+        const double us = 0.85 * ((pieces + r - 1) / r) + sums * r + 2.5;
         if (us < least) {
             least = us;
             best = r;
@@ -122,15 +122,7 @@ struct Int4Memory {
 };
 
 template <typename T, bool I8, int FL> static int int4_tiles(const Int4Args &a, const Int4Memory &memory, hipStream_t s) {
-    const int columns = (a.N + Int4Tile<I8, FL>::BN - 1) / Int4Tile<I8, FL>::BN;
     Int4Ranges ranges{int4_ranges(a.M, a.N, a.K), nullptr};
-    const Int4Rows rows = int4_row_tiles(a.M, columns * ranges.count, I8 ? 2.2 : 1.5, ranges.count > 1 ? 2 : 4);
-    MYNN_REQUIRE((long long)rows.tiles * columns < 1 << 30, MYNN_ERR_UNSUPPORTED, "4-bit product: M=%d N=%d", a.M, a.N);
-    static bool lds_set = false;
-    if (!lds_set) {
-        MYNN_HIP(hipFuncSetAttribute((const void *)int4_tile_kernel<T, I8, FL>, hipFuncAttributeMaxDynamicSharedMemorySize, kI4Lds));
-        lds_set = true;
-    }
     const size_t total = (size_t)a.M * a.N;
     StreamBlocks::Lease block;
     if (ranges.count > 1 && memory.given) ranges.part = (float *)memory.ptr;
@@ -138,18 +130,34 @@ template <typename T, bool I8, int FL> static int int4_tiles(const Int4Args &a, 
         if (const int rc = g_int4_blocks.lease(s, false, int4_workspace(a), 0, "4-bit product", &block)) return rc;
         ranges.part = (float *)block.ptr;
     }
-    MYNN_LAUNCH((int4_tile_kernel<T, I8, FL>), dim3(rows.tiles * columns * (ranges.part ? ranges.count : 1)), dim3(512), kI4Lds, s, a, rows, ranges);
-    if (ranges.part) {
-        // (two values a thread where rows are whole pairs)
-        auto join = [&](auto v) {
-            constexpr int V = decltype(v)::value;
-            MYNN_LAUNCH((int4_join_kernel<T, I8, V>), dim3((unsigned)((total / V + 255) / 256)), dim3(256), 0, s, (T *)a.out, (const float *)ranges.part,
-                        (const T *)a.act_scale, ranges.count, (uint32_t)a.N, (uint32_t)total);
-        };
-        if (a.N % 2 == 0) join(std::integral_constant<int, 2>{});
-        else join(std::integral_constant<int, 1>{});
-    }
-    return launch_status("int4_tile_kernel");
+    const int side = ranges.part ? ranges.count : 1;  // ranges side by side
+    auto go = [&](auto nw_, const Int4Rows &rows) {
+        constexpr int NW = decltype(nw_)::value;
+        using G = Int4Tile<I8, FL, NW>;
+        const long long blocks = (long long)rows.tiles * ((a.N + G::BN - 1) / G::BN) * side;
+        MYNN_REQUIRE(blocks < 1 << 30, MYNN_ERR_UNSUPPORTED, "4-bit product: M=%d N=%d", a.M, a.N);
+        static bool lds_set = false;
+        if (!lds_set) {
+            MYNN_HIP(hipFuncSetAttribute((const void *)int4_tile_kernel<T, I8, FL, NW>, hipFuncAttributeMaxDynamicSharedMemorySize, G::LDS));
+            lds_set = true;
+        }
+        MYNN_LAUNCH((int4_tile_kernel<T, I8, FL, NW>), dim3((unsigned)blocks), dim3(64 * NW), G::LDS, s, a, rows, ranges);
+        return launch_status("int4_tile_kernel");
+    };
+    // Tiles of at most 64 rows: two workgroups of four waves a compute unit, one computes while the other meets at its barrier (us, one of eight / two of
+    // four: 128 x 4096 x 4096 19.7 / 16.4, 339 x 2560 x 2048 of int8 23 / 18.5, 64 x 28672 x 4096 35.8 / 34.3; taller tiles are the better ones where
+    // there are rows for them, 777 x 28672 x 4096 266 / 231, and three of their stages do not fit twice)
+    const Int4Rows rows = int4_row_tiles(a.M, (a.N + 255) / 256 * ranges.count, I8 ? 2.2 : 1.5, ranges.count > 1 ? 2 : 4);
+    const int rc = rows.high <= 2 ? go(std::integral_constant<int, 4>{}, rows) : go(std::integral_constant<int, 8>{}, rows);
+    if (rc || !ranges.part) return rc;
+    // (two values a thread where rows are whole pairs)
+    auto join = [&](auto v) {
+        constexpr int V = decltype(v)::value;
+        MYNN_LAUNCH((int4_join_kernel<T, I8, V>), dim3((unsigned)((total / V + 255) / 256)), dim3(256), 0, s, (T *)a.out, (const float *)ranges.part,
+                    (const T *)a.act_scale, ranges.count, (uint32_t)a.N, (uint32_t)total);
+        return launch_status("int4_join_kernel");
+    };
+    return a.N % 2 == 0 ? join(std::integral_constant<int, 2>{}) : join(std::integral_constant<int, 1>{});
 }
 
 template <typename T, bool I8, int FL> static int int4_product_of(const Int4Args &a, const Int4Memory &memory, hipStream_t s) {

@@ -58,15 +58,15 @@ struct Int4ZeroI8 {
 
 // LDS of a stage: codes, then a dword for each column's scale and one for its zero point, for each group of a piece, then activations of
 // 32 TI rows; as many stages as there is room for, up to six: short tiles wait for memory, not for the matrix cores.
-constexpr int kI4Lds = 160 * 1024;
-template <bool I8, int FL> struct Int4Tile {
-    static constexpr int BN = 256, PARTS = 4 / FL;
+template <bool I8, int FL, int NW> struct Int4Tile {
+    static constexpr int LDS = NW * 20 * 1024;  // (a compute unit has 160 KB and takes eight waves)
+    static constexpr int BN = 32 * NW, PARTS = 4 / FL;
     static constexpr int ROW = I8 ? 128 : 256;  // bytes of a piece of an activation row
     static constexpr int W = BN * 64, S = BN * 4 * PARTS, HEAD = W + 2 * S;
-    static constexpr int LW = W / 8192, LS = PARTS;  // load instructions of a wave and stage, codes and scales
-    static constexpr int loads(int ti) { return (32 * ti * ROW + 8191) / 8192; }
-    static constexpr int stage(int ti) { return HEAD + 8192 * loads(ti); }
-    static constexpr int stages(int ti) { return kI4Lds / stage(ti) < 6 ? kI4Lds / stage(ti) : 6; }
+    static constexpr int LW = 2, LS = PARTS;  // load instructions of a wave and stage, codes and scales
+    static constexpr int loads(int ti) { return (32 * ti * ROW + 1024 * NW - 1) / (1024 * NW); }
+    static constexpr int stage(int ti) { return HEAD + 1024 * NW * loads(ti); }
+    static constexpr int stages(int ti) { return LDS / stage(ti) < 6 ? LDS / stage(ti) : 6; }
 };
 
 // 2 bytes or one a lane to LDS dword lds + 4 * lane, from base + off (base wave-uniform)
@@ -100,9 +100,9 @@ template <int LOADS, int MOST> __device__ inline void wait_stages(int ahead) {
     } else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 }
 
-template <typename T, bool I8, int FL>
-__global__ __launch_bounds__(512, 2) void int4_tile_kernel(Int4Args p, Int4Rows rows, Int4Ranges ranges) {
-    using G = Int4Tile<I8, FL>;
+template <typename T, bool I8, int FL, int NW>
+__global__ __launch_bounds__(64 * NW, 2) void int4_tile_kernel(Int4Args p, Int4Rows rows, Int4Ranges ranges) {
+    using G = Int4Tile<I8, FL, NW>;
     constexpr int EB = I8 ? 1 : 2, ROW = G::ROW, PARTS = G::PARTS;
     constexpr int SP = (I8 ? 1 : 2) * FL;  // instructions to a scale
     constexpr int CPR = ROW / 16;          // 16-byte chunks of a row
@@ -162,8 +162,8 @@ __global__ __launch_bounds__(512, 2) void int4_tile_kernel(Int4Args p, Int4Rows 
         }
 #pragma unroll
         for (int i = 0; i < G::LS; i++) {
-            const int v = wave * G::LS + i, row = min(64 * (v & 3) + lane, p.N - 1 - n0);
-            soff[i] = (uint32_t)row * (uint32_t)groups * (v < 4 * PARTS ? 2u : p.zero ? 1u : 0u);
+            const int v = wave * G::LS + i, row = min(64 * (v % (NW / 2)) + lane, p.N - 1 - n0);
+            soff[i] = (uint32_t)row * (uint32_t)groups * (v < NW / 2 * PARTS ? 2u : p.zero ? 1u : 0u);
         }
         auto load = [&](int i, int c, int slot) {
             const uint32_t to = at0 + slot * STAGE;
@@ -186,10 +186,10 @@ __global__ __launch_bounds__(512, 2) void int4_tile_kernel(Int4Args p, Int4Rows 
                 load_to_lds(wbase + (size_t)c * 64, off, to + (wave * G::LW + i) * 1024);
             } else {
                 i -= LA + G::LW;
-                const int v = wave * G::LS + i, part = (v >> 2) % PARTS;  // (of the wave alike)
+                const int v = wave * G::LS + i, part = v / (NW / 2) % PARTS;  // (of the wave alike)
                 const int g = FL == 4 ? (p.pieces_magic ? (int)__umulhi((uint32_t)c, p.pieces_magic) : c) : min(c * PARTS + part, groups - 1);
                 const size_t first = (size_t)n0 * groups + g;
-                if (v >= 4 * PARTS && p.zero) load_small_to_lds<1>((const char *)p.zero + first, soff[i], to + G::W + v * 256);
+                if (v >= NW / 2 * PARTS && p.zero) load_small_to_lds<1>((const char *)p.zero + first, soff[i], to + G::W + v * 256);
                 else load_small_to_lds<2>((const char *)p.scale + first * 2, soff[i], to + G::W + v * 256);
             }
         };
@@ -259,7 +259,7 @@ __global__ __launch_bounds__(512, 2) void int4_tile_kernel(Int4Args p, Int4Rows 
 #pragma unroll
                 for (int part = 0; part < PARTS; part++) {
                     if (FL < 4 && 128 * c + 32 * FL * part >= p.K) break;
-                    const char *sz = at + G::W + (part * 256 + 32 * wave + c32) * 4;
+                    const char *sz = at + G::W + (part * G::BN + 32 * wave + c32) * 4;
                     const uint16_t half = *(const uint16_t *)sz;
                     const float s = Elem<T>::ld((const T *)&half, 0);
                     const std::conditional_t<I8, Int4ZeroI8, Int4Zero<T>> conv(p.zero ? *(const uint32_t *)(sz + G::S) & 15u : 8u);
@@ -310,9 +310,14 @@ __global__ __launch_bounds__(512, 2) void int4_tile_kernel(Int4Args p, Int4Rows 
             }
     };
     // (a loop for each height: the sums and fragments are registers)
-    if (height == 4) run(std::integral_constant<int, 4>{});
-    else if (height == 3) run(std::integral_constant<int, 3>{});
-    else if (height == 2) run(std::integral_constant<int, 2>{});
+    if constexpr (NW == 8) {
+        if (height >= 3) {
+            if (height == 4) run(std::integral_constant<int, 4>{});
+            else run(std::integral_constant<int, 3>{});
+            return;
+        }
+    }
+    if (height == 2) run(std::integral_constant<int, 2>{});
     else run(std::integral_constant<int, 1>{});
 }
 
