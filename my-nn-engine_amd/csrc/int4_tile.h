@@ -1,15 +1,18 @@
-// Many rows of activations times 4-bit weights: eight waves of 64 x 64, as 128 rows x 256 columns or 64 x 512.
+// Many rows of activations times 4-bit weights: tiles of 32 TI rows (TI = 1 .. 4), a wave 32 TI x 32; eight waves side by side where tiles are tall, two
+// workgroups of four a compute unit where they are not.
 //
 // Activations, codes, scales and zero points go from memory to LDS without passing registers (global_load_lds), a piece of 128 columns
-// a stage, three stages where they fit: a piece is asked for two pieces ahead, because a weight tile's first reader waits for HBM.
-// (Weights and scales loaded into registers instead were waited for at every piece, with all that had been asked for since: 304 us
-// for 777 x 28672 x 4096, 231 with those loads left out.)  The codes are converted in registers, by each wave for its columns.
+// a stage, so that a piece is asked for two to five pieces ahead.  (Weights and scales loaded into registers were waited for at every piece, with all
+// that had been asked for since: 777 x 28672 x 4096 fp16 304 us, 231 with those loads left out.)  Each wave converts the codes of its columns in
+// registers, once for all rows of the tile; taller waves were better than wider ones (128 x 32 against 64 x 64: 275 against 282 us).
 // v_mfma 32x32 with the activations as the rows, so that a lane's 16 sums belong to one weight row and meet one scale.  A group's sum
 // starts from zero in registers of its own and is added, scaled, to the total: the codes' differences are exact in every type, so nothing
 // is rounded before the store, where weights dequantised to 16 bits would be rounded once each.
 //
-// What bounds it: MFMAs against the vector operations of two waves a SIMD -- for 32 MFMAs (int8: 16) of a wave and piece, 16 dwords of codes
-// (12 operations each in fp16, 19 in bf16, 9 to int8) and 64 sums to scale (int8: a conversion more).
+// What bounds it.  Tall tiles: of a piece (128 rows x 256 columns, 2.2 us in rounds that fill the device) the MFMAs alone are 1.6; the rest is what the
+// vector operations (12 for eight codes in fp16, 19 in bf16, 9 to int8; 64 sums to scale; a wave's seven loads) do not hide behind them.  2048 x 28672 x
+// 4096 fp16 501 - 514 us, 0.95 PFLOP/s; 128 x 65536 x 4096 of int8 66 us, 1.04 POP/s.  Short ones: the steps of a piece one after the other, 0.65 us
+// with 32 rows, 0.85 with 64 (its barrier and its reads from LDS are half of that; read a piece ahead they cost as much elsewhere).
 #pragma once
 #include "int4_codes.h"
 

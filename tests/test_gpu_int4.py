@@ -70,6 +70,34 @@ def test_decoder_shapes(kind, dtype, M, N, K, group):
     ref.assert_close(call(kind, ops), *want(kind, ops))
 
 
+# rows so long that a workgroup goes over K in rounds, and matrices of so many rows that a wave goes through a ring of them
+@KINDS
+@pytest.mark.parametrize("M,N,K,group,zero", [(1, 70, 40960, 64, True), (2, 100, 24576, 32, False), (3, 66, 32768, 128, True), (8, 40, 14336, 64, True),
+                                              (5, 41, 20480, 32, True), (7, 33, 16512, 128, False), (1, 128256, 256, 128, True), (12, 70000, 512, 64, False),
+                                              (20, 40000, 384, 32, True), (6, 50001, 640, 128, True)])
+def test_long_rows_and_many(kind, M, N, K, group, zero):
+    ops = operands(kind, M, N, K, group, BF16 if M % 2 else F16, zero)
+    ref.assert_close(call(kind, ops), *want(kind, ops))
+    if kind == "linear" and N <= 100:
+        clean = call(kind, ops)
+        ops[0][M - 1, K - 5] = float("-inf")
+        out = call(kind, ops)
+        d, _ = ref.differences(*ops[1:])
+        expected = d[:, K - 5] * float("-inf")
+        assert torch.equal(out[: M - 1], clean[: M - 1]) and torch.equal(out[M - 1].isnan(), expected.isnan())
+        assert torch.equal(out[M - 1].double().nan_to_num(nan=0.0, posinf=1.0, neginf=-1.0), expected.sign().nan_to_num(nan=0.0))
+
+
+# both sides of every border between the forms: rows, columns, lengths, groups
+@KINDS
+@pytest.mark.parametrize("M", [8, 9, 16, 17, 32, 33])
+@pytest.mark.parametrize("N", [15, 16, 17])
+@pytest.mark.parametrize("K,group", [(1024, 32), (1152, 32), (2048, 128), (2176, 64), (4096, 32), (4096, 128), (4224, 128), (4128, 32)])
+def test_borders(kind, M, N, K, group):
+    ops = operands(kind, M, N, K, group, F16, True)
+    ref.assert_close(call(kind, ops), *want(kind, ops))
+
+
 @pytest.mark.parametrize("dtype", [F16, BF16])
 def test_leading_dimensions(dtype):
     act, wq, scale, zero = operands("linear", 30, 48, 256, 64, dtype, True)

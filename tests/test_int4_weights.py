@@ -86,6 +86,7 @@ def test_products_refuse_before_they_launch():
         for group in (0, -128, 16, 48, 96, 130, 192):
             assert f(K=128 * 3 * 5 * 13, group=group) == -2, group
         assert f(K=192) == -1 and f(K=100, group=32) == -1
+        assert f(K=(1 << 22) + 128) == -2
         assert f(act=odd) == -1 and f(wq=odd) == -1
         for dtype in (mynn.F32, mynn.I8, 9):
             assert f(dtype=dtype) == -2
@@ -110,3 +111,41 @@ def test_norm_refuses_before_it_launches():
             assert f(**{k: 0}) == -1 and f(**{k: -1}) == -1
         assert f(dtype=9) == -1
     assert norm(total=p) == -1 and qnorm(ys=None) == -1
+
+
+def test_workspaces_are_asked_for_before_a_launch():
+    lib = mynn.lib()
+    need = lib.mynn_matmul_int4_workspace_bytes(48, 4096, 4096, 128)
+    assert need > 0 and need % (48 * 4096 * 4) == 0
+    # (few rows, and tiles that fill the device: none)
+    assert lib.mynn_matmul_int4_workspace_bytes(1, 4096, 4096, 128) == 0 and lib.mynn_matmul_int4_workspace_bytes(2048, 28672, 4096, 128) == 0
+    for bad in ((0, 4096, 4096, 128), (48, 0, 4096, 128), (48, 4096, -1, 128), (48, 4096, 4096, 0)):
+        assert lib.mynn_matmul_int4_workspace_bytes(*bad) == 0
+    buf = C.create_string_buffer(4096 + 16)
+    p = (C.addressof(buf) + 15) & ~15
+    for ws, size in ((None, 1 << 40), (p, need - 1), (p + 4, need)):
+        assert lib.mynn_dequant_matmul_int4_ws(p, p, p, p, None, 48, 4096, 4096, 128, mynn.F16, ws, size, None) == -1
+        assert b"workspace" in lib.mynn_last_error()
+        assert lib.mynn_quantized_matmul_int4_ws(p, p, p, p, p, None, 48, 4096, 4096, 128, mynn.F16, ws, size, None) == -1
+
+
+def test_kernels_use_no_scratch_memory(tmp_path):
+    """sums, fragments and codes are registers in every form"""
+    import os
+    import re
+    import subprocess
+
+    from test_kernel_registers import LIB, READELF, device_code
+
+    if not (os.path.exists(READELF) and os.path.exists(LIB)):
+        pytest.skip("needs the built library and llvm-readelf")
+    forms = {}
+    for code in device_code(open(LIB, "rb").read()):
+        if b"int4_tile_kernel" not in code and b"add_norm_vec_kernel" not in code:
+            continue
+        (tmp_path / "code").write_bytes(code)
+        notes = subprocess.check_output([READELF, "--notes", str(tmp_path / "code")], text=True)
+        for name, scratch in re.findall(r"\.name:\s+(\S*(?:int4|add_norm)\S*)\n(?:(?!\.name:).)*?\.private_segment_fixed_size:\s+(\d+)", notes, re.S):
+            forms[name] = int(scratch)
+    assert sum("int4_tile" in n for n in forms) == 24 and sum("int4_stream" in n for n in forms) >= 72 and sum("add_norm_vec" in n for n in forms) == 24
+    assert not {k: v for k, v in forms.items() if v}
