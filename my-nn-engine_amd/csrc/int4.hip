@@ -131,18 +131,27 @@ template <typename T, bool I8, int FL> static int int4_tiles(const Int4Args &a, 
         ranges.part = (float *)block.ptr;
     }
     const int side = ranges.part ? ranges.count : 1;  // ranges side by side
-    auto go = [&](auto nw_, const Int4Rows &rows) {
+    auto launch = [&](auto nw_, auto wide, const Int4Rows &rows) {
         constexpr int NW = decltype(nw_)::value;
-        using G = Int4Tile<I8, FL, NW>;
+        constexpr bool WIDE = decltype(wide)::value;
+        using G = Int4Tile<I8, FL, NW, WIDE>;
         const long long blocks = (long long)rows.tiles * ((a.N + G::BN - 1) / G::BN) * side;
         MYNN_REQUIRE(blocks < 1 << 30, MYNN_ERR_UNSUPPORTED, "4-bit product: M=%d N=%d", a.M, a.N);
         static bool lds_set = false;
         if (!lds_set) {
-            MYNN_HIP(hipFuncSetAttribute((const void *)int4_tile_kernel<T, I8, FL, NW>, hipFuncAttributeMaxDynamicSharedMemorySize, G::LDS));
+            MYNN_HIP(hipFuncSetAttribute((const void *)int4_tile_kernel<T, I8, FL, NW, WIDE>, hipFuncAttributeMaxDynamicSharedMemorySize, G::LDS));
             lds_set = true;
         }
-        MYNN_LAUNCH((int4_tile_kernel<T, I8, FL, NW>), dim3((unsigned)blocks), dim3(64 * NW), G::LDS, s, a, rows, ranges);
+        MYNN_LAUNCH((int4_tile_kernel<T, I8, FL, NW, WIDE>), dim3((unsigned)blocks), dim3(64 * NW), G::LDS, s, a, rows, ranges);
         return launch_status("int4_tile_kernel");
+    };
+    auto go = [&](auto nw, const Int4Rows &rows) {
+        // (us, without / with: 24 x 4096 x 14336 of int8, groups of 64 and zero points 22.8 / 21, 64 x 28672 x 4096, groups of 32 and zero points 68 / 56, 411 x 4096 x
+        // 14336 125 / 115; groups of 64 without zero points no difference)
+        if constexpr (FL < 4) {
+            if ((FL == 1 || a.zero) && a.K % 128 == 0 && ((uintptr_t)a.scale & 3) == 0 && ((uintptr_t)a.zero & (FL == 1 ? 3 : 1)) == 0) return launch(nw, std::true_type{}, rows);
+        }
+        return launch(nw, std::false_type{}, rows);
     };
     // Tiles of at most 64 rows: two workgroups of four waves a compute unit, one computes while the other meets at its barrier (us, one of eight / two of
     // four: 128 x 4096 x 4096 19.7 / 16.4, 339 x 2560 x 2048 of int8 23 / 18.5, 64 x 28672 x 4096 35.8 / 34.3; taller tiles are the better ones where

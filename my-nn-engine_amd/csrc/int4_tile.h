@@ -61,24 +61,27 @@ struct Int4ZeroI8 {
 
 // LDS of a stage: codes, then a dword for each column's scale and one for its zero point, for each group of a piece, then activations of
 // 32 TI rows; as many stages as there is room for, up to six: short tiles wait for memory, not for the matrix cores.
-template <bool I8, int FL, int NW> struct Int4Tile {
+// WIDE (groups of 32 and 64): a piece's scales of a column as one dword or two and its zero points as one, where rows are whole pieces and addresses
+// allow it, instead of a load for each, every one of which asks for a line of its own.
+template <bool I8, int FL, int NW, bool WIDE> struct Int4Tile {
     static constexpr int LDS = NW * 20 * 1024;  // (a compute unit has 160 KB and takes eight waves)
     static constexpr int BN = 32 * NW, PARTS = 4 / FL;
     static constexpr int ROW = I8 ? 128 : 256;  // bytes of a piece of an activation row
     static constexpr int W = BN * 64, S = BN * 4 * PARTS, HEAD = W + 2 * S;
-    static constexpr int LW = 2, LS = PARTS;  // load instructions of a wave and stage, codes and scales
+    static constexpr int LW = 2, LS = !WIDE ? PARTS : FL == 1 ? 2 : 1;  // load instructions of a wave and stage, codes and scales
     static constexpr int loads(int ti) { return (32 * ti * ROW + 1024 * NW - 1) / (1024 * NW); }
     static constexpr int stage(int ti) { return HEAD + 1024 * NW * loads(ti); }
     static constexpr int stages(int ti) { return LDS / stage(ti) < 6 ? LDS / stage(ti) : 6; }
 };
 
-// 2 bytes or one a lane to LDS dword lds + 4 * lane, from base + off (base wave-uniform)
+// 4 bytes, 2 or one a lane to LDS dword lds + 4 * lane, from base + off (base wave-uniform)
 #pragma clang diagnostic push
 #pragma clang diagnostic ignored "-Winline-asm"
 template <int BYTES> __device__ inline void load_small_to_lds(const char *base, uint32_t off, uint32_t lds) {
     lds = __builtin_amdgcn_readfirstlane(lds);
     base = scalar_pointer(base);
-    if constexpr (BYTES == 2) asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_ushort %1, %2" ::"s"(lds), "v"(off), "s"(base) : "memory", "m0");
+    if constexpr (BYTES == 4) asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" ::"s"(lds), "v"(off), "s"(base) : "memory", "m0");
+    else if constexpr (BYTES == 2) asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_ushort %1, %2" ::"s"(lds), "v"(off), "s"(base) : "memory", "m0");
     else asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_ubyte %1, %2" ::"s"(lds), "v"(off), "s"(base) : "memory", "m0");
 }
 #pragma clang diagnostic pop
@@ -103,9 +106,9 @@ template <int LOADS, int MOST> __device__ inline void wait_stages(int ahead) {
     } else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 }
 
-template <typename T, bool I8, int FL, int NW>
+template <typename T, bool I8, int FL, int NW, bool WIDE>
 __global__ __launch_bounds__(64 * NW, 2) void int4_tile_kernel(Int4Args p, Int4Rows rows, Int4Ranges ranges) {
-    using G = Int4Tile<I8, FL, NW>;
+    using G = Int4Tile<I8, FL, NW, WIDE>;
     constexpr int EB = I8 ? 1 : 2, ROW = G::ROW, PARTS = G::PARTS;
     constexpr int SP = (I8 ? 1 : 2) * FL;  // instructions to a scale
     constexpr int CPR = ROW / 16;          // 16-byte chunks of a row
@@ -166,7 +169,8 @@ __global__ __launch_bounds__(64 * NW, 2) void int4_tile_kernel(Int4Args p, Int4R
 #pragma unroll
         for (int i = 0; i < G::LS; i++) {
             const int v = wave * G::LS + i, row = min(64 * (v % (NW / 2)) + lane, p.N - 1 - n0);
-            soff[i] = (uint32_t)row * (uint32_t)groups * (v < NW / 2 * PARTS ? 2u : p.zero ? 1u : 0u);
+            if constexpr (WIDE) soff[i] = (uint32_t)row * (uint32_t)groups * (v < NW / (3 - G::LS) ? 2u : p.zero && v < NW / (3 - G::LS) + NW / 2 ? 1u : 0u);
+            else soff[i] = (uint32_t)row * (uint32_t)groups * (v < NW / 2 * PARTS ? 2u : p.zero ? 1u : 0u);
         }
         auto load = [&](int i, int c, int slot) {
             const uint32_t to = at0 + slot * STAGE;
@@ -189,6 +193,16 @@ __global__ __launch_bounds__(64 * NW, 2) void int4_tile_kernel(Int4Args p, Int4R
                 load_to_lds(wbase + (size_t)c * 64, off, to + (wave * G::LW + i) * 1024);
             } else {
                 i -= LA + G::LW;
+                if constexpr (WIDE) {
+                    // dword `which` of the scales, then the zero points, then (groups of 32) nothing: one scale for all lanes
+                    constexpr int scales = NW / (3 - G::LS);
+                    const int v = wave * G::LS + i, which = v / (NW / 2);
+                    const size_t first = (size_t)n0 * groups + c * PARTS;
+                    const uint32_t where = to + G::W + (v < scales ? v * 256 : G::S + (v - scales) * 256);
+                    if (v >= scales && v < scales + NW / 2 && p.zero) load_small_to_lds<FL == 1 ? 4 : 2>((const char *)p.zero + first, soff[i], where);
+                    else load_small_to_lds<4>((const char *)p.scale + (v < scales ? first * 2 + 4 * which : 0), soff[i], where);
+                    return;
+                }
                 const int v = wave * G::LS + i, part = v / (NW / 2) % PARTS;  // (of the wave alike)
                 const int g = FL == 4 ? (p.pieces_magic ? (int)__umulhi((uint32_t)c, p.pieces_magic) : c) : min(c * PARTS + part, groups - 1);
                 const size_t first = (size_t)n0 * groups + g;
@@ -262,10 +276,11 @@ __global__ __launch_bounds__(64 * NW, 2) void int4_tile_kernel(Int4Args p, Int4R
 #pragma unroll
                 for (int part = 0; part < PARTS; part++) {
                     if (FL < 4 && 128 * c + 32 * FL * part >= p.K) break;
-                    const char *sz = at + G::W + (part * G::BN + 32 * wave + c32) * 4;
-                    const uint16_t half = *(const uint16_t *)sz;
+                    const char *sz = at + G::W + ((WIDE ? part >> 1 : part) * G::BN + 32 * wave + c32) * 4;
+                    const uint16_t half = *(const uint16_t *)(sz + (WIDE ? 2 * (part & 1) : 0));
                     const float s = Elem<T>::ld((const T *)&half, 0);
-                    const std::conditional_t<I8, Int4ZeroI8, Int4Zero<T>> conv(p.zero ? *(const uint32_t *)(sz + G::S) & 15u : 8u);
+                    const char *zs = WIDE ? at + G::W + G::S + (32 * wave + c32) * 4 + part : sz + G::S;
+                    const std::conditional_t<I8, Int4ZeroI8, Int4Zero<T>> conv(p.zero ? *(const uint8_t *)zs & 15u : 8u);
                     std::conditional_t<I8, i16v_t, f16x_t> acc[TI] = {};
 #pragma unroll
                     for (int k = 0; k < SP; k++) {

@@ -206,7 +206,7 @@ def test_small_values(dtype, M):
 
 # scales, zero points and outputs at any element; what lies around the output stays as it was
 @KINDS
-@pytest.mark.parametrize("M,N,K,group", [(1, 37, 160, 32), (9, 50, 384, 128), (33, 65, 192, 64), (140, 131, 256, 128)])
+@pytest.mark.parametrize("M,N,K,group", [(1, 37, 160, 32), (3, 37, 256, 32), (9, 50, 384, 128), (33, 65, 192, 64), (33, 65, 256, 64), (40, 70, 384, 32), (140, 131, 256, 128)])
 def test_odd_places(kind, M, N, K, group):
     ops = list(operands(kind, M, N, K, group, BF16, True))
     expected = call(kind, ops)

@@ -147,5 +147,5 @@ def test_kernels_use_no_scratch_memory(tmp_path):
         notes = subprocess.check_output([READELF, "--notes", str(tmp_path / "code")], text=True)
         for name, scratch in re.findall(r"\.name:\s+(\S*(?:int4|add_norm)\S*)\n(?:(?!\.name:).)*?\.private_segment_fixed_size:\s+(\d+)", notes, re.S):
             forms[name] = int(scratch)
-    assert sum("int4_tile" in n for n in forms) == 24 and sum("int4_stream" in n for n in forms) >= 72 and sum("add_norm_vec" in n for n in forms) == 24
+    assert sum("int4_tile" in n for n in forms) == 40 and sum("int4_stream" in n for n in forms) >= 72 and sum("add_norm_vec" in n for n in forms) == 24
     assert not {k: v for k, v in forms.items() if v}
