@@ -321,7 +321,7 @@ bool addresses(PyObject *const *args, int count, void **p) {
     return true;
 }
 
-// (exception class, addresses of mynn_last_error and of the four operators)
+// (exception class, addresses of mynn_last_error and of the first four operators)
 PyObject *bind(PyObject *, PyObject *const *args, Py_ssize_t n) {
     if (n != 6) {
         PyErr_SetString(PyExc_TypeError, "bind: six arguments");
