@@ -3,6 +3,7 @@
 // to the storage type or, per row, to 8 bits: step = max|y| / 127 (1 for a row of zeros), code = y / step rounded half away from zero.
 // Statistics and y are held in 32 bits; y goes to 8 bits without a rounding to T in between.  A row whose y is not all finite
 // gets the step NaN and codes of zero, so that a product of it is NaN and not some number.
+#include <algorithm>
 #include <type_traits>
 
 #include "mfma.h"
@@ -180,9 +181,22 @@ __global__ __launch_bounds__(64 * W) void add_norm_vec_kernel(void *out_, const 
     }
 }
 
+constexpr int kAnRows = 1 << 21;  // rows of a launch: with 1024 threads each it stays below the 2^32 that one may have
+
 template <bool Q8>
 static int add_norm(void *out, void *y_scale, void *sum, const void *x, const void *residual, const void *w, int rows, int dim, float eps, int dtype,
                     hipStream_t s) {
+    if (rows > kAnRows) {
+        const size_t bytes = dtype == MYNN_F32 ? 4 : 2, step = (size_t)kAnRows * dim;
+        for (int r = 0; r < rows; r += std::min(kAnRows, rows - r)) {
+            const size_t i = r / kAnRows;
+            auto at = [&](const void *p) { return p ? (char *)p + i * step * bytes : nullptr; };
+            if (const int rc = add_norm<Q8>((char *)out + i * step * (Q8 ? 1 : bytes), Q8 ? (char *)y_scale + i * kAnRows * bytes : nullptr, at(sum), at(x), at(residual),
+                                            w, std::min(kAnRows, rows - r), dim, eps, dtype, s))
+                return rc;
+        }
+        return 0;
+    }
     return dispatch_dtype(dtype, [&](auto *t) {
         using T = std::remove_pointer_t<decltype(t)>;
         if constexpr (sizeof(T) == 2) {

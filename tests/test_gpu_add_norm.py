@@ -179,6 +179,21 @@ def test_offsets_beyond_32_bits():
     assert not bool(codes[100].any())
 
 
+@pytest.mark.parametrize("dtype,dim", [(F16, 8), (F32, 3)])
+def test_more_rows_than_a_launch_has_room_for(dtype, dim):
+    rows = (1 << 24) + 5
+    x, r, w = operands(rows, dim, dtype)
+    out, total = mynn.add_rms_norm(x, r, w, EPS)
+    codes, scale, again = mynn.add_rms_norm_quantize(x, r, w, EPS)
+    assert torch.equal(total, again)
+    for at in (0, (1 << 21) - 3, (1 << 22) - 3, 5 << 21, (1 << 24) - 3):
+        rows = slice(at, at + 8)
+        check_sum(total[rows], x[rows], r[rows])
+        y, rel = exact_norm(total[rows], w)
+        assert bool(((out[rows].double() - y).abs() <= y.abs() * (half_step(dtype) * (1 + rel) + rel) + torch.finfo(dtype).smallest_normal * half_step(dtype)).all())
+        check_codes(codes[rows], scale[rows], total[rows], w)
+
+
 @pytest.mark.parametrize("rows,dim", [(1, 4096), (300, 2048), (4096, 1024)])
 def test_captured_calls(rows, dim):
     x, r, w = operands(rows, dim, F16)
