@@ -369,11 +369,20 @@ def quantized_matmul(lhs, lhs_scale, rhs, rhs_scale, want_acc=True):
     return out, acc
 
 
+def _on_current_device(name, *tensors):
+    """a launch goes to the current device's stream: operands of another GPU are refused"""
+    for t in tensors:
+        if t is not None and t.device.type == "cuda" and t.device.index != _t()._C._cuda_getDevice():
+            raise MynnError("%s: an operand is on %s, which is not the current device" % (name, t.device))
+
+
 def _int4_shape(wq, scale, zero):
     """(N, K, group) of a 4-bit matrix: wq uint8 [N, K/2], scale [N, K/group], zero like scale in uint8 or None"""
+    if wq.dim() != 2 or scale.dim() != 2:
+        raise MynnError("4-bit weights: wq %s and scale %s have to be matrices" % (tuple(wq.shape), tuple(scale.shape)))
     N, half = wq.shape
     groups = scale.shape[1]
-    if scale.shape[0] != N or groups < 1 or 2 * half % groups or wq.dtype != _torch.uint8 or (
+    if scale.shape[0] != N or groups < 1 or half < 1 or 2 * half % groups or N >= 1 << 31 or wq.dtype != _torch.uint8 or (
             zero is not None and (zero.shape != scale.shape or zero.dtype != _torch.uint8)):
         raise MynnError("4-bit weights: wq %s %s, scale %s, zero %s do not fit together" % (
             tuple(wq.shape), wq.dtype, tuple(scale.shape), None if zero is None else (tuple(zero.shape), zero.dtype)))
@@ -394,7 +403,8 @@ def dequant_matmul_int4(act, wq, scale, zero=None):
             return out
     _t()
     N, K, group = _int4_shape(wq, scale, zero)
-    if act.shape[-1] != K or act.dtype != scale.dtype:
+    _on_current_device("dequant_matmul_int4", act, wq, scale, zero)
+    if act.dim() < 1 or act.shape[-1] != K or act.numel() // K >= 1 << 31 or act.dtype != scale.dtype:
         raise MynnError("dequant_matmul_int4: act %s %s, scale %s and K=%d do not fit together" % (tuple(act.shape), act.dtype, scale.dtype, K))
     out = wq.new_empty(act.shape[:-1] + (N,), dtype=scale.dtype)
     M = act.numel() // K
@@ -412,7 +422,8 @@ def quantized_matmul_int4(lhs, lhs_scale, wq, scale, zero=None):
             return out
     _t()
     N, K, group = _int4_shape(wq, scale, zero)
-    if lhs.dim() != 2 or lhs.shape[1] != K or lhs.dtype != _torch.int8 or lhs_scale.numel() != lhs.shape[0] or lhs_scale.dtype != scale.dtype:
+    _on_current_device("quantized_matmul_int4", lhs, lhs_scale, wq, scale, zero)
+    if lhs.dim() != 2 or lhs.shape[1] != K or lhs.shape[0] >= 1 << 31 or lhs.dtype != _torch.int8 or lhs_scale.numel() != lhs.shape[0] or lhs_scale.dtype != scale.dtype:
         raise MynnError("quantized_matmul_int4: lhs %s %s, lhs_scale %s %s, scale %s and K=%d do not fit together" % (
             tuple(lhs.shape), lhs.dtype, tuple(lhs_scale.shape), lhs_scale.dtype, scale.dtype, K))
     M = lhs.shape[0]
@@ -677,8 +688,9 @@ def rms_norm(x, w, eps):
 
 
 def _add_norm_shape(name, x, residual, w):
-    dim = x.shape[-1]
-    if (residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype)) or w.numel() != dim or w.dtype != x.dtype:
+    _on_current_device(name, x, residual, w)
+    dim = x.shape[-1] if x.dim() else 0
+    if x.numel() // max(dim, 1) >= 1 << 31 or dim >= 1 << 31 or (residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype)) or w.numel() != dim or w.dtype != x.dtype:
         raise MynnError("%s: x %s %s, residual %s, w %s %s do not fit together" % (
             name, tuple(x.shape), x.dtype, None if residual is None else (tuple(residual.shape), residual.dtype), tuple(w.shape), w.dtype))
     return x.numel() // max(dim, 1), dim

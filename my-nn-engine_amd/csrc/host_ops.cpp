@@ -42,6 +42,12 @@ const at::Tensor *plain(PyObject *o) {
     const at::Tensor &t = THPVariable_Unpack(o);
     return t.defined() && t.has_storage() && t.is_cuda() && t.layout() == at::kStrided && t.is_contiguous() ? &t : nullptr;
 }
+// ... and on the current device
+const at::Tensor *here(PyObject *o) {
+    const at::Tensor *t = plain(o);
+    return t && t->get_device() == c10::hip::current_device() ? t : nullptr;
+}
+bool fits_int(int64_t v) { return v <= INT32_MAX; }
 void *data(const at::Tensor &t) { return t.data_ptr(); }
 mynn_stream current_stream() { return (mynn_stream)c10::hip::getCurrentHIPStream().stream(); }
 at::Tensor make(at::IntArrayRef sizes, const at::Tensor &like, at::ScalarType type) { return at::empty(sizes, like.options().dtype(type)); }
@@ -171,11 +177,11 @@ struct Int4 {
     const at::Tensor *wq, *scale, *zero = nullptr;
     int64_t N = 0, K = 0, groups = 0;
     int code = -1;
-    Int4(PyObject *w, PyObject *s, PyObject *z) : wq(plain(w)), scale(plain(s)) {
-        if (!wq || !scale || wq->dim() != 2 || scale->dim() != 2 || wq->scalar_type() != at::kByte || (z != Py_None && !(zero = plain(z)))) return;
+    Int4(PyObject *w, PyObject *s, PyObject *z) : wq(here(w)), scale(here(s)) {
+        if (!wq || !scale || wq->dim() != 2 || scale->dim() != 2 || wq->scalar_type() != at::kByte || (z != Py_None && !(zero = here(z)))) return;
         N = wq->size(0), groups = scale->size(1);
         const int64_t cols = 2 * wq->size(1);
-        if (scale->size(0) != N || groups < 1 || cols % groups || (zero && (zero->scalar_type() != at::kByte || zero->sizes() != scale->sizes()))) return;
+        if (scale->size(0) != N || groups < 1 || cols % groups || !fits_int(N) || !fits_int(cols) || (zero && (zero->scalar_type() != at::kByte || zero->sizes() != scale->sizes()))) return;
         K = cols;
         code = code_of(scale->scalar_type());
     }
@@ -191,10 +197,11 @@ struct Int4 {
 PyObject *dequant_matmul_int4(PyObject *, PyObject *const *args, Py_ssize_t n) {
     if (n != 4) return none();
     return guarded([&]() -> PyObject * {
-        const at::Tensor *act = plain(args[0]);
+        const at::Tensor *act = here(args[0]);
         const Int4 w(args[1], args[2], args[3]);
         if (!act || !w || act->dim() < 1 || act->size(-1) != w.K || act->scalar_type() != w.scale->scalar_type()) return none();
         const int64_t M = act->numel() / w.K;
+        if (!fits_int(M)) return none();
         c10::SmallVector<int64_t, 4> sizes(act->sizes().begin(), act->sizes().end());
         sizes.back() = w.N;
         const at::Tensor out = make(sizes, *w.wq, w.scale->scalar_type());
@@ -214,12 +221,13 @@ PyObject *dequant_matmul_int4(PyObject *, PyObject *const *args, Py_ssize_t n) {
 PyObject *quantized_matmul_int4(PyObject *, PyObject *const *args, Py_ssize_t n) {
     if (n != 5) return none();
     return guarded([&]() -> PyObject * {
-        const at::Tensor *lhs = plain(args[0]), *ls = plain(args[1]);
+        const at::Tensor *lhs = here(args[0]), *ls = here(args[1]);
         const Int4 w(args[2], args[3], args[4]);
         if (!lhs || !ls || !w || lhs->dim() != 2 || lhs->size(1) != w.K || lhs->scalar_type() != at::kChar || ls->numel() != lhs->size(0) ||
             ls->scalar_type() != w.scale->scalar_type())
             return none();
         const int64_t M = lhs->size(0);
+        if (!fits_int(M)) return none();
         const at::Tensor out = make({M, w.N}, *w.wq, w.scale->scalar_type());
         void *o = data(out), *l = data(*lhs), *lsp = data(*ls), *q = data(*w.wq), *s = data(*w.scale), *z = w.zero ? data(*w.zero) : nullptr;
         const at::Tensor ws = w.workspace(M);
@@ -240,13 +248,14 @@ struct NormArgs {
     int64_t rows = 0, dim = 0;
     int code = -1;
     float eps = 0.f;
-    explicit NormArgs(PyObject *const *args) : x(plain(args[0])), w(plain(args[2])) {
-        if (!x || !w || x->dim() < 1 || (args[1] != Py_None && !(residual = plain(args[1]))) || !PyFloat_CheckExact(args[3])) return;
+    explicit NormArgs(PyObject *const *args) : x(here(args[0])), w(here(args[2])) {
+        if (!x || !w || x->dim() < 1 || (args[1] != Py_None && !(residual = here(args[1]))) || !PyFloat_CheckExact(args[3])) return;
         if (x->size(-1) < 1 || w->numel() != x->size(-1) || w->scalar_type() != x->scalar_type() ||
             (residual && (residual->sizes() != x->sizes() || residual->scalar_type() != x->scalar_type())))
             return;
         dim = x->size(-1);
         rows = x->numel() / dim;
+        if (!fits_int(rows) || !fits_int(dim)) return;
         eps = (float)PyFloat_AS_DOUBLE(args[3]);
         code = code_of(x->scalar_type());
     }

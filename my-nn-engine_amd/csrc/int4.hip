@@ -4,6 +4,7 @@
 //   out[m, n] = T( sum over groups of scale[n, g] * sum over k in g of act[m, k] * (code[n, k] - zero[n, g]) )
 // in 32 bits, rounded at the store; with int8 activations the inner sum is exact in int32 and the row's scale is applied last.
 #include <algorithm>
+#include <atomic>
 
 #include "int4_stream.h"
 #include "int4_tile.h"
@@ -19,6 +20,17 @@ constexpr int kCus = 256;
 static bool int4_streams(const Int4Args &a) {
     const int rows = a.M <= 8 ? 1 : a.M <= 16 ? 4096 : a.M <= 32 ? 2048 : 0;
     return (rows == 1 || a.K <= (a.group == 32 ? rows / 2 : rows)) && a.K % 128 == 0 && a.N >= 16 && (size_t)8 * a.K < 1u << 31;
+}
+
+// room for `bytes` of LDS a workgroup, asked for once a kernel and device (done: the devices' bits)
+static int int4_lds(const void *kernel, int bytes, std::atomic<uint64_t> &done) {
+    int device = 0;
+    MYNN_HIP(hipGetDevice(&device));
+    const uint64_t bit = (uint64_t)1 << (device & 63);
+    if (device < 64 && (done.load(std::memory_order_relaxed) & bit)) return 0;
+    MYNN_HIP(hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes));
+    done.fetch_or(bit, std::memory_order_relaxed);
+    return 0;
 }
 
 template <typename T, bool I8, int FL> static int int4_stream(const Int4Args &a, hipStream_t s) {
@@ -37,11 +49,8 @@ template <typename T, bool I8, int FL> static int int4_stream(const Int4Args &a,
         plan.tiles = turns * plan.per_wave;
         const size_t lds = (size_t)plan.tiles * plan.over_k * OUT * sizeof(float);
         if (MP == 16) {
-            static bool lds_set = false;
-            if (!lds_set) {
-                MYNN_HIP(hipFuncSetAttribute((const void *)int4_stream_kernel<T, I8, FL, MP, P, D, MT>, hipFuncAttributeMaxDynamicSharedMemorySize, 128 * 1024));
-                lds_set = true;
-            }
+            static std::atomic<uint64_t> set{0};
+            if (const int rc = int4_lds((const void *)int4_stream_kernel<T, I8, FL, MP, P, D, MT>, 128 * 1024, set)) return rc;
         }
         MYNN_LAUNCH((int4_stream_kernel<T, I8, FL, MP, P, D, MT>), dim3((tiles + plan.tiles - 1) / plan.tiles), dim3(64 * turns * plan.over_k), lds, s, a, plan);
         return launch_status("int4_stream_kernel");
@@ -136,12 +145,9 @@ template <typename T, bool I8, int FL> static int int4_tiles(const Int4Args &a, 
         constexpr bool WIDE = decltype(wide)::value;
         using G = Int4Tile<I8, FL, NW, WIDE>;
         const long long blocks = (long long)rows.tiles * ((a.N + G::BN - 1) / G::BN) * side;
-        MYNN_REQUIRE(blocks < 1 << 30, MYNN_ERR_UNSUPPORTED, "4-bit product: M=%d N=%d", a.M, a.N);
-        static bool lds_set = false;
-        if (!lds_set) {
-            MYNN_HIP(hipFuncSetAttribute((const void *)int4_tile_kernel<T, I8, FL, NW, WIDE>, hipFuncAttributeMaxDynamicSharedMemorySize, G::LDS));
-            lds_set = true;
-        }
+        MYNN_REQUIRE(blocks < (1ll << 32) / (64 * NW), MYNN_ERR_UNSUPPORTED, "4-bit product: M=%d N=%d", a.M, a.N);  // (the threads of a launch)
+        static std::atomic<uint64_t> set{0};
+        if (const int rc = int4_lds((const void *)int4_tile_kernel<T, I8, FL, NW, WIDE>, G::LDS, set)) return rc;
         MYNN_LAUNCH((int4_tile_kernel<T, I8, FL, NW, WIDE>), dim3((unsigned)blocks), dim3(64 * NW), G::LDS, s, a, rows, ranges);
         return launch_status("int4_tile_kernel");
     };
@@ -191,7 +197,7 @@ static int check_int4(const char *who, const void *out, const void *act, const v
     MYNN_REQUIRE(out && act && wq && scale && M > 0 && N > 0 && K > 0, MYNN_ERR_INVALID, "%s: bad operand (M=%d N=%d K=%d)", who, M, N, K);
     MYNN_REQUIRE(group == 32 || group == 64 || (group > 0 && group % 128 == 0), MYNN_ERR_UNSUPPORTED, "%s: group=%d (32, 64 or a multiple of 128)", who, group);
     MYNN_REQUIRE(K % group == 0, MYNN_ERR_INVALID, "%s: K=%d is no multiple of the group of %d", who, K, group);
-    MYNN_REQUIRE(K <= 1 << 22, MYNN_ERR_UNSUPPORTED, "%s: K=%d", who, K);
+    MYNN_REQUIRE(K <= 1 << 22 && M <= 1 << 30 && N <= 1 << 30, MYNN_ERR_UNSUPPORTED, "%s: M=%d N=%d K=%d", who, M, N, K);
     MYNN_REQUIRE(aligned16(act) && aligned16(wq), MYNN_ERR_INVALID, "%s: activations and weights have to be 16-byte aligned", who);
     return 0;
 }
@@ -213,7 +219,7 @@ static int quantized_matmul_int4(void *out, const int8_t *lhs, const void *lhs_s
 }
 
 extern "C" size_t mynn_matmul_int4_workspace_bytes(int M, int N, int K, int group) {
-    if (M < 1 || N < 1 || K < 1 || group < 1) return 0;
+    if (M < 1 || N < 1 || K < 1 || group < 1 || M > 1 << 30 || N > 1 << 30 || K > 1 << 22) return 0;
     Int4Args a{};
     a.M = M, a.N = N, a.K = K, a.group = group;
     return int4_workspace(a);

@@ -87,10 +87,46 @@ def test_products_refuse_before_they_launch():
             assert f(K=128 * 3 * 5 * 13, group=group) == -2, group
         assert f(K=192) == -1 and f(K=100, group=32) == -1
         assert f(K=(1 << 22) + 128) == -2
+        assert f(M=(1 << 30) + 1) == -2 and f(N=(1 << 31) - 1) == -2
         assert f(act=odd) == -1 and f(wq=odd) == -1
         for dtype in (mynn.F32, mynn.I8, 9):
             assert f(dtype=dtype) == -2
     assert qlinear(ls=None) == -1
+
+
+def test_wrappers_refuse_before_they_call():
+    import types
+
+    import torch
+
+    act, ls = torch.zeros((2, 64), dtype=torch.float16), torch.ones((2,), dtype=torch.float16)
+    wq, scale, zero = torch.zeros((4, 32), dtype=torch.uint8), torch.ones((4, 2), dtype=torch.float16), torch.zeros((4, 2), dtype=torch.uint8)
+    for bad in ((wq[0], scale, zero), (wq[None], scale, zero), (wq, scale[0], None), (wq, scale, zero[:1]), (wq[:, :0], scale, zero), (wq, scale[:, :0], None)):
+        with pytest.raises(mynn.MynnError, match="4-bit weights"):
+            mynn.dequant_matmul_int4(act, *bad)
+        with pytest.raises(mynn.MynnError, match="4-bit weights"):
+            mynn.quantized_matmul_int4(act.to(torch.int8), ls, *bad)
+    for bad in (act[0, 0], act[:, :32], act.float(), act[None, :, :0]):
+        with pytest.raises(mynn.MynnError, match="fit together"):
+            mynn.dequant_matmul_int4(bad, wq, scale, zero)
+    for bad in ((act.to(torch.int8)[0], ls), (act, ls), (act.to(torch.int8), ls[:1])):
+        with pytest.raises(mynn.MynnError, match="fit together"):
+            mynn.quantized_matmul_int4(*bad, wq, scale, zero)
+    # more rows than an int counts (a broadcast view: no memory)
+    with pytest.raises(mynn.MynnError, match="fit together"):
+        mynn.dequant_matmul_int4(act[:1].expand((1 << 32) + 2, 64), wq, scale, zero)
+    for norm in (mynn.add_rms_norm, mynn.add_rms_norm_quantize):
+        for x, w in ((act[0, 0], act[0]), (act, act[0, :32]), (act[:1].expand((1 << 32) + 2, 64), act[0])):
+            with pytest.raises(mynn.MynnError, match="fit together"):
+                norm(x, None, w, 1e-5)
+    # an operand of another device than the current one
+    current = types.SimpleNamespace(_cuda_getDevice=lambda: 1)
+    with pytest.MonkeyPatch.context() as m:
+        m.setattr(mynn, "_t", lambda: types.SimpleNamespace(_C=current))
+        on = [types.SimpleNamespace(device=torch.device("cuda", i)) for i in range(2)]
+        mynn._on_current_device("f", on[1], None)
+        with pytest.raises(mynn.MynnError, match="cuda:0"):
+            mynn._on_current_device("f", on[1], on[0])
 
 
 def test_norm_refuses_before_it_launches():
