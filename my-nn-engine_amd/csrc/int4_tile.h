@@ -175,7 +175,7 @@ __global__ __launch_bounds__(64 * NW, 2) void int4_tile_kernel(Int4Args p, Int4R
         auto load = [&](int i, int c, int slot) {
             const uint32_t to = at0 + slot * STAGE;
             // (of a broken piece: chunks behind the row are not multiplied, its last one in their place)
-            const bool broken = FL < 4 && 128 * c + 128 > p.K;
+            const bool broken = FL < 4 && !WIDE && 128 * c + 128 > p.K;
             if (i < LA) {
                 uint32_t off = aoff[i];
                 if (broken) {
@@ -255,6 +255,17 @@ __global__ __launch_bounds__(64 * NW, 2) void int4_tile_kernel(Int4Args p, Int4R
                         }
                     }
                 }
+                // WIDE has whole pieces alone: a column's scales and zero points are read at once, and a piece's groups are one block of code (365 x 2560 x
+                // 2048 of int8 in groups of 32 31.5 -> 26.4 us, 411 x 4096 x 14336 114 -> 103).  Not in the tallest tiles (nor the next in fp16,
+                // whose conversion holds constants), which have no registers for two groups' sums: the branch keeps their groups apart.
+                constexpr bool AT_ONCE = WIDE && TI <= (std::is_same<T, f16_t>::value && !I8 && FL == 1 ? 2 : 3);
+                const char *column = at + G::W + (32 * wave + c32) * 4;
+                uint32_t sw[2] = {}, zw = 0x08080808u;
+                if constexpr (AT_ONCE) {
+                    sw[0] = *(const uint32_t *)column;
+                    if constexpr (FL == 1) sw[1] = *(const uint32_t *)(column + G::BN * 4);
+                    if (p.zero) zw = *(const uint32_t *)(column + G::S);
+                }
                 // Fragments are read an instruction ahead, in short tiles, whose products do not cover the way to LDS, all of a piece at once; the
                 // loads of a later piece are asked for between the products, one here and there: the eight waves' together keep the memory pipe busy for
                 // most of a piece, and a wave that waits to hand it the next one does nothing else.
@@ -275,12 +286,12 @@ __global__ __launch_bounds__(64 * NW, 2) void int4_tile_kernel(Int4Args p, Int4R
                 const bool more = c + NS - 1 < c1;
 #pragma unroll
                 for (int part = 0; part < PARTS; part++) {
-                    if (FL < 4 && 128 * c + 32 * FL * part >= p.K) break;
-                    const char *sz = at + G::W + ((WIDE ? part >> 1 : part) * G::BN + 32 * wave + c32) * 4;
-                    const uint16_t half = *(const uint16_t *)(sz + (WIDE ? 2 * (part & 1) : 0));
+                    if (FL < 4 && !AT_ONCE && 128 * c + 32 * FL * part >= p.K) break;
+                    const char *sz = column + (WIDE ? part >> 1 : part) * G::BN * 4;
+                    const uint16_t half = AT_ONCE ? (uint16_t)(sw[part >> 1] >> (16 * (part & 1))) : *(const uint16_t *)(sz + (WIDE ? 2 * (part & 1) : 0));
                     const float s = Elem<T>::ld((const T *)&half, 0);
-                    const char *zs = WIDE ? at + G::W + G::S + (32 * wave + c32) * 4 + part : sz + G::S;
-                    const std::conditional_t<I8, Int4ZeroI8, Int4Zero<T>> conv(p.zero ? *(const uint8_t *)zs & 15u : 8u);
+                    const uint32_t zero = AT_ONCE ? (zw >> (8 * part)) & 15u : p.zero ? *(const uint8_t *)(WIDE ? column + G::S + part : sz + G::S) & 15u : 8u;
+                    const std::conditional_t<I8, Int4ZeroI8, Int4Zero<T>> conv(zero);
                     std::conditional_t<I8, i16v_t, f16x_t> acc[TI] = {};
 #pragma unroll
                     for (int k = 0; k < SP; k++) {
