@@ -336,8 +336,9 @@ int mynn_add_rms_norm(void *out, void *sum, const void *x, const void *residual,
                       float eps, int dtype, mynn_stream s);
 /* The same with the normalised rows in 8 bits, as mynn_quantized_matmul and mynn_quantized_matmul_int4 take them:
  * y_scale[row] = amax/127 of the normalised row (1 for a row of zeros), y = clamp(round_half_away(value/scale),
- * -127,127) as in mynn_dynamic_quantize_linear, from the 32-bit values (they are not rounded to T in between).  A row
- * with a value that is not finite gets the scale NaN and codes of zero. */
+ * -127,127) from the 32-bit values (they are not rounded to T in between), their 32-bit quotient and the scale before
+ * it is rounded to T (mynn_dynamic_quantize_linear takes the product with the reciprocal: another code for some values
+ * next to a tie).  A row with a value that is not finite gets the scale NaN and codes of zero. */
 int mynn_add_rms_norm_quantize(int8_t *y, void *y_scale, void *sum, const void *x, const void *residual, const void *w,
                                int rows, int dim, float eps, int dtype, mynn_stream s);
 
