@@ -221,8 +221,8 @@ __global__ __launch_bounds__(512) void int4_stream_kernel(Int4Args p, Int4Stream
         const float *from = red + tile * plan.over_k * OUT + m / MP * MP * MP + w * MP + m % MP;
         float sum = from[0];
         for (int k = 1; k < plan.over_k; k++) sum += from[k * OUT];
-        const int n = min((first + tile) * MP, p.N - MP) + w;
-        if (m < p.M) {
+        const int own = (first + tile) * MP, n = min(own, p.N - MP) + w;
+        if (m < p.M && n >= own) {  // (rows of the tile before are that tile's alone: one store to a place)
             if constexpr (I8) sum *= Elem<T>::ld((const T *)p.act_scale, m);
             Elem<T>::st((T *)p.out, (size_t)m * p.N + n, sum);
         }
