@@ -139,9 +139,9 @@ int mynn_quantized_matmul(void *out, int32_t *acc_out, const int8_t *lhs, const 
  * odd column behind it in the high four.  Columns come in groups of `group` (32, 64 or a multiple of 128, dividing K);
  * scale [N, K/group] in dtype, zero uint8 [N, K/group] (its low four bits) or NULL for 8 everywhere:
  *   w[n,k] = scale[n, k/group] * (wq[n,k] - zero[n, k/group]).
- * A group's sum meets the scale once, in f32; one rounding at the store.  It runs over the codes' differences, which are exact; with few
- * rows in 16 bits over the codes, the zero point times the sum of act taken off it, unless that is not finite.  An infinity or a
- * NaN of act goes where the formula takes it: to its own row of out.  K up to 2^22, M and N to 2^30.
+ * A group's sum meets the scale once, in f32; one rounding at the store.  It runs over the codes' differences, which are exact.  An
+ * infinity or a NaN of act goes where the formula takes it, to its own row of out, and one of scale to its own column; the other values keep
+ * their bits.  K up to 2^22, M and N to 2^30.
  * Where the tiles of more than 8 rows leave the device idle, the f32 sums run over several ranges of K, added in their order; their
  * number is a function of M, N, K and the group alone, and every form of a call gives the same bits.  The ranges' sums need
  * mynn_matmul_int4_workspace_bytes(...) bytes (0: no ranges): the _ws forms take them from the caller (16-byte aligned;

@@ -3,11 +3,11 @@
 // A dword holds eight codes, the first in its lowest four bits.  A lane of v_mfma 16x16x32 takes the eight of a dword, one of v_mfma 32x32x16 too,
 // one of v_mfma 32x32x32 (int8) those of two.
 //
-// To 16 bits as they are, nine vector operations for eight: a nibble as a byte is 2^-9 times its value as an fp8 number (e4m3: below 8
-// subnormal, from 8 on the first binade, one line), so v_cvt_scalef32_pk makes two exact values of T from two bytes.  The zero point then comes
-// off the sums: sum a (q - z) = sum a q - z sum a.  Both sums may overflow, or meet an infinity, where their difference does not: who uses
-// them looks at the result and starts again with the differences themselves where it is not finite.
+// The zero point comes off each code, exactly, before the code meets an activation.  (Sums of act * code less the zero point times the sum of act took two
+// operations fewer for eight codes; but an activation whose code is the zero point, which is to count for nothing, left the rounding of both sums, and an
+// infinite one more than that.)
 // To int8: nibbles to bytes, the zero point taken off inside the bytes (a bit set above them: no borrow).
+// To fp16: a nibble under an exponent that makes it 1024 + n, or, four bits further up, 64 + n; one addition takes 1024 or 64 and the zero point off two.
 #pragma once
 #include <type_traits>
 
@@ -19,42 +19,35 @@ namespace mynn {
 typedef float f4_t __attribute__((ext_vector_type(4)));
 typedef int i4_t __attribute__((ext_vector_type(4)));
 
-template <typename T> __device__ inline f4_t mfma16(const U4 &a, const U4 &b, f4_t c) {
-    if constexpr (std::is_same<T, f16_t>::value)
-        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8_t, a), __builtin_bit_cast(h8_t, b), c, 0, 0, 0);
-    else
-        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8_t, a), __builtin_bit_cast(b8_t, b), c, 0, 0, 0);
+__device__ inline f4_t mfma16(const U4 &a, const U4 &b, f4_t c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8_t, a), __builtin_bit_cast(h8_t, b), c, 0, 0, 0);
 }
 
-// the eight codes of a dword as bytes, in their order
-__device__ inline uint2 int4_bytes(uint32_t w) {
-    const uint32_t e = w & 0x0F0F0F0Fu, o = (w >> 4) & 0x0F0F0F0Fu;
-    return uint2{__builtin_amdgcn_perm(o, e, 0x05010400u), __builtin_amdgcn_perm(o, e, 0x07030602u)};
-}
 // code - zero of the eight as int8 (zz: the zero point in each byte): 0x80 + code - zero never borrows from its neighbour
 __device__ inline uint2 int4_to_i8(uint32_t w, uint32_t zz) {
     const uint32_t e = ((w & 0x0F0F0F0Fu) | 0x80808080u) - zz, o = (((w >> 4) & 0x0F0F0F0Fu) | 0x80808080u) - zz;
     return uint2{__builtin_amdgcn_perm(o, e, 0x05010400u) ^ 0x80808080u, __builtin_amdgcn_perm(o, e, 0x07030602u) ^ 0x80808080u};
 }
-// the eight codes as T
-template <typename T> __device__ inline U4 int4_codes(uint32_t w) {
-    const uint2 b = int4_bytes(w);
-    if constexpr (std::is_same<T, f16_t>::value)
-        return U4{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)b.x, 512.f, false)),
-                  __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)b.x, 512.f, true)),
-                  __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)b.y, 512.f, false)),
-                  __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)b.y, 512.f, true))};
-    else
-        return U4{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)b.x, 512.f, false)),
-                  __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)b.x, 512.f, true)),
-                  __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)b.y, 512.f, false)),
-                  __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)b.y, 512.f, true))};
-}
-// code - zero of the eight as T
-template <typename T> __device__ inline U4 int4_differences(uint32_t w, int z) {
-    auto two = [&](int i) { return pack2<T>((float)((int)((w >> (8 * i)) & 15u) - z), (float)((int)((w >> (8 * i + 4)) & 15u) - z)); };
-    return U4{two(0), two(1), two(2), two(3)};
-}
+// code - zero of a dword's eight as fp16, in pairs (0, 4), (1, 5), (2, 6), (3, 7): where the other operand can be in that order too, one shift takes the
+// place of the four byte selections, nine operations in all.
+struct Int4Pairs {
+    h2_t low, high;
+    uint32_t nibbles0 = 0x000F000Fu, nibbles1 = 0x00F000F0u;
+    // (in vector registers: one instruction takes both, but at most one constant from elsewhere)
+    __device__ Int4Pairs() { asm volatile("" : "+v"(nibbles0), "+v"(nibbles1)); }
+    __device__ void at(uint32_t z) {
+        low = __builtin_bit_cast(h2_t, 0xE400E400u + z * 0x00010001u);
+        high = __builtin_bit_cast(h2_t, 0xD400D400u + z * 0x00100010u);
+    }
+    __device__ U4 operator()(uint32_t w) const {
+        auto two = [&](uint32_t v, uint32_t nibbles, uint32_t exponents, h2_t off) {
+            const uint32_t n = (v & nibbles) | exponents;
+            return __builtin_bit_cast(uint32_t, __builtin_bit_cast(h2_t, n) + off);
+        };
+        const uint32_t v = w >> 8;
+        return U4{two(w, nibbles0, 0x64006400u, low), two(w, nibbles1, 0x54005400u, high), two(v, nibbles0, 0x64006400u, low), two(v, nibbles1, 0x54005400u, high)};
+    }
+};
 // dword j of lane group g (16 lanes each) <-> dword g of lane group j
 __device__ inline void int4_transpose(U4 &d) {
     typedef uint32_t u2_t __attribute__((ext_vector_type(2)));
