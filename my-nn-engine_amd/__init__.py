@@ -288,14 +288,22 @@ def device_info():
 
 
 def dequantize_linear(x_i8, scale):
+    """codes times a scale for each row: scale has as many values as the first dimension of x_i8, or as several leading ones together (the codes
+    [.., dim] and scales of add_rms_norm_quantize and dynamic_quantize_linear)"""
     if x_i8.is_cuda:
         out = (_ops or _host_ops()).dequantize_linear(x_i8, scale)
         if out is not None:
             return out
     import torch
 
+    rows = x_i8.shape[0] if x_i8.dim() else 0
+    for d in range(1, x_i8.dim()):
+        if rows < scale.numel():
+            rows *= x_i8.shape[d]
+    if rows != scale.numel() or not x_i8.numel():
+        raise MynnError("dequantize_linear: x %s and scale %s do not fit together" % (tuple(x_i8.shape), tuple(scale.shape)))
+    _on_current_device("dequantize_linear", x_i8, scale)
     out = torch.empty(x_i8.shape, dtype=scale.dtype, device=x_i8.device)
-    rows = x_i8.shape[0]
     check(lib().mynn_dequantize_linear(_ptr(out), _ptr(x_i8), _ptr(scale), rows, x_i8.numel() // rows, _dt(scale),
                                        _stream()))
     return out

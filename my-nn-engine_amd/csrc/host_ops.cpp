@@ -302,13 +302,16 @@ PyObject *add_rms_norm_quantize(PyObject *, PyObject *const *args, Py_ssize_t n)
     });
 }
 
-// (codes [rows, ..], scale [rows]) -> what the codes stand for, in the scale's type
+// (codes, a scale for each row: for each index of as many of the leading dimensions as give that many) -> what the codes stand for, in the scale's type
 PyObject *dequantize_linear(PyObject *, PyObject *const *args, Py_ssize_t n) {
     if (n != 2) return none();
     return guarded([&]() -> PyObject * {
-        const at::Tensor *x = plain(args[0]), *scale = plain(args[1]);
-        if (!x || !scale || x->dim() < 1 || x->size(0) < 1 || x->scalar_type() != at::kChar || code_of(scale->scalar_type()) < 0) return none();
-        const int64_t rows = x->size(0), inner = x->numel() / rows;
+        const at::Tensor *x = here(args[0]), *scale = here(args[1]);
+        if (!x || !scale || x->dim() < 1 || x->numel() < 1 || x->scalar_type() != at::kChar || code_of(scale->scalar_type()) < 0) return none();
+        int64_t rows = x->size(0);
+        for (int64_t d = 1; d < x->dim() && rows < scale->numel(); d++) rows *= x->size(d);
+        if (rows != scale->numel()) return none();
+        const int64_t inner = x->numel() / rows;
         const at::Tensor out = make(x->sizes(), *x, scale->scalar_type());
         void *o = data(out), *xp = data(*x), *sp = data(*scale);
         const int code = code_of(scale->scalar_type());
