@@ -331,11 +331,11 @@ int mynn_rms_norm(void *out, const void *x, const void *w, int rows, int dim, fl
 /* A residual's addition with the norm behind it (mynn_add, then mynn_rms_norm, in one pass over the rows):
  *   sum = T(x + residual), out = T((sum * (1/sqrt(mean(sum^2)+eps))) * w) per row of dim values.
  * residual NULL: sum = x.  sum NULL: not stored.  sum may be x or residual itself; out may be either of the two that sum
- * is not. */
+ * is not.  A finite row whose squares have no 32-bit sum is normalised all the same (mynn_rms_norm gives zeros there). */
 int mynn_add_rms_norm(void *out, void *sum, const void *x, const void *residual, const void *w, int rows, int dim,
                       float eps, int dtype, mynn_stream s);
 /* The same with the normalised rows in 8 bits, as mynn_quantized_matmul and mynn_quantized_matmul_int4 take them:
- * y_scale[row] = amax/127 of the normalised row (1 for a row of zeros), y = clamp(round_half_away(value/scale),
+ * y_scale[row] = amax/127 of the normalised row (1 for a row of zeros, or of nothing from 2^-120 on: codes of zero), y = clamp(round_half_away(value/scale),
  * -127,127) from the 32-bit values (they are not rounded to T in between), their 32-bit quotient and the scale before
  * it is rounded to T (mynn_dynamic_quantize_linear takes the product with the reciprocal: another code for some values
  * next to a tie).  A row with a value that is not finite gets the scale NaN and codes of zero. */

@@ -47,6 +47,19 @@ struct AnStep {
     }
 };
 
+// A row whose squares have no 32-bit sum (values of 1e19 and more), or whose mean square and eps are so small that squares get lost (eps 0), is summed
+// again, each value times this: the sum then lies between 2^-64 and 2^126.  0: neither (and what is not a number stays so).
+__device__ inline float an_unit(float ss, int dim, float eps) { return ss == INFINITY ? 0x1p-96f : ss / (float)dim + eps < 0x1p-100f ? 0x1p96f : 0.f; }
+// y = (h * first) * inv * w of such a row; large ones in two factors, because their product may be below the normal numbers
+struct AnRange {
+    float first, inv;
+    __device__ AnRange(float unit, float ss, int dim, float eps) {
+        const bool large = unit < 1.0f;
+        first = large ? 0x1p-32f : unit;
+        inv = (large ? 0x1p-64f : 1.0f) / sqrtf(ss / (float)dim + eps * unit * unit);
+    }
+};
+
 // Rows of any length, at any address, of any type: a workgroup per row, an element a thread and step.  What a thread wrote of `sum`
 // it reads again itself, so `sum` may be x or the residual, and so may `out` where no sum is asked for.
 template <typename T, bool Q8>
@@ -64,15 +77,27 @@ __global__ __launch_bounds__(kAnThreads) void add_norm_kernel(void *out_, T *y_s
         if (sum) Elem<T>::st(sum, base + i, h);
         ss += h * h;
     }
-    const float inv = 1.0f / sqrtf(an_sum(ss, red) / (float)dim + eps);
+    ss = an_sum(ss, red);
+    float first = 1.0f, inv = 1.0f / sqrtf(ss / (float)dim + eps);
+    if (const float unit = an_unit(ss, dim, eps); unit != 0.f) {  // (all threads alike)
+        ss = 0.f;
+        for (int i = threadIdx.x; i < dim; i += kAnThreads) {
+            const float h = again(i) * unit;
+            ss += h * h;
+        }
+        const AnRange range(unit, an_sum(ss, red), dim, eps);
+        first = range.first;
+        inv = range.inv;
+    }
+    auto y = [&](int i) { return ((again(i) * first) * inv) * Elem<T>::ld(w, i); };
     if constexpr (!Q8) {
-        for (int i = threadIdx.x; i < dim; i += kAnThreads) Elem<T>::st((T *)out_, base + i, (again(i) * inv) * Elem<T>::ld(w, i));
+        for (int i = threadIdx.x; i < dim; i += kAnThreads) Elem<T>::st((T *)out_, base + i, y(i));
     } else {
         __shared__ uint32_t peak[4];
         uint32_t amax = 0;
-        for (int i = threadIdx.x; i < dim; i += kAnThreads) amax = max(amax, an_bits((again(i) * inv) * Elem<T>::ld(w, i)));
+        for (int i = threadIdx.x; i < dim; i += kAnThreads) amax = max(amax, an_bits(y(i)));
         const AnStep step(an_max(amax, peak));
-        for (int i = threadIdx.x; i < dim; i += kAnThreads) ((int8_t *)out_)[base + i] = (int8_t)step.code((again(i) * inv) * Elem<T>::ld(w, i));
+        for (int i = threadIdx.x; i < dim; i += kAnThreads) ((int8_t *)out_)[base + i] = (int8_t)step.code(y(i));
         if (threadIdx.x == 0) Elem<T>::st(y_scale, blockIdx.x, step.step);
     }
 }
@@ -145,7 +170,28 @@ __global__ __launch_bounds__(64 * W) void add_norm_vec_kernel(void *out_, const 
 #pragma unroll
         for (int i = 0; i < 8; i++) ss += f[i] * f[i];
     }
-    const float inv = 1.0f / sqrtf(an_row_sum<W>(ss, red) / (float)dim + eps);
+    ss = an_row_sum<W>(ss, red);
+    float inv = 1.0f / sqrtf(ss / (float)dim + eps);
+    if constexpr (std::is_same<T, bf16_t>::value) {  // (fp16 values have squares between)
+        if (const float unit = an_unit(ss, dim, eps); unit != 0.f) {  // (all threads alike)
+            auto times = [&](float by, bool keep) {
+                float sum_ = 0.f;
+#pragma unroll
+                for (int q = 0; q < NCH; q++) {
+                    float f[8];
+                    widen8<T>(v[q], f);
+#pragma unroll
+                    for (int i = 0; i < 8; i++) sum_ += (f[i] *= by) * f[i];
+                    if (keep) v[q] = U4{pack2<T>(f[0], f[1]), pack2<T>(f[2], f[3]), pack2<T>(f[4], f[5]), pack2<T>(f[6], f[7])};
+                }
+                return sum_;
+            };
+            __syncthreads();
+            const AnRange range(unit, an_row_sum<W>(times(unit, false), red), dim, eps);
+            times(range.first, true);  // (a power of two; of a large row, what has no bf16 number is nothing beside the rest)
+            inv = range.inv;
+        }
+    }
     if constexpr (!Q8) {
 #pragma unroll
         for (int q = 0; q < NCH; q++) {
