@@ -390,7 +390,7 @@ def _int4_shape(wq, scale, zero):
         raise MynnError("4-bit weights: wq %s and scale %s have to be matrices" % (tuple(wq.shape), tuple(scale.shape)))
     N, half = wq.shape
     groups = scale.shape[1]
-    if scale.shape[0] != N or groups < 1 or half < 1 or 2 * half % groups or N >= 1 << 31 or wq.dtype != _torch.uint8 or (
+    if scale.shape[0] != N or groups < 1 or half < 1 or 2 * half % groups or N >= 1 << 31 or half >= 1 << 30 or wq.dtype != _torch.uint8 or (
             zero is not None and (zero.shape != scale.shape or zero.dtype != _torch.uint8)):
         raise MynnError("4-bit weights: wq %s %s, scale %s, zero %s do not fit together" % (
             tuple(wq.shape), wq.dtype, tuple(scale.shape), None if zero is None else (tuple(zero.shape), zero.dtype)))
@@ -1164,6 +1164,8 @@ def quantize_int4_groups(w_f32, group, scale_dt, symmetric=True):
 
     w = np.ascontiguousarray(np.asarray(w_f32, np.float32))
     rows, cols = w.shape
+    if not 0 < int(group) < 1 << 31:  # (the library's is an int: what is left of a larger one would not be what the arrays below are made for)
+        raise MynnError("quantize_int4_groups: group=%d (32, 64 or a multiple of 128)" % group)
     q = np.empty((rows, cols // 2), np.uint8)
     s = np.empty((rows, max(cols // max(int(group), 1), 1)), np.uint16)
     z = None if symmetric else np.empty(s.shape, np.uint8)
