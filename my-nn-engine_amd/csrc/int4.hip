@@ -19,7 +19,7 @@ constexpr int kCus = 256;
 // 12.3 and 17).  Up to eight rows are always streamed (8 rows of 4096 x 14336 18).
 static bool int4_streams(const Int4Args &a) {
     const int rows = a.M <= 8 ? 1 : a.M <= 16 ? 4096 : a.M <= 32 ? 2048 : 0;
-    return (rows == 1 || a.K <= (a.group == 32 ? rows / 2 : rows)) && a.K % 128 == 0 && a.N >= 16 && (size_t)8 * a.K < 1u << 31;
+    return (rows == 1 || a.K <= (a.group == 32 ? rows / 2 : rows)) && a.K % 128 == 0 && a.N >= 16;
 }
 
 // room for `bytes` of LDS a workgroup, asked for once a kernel and device (done: the devices' bits)
