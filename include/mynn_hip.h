@@ -19,7 +19,7 @@
  * configuration as an argument and touches nothing global); (b) the scratch memory of the entry
  * points that need some and are not given any: `mynn_dequant_matmul` (M >= 2), `mynn_quantized_matmul`
  * (M >= 3), `mynn_attention` (a cache split over workgroups), `mynn_attention_streaming` and the products with 4-bit weights
- * (more than 8 rows).  Each of these groups keeps one grown-on-demand block PER STREAM, locked until the call's launches are
+ * (where `mynn_matmul_int4_workspace_bytes` is not 0).  Each of these groups keeps one grown-on-demand block PER STREAM, locked until the call's launches are
  * made, so calls on different streams never share one and several host threads may call on one stream.
  * Growing synchronises that stream and cannot happen while the stream is being captured: a captured call
  * that needs a larger block than there is fails with MYNN_ERR_STATE (make it once before the capture).
@@ -141,8 +141,10 @@ int mynn_quantized_matmul(void *out, int32_t *acc_out, const int8_t *lhs, const 
  *   w[n,k] = scale[n, k/group] * (wq[n,k] - zero[n, k/group]).
  * A group's sum meets the scale once, in f32; one rounding at the store.  It runs over the codes' differences, which are exact.  An
  * infinity or a NaN of act goes where the formula takes it, to its own row of out, and one of scale to its own column; the other values keep
- * their bits.  K up to 2^22, M and N to 2^30.
- * Where the tiles of more than 8 rows leave the device idle, the f32 sums run over several ranges of K, added in their order; their
+ * their bits.  K up to 2^22, M and N to 2^30, and no more than 2^23 - 1 tiles of 128 x 256 values of out: more are MYNN_ERR_UNSUPPORTED.
+ * Few rows (up to 8, to 16 where K <= 4096, to 32 where K <= 2048, half as long in groups of 32) are streamed where K is a multiple of 128 and N
+ * at least 16: one launch, no memory.  bf16 rows whose values lie more than 31 binades apart take another pass there (1 x 28672 x 4096: 15 us, 32).
+ * All others go in tiles.  Where those leave the device idle, the f32 sums run over several ranges of K, added in their order; their
  * number is a function of M, N, K and the group alone, and every form of a call gives the same bits.  The ranges' sums need
  * mynn_matmul_int4_workspace_bytes(...) bytes (0: no ranges): the _ws forms take them from the caller (16-byte aligned;
  * nothing global is touched, and calls whose workspaces differ may overlap), the others from a block of the stream's; while being

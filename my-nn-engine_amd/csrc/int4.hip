@@ -15,8 +15,10 @@ namespace mynn {
 constexpr int kCus = 256;
 
 // Few rows, of whole slices of 128 columns, for which eight waves hold the activations of all of K: more rows would be read several times over
-// (4096 x 14336, 16 rows, us: 40 this way, 20 as tiles; 4096 x 4096 12.8 against 14.9, 28672 x 4096 27.6 and 26.8, 24 rows of 11264 x 2048
-// 12.3 and 17).  Up to eight rows are always streamed (8 rows of 4096 x 14336 18).
+// (4096 x 14336, 16 rows, us: 40 this way, 17 as tiles).  Up to eight rows are always streamed (8 rows of 4096 x 14336 18).  From nine on it is not the
+// faster form everywhere (us, this way and as tiles: fp16, 16 rows of 2560 x 2048 7.1 and 9.1, 11264 x 2048 12.9 and 12.6, 28672 x 4096 27 and 25.6, 4096 x
+// 4096 12.6 and 9.8; 24 rows of 2560 x 2048 8.5 and 9.4, 11264 x 2048 11.9 and 13.2; 32 rows of 32000 x 2048 19.6 and 15.1), but the one that
+// needs no workspace and one launch, captured too.
 static bool int4_streams(const Int4Args &a) {
     const int rows = a.M <= 8 ? 1 : a.M <= 16 ? 4096 : a.M <= 32 ? 2048 : 0;
     return (rows == 1 || a.K <= (a.group == 32 ? rows / 2 : rows)) && a.K % 128 == 0 && a.N >= 16;
@@ -57,7 +59,7 @@ template <typename T, bool I8, int FL> static int int4_stream(const Int4Args &a,
     };
     using std::integral_constant;
     // (P, D): units of 128 S columns of a wave's share, tiles in flight.  Larger shares where eight waves do not cover K otherwise (4096 x 14336, us,
-    // four rows: 14.4 -> 12.5, eight 19.7 -> 18.1; elsewhere slower: 28672 x 4096, one row 14.1 -> 20.6).
+    // four rows: 14.4 -> 12.1, eight 19.4 -> 17.6; elsewhere slower: 28672 x 4096, one row 14 -> 21).
     auto shares = [&](auto mp) {
         constexpr int MP = decltype(mp)::value;
         if constexpr (FL > 1) {
@@ -76,8 +78,8 @@ template <typename T, bool I8, int FL> static int int4_stream(const Int4Args &a,
 }
 
 // Heights of the row tiles, in blocks of 32 rows: four as often as they go and the rest in a short tile, or all (but for one block) alike, by
-// how long the last compute unit is busy.  A tile of h blocks takes h + 1.5 units, of int8 h + 2.2 (one round of K = 4096, us: 46, 58,
-// 80, 104 for one to four blocks of fp16, 40, 48, 60, 75 of int8).
+// how long the last compute unit is busy.  A tile of h blocks takes some h + 1.5 units, of int8 h + 2.2 (one round of K = 4096, us: 44, 54,
+// 69, 90 for one to four blocks of fp16, 42, 51, 61, 68 of int8).
 static Int4Rows int4_row_tiles(int M, int columns, double fixed, int most) {
     const int blocks = (M + 31) / 32;
     auto busy = [&](const Int4Rows &r) {

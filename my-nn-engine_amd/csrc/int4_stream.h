@@ -5,7 +5,8 @@
 // those with a = b are the product's.  A slice is 128 columns, so an instruction's operands cover 128 S columns (with one row 2048: a kilobyte
 // of one weight row, 64 bytes a slice, 16 a lane), the wave's activations stay in 16 registers for each 128 S columns of its share of K
 // for all the weight rows it takes, and a tile asks for its codes, scales and zero points alone.  (With the activations loaded again for every 16 weight
-// rows, four loads for each one of weights, 128256 x 4096 took 92 us for one row; now 50, 5.4 TB/s.)
+// rows, four loads for each one of weights, 128256 x 4096 took 92 us for one row; now 48 to 49, 5.6 TB/s, part of
+// it from the 256 MB cache.)
 //
 // From nine rows on MP is 16: one slice, MT tiles of 16 rows, nothing to be summed inside a wave.
 //

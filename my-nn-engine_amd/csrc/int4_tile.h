@@ -11,7 +11,7 @@
 //
 // What bounds it.  Tall tiles: of a piece (128 rows x 256 columns, 2.2 us in rounds that fill the device) the MFMAs alone are 1.6; the rest is what the
 // vector operations (12 for eight codes in fp16, 19 in bf16, 9 to int8; 64 sums to scale; a wave's seven loads) do not hide behind them.  2048 x 28672 x
-// 4096 fp16 501 - 514 us, 0.95 PFLOP/s; 128 x 65536 x 4096 of int8 66 us, 1.04 POP/s.  Short ones: the steps of a piece one after the other, 0.65 us
+// 4096 fp16 501 - 514 us, 0.95 PFLOP/s; 128 x 65536 x 4096 of int8 66 - 68 us, 1.02 POP/s.  Short ones: the steps of a piece one after the other, 0.65 us
 // with 32 rows, 0.85 with 64 (its barrier and its reads from LDS are half of that; read a piece ahead they cost as much elsewhere).
 #pragma once
 #include "int4_codes.h"
