@@ -121,7 +121,8 @@ def _quantize4(x, group, dtype):
     """rows [.., D] of 32-bit numbers -> (codes [.., D/2], scales [.., D/group], zero points like the scales)"""
     v = x.reshape(*x.shape[:-1], x.shape[-1] // group, group)
     lo, hi = v.amin(-1).clamp_max(0.0), v.amax(-1).clamp_min(0.0)
-    s = (hi / 15.0 - lo / 15.0).to(dtype)
+    fifteen = torch.full_like(hi, 15.0)  # (by a number, a tensor is multiplied with its rounded reciprocal)
+    s = (hi / fifteen - lo / fifteen).to(dtype)
     s = torch.where(s == 0, torch.ones_like(s), s)
     z = _round(-lo / s.float()).clamp_max(15.0)
     c = (_round(v / s.float()[..., None]) + z[..., None]).clamp(0.0, 15.0).to(torch.uint8).reshape(x.shape)
@@ -223,7 +224,7 @@ def _plain_append(s):
         x = x.float()
         if s["bits"] == 8:
             peak = x.abs().amax(-1, keepdim=True)
-            y = x * torch.where(peak == 0, torch.zeros_like(peak), 127.0 / peak)
+            y = x * torch.where(peak == 0, torch.zeros_like(peak), torch.full_like(peak, 127.0) / peak)
             codes, scale = (y + torch.where(y >= 0, 0.5, -0.5)).trunc().clamp(-128, 127).to(torch.int8), (peak * (1.0 / 127.0)).to(dtype)
             s["pools"][side][put], s["pools"][2 + side][put] = codes, scale[..., 0]
             x = codes.float() * scale.float()
