@@ -270,6 +270,59 @@ const int32_t *mynn_kv_pages_table(const mynn_kv_pages *pages);          /* devi
 int mynn_kv_pages_table_host(const mynn_kv_pages *pages, int32_t *out);  /* the same, copied to host memory */
 int mynn_kv_pages_destroy(mynn_kv_pages *pages);
 
+/* Sequences of different lengths over a paged cache of 16, 8 or 4 bits.  No counterpart in the reference.
+ * The pools of a cache, for keys and for values, as mynn_attention_paged has them: kv_bits 16: [n_pages, Hkv, page_rows, D] in
+ * dtype; 8: int8 codes, scales [n_pages, Hkv, page_rows] in dtype; 4: codes uint8 [n_pages, Hkv, page_rows, D/2] (the even column in
+ * the low four bits), scales [n_pages, Hkv, page_rows, D/group] in dtype and zero points uint8 like the scales (their low four
+ * bits): a value is scale * (code - zero).  All 16-byte aligned; head_dim 64 or 128, group 32, 64 or 128 and at most head_dim, dtype
+ * MYNN_F16 or MYNN_BF16.  page_table: device int32 [B, pages_per_seq]; a page number outside [0, n_pages) (an unmapped page is
+ * -1) is a page that is not there.  past_lens: device int32 [B], the rows of each sequence in the cache before this step;
+ * new_lens: device int32 [B] or NULL, how many of the call's S tokens are the sequence's own (0 .. S; NULL: all): token i
+ * of sequence b is cache row past_lens[b] + i.  Both are read on the device: a captured call follows them.
+ *
+ * RoPE of q and k (as mynn_rope), and k and v to the cache: in 16 bits as they are, in 8 by the rule of
+ * mynn_quantizing_kvcache_update, in 4 by that of mynn_quantize_int4_groups (of the row in dtype; a group with a value that is
+ * not finite gets the scale NaN).  q [B,Hq,S,D], k, v [B,Hkv,S,D] at any strides (strides: host int64 [9], in elements: sequence, head
+ * and row of q, of k, of v; a row's values lie together); q_out [B,Hq,S,D] contiguous, 16-byte aligned, and may be q where
+ * q lies so.  q and q_out NULL: k and v alone.  cos, sin [table_rows, D]; position: device int64 [B,S], the table row of each token,
+ * or NULL for its cache row.  A token whose cache row or table row does not exist, and every token from new_lens on, is not
+ * appended and its q_out row is zeros; what the cache holds besides the appended rows stays as it is.  No two rows of a call may be
+ * the same row of the cache.  k and v must not overlap the pools. */
+int mynn_rope_append_paged(void *q_out, const void *q, const void *k, const void *v, const int64_t *strides,
+                           const void *cos_t, const void *sin_t, int table_rows, const int64_t *position,
+                           void *k_pool, void *v_pool, void *k_scale_pool, void *v_scale_pool,
+                           uint8_t *k_zero_pool, uint8_t *v_zero_pool,
+                           const int32_t *page_table, int n_pages, int pages_per_seq, int page_rows,
+                           const int32_t *past_lens, const int32_t *new_lens, int B, int S,
+                           int num_q_heads, int num_kv_heads, int head_dim, int dtype, int kv_bits, int group,
+                           mynn_stream s);
+/* Rows of a cache as plain rows (of 8 and 4 bits: what they stand for, rounded to dtype): k_out, v_out [B,Hkv,S,D], either may be NULL;
+ * row i of sequence b is cache row first_rows[b] + i for i < n_rows[b] (device; NULL: S).  Rows that are not there are zeros. */
+int mynn_kv_rows_paged(void *k_out, void *v_out, const void *k_pool, const void *v_pool,
+                       const void *k_scale_pool, const void *v_scale_pool,
+                       const uint8_t *k_zero_pool, const uint8_t *v_zero_pool,
+                       const int32_t *page_table, int n_pages, int pages_per_seq, int page_rows,
+                       const int32_t *first_rows, const int32_t *n_rows, int B, int S,
+                       int num_kv_heads, int head_dim, int dtype, int kv_bits, int group, mynn_stream s);
+/* Attention over a cache of 4 bits.  Q, out [B,Hq,Sq,D] contiguous, 16-byte aligned; kv head = q head / (Hq/Hkv).  The Sq rows of
+ * a sequence are its newest tokens, which the cache holds already: row i sees the keys [0, past_lens[b] + i + 1) where is_causal,
+ * else all past_lens[b] + new_lens[b].  Keys on a page that is not there are left out.  A row that sees no key, and every row
+ * from new_lens on, is zeros.
+ * workspace: mynn_attention_paged_int4_workspace_bytes(...) bytes, 16-byte aligned (0: none needed).  counters: device int32
+ * [B * Hkv] that are zero, and are zero again behind the call, or NULL: with them the parts of a sequence that several workgroups
+ * share are joined inside the launch, without them by a second one; the results are the same bits.  Calls that may overlap
+ * need workspaces and counters of their own; nothing global is touched. */
+size_t mynn_attention_paged_int4_workspace_bytes(int B, int Sq, int pages_per_seq, int page_rows,
+                                                 int num_q_heads, int num_kv_heads, int head_dim);
+int mynn_attention_paged_int4(void *out, const void *Q, const uint8_t *k_pool, const uint8_t *v_pool,
+                              const void *k_scale_pool, const void *v_scale_pool,
+                              const uint8_t *k_zero_pool, const uint8_t *v_zero_pool,
+                              const int32_t *page_table, int n_pages, int pages_per_seq, int page_rows,
+                              float scale, int is_causal, int B, int Sq, const int32_t *past_lens,
+                              const int32_t *new_lens, int num_q_heads, int num_kv_heads, int head_dim,
+                              int dtype, int group, void *workspace, size_t workspace_bytes, int32_t *counters,
+                              mynn_stream s);
+
 /* KVCacheUpdate -- kvcache_update.cuh:6-26: cache[bh, offset+t, :] = new[bh, t, :] in place. */
 int mynn_kvcache_update(void *cache, const void *new_kv, int offset, int BH, int S_new,
                         int max_seq, int D, int dtype, mynn_stream s);

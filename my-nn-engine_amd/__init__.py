@@ -94,6 +94,11 @@ SIGNATURES = {
     "mynn_attention_paged_workspace_bytes": (_sz, [_i, _i, _i, _i, _i, _i, _i]),
     "mynn_attention_paged": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _f, _i, _i, _i, _i, _vp, _i, _i, _i, _i, _i, _i, _vp, _sz, _vp]),
     "mynn_kvcache_update_paged": (_i, [_vp, _vp, _i, _i, _i, _i, _i, _i, _vp, _i, _i, _vp]),
+    "mynn_rope_append_paged": (_i, [_vp, _vp, _vp, _vp, C.POINTER(_i64), _vp, _vp, _i, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _vp, _vp, _i, _i, _i, _i, _i, _i,
+                                    _i, _i, _vp]),
+    "mynn_kv_rows_paged": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _vp]),
+    "mynn_attention_paged_int4_workspace_bytes": (_sz, [_i, _i, _i, _i, _i, _i, _i]),
+    "mynn_attention_paged_int4": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _f, _i, _i, _i, _vp, _vp, _i, _i, _i, _i, _i, _vp, _sz, _vp, _vp]),
     "mynn_kv_pool_create": (_vp, [_i, _i]),
     "mynn_kv_pool_free_pages": (_i, [_vp]),
     "mynn_kv_pool_destroy": (_i, [_vp]),
@@ -545,9 +550,11 @@ class KvPool:
     def free_pages(self):
         return lib().mynn_kv_pool_free_pages(self.handle)
 
-    def buffers(self, n_layers, n_kv_heads, head_dim, dtype, fill=None, kv_int8=False):
+    def buffers(self, n_layers, n_kv_heads, head_dim, dtype, fill=None, kv_int8=False, kv_int4_group=0):
         """One (K pool, V pool) per layer, [n_pages, Hkv, page_rows, D] in `dtype`; kv_int8: (K codes, V codes, K scales,
-        V scales) with int8 code pools and scale pools [n_pages, Hkv, page_rows] in `dtype`."""
+        V scales) with int8 code pools and scale pools [n_pages, Hkv, page_rows] in `dtype`; kv_int4_group (32, 64 or 128): a cache of 4
+        bits, (K codes, V codes, K scales, V scales, K zero points, V zero points) with codes uint8 [n_pages, Hkv, page_rows, D/2],
+        scales [.., D/kv_int4_group] in `dtype` and zero points uint8 like them."""
         import torch
 
         shape = (self.n_pages, n_kv_heads, self.page_rows, head_dim)
@@ -555,6 +562,13 @@ class KvPool:
         def make(sh, dt):
             return torch.zeros(sh, dtype=dt, device="cuda") if fill is None else torch.full(sh, fill, dtype=dt, device="cuda")
 
+        if kv_int4_group:
+            if kv_int8 or kv_int4_group not in (32, 64, 128) or head_dim % kv_int4_group:
+                raise MynnError("kv_pool buffers: kv_int4_group=%s of head_dim %d (32, 64 or 128), kv_int8=%s" % (kv_int4_group, head_dim, kv_int8))
+            groups = shape[:3] + (head_dim // kv_int4_group,)
+            codes = shape[:3] + (head_dim // 2,)
+            return [(torch.zeros(codes, dtype=torch.uint8, device="cuda"), torch.zeros(codes, dtype=torch.uint8, device="cuda"), make(groups, dtype), make(groups, dtype),
+                     torch.zeros(groups, dtype=torch.uint8, device="cuda"), torch.zeros(groups, dtype=torch.uint8, device="cuda")) for _ in range(n_layers)]
         if kv_int8:
             return [(torch.zeros(shape, dtype=torch.int8, device="cuda"), torch.zeros(shape, dtype=torch.int8, device="cuda"),
                      make(shape[:3], dtype), make(shape[:3], dtype)) for _ in range(n_layers)]
@@ -631,6 +645,148 @@ def kvcache_update_paged(pool, new_kv, offset, table, page_rows):
     check(lib().mynn_kvcache_update_paged(_ptr(pool), _ptr(new_kv), int(offset), B, Hkv, S_new, D, _dt(new_kv), _ptr(table),
                                           table.shape[1], int(page_rows), _stream()))
     return pool
+
+
+class _Paged:
+    """The pools of a layer (KvPool.buffers) and a page table (KvPages, or a cuda int32 tensor [B, pages_per_seq]) as the calls for sequences of
+    different lengths take them; what does not fit together is refused here."""
+
+    def __init__(self, name, pools, table, past, new):
+        torch = _t()
+        pools = tuple(pools)
+        kinds = {2: (16, None), 4: (8, torch.int8), 6: (4, torch.uint8)}
+        if len(pools) not in kinds or not all(t.dim() >= 3 for t in pools):
+            raise MynnError("%s: %d pools (2 of 16 bits, 4 of an int8 cache, 6 of a cache of 4 bits)" % (name, len(pools)))
+        self.bits, codes = kinds[len(pools)]
+        k = pools[0]
+        self.n_pages, self.heads, self.rows = k.shape[:3]
+        self.dtype = k.dtype if self.bits == 16 else pools[2].dtype
+        self.dim = k.shape[-1] * (2 if self.bits == 4 else 1)
+        groups = pools[2].shape[-1] if self.bits == 4 else 1
+        self.group = self.dim // max(groups, 1) if self.bits == 4 else 0
+        lead = (self.n_pages, self.heads, self.rows)
+        shapes = {16: [(self.dim,)], 8: [(self.dim,), ()], 4: [(self.dim // 2,), (groups,), (groups,)]}[self.bits]
+        types = [codes or self.dtype, self.dtype, torch.uint8]
+        for n, t in enumerate(pools):
+            if k.dim() != 4 or tuple(t.shape) != lead + shapes[n // 2] or t.dtype != types[n // 2]:
+                raise MynnError("%s: pools %s do not fit together" % (name, [(tuple(t.shape), t.dtype) for t in pools]))
+        if self.dtype not in (torch.float16, torch.bfloat16) or (self.bits == 4 and (groups < 1 or self.dim % groups)):
+            raise MynnError("%s: pools %s (16-bit values or scales)" % (name, [(tuple(t.shape), t.dtype) for t in pools]))
+        if isinstance(table, KvPages):
+            if table.pool.page_rows != self.rows or table.pool.n_pages > self.n_pages:
+                raise MynnError("%s: pages of %d rows out of %d, pools of %d pages of %d" % (name, table.pool.page_rows, table.pool.n_pages, self.n_pages, self.rows))
+            self.batch, self.pages, self.table = table.batch, table.pages_per_seq, table.table_ptr
+            table = None
+        else:
+            if table.dim() != 2 or table.dtype != torch.int32:
+                raise MynnError("%s: page table %s %s (int32 [B, pages])" % (name, tuple(table.shape), table.dtype))
+            self.batch, self.pages = table.shape
+            self.table = _ptr(table)
+        for what in (past, new):
+            if what is not None and (what.dtype != torch.int32 or tuple(what.shape) != (self.batch,)):
+                raise MynnError("%s: lengths %s %s (int32 [%d])" % (name, tuple(what.shape), what.dtype, self.batch))
+        _on_current_device(name, *pools, table, past, new)
+        self.past, self.new = _ptr(past), _ptr(new)
+        self.ptrs = [_ptr(t) for t in pools] + [None] * (6 - len(pools))
+        self.where = [self.table, self.n_pages, self.pages, self.rows]
+
+    def rows_of(self, name, x, heads=None):
+        """(S) of [B, H, S, D] rows in the cache's type"""
+        if x.dim() != 4 or x.shape[0] != self.batch or x.shape[3] != self.dim or x.dtype != self.dtype or (heads is not None and x.shape[1] != heads) or x.shape[2] >= 1 << 31:
+            raise MynnError("%s: rows %s %s over a cache of %d sequences, %d heads of %d, %s" % (
+                name, tuple(x.shape), x.dtype, self.batch, self.heads, self.dim, self.dtype))
+        return x.shape[2]
+
+
+def rope_append_paged(q, k, v, cos_t, sin_t, pools, table, past_lens, new_lens=None, positions=None, out=None):
+    """mynn_rope_append_paged: rotates q [B,Hq,S,D] (None: keys and values alone) and k [B,Hkv,S,D] and appends k, v to the pools (KvPool.buffers) from row
+    past_lens[b] (cuda int32 [B]) on; new_lens (cuda int32 [B]): how many of the S tokens are a sequence's own; positions (cuda int64 [B,S]): the
+    table rows, where they are not the cache rows.  q, k, v may be views (of the projection's rows, say) whose last dimension lies together.
+    Returns the rotated q, contiguous (out, where given)."""
+    torch = _t()
+    name = "rope_append_paged"
+    c = _Paged(name, pools, table, past_lens, new_lens)
+    S = c.rows_of(name, k, c.heads)
+    heads = 0 if q is None else q.shape[1]
+    if c.rows_of(name, v, c.heads) != S or (q is not None and c.rows_of(name, q) != S) or cos_t.dim() != 2 or sin_t.shape != cos_t.shape or cos_t.shape[1] != c.dim or (
+            cos_t.dtype != c.dtype or sin_t.dtype != c.dtype or cos_t.shape[0] >= 1 << 31):
+        raise MynnError("%s: q %s, k %s, v %s, tables %s %s do not fit together" % (
+            name, None if q is None else tuple(q.shape), tuple(k.shape), tuple(v.shape), tuple(cos_t.shape), tuple(sin_t.shape)))
+    if positions is not None and (positions.dtype != torch.int64 or tuple(positions.shape) != (c.batch, S)):
+        raise MynnError("%s: positions %s %s (int64 [%d, %d])" % (name, tuple(positions.shape), positions.dtype, c.batch, S))
+    strides = []
+    for x in (q, k, v):
+        if x is None:
+            strides += [0, 0, 0]
+            continue
+        if not x.is_cuda or x.stride(3) != 1:
+            raise MynnError("%s: rows whose values do not lie together, or on %s" % (name, x.device))
+        strides += [x.stride(d) if x.shape[d] > 1 else 0 for d in range(3)]
+    if q is None:
+        out = None
+    elif out is None:
+        out = q.new_empty(q.shape)
+    elif out.shape != q.shape or out.dtype != q.dtype:
+        raise MynnError("%s: out %s %s for q %s %s" % (name, tuple(out.shape), out.dtype, tuple(q.shape), q.dtype))
+    _on_current_device(name, q, k, v, cos_t, sin_t, positions, out)
+    check(lib().mynn_rope_append_paged(_ptr(out), None if q is None else q.data_ptr(), k.data_ptr(), v.data_ptr(), (_i64 * 9)(*strides), _ptr(cos_t), _ptr(sin_t),
+                                       cos_t.shape[0], _ptr(positions), *c.ptrs, *c.where, c.past, c.new, c.batch, S, max(heads, 1), c.heads, c.dim, _dt(k), c.bits,
+                                       c.group, _stream()))
+    return out
+
+
+def kv_rows_paged(pools, table, first_rows, n, n_rows=None):
+    """mynn_kv_rows_paged: (k, v) [B,Hkv,n,D], what the cache's rows first_rows[b] (cuda int32 [B]) .. stand for; zeros from n_rows[b] on"""
+    c = _Paged("kv_rows_paged", pools, table, first_rows, n_rows)
+    n = int(n)
+    if not 0 < n < 1 << 31:
+        raise MynnError("kv_rows_paged: %d rows" % n)
+    k = pools[0].new_empty((c.batch, c.heads, n, c.dim), dtype=c.dtype)
+    v = pools[0].new_empty((c.batch, c.heads, n, c.dim), dtype=c.dtype)
+    check(lib().mynn_kv_rows_paged(_ptr(k), _ptr(v), *c.ptrs, *c.where, c.past, c.new, c.batch, n, c.heads, c.dim, _codes[c.dtype], c.bits, c.group, _stream()))
+    return k, v
+
+
+def attention_paged_int4_workspace(q, pools, table):
+    """Memory for attention_paged_int4 on operands like these, to be kept from call to call (one for calls that may overlap each): its first words
+    are counters, zero here and zero again behind every call."""
+    B, Hq, Sq, D = q.shape
+    pages = table.pages_per_seq if isinstance(table, KvPages) else table.shape[1]
+    Hkv, rows = pools[0].shape[1:3]
+    need = lib().mynn_attention_paged_int4_workspace_bytes(B, Sq, pages, rows, Hq, Hkv, D)
+    return _t().zeros((_counter_bytes(B, Hkv) + need,), dtype=_torch.uint8, device=q.device)
+
+
+def _counter_bytes(B, Hkv):
+    return (4 * B * Hkv + 255) // 256 * 256
+
+
+def attention_paged_int4(q, pools, table, scale, past_lens, new_lens=None, is_causal=True, workspace=None, out=None):
+    """mynn_attention_paged_int4: q [B,Hq,Sq,D], the newest tokens of each sequence, over a cache of 4 bits (KvPool.buffers with kv_int4_group) that holds
+    their rows already (rope_append_paged with the same past_lens and new_lens).  workspace: attention_paged_int4_workspace(...), kept by
+    the caller; without one the call allocates its own, and takes a launch more where a sequence is shared by several workgroups."""
+    name = "attention_paged_int4"
+    c = _Paged(name, pools, table, past_lens, new_lens)
+    if c.bits != 4:
+        raise MynnError("%s: a cache of %d bits" % (name, c.bits))
+    Sq, Hq = c.rows_of(name, q), q.shape[1]
+    if out is None:
+        out = q.new_empty(q.shape)
+    elif out.shape != q.shape or out.dtype != q.dtype:
+        raise MynnError("%s: out %s %s for q %s %s" % (name, tuple(out.shape), out.dtype, tuple(q.shape), q.dtype))
+    _on_current_device(name, q, out, workspace)
+    need = lib().mynn_attention_paged_int4_workspace_bytes(c.batch, Sq, c.pages, c.rows, Hq, c.heads, c.dim)
+    counters, at = None, 0
+    if workspace is None:
+        workspace = q.new_empty((need,), dtype=_torch.uint8) if need else None
+    else:
+        at = _counter_bytes(c.batch, c.heads)
+        if workspace.dtype != _torch.uint8 or workspace.numel() < at + need:
+            raise MynnError("%s: a workspace of %d bytes, %d needed" % (name, workspace.numel(), at + need))
+        counters = _ptr(workspace)
+    check(lib().mynn_attention_paged_int4(_ptr(out), _ptr(q), *c.ptrs, *c.where, float(scale), int(is_causal), c.batch, Sq, c.past, c.new, Hq, c.heads, c.dim, _dt(q), c.group,
+                                          None if workspace is None else _ptr(workspace) + at, need, counters, _stream()))
+    return out
 
 
 def kvcache_update_streaming(cache, new_kv, offset, ring_sink, ring_window, ring_start):

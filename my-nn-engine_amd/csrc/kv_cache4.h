@@ -1,0 +1,59 @@
+// Paged caches as the operators for sequences of different lengths see them: which rows there are, where a row lies, and the 4-bit
+// form of a row (codes, scales and zero points of groups of columns, as the 4-bit weights have them).
+#pragma once
+#include "mynn_common.h"
+
+namespace mynn {
+
+// The pools of a cache and the page table of B sequences.  A page number outside [0, n_pages) stands for a page that is not there:
+// no address is made of it.
+struct PagedKv {
+    void *k, *v;              // T, int8 or pairs of 4-bit codes: [n_pages, Hkv, P, D]
+    void *k_scale, *v_scale;  // T: int8 [n_pages, Hkv, P], 4 bits [n_pages, Hkv, P, D / group]
+    uint8_t *k_zero, *v_zero;  // 4 bits: as the scales
+    const int32_t *table;     // [B, pages_per_seq]
+    const int32_t *past, *fresh;  // [B] rows in the cache before the S new ones, and how many of those there are (null: S)
+    int n_pages, pages_per_seq, page_shift, Hkv;
+};
+
+// A sequence: rows [0, past) were there before, [past, len) are new.  (An int holds every sum below: a past that no cache could have is cut off.)
+struct PagedSeq {
+    int past, fresh, len, cap;
+    __device__ PagedSeq(const PagedKv &c, int b, int S) {
+        cap = c.pages_per_seq << c.page_shift;
+        past = min(max(c.past[b], -S), cap);
+        fresh = c.fresh ? min(max(c.fresh[b], 0), S) : S;
+        len = fresh ? min(max(past + fresh, 0), cap) : 0;
+    }
+    // keys that query row i sees
+    __device__ int bound(int i, bool causal) const { return i >= fresh ? 0 : causal ? min(max(past + i + 1, 0), len) : len; }
+};
+
+// the page that row r of sequence b lies in, -1: none
+__device__ inline int paged_page(const PagedKv &c, int b, int r) {
+    const int page = c.table[(size_t)b * c.pages_per_seq + (r >> c.page_shift)];
+    return (unsigned)page < (unsigned)c.n_pages ? page : -1;
+}
+// ... and the index of its row for kv head h, in rows
+__device__ inline size_t paged_row(const PagedKv &c, int page, int h, int r) {
+    return (((size_t)page * c.Hkv + h) << c.page_shift) + (size_t)(r & ((1 << c.page_shift) - 1));
+}
+
+// The 4-bit form of a group of columns with least value lo <= 0 and largest hi >= 0 (zero among them: a value of zero stays zero):
+//   s = T(hi/15 - lo/15), z = round(-lo/s), code = round(x/s) + z in 0 .. 15, which stands for s * (code - z)
+// -- mynn_quantize_int4_groups for a row.  A group with a value that is not finite stands for NaN.
+template <typename T> struct Int4Row {
+    float s, z;
+    __device__ Int4Row(float lo, float hi, bool finite) {
+        s = Elem<T>::rnd(hi / 15.0f - lo / 15.0f);
+        if (s == 0.f) s = 1.f;
+        z = fminf(roundf(-lo / s), 15.f);
+        if (!finite) s = __builtin_nanf(""), z = 0.f;
+    }
+    __device__ uint32_t code(float x) const {
+        const float c = fminf(fmaxf(roundf(x / s) + z, 0.f), 15.f);
+        return c == c ? (uint32_t)c : 0u;
+    }
+};
+
+}  // namespace mynn
