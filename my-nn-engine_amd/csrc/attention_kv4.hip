@@ -1,19 +1,10 @@
 // Attention over a paged cache held in 4 bits, for sequences of different lengths.
-#include "kv_cache4.h"
-#include "mfma.h"
+#include "attention_kv4_stream.h"
 
 namespace mynn {
 
 int paged_kv_check(const char *who, const PagedKv &c, int page_rows, int kv_bits, int group, int D);
 int paged_shift(int page_rows);
-
-struct Kv4Args {
-    PagedKv c;
-    void *out;
-    const void *q;
-    float scale;
-    int causal, B, Sq, Hq;
-};
 
 // One wave for a query row of a head: 64 keys at a time, a key a lane; then a lane's dims over those keys.
 template <typename T, int D> __global__ __launch_bounds__(64) void attn_kv4_row_kernel(Kv4Args a, int group) {
@@ -67,12 +58,42 @@ template <typename T, int D> __global__ __launch_bounds__(64) void attn_kv4_row_
     for (int e = 0; e < D / 64; e++) Elem<T>::st((T *)a.out, line + lane + 64 * e, l == 0.f ? 0.f : o[e] / l);
 }
 
+static int kv4_cus() {
+    static int cus = 0;
+    if (!cus) {
+        int dev = 0, n = 0;
+        if (hipGetDevice(&dev) != hipSuccess || hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess) {
+            (void)hipGetLastError();
+            n = 256;
+        }
+        cus = n;
+    }
+    return cus;
+}
+static bool kv4_few_rows(int Hq, int Hkv, int Sq) { return (long)(Hq / Hkv) * Sq <= 16; }
+// workgroups of the form for few rows: as many as run at once, no more than there can be units
+static int kv4_stream_grid(int B, int Hkv, long rows) {
+    const long units = (long)B * Hkv * ((rows + kKv4Unit - 1) / kKv4Unit), most = 2l * kv4_cus();
+    return (int)(units < most ? units : most);
+}
+
+template <typename T, int D, int NG> static int kv4_stream_go(const Kv4Args &a, hipStream_t s) {
+    const int R = a.Hq / a.c.Hkv * a.Sq, tile = 32 * (D / 2 + 16), wave = tile > R * D * 4 ? tile : R * D * 4;
+    MYNN_LAUNCH((attn_kv4_stream_kernel<T, D, NG>), dim3(a.grid), dim3(kKv4Waves * 64), kKv4Waves * (wave + 128), s, a);
+    if (const int rc = launch_status("attn_kv4_stream_kernel")) return rc;
+    if (a.grid == a.B * a.c.Hkv && a.c.pages_per_seq << a.c.page_shift <= kKv4Unit) return 0;  // (a unit each: nothing is shared)
+    MYNN_LAUNCH((attn_kv4_join_kernel<T, D>), dim3(a.B * a.c.Hkv), dim3(256), 0, s, a);
+    return launch_status("attn_kv4_join_kernel");
+}
+
 }  // namespace mynn
 
 using namespace mynn;
 
 extern "C" size_t mynn_attention_paged_int4_workspace_bytes(int B, int Sq, int pages_per_seq, int page_rows, int num_q_heads, int num_kv_heads, int head_dim) {
-    return 0;
+    if (B <= 0 || Sq <= 0 || pages_per_seq <= 0 || page_rows <= 0 || num_kv_heads <= 0 || num_q_heads < num_kv_heads || !kv4_few_rows(num_q_heads, num_kv_heads, Sq)) return 0;
+    const size_t R = (size_t)(num_q_heads / num_kv_heads) * Sq;
+    return 2 * (size_t)kv4_stream_grid(B, num_kv_heads, (long)pages_per_seq * page_rows) * R * (head_dim + 4) * sizeof(float);
 }
 
 extern "C" int mynn_attention_paged_int4(void *out, const void *Q, const uint8_t *k_pool, const uint8_t *v_pool, const void *k_scale_pool, const void *v_scale_pool,
@@ -85,10 +106,27 @@ extern "C" int mynn_attention_paged_int4(void *out, const void *Q, const uint8_t
                  num_q_heads, num_kv_heads);
     Kv4Args a{{(void *)k_pool, (void *)v_pool, (void *)k_scale_pool, (void *)v_scale_pool, (uint8_t *)k_zero_pool, (uint8_t *)v_zero_pool, page_table, past_lens, new_lens,
                n_pages, pages_per_seq, 0, num_kv_heads},
-              out, Q, scale, is_causal, B, Sq, num_q_heads};
+              out, Q, scale, is_causal, B, Sq, num_q_heads, nullptr, nullptr, nullptr, 0};
     if (const int rc = paged_kv_check(who, a.c, page_rows, 4, group, head_dim)) return rc;
     a.c.page_shift = paged_shift(page_rows);
     MYNN_REQUIRE((long)num_q_heads * Sq < 1l << 31 && B <= 65535, MYNN_ERR_UNSUPPORTED, "%s: B=%d Sq=%d heads %d", who, B, Sq, num_q_heads);
+    if (kv4_few_rows(num_q_heads, num_kv_heads, Sq)) {
+        const size_t need = mynn_attention_paged_int4_workspace_bytes(B, Sq, pages_per_seq, page_rows, num_q_heads, num_kv_heads, head_dim);
+        MYNN_REQUIRE(need == 0 || (workspace && aligned16(workspace) && workspace_bytes >= need), MYNN_ERR_INVALID, "%s: %zu bytes of workspace, %zu needed", who,
+                     workspace_bytes, need);
+        MYNN_REQUIRE((long)B * num_kv_heads * (((long)pages_per_seq * page_rows + kKv4Unit - 1) / kKv4Unit) < 1l << 30, MYNN_ERR_UNSUPPORTED,
+                     "%s: %d sequences of %d heads of %ld rows", who, B, num_kv_heads, (long)pages_per_seq * page_rows);
+        a.grid = kv4_stream_grid(B, num_kv_heads, (long)pages_per_seq * page_rows);
+        const size_t R = (size_t)(num_q_heads / num_kv_heads) * Sq;
+        a.part_o = (float *)workspace;
+        a.part_ml = a.part_o + 2 * (size_t)a.grid * R * head_dim;
+        a.counters = counters;
+        return dispatch_dtype16(dtype, [&](auto *t) {
+            using T = std::remove_pointer_t<decltype(t)>;
+            if (head_dim == 64) return group == 64 ? kv4_stream_go<T, 64, 1>(a, as_stream(s)) : kv4_stream_go<T, 64, 2>(a, as_stream(s));
+            return group == 128 ? kv4_stream_go<T, 128, 1>(a, as_stream(s)) : group == 64 ? kv4_stream_go<T, 128, 2>(a, as_stream(s)) : kv4_stream_go<T, 128, 4>(a, as_stream(s));
+        });
+    }
     return dispatch_dtype16(dtype, [&](auto *t) {
         using T = std::remove_pointer_t<decltype(t)>;
         const dim3 grid(num_q_heads * Sq, B);
