@@ -1,62 +1,13 @@
 // Attention over a paged cache held in 4 bits, for sequences of different lengths.
 #include "attention_kv4_stream.h"
+#include "attention_kv4_tile.h"
 
 namespace mynn {
 
 int paged_kv_check(const char *who, const PagedKv &c, int page_rows, int kv_bits, int group, int D);
 int paged_shift(int page_rows);
 
-// One wave for a query row of a head: 64 keys at a time, a key a lane; then a lane's dims over those keys.
-template <typename T, int D> __global__ __launch_bounds__(64) void attn_kv4_row_kernel(Kv4Args a, int group) {
-    __shared__ float q_s[D], p_s[64];
-    __shared__ size_t r_s[64];
-    const int lane = threadIdx.x, i = blockIdx.x % a.Sq, head = blockIdx.x / a.Sq, b = blockIdx.y;
-    const int h = head / (a.Hq / a.c.Hkv), groups = D / group;
-    const PagedSeq seq(a.c, b, a.Sq);
-    const int bound = seq.bound(i, a.causal);
-    const size_t line = (((size_t)b * a.Hq + head) * a.Sq + i) * D;
-    for (int d = lane; d < D; d += 64) q_s[d] = Elem<T>::ld((const T *)a.q, line + d);
-    float m = -INFINITY, l = 0.f, o[D / 64] = {};
-    for (int k0 = 0; k0 < bound; k0 += 64) {
-        __syncthreads();
-        const int key = k0 + lane, page = key < bound ? paged_page(a.c, b, key) : -1;
-        const size_t r = page >= 0 ? paged_row(a.c, page, h, key) : 0;
-        float s = -INFINITY;
-        if (page >= 0) {
-            s = 0.f;
-            for (int g = 0; g < groups; g++) {
-                float x = 0.f;
-                const float z = (float)(a.c.k_zero[r * groups + g] & 15);
-                for (int d = g * group; d < (g + 1) * group; d++) {
-                    const uint32_t w = ((const uint8_t *)a.c.k)[r * (D / 2) + d / 2];
-                    x = fmaf(q_s[d], (float)(d & 1 ? w >> 4 : w & 15u) - z, x);
-                }
-                s = fmaf(x, Elem<T>::ld((const T *)a.c.k_scale, r * groups + g), s);
-            }
-            s *= a.scale;
-        }
-        const float mn = fmaxf(m, wave_max(s)), ref = mn == -INFINITY ? 0.f : mn;
-        const float p = page >= 0 ? expf(s - ref) : 0.f, corr = expf(m - ref);
-        m = mn;
-        l = l * corr + wave_sum(p);
-        p_s[lane] = p;
-        r_s[lane] = page >= 0 ? r : ~(size_t)0;
-        __syncthreads();
-        for (int e = 0; e < D / 64; e++) {
-            const int d = lane + 64 * e, g = d / group;
-            float x = 0.f;
-            for (int k = 0; k < 64; k++) {
-                const size_t rk = r_s[k];
-                if (rk == ~(size_t)0) continue;
-                const uint32_t w = ((const uint8_t *)a.c.v)[rk * (D / 2) + d / 2];
-                const float z = (float)(a.c.v_zero[rk * groups + g] & 15), sc = Elem<T>::ld((const T *)a.c.v_scale, rk * groups + g);
-                x = fmaf(p_s[k], ((float)(d & 1 ? w >> 4 : w & 15u) - z) * sc, x);
-            }
-            o[e] = o[e] * corr + x;
-        }
-    }
-    for (int e = 0; e < D / 64; e++) Elem<T>::st((T *)a.out, line + lane + 64 * e, l == 0.f ? 0.f : o[e] / l);
-}
+template <int N> using Int = std::integral_constant<int, N>;
 
 static int kv4_cus() {
     static int cus = 0;
@@ -86,13 +37,49 @@ template <typename T, int D, int NG> static int kv4_stream_go(const Kv4Args &a, 
     return launch_status("attn_kv4_join_kernel");
 }
 
+// Rows of a workgroup of the form for many rows, and the ranges that its keys come in where blocks of rows leave the device idle.
+struct Kv4TilePlan {
+    int rows, blocks, ranges;
+};
+static Kv4TilePlan kv4_tile_plan(int B, int Sq, int Hq, int Hkv, long rows) {
+    const long R = (long)(Hq / Hkv) * Sq;
+    Kv4TilePlan p;
+    p.rows = R <= 64 ? 64 : 128;
+    p.blocks = (int)((R + p.rows - 1) / p.rows);
+    const long wgs = (long)B * Hkv * p.blocks, most = (rows + 255) / 256, want = 2l * kv4_cus() / wgs;
+    p.ranges = (int)(want < 1 ? 1 : want > most ? most : want);
+    return p;
+}
+
+template <typename T, int D, int NG, int QW, int KW> static int kv4_tile_launch(const Kv4Args &a, const Kv4TilePlan &p, hipStream_t s) {
+    using Block = Kv4Block<D, NG, QW, KW, 64>;
+    static bool set = false;
+    if (!set && Block::LDS > 64 * 1024) {
+        MYNN_HIP(hipFuncSetAttribute((const void *)attn_kv4_tile_kernel<T, D, NG, QW, KW, 64>, hipFuncAttributeMaxDynamicSharedMemorySize, Block::LDS));
+        set = true;
+    }
+    MYNN_LAUNCH((attn_kv4_tile_kernel<T, D, NG, QW, KW, 64>), dim3(a.B * a.c.Hkv, p.blocks, p.ranges), dim3(Block::THREADS), Block::LDS, s, a);
+    return launch_status("attn_kv4_tile_kernel");
+}
+template <typename T, int D, int NG> static int kv4_tile_go(const Kv4Args &a, const Kv4TilePlan &p, hipStream_t s) {
+    const int rc = p.rows == 64 ? kv4_tile_launch<T, D, NG, 2, 2>(a, p, s) : kv4_tile_launch<T, D, NG, 4, 1>(a, p, s);
+    if (rc || p.ranges == 1) return rc;
+    const size_t threads = (size_t)a.B * a.Hq * a.Sq * (D / 4);
+    MYNN_LAUNCH((attn_kv4_ranges_kernel<T, D>), dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, s, a, p.ranges, p.rows);
+    return launch_status("attn_kv4_ranges_kernel");
+}
+
 }  // namespace mynn
 
 using namespace mynn;
 
 extern "C" size_t mynn_attention_paged_int4_workspace_bytes(int B, int Sq, int pages_per_seq, int page_rows, int num_q_heads, int num_kv_heads, int head_dim) {
-    if (B <= 0 || Sq <= 0 || pages_per_seq <= 0 || page_rows <= 0 || num_kv_heads <= 0 || num_q_heads < num_kv_heads || !kv4_few_rows(num_q_heads, num_kv_heads, Sq)) return 0;
+    if (B <= 0 || Sq <= 0 || pages_per_seq <= 0 || page_rows <= 0 || num_kv_heads <= 0 || num_q_heads < num_kv_heads) return 0;
     const size_t R = (size_t)(num_q_heads / num_kv_heads) * Sq;
+    if (!kv4_few_rows(num_q_heads, num_kv_heads, Sq)) {
+        const int ranges = kv4_tile_plan(B, Sq, num_q_heads, num_kv_heads, (long)pages_per_seq * page_rows).ranges;
+        return ranges == 1 ? 0 : (size_t)ranges * B * num_kv_heads * R * (head_dim + 4) * sizeof(float);
+    }
     return 2 * (size_t)kv4_stream_grid(B, num_kv_heads, (long)pages_per_seq * page_rows) * R * (head_dim + 4) * sizeof(float);
 }
 
@@ -109,29 +96,29 @@ extern "C" int mynn_attention_paged_int4(void *out, const void *Q, const uint8_t
               out, Q, scale, is_causal, B, Sq, num_q_heads, nullptr, nullptr, nullptr, 0};
     if (const int rc = paged_kv_check(who, a.c, page_rows, 4, group, head_dim)) return rc;
     a.c.page_shift = paged_shift(page_rows);
-    MYNN_REQUIRE((long)num_q_heads * Sq < 1l << 31 && B <= 65535, MYNN_ERR_UNSUPPORTED, "%s: B=%d Sq=%d heads %d", who, B, Sq, num_q_heads);
+    MYNN_REQUIRE((long)num_q_heads * Sq < 1l << 30 && (long)B * num_kv_heads < 1l << 30, MYNN_ERR_UNSUPPORTED, "%s: B=%d Sq=%d heads %d", who, B, Sq, num_q_heads);
+    const long rows = (long)pages_per_seq * page_rows;
+    const size_t need = mynn_attention_paged_int4_workspace_bytes(B, Sq, pages_per_seq, page_rows, num_q_heads, num_kv_heads, head_dim);
+    MYNN_REQUIRE(need == 0 || (workspace && aligned16(workspace) && workspace_bytes >= need), MYNN_ERR_INVALID, "%s: %zu bytes of workspace, %zu needed", who, workspace_bytes,
+                 need);
+    const size_t R = (size_t)(num_q_heads / num_kv_heads) * Sq;
+    a.part_o = (float *)workspace;
+    auto pick = [&](auto &&go) {
+        return dispatch_dtype16(dtype, [&](auto *t) {
+            if (head_dim == 64) return group == 64 ? go(t, Int<64>{}, Int<1>{}) : go(t, Int<64>{}, Int<2>{});
+            return group == 128 ? go(t, Int<128>{}, Int<1>{}) : group == 64 ? go(t, Int<128>{}, Int<2>{}) : go(t, Int<128>{}, Int<4>{});
+        });
+    };
     if (kv4_few_rows(num_q_heads, num_kv_heads, Sq)) {
-        const size_t need = mynn_attention_paged_int4_workspace_bytes(B, Sq, pages_per_seq, page_rows, num_q_heads, num_kv_heads, head_dim);
-        MYNN_REQUIRE(need == 0 || (workspace && aligned16(workspace) && workspace_bytes >= need), MYNN_ERR_INVALID, "%s: %zu bytes of workspace, %zu needed", who,
-                     workspace_bytes, need);
-        MYNN_REQUIRE((long)B * num_kv_heads * (((long)pages_per_seq * page_rows + kKv4Unit - 1) / kKv4Unit) < 1l << 30, MYNN_ERR_UNSUPPORTED,
-                     "%s: %d sequences of %d heads of %ld rows", who, B, num_kv_heads, (long)pages_per_seq * page_rows);
-        a.grid = kv4_stream_grid(B, num_kv_heads, (long)pages_per_seq * page_rows);
-        const size_t R = (size_t)(num_q_heads / num_kv_heads) * Sq;
-        a.part_o = (float *)workspace;
+        MYNN_REQUIRE((long)B * num_kv_heads * ((rows + kKv4Unit - 1) / kKv4Unit) < 1l << 30, MYNN_ERR_UNSUPPORTED, "%s: %d sequences of %d heads of %ld rows", who, B, num_kv_heads,
+                     rows);
+        a.grid = kv4_stream_grid(B, num_kv_heads, rows);
         a.part_ml = a.part_o + 2 * (size_t)a.grid * R * head_dim;
         a.counters = counters;
-        return dispatch_dtype16(dtype, [&](auto *t) {
-            using T = std::remove_pointer_t<decltype(t)>;
-            if (head_dim == 64) return group == 64 ? kv4_stream_go<T, 64, 1>(a, as_stream(s)) : kv4_stream_go<T, 64, 2>(a, as_stream(s));
-            return group == 128 ? kv4_stream_go<T, 128, 1>(a, as_stream(s)) : group == 64 ? kv4_stream_go<T, 128, 2>(a, as_stream(s)) : kv4_stream_go<T, 128, 4>(a, as_stream(s));
-        });
+        return pick([&](auto *t, auto d, auto n) { return kv4_stream_go<std::remove_pointer_t<decltype(t)>, decltype(d)::value, decltype(n)::value>(a, as_stream(s)); });
     }
-    return dispatch_dtype16(dtype, [&](auto *t) {
-        using T = std::remove_pointer_t<decltype(t)>;
-        const dim3 grid(num_q_heads * Sq, B);
-        if (head_dim == 64) MYNN_LAUNCH((attn_kv4_row_kernel<T, 64>), grid, dim3(64), 0, as_stream(s), a, group);
-        else MYNN_LAUNCH((attn_kv4_row_kernel<T, 128>), grid, dim3(64), 0, as_stream(s), a, group);
-        return launch_status("attn_kv4_row_kernel");
-    });
+    const Kv4TilePlan plan = kv4_tile_plan(B, Sq, num_q_heads, num_kv_heads, rows);
+    MYNN_REQUIRE(plan.blocks <= 65535 && plan.ranges <= 65535, MYNN_ERR_UNSUPPORTED, "%s: Sq=%d heads %d/%d", who, Sq, num_q_heads, num_kv_heads);
+    a.part_ml = a.part_o + (size_t)plan.ranges * B * num_kv_heads * R * head_dim;
+    return pick([&](auto *t, auto d, auto n) { return kv4_tile_go<std::remove_pointer_t<decltype(t)>, decltype(d)::value, decltype(n)::value>(a, plan, as_stream(s)); });
 }

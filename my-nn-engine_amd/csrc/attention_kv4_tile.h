@@ -1,0 +1,334 @@
+// The form for many rows: blocks of 32 query rows of a kv head (query heads times new tokens, the heads of a token next to each other) as the columns of
+// v_mfma_f32_32x32x16_f16.
+//
+// A workgroup of QW x KW waves has QW blocks of rows and walks their keys in tiles of KEYS, a KW-th of each tile a wave.  Codes travel global -> registers (a tile ahead)
+// -> (code - zero) in fp16 -> LDS, once for all rows of the workgroup: two stages, one barrier a tile.
+//   S^T = K . Q^T      per group of columns; a key's scale meets the group's sum
+//   softmax            a lane has ONE row and half of the keys of each 32; the reference with the value scales in it (attention_kv4.h)
+//   O^T += V^T . P^T   p * vs rounded to fp16 once; P stays in registers (the D layout of S^T is the B layout of P^T with the keys in the order 4g+0..3, 8+4g+0..3), V^T
+//                      comes from the row-major tile by transposing reads
+// Codes leave a dword in the order of kv4_pairs, so columns lie in that order inside every 8: queries are put in the same order when they are read, results back when stored.
+#pragma once
+#include "attention_kv4.h"
+
+namespace mynn {
+
+template <int D, int NG, int QW, int KW, int KEYS> struct Kv4Block {
+    static constexpr int ROWB = D * 2, TILEB = KEYS * ROWB, THREADS = QW * KW * 64, ROWS = QW * 32, NH = KEYS / 32 / KW, UNITS = KEYS * 4 / THREADS;
+    static constexpr int SCALES = (2 * NG + 1) * KEYS * 4, FLAGS = KEYS / 16 * 4;
+    static constexpr int STAGE = 2 * TILEB + SCALES + FLAGS;
+    static constexpr int WORDS = D / 2 + 2;  // of a lane's result: reference, sum, O^T
+    static constexpr int MERGE = KW > 1 ? QW * KW * 64 * WORDS * 4 : 0;
+    static constexpr int LDS = 2 * STAGE > MERGE ? 2 * STAGE : MERGE;
+    static_assert(NH >= 1 && UNITS >= 1 && STAGE % 16 == 0, "whole 32s of keys a wave, whole quarter rows a thread");
+};
+
+template <typename T, int D, int NG, int QW, int KW, int KEYS> __global__ __launch_bounds__(QW *KW * 64, 2) void attn_kv4_tile_kernel(Kv4Args a) {
+    using B = Kv4Block<D, NG, QW, KW, KEYS>;
+    constexpr int KS = D / 16, DT = D / 32, NH = B::NH, DW = D / 32, ROWB = B::ROWB, KPG = KS / NG, TPG = DT / NG;
+    extern __shared__ __align__(16) char sm[];
+    const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), wave = w % QW, kg = w / QW, col = lane & 31, g = lane >> 5;
+    const int G = a.Hq / a.c.Hkv, R = G * a.Sq;
+    const int b = blockIdx.x / a.c.Hkv, h = blockIdx.x % a.c.Hkv, nz = gridDim.z;
+    const int row0 = ((int)gridDim.y - 1 - (int)blockIdx.y) * B::ROWS;  // (the rows with the most keys are dispatched first)
+    const PagedSeq seq(a.c, b, a.Sq);
+    const int valid = seq.fresh * G;  // rows behind it are zeros
+    auto out_row = [&](int r) { return (T *)a.out + (((size_t)b * a.Hq + h * G + r % G) * a.Sq + r / G) * D; };
+    if (row0 >= valid) {
+        if (blockIdx.z == 0)
+            for (int x = tid; x < min(B::ROWS, R - row0) * (D / 8); x += B::THREADS) *(U4 *)(out_row(row0 + x / (D / 8)) + x % (D / 8) * 8) = U4{0u, 0u, 0u, 0u};
+        return;
+    }
+    auto bound_of = [&](int r) { return seq.bound(min(r, valid - 1) / G, a.causal); };
+    const int ntiles = (bound_of(row0 + B::ROWS - 1) + KEYS - 1) / KEYS;
+    const int t0 = (int)((long)ntiles * blockIdx.z / nz), t1 = (int)((long)ntiles * (blockIdx.z + 1) / nz);
+    const int row = row0 + 32 * wave + col, row_c = min(row, valid - 1);
+    const int bound = bound_of(row), wave_first = bound_of(row0 + 32 * wave), wave_last = row0 + 32 * wave < valid ? bound_of(row0 + 32 * wave + 31) : 0;
+
+    // ---- staging: a thread has a quarter of a row of K and of V, UNITS times
+    constexpr int QUARTERS = B::THREADS / 4;
+    const int quarter = tid & 3, sg = quarter * NG / 4;
+    const int psh = a.c.page_shift, pmask = (1 << psh) - 1;
+    int pages = -1, pages_at = -(1 << 30);
+    struct Raw {
+        uint32_t k[DW], v[DW];
+        T ks, vs;
+        uint8_t kz, vz;
+        int there;
+    } raw[B::UNITS];
+    auto load = [&](int t) {
+#pragma unroll
+        for (int u = 0; u < B::UNITS; u++) {
+            Raw &x = raw[u];
+            // (a wave's 16 rows lie in one page)
+            const int first = t * KEYS + u * QUARTERS + 16 * w, p = first >> psh;
+            if (p - pages_at >= 64 || p < pages_at) {
+                pages_at = p;
+                pages = p + lane < a.c.pages_per_seq ? a.c.table[(size_t)b * a.c.pages_per_seq + p + lane] : -1;
+                if ((unsigned)pages >= (unsigned)a.c.n_pages) pages = -1;
+            }
+            const int page = __builtin_amdgcn_readlane(pages, p - pages_at);
+            x.there = page >= 0;
+            const size_t r = (((size_t)max(page, 0) * a.c.Hkv + h) << psh) + (size_t)(first & pmask) + (lane >> 2);
+            __builtin_memcpy(&x.k, __builtin_assume_aligned((const uint8_t *)a.c.k + r * (D / 2) + quarter * (D / 8), D / 8), D / 8);
+            __builtin_memcpy(&x.v, __builtin_assume_aligned((const uint8_t *)a.c.v + r * (D / 2) + quarter * (D / 8), D / 8), D / 8);
+            x.ks = ((const T *)a.c.k_scale)[r * NG + sg];
+            x.vs = ((const T *)a.c.v_scale)[r * NG + sg];
+            x.kz = a.c.k_zero[r * NG + sg];
+            x.vz = a.c.v_zero[r * NG + sg];
+        }
+    };
+    auto k_swz = [](int r) { return D == 128 ? r & 15 : (r >> 1) & 7; };
+    auto v_swz = [](int r) { return D == 128 ? (r & 3) * 5 : (((r >> 1) ^ r) & 1) << 2; };
+    Int4Pairs pairs;
+    auto store = [&](char *stage) {
+        float *ksc = (float *)(stage + 2 * B::TILEB), *vsc = ksc + NG * KEYS, *lift = vsc + NG * KEYS;
+        int *there = (int *)(lift + KEYS);
+#pragma unroll
+        for (int u = 0; u < B::UNITS; u++) {
+            const Raw &x = raw[u];
+            const int r = u * QUARTERS + (tid >> 2);
+            pairs.at(x.kz & 15u);
+#pragma unroll
+            for (int i = 0; i < DW; i++) *(U4 *)(stage + r * ROWB + (((quarter * DW + i) ^ k_swz(r)) << 4)) = pairs(x.k[i]);
+            pairs.at(x.vz & 15u);
+#pragma unroll
+            for (int i = 0; i < DW; i++) *(U4 *)(stage + B::TILEB + r * ROWB + (((quarter * DW + i) ^ v_swz(r)) << 4)) = pairs(x.v[i]);
+            const float vs = Elem<T>::ld(&x.vs, 0);
+            if (quarter % (4 / NG) == 0) {
+                ksc[sg * KEYS + r] = Elem<T>::ld(&x.ks, 0);
+                vsc[sg * KEYS + r] = vs;
+            }
+            const float big = group_max<4>(fabsf(vs));
+            if (quarter == 0) lift[r] = kv4_lift(big);
+            if (lane == 0) there[r >> 4] = x.there;
+        }
+    };
+    if (t0 < t1) load(t0);
+
+    // ---- Q^T: B operand, columns 16 ks + 8 g .. +7 in the codes' order, as fp16 times a power of two of the row
+    U4 qf[KS];
+    float csc;
+    {
+        const T *q = (const T *)a.q + (((size_t)b * a.Hq + h * G + row_c % G) * a.Sq + row_c / G) * D;
+        U4 x[KS];
+        float f[8], peak = 0.f;
+#pragma unroll
+        for (int ks = 0; ks < KS; ks++) {
+            x[ks] = *(const U4 *)(q + 16 * ks + 8 * g);
+            widen8<T>(x[ks], f);
+#pragma unroll
+            for (int e = 0; e < 8; e++) peak = fmaxf(peak, fabsf(f[e]));
+        }
+        peak = xor32_max(peak);
+        const int e10 = peak > 0.f ? 10 - __builtin_amdgcn_frexp_expf(peak) : 0;
+#pragma unroll
+        for (int ks = 0; ks < KS; ks++) {
+            widen8<T>(x[ks], f);
+#pragma unroll
+            for (int e = 0; e < 8; e++) f[e] = __builtin_amdgcn_ldexpf(f[e], e10);
+            qf[ks] = U4{pack2<f16_t>(f[0], f[4]), pack2<f16_t>(f[1], f[5]), pack2<f16_t>(f[2], f[6]), pack2<f16_t>(f[3], f[7])};
+        }
+        csc = __builtin_amdgcn_ldexpf(a.scale * 1.4426950408889634f, -e10);
+    }
+    f16x_t o[DT];
+#pragma unroll
+    for (int t = 0; t < DT; t++)
+#pragma unroll
+        for (int e = 0; e < 16; e++) o[t][e] = 0.f;
+    float M = -INFINITY, l = 0.f;
+    const int krow = col * ROWB + ((g ^ k_swz(col)) << 4);
+    int vrow[DT];
+    {
+        const int i = lane & 15, r = 4 * g + (i >> 2);
+#pragma unroll
+        for (int t2 = 0; t2 < DT; t2++) vrow[t2] = r * ROWB + (((4 * t2 + 2 * ((lane >> 4) & 1) + ((i & 3) >> 1)) ^ v_swz(r)) << 4) + 8 * (i & 1);
+    }
+
+    auto tile = [&](const char *stage, int key0, auto masked) {
+        constexpr bool MASKED = decltype(masked)::value;
+        const int off = kg * 32 * NH;  // this wave's keys of the tile
+        const char *kt = stage + off * ROWB, *vt = kt + B::TILEB;
+        const float *ksc = (const float *)(stage + 2 * B::TILEB) + off, *vsc = ksc + NG * KEYS, *lift = vsc + NG * KEYS;
+        const int *there = (const int *)(lift + KEYS - off + off / 16);
+        f16x_t s[NH];
+#pragma unroll
+        for (int gr = 0; gr < NG; gr++)
+#pragma unroll
+            for (int hf = 0; hf < NH; hf++) {
+                f16x_t x;
+#pragma unroll
+                for (int e = 0; e < 16; e++) x[e] = 0.f;
+#pragma unroll
+                for (int ks = gr * KPG; ks < (gr + 1) * KPG; ks++) x = Mfma<f16_t>::run(*(const U4 *)(kt + (krow ^ (32 * ks)) + 32 * hf * ROWB), qf[ks], x);
+#pragma unroll
+                for (int e4 = 0; e4 < 4; e4++) {
+                    const f4_t f = *(const f4_t *)&ksc[gr * KEYS + 32 * hf + 8 * e4 + 4 * g];
+#pragma unroll
+                    for (int e = 0; e < 4; e++) s[hf][4 * e4 + e] = gr == 0 ? x[4 * e4 + e] * f[e] : fmaf(x[4 * e4 + e], f[e], s[hf][4 * e4 + e]);
+                }
+            }
+        float top = -INFINITY;
+        uint32_t seen[NH];  // MASKED: a bit for each of the lane's keys of a 32
+#pragma unroll
+        for (int hf = 0; hf < NH; hf++) {
+            seen[hf] = ~0u;
+            if (MASKED) {
+                seen[hf] = 0;
+                const int room = bound - key0 - 32 * hf - 4 * g;
+#pragma unroll
+                for (int e = 0; e < 16; e++) {
+                    const bool in = 8 * (e >> 2) + (e & 3) < room && there[2 * hf + (e >> 3)];
+                    seen[hf] |= (uint32_t)in << e;
+                    if (!in) s[hf][e] = -INFINITY;
+                }
+            }
+#pragma unroll
+            for (int e4 = 0; e4 < 4; e4++) {
+                const f4_t f = *(const f4_t *)&lift[32 * hf + 8 * e4 + 4 * g];
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const float t = fmaf(s[hf][4 * e4 + e], csc, f[e]);
+                    top = fmaxf(top, MASKED ? (seen[hf] >> (4 * e4 + e) & 1 ? t : -INFINITY) : t);
+                }
+            }
+        }
+        top = xor32_max(top);
+        const bool up = top > M;
+        if (__builtin_amdgcn_ballot_w64(up) != 0) {
+            const float mn = up ? top : M, corr = up ? __builtin_amdgcn_exp2f(M - mn) : 1.f;
+            M = mn;
+            l *= corr;
+#pragma unroll
+            for (int t2 = 0; t2 < DT; t2++)
+#pragma unroll
+                for (int e = 0; e < 16; e++) o[t2][e] *= corr;
+        }
+        const float ref = M == -INFINITY ? 0.f : M;
+        float lt = 0.f;
+#pragma unroll
+        for (int hf = 0; hf < NH; hf++)
+#pragma unroll
+            for (int e = 0; e < 16; e++) {
+                const float p = __builtin_amdgcn_exp2f(fmaf(s[hf][e], csc, -ref));
+                s[hf][e] = MASKED ? (seen[hf] >> e & 1 ? p : 0.f) : p;
+                lt += s[hf][e];
+            }
+        l += lt;
+#pragma unroll
+        for (int gr = 0; gr < NG; gr++)
+#pragma unroll
+            for (int st = 0; st < 2 * NH; st++) {
+                const int e0 = 8 * (st & 1);
+                float p[8];
+#pragma unroll
+                for (int e4 = 0; e4 < 2; e4++) {
+                    const f4_t f = *(const f4_t *)&vsc[gr * KEYS + 16 * st + 8 * e4 + 4 * g];
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        const float x = s[st >> 1][e0 + 4 * e4 + e];
+                        p[4 * e4 + e] = MASKED ? (seen[st >> 1] >> (e0 + 4 * e4 + e) & 1 ? x * f[e] : 0.f) : x * f[e];
+                    }
+                }
+                const U4 pf = U4{cvt2<f16_t>(p[0], p[1]), cvt2<f16_t>(p[2], p[3]), cvt2<f16_t>(p[4], p[5]), cvt2<f16_t>(p[6], p[7])};
+#pragma unroll
+                for (int t2 = gr * TPG; t2 < (gr + 1) * TPG; t2++) {
+                    const char *vr = vt + vrow[t2] + 16 * st * ROWB;
+                    const uint2 lo = lds_read_tr16(vr), hi = lds_read_tr16(vr + 8 * ROWB);
+                    o[t2] = Mfma<f16_t>::run(U4{lo.x, lo.y, hi.x, hi.y}, pf, o[t2]);
+                }
+            }
+    };
+
+    for (int t = t0, stage = 0; t < t1; t++, stage ^= 1) {
+        char *here = sm + stage * B::STAGE;
+        store(here);  // (tile t - 2, which lay here, is behind the last barrier for every wave)
+        if (t + 1 < t1) load(t + 1);
+        __syncthreads();
+        const int key0 = t * KEYS + kg * 32 * NH;
+        if (key0 >= wave_last) continue;
+        const int *there = (const int *)(here + 2 * B::TILEB + B::SCALES) + kg * 2 * NH;
+        int all = 1;
+#pragma unroll
+        for (int x = 0; x < 2 * NH; x++) all &= there[x];
+        if (key0 + 32 * NH <= wave_first && __builtin_amdgcn_readfirstlane(all)) tile(here, key0, std::false_type{});
+        else tile(here, key0, std::true_type{});
+    }
+
+    l = xor32_sum(l);
+    if constexpr (KW > 1) {
+        // the waves that shared a block of rows: the first of them takes the others' results in
+        __syncthreads();
+        float *to = (float *)sm + (size_t)w * 64 * B::WORDS + lane;
+        if (kg > 0) {
+            to[0] = M;
+            to[64] = l;
+#pragma unroll
+            for (int t2 = 0; t2 < DT; t2++)
+#pragma unroll
+                for (int e = 0; e < 16; e++) to[(2 + 16 * t2 + e) * 64] = o[t2][e];
+        }
+        __syncthreads();
+        if (kg > 0) return;
+#pragma unroll
+        for (int k = 1; k < KW; k++) {
+            const float *from = (const float *)sm + (size_t)(k * QW + wave) * 64 * B::WORDS + lane;
+            const float mo = from[0], mn = fmaxf(M, mo);
+            const float ca = M == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(M - mn), cb = mo == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mo - mn);
+            l = l * ca + from[64] * cb;
+            M = mn;
+#pragma unroll
+            for (int t2 = 0; t2 < DT; t2++)
+#pragma unroll
+                for (int e = 0; e < 16; e++) o[t2][e] = o[t2][e] * ca + from[(2 + 16 * t2 + e) * 64] * cb;
+        }
+    }
+    const float inv = nz > 1 ? 1.f : row >= valid || l == 0.f ? 0.f : 1.0f / l;
+    const size_t line = ((size_t)blockIdx.x * R + row) * nz + blockIdx.z;
+#pragma unroll
+    for (int t2 = 0; t2 < DT; t2++)
+#pragma unroll
+        for (int e4 = 0; e4 < 4; e4++) {
+            // columns 0, 4, 1, 5 of an 8 in the lower lanes, 2, 6, 3, 7 in the upper: 0 .. 3 and 4 .. 7
+            float x0 = o[t2][4 * e4], x2 = o[t2][4 * e4 + 1], x1 = o[t2][4 * e4 + 2], x3 = o[t2][4 * e4 + 3];
+            permlane32_swap(x0, x2);
+            permlane32_swap(x1, x3);
+            const int d = 32 * t2 + 8 * e4 + 4 * g;
+            if (row >= R) continue;
+            if (nz > 1) *(f4_t *)(a.part_o + line * D + d) = f4_t{x0, x1, x2, x3};
+            else if (row >= valid) *(uint2 *)(out_row(row) + d) = uint2{0u, 0u};
+            else *(uint2 *)(out_row(row) + d) = uint2{pack2<T>(x0 * inv, x1 * inv), pack2<T>(x2 * inv, x3 * inv)};
+        }
+    if (nz > 1 && g == 0 && row < R) *(float2 *)(a.part_ml + line * 2) = float2{M, l};
+}
+
+// Joins the ranges of keys of each row.  Rows of a block that has none of the sequence's own are zeros already.
+template <typename T, int D> __global__ __launch_bounds__(256) void attn_kv4_ranges_kernel(Kv4Args a, int nz, int block_rows) {
+    const int G = a.Hq / a.c.Hkv, R = G * a.Sq;
+    const size_t at = (size_t)blockIdx.x * 256 + threadIdx.x, line = at / (D / 4);
+    const int d = (int)(at % (D / 4)) * 4;
+    if (line >= (size_t)a.B * a.c.Hkv * R) return;
+    const int pair = (int)(line / R), r = (int)(line % R), b = pair / a.c.Hkv, h = pair % a.c.Hkv;
+    const PagedSeq seq(a.c, b, a.Sq);
+    const int valid = seq.fresh * G;
+    if (r / block_rows * block_rows >= valid) return;
+    const float *ml = a.part_ml + line * nz * 2, *po = a.part_o + line * nz * D + d;
+    float mt = -INFINITY;
+    for (int z = 0; z < nz; z++) mt = fmaxf(mt, ml[2 * z]);
+    float lt = 0.f;
+    f4_t o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (int z = 0; z < nz; z++) {
+        const float c = ml[2 * z] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml[2 * z] - mt);
+        const f4_t oz = *(const f4_t *)(po + (size_t)z * D);
+        lt = fmaf(ml[2 * z + 1], c, lt);
+#pragma unroll
+        for (int e = 0; e < 4; e++) o[e] = fmaf(oz[e], c, o[e]);
+    }
+    const float inv = r >= valid || lt == 0.f ? 0.f : 1.0f / lt;
+    uint2 x = uint2{pack2<T>(o[0] * inv, o[1] * inv), pack2<T>(o[2] * inv, o[3] * inv)};
+    if (r >= valid) x = uint2{0u, 0u};
+    *(uint2 *)((T *)a.out + (((size_t)b * a.Hq + h * G + r % G) * a.Sq + r / G) * D + d) = x;
+}
+
+}  // namespace mynn
