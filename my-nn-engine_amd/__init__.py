@@ -266,6 +266,8 @@ def _load_host_ops():
     module.bind_int4(*(C.cast(getattr(l, n), _vp).value for n in (
         "mynn_dequant_matmul_int4_ws", "mynn_quantized_matmul_int4_ws", "mynn_add_rms_norm", "mynn_add_rms_norm_quantize",
         "mynn_dequantize_linear", "mynn_matmul_int4_workspace_bytes")))
+    module.bind_paged(*(C.cast(getattr(l, n), _vp).value for n in (
+        "mynn_rope_append_paged", "mynn_kv_rows_paged", "mynn_attention_paged_int4_workspace_bytes", "mynn_attention_paged_int4")))
     return module
 
 
@@ -703,6 +705,10 @@ def rope_append_paged(q, k, v, cos_t, sin_t, pools, table, past_lens, new_lens=N
     past_lens[b] (cuda int32 [B]) on; new_lens (cuda int32 [B]): how many of the S tokens are a sequence's own; positions (cuda int64 [B,S]): the
     table rows, where they are not the cache rows.  q, k, v may be views (of the projection's rows, say) whose last dimension lies together.
     Returns the rotated q, contiguous (out, where given)."""
+    if k.is_cuda:
+        done = (_ops or _host_ops()).rope_append_paged(q, k, v, cos_t, sin_t, pools, table, past_lens, new_lens, positions, out)
+        if done is not None:
+            return done
     torch = _t()
     name = "rope_append_paged"
     c = _Paged(name, pools, table, past_lens, new_lens)
@@ -737,6 +743,10 @@ def rope_append_paged(q, k, v, cos_t, sin_t, pools, table, past_lens, new_lens=N
 
 def kv_rows_paged(pools, table, first_rows, n, n_rows=None):
     """mynn_kv_rows_paged: (k, v) [B,Hkv,n,D], what the cache's rows first_rows[b] (cuda int32 [B]) .. stand for; zeros from n_rows[b] on"""
+    if first_rows.is_cuda:
+        done = (_ops or _host_ops()).kv_rows_paged(pools, table, first_rows, n, n_rows)
+        if done is not None:
+            return done
     c = _Paged("kv_rows_paged", pools, table, first_rows, n_rows)
     n = int(n)
     if not 0 < n < 1 << 31:
@@ -765,6 +775,10 @@ def attention_paged_int4(q, pools, table, scale, past_lens, new_lens=None, is_ca
     """mynn_attention_paged_int4: q [B,Hq,Sq,D], the newest tokens of each sequence, over a cache of 4 bits (KvPool.buffers with kv_int4_group) that holds
     their rows already (rope_append_paged with the same past_lens and new_lens).  workspace: attention_paged_int4_workspace(...), kept by
     the caller; without one the call allocates its own, and takes a launch more where a sequence is shared by several workgroups."""
+    if q.is_cuda:
+        done = (_ops or _host_ops()).attention_paged_int4(q, pools, table, scale, past_lens, new_lens, is_causal, workspace, out)
+        if done is not None:
+            return done
     name = "attention_paged_int4"
     c = _Paged(name, pools, table, past_lens, new_lens)
     if c.bits != 4:

@@ -26,6 +26,10 @@ decltype(&mynn_quantized_matmul_int4_ws) g_quantized_matmul_int4;
 decltype(&mynn_add_rms_norm) g_add_rms_norm;
 decltype(&mynn_add_rms_norm_quantize) g_add_rms_norm_quantize;
 decltype(&mynn_dequantize_linear) g_dequantize_linear;
+decltype(&mynn_rope_append_paged) g_rope_append_paged;
+decltype(&mynn_kv_rows_paged) g_kv_rows_paged;
+decltype(&mynn_attention_paged_int4_workspace_bytes) g_kv4_bytes;
+decltype(&mynn_attention_paged_int4) g_attention_paged_int4;
 PyObject *g_error;
 
 int code_of(at::ScalarType t) {
@@ -321,6 +325,136 @@ PyObject *dequantize_linear(PyObject *, PyObject *const *args, Py_ssize_t n) {
     });
 }
 
+// The pools of a layer (a tuple or list of 2, 4 or 6 tensors), a page table [B, pages] and lengths [B] (or None), as the calls over paged caches take them
+struct Paged {
+    const at::Tensor *pool[6] = {}, *table, *past, *fresh = nullptr;
+    void *p[6] = {}, *table_p = nullptr, *past_p = nullptr, *fresh_p = nullptr;
+    int64_t B = 0, pages = 0, n_pages = 0, heads = 0, rows = 0, dim = 0, groups = 1;
+    int bits = 0, code = -1;
+    at::ScalarType type = at::kHalf;
+    Paged(PyObject *pools, PyObject *tab, PyObject *pst, PyObject *nw) : table(here(tab)), past(here(pst)) {
+        if (!(PyTuple_CheckExact(pools) || PyList_CheckExact(pools)) || !table || !past || (nw != Py_None && !(fresh = here(nw)))) return;
+        const Py_ssize_t n = PySequence_Fast_GET_SIZE(pools);
+        if (n != 2 && n != 4 && n != 6) return;
+        for (Py_ssize_t i = 0; i < n; i++)
+            if (!(pool[i] = here(PySequence_Fast_GET_ITEM(pools, i)))) return;
+        const at::Tensor &k = *pool[0];
+        if (k.dim() != 4 || table->dim() != 2 || table->scalar_type() != at::kInt) return;
+        B = table->size(0), pages = table->size(1), n_pages = k.size(0), heads = k.size(1), rows = k.size(2), dim = k.size(3) * (n == 6 ? 2 : 1);
+        type = n == 2 ? k.scalar_type() : pool[2]->scalar_type();
+        if (n == 6) {
+            if (pool[2]->dim() != 4) return;
+            groups = pool[2]->size(3);
+            if (groups < 1 || dim % groups) return;
+        }
+        const at::ScalarType kinds[3] = {n == 2 ? type : n == 4 ? at::kChar : at::kByte, type, at::kByte};
+        for (Py_ssize_t i = 0; i < n; i++) {
+            const at::Tensor &x = *pool[i];
+            const int64_t last = i < 2 ? k.size(3) : groups;
+            if (x.scalar_type() != kinds[i / 2] || x.dim() != (n == 4 && i >= 2 ? 3 : 4) || x.size(0) != n_pages || x.size(1) != heads || x.size(2) != rows ||
+                (x.dim() == 4 && x.size(3) != last))
+                return;
+        }
+        for (const at::Tensor *x : {past, fresh})
+            if (x && (x->scalar_type() != at::kInt || x->dim() != 1 || x->size(0) != B)) return;
+        if (!fits_int(B) || !fits_int(pages) || !fits_int(n_pages) || !fits_int(heads) || !fits_int(rows) || !fits_int(dim) || B < 1 || (type != at::kHalf && type != at::kBFloat16)) return;
+        for (Py_ssize_t i = 0; i < n; i++) p[i] = data(*pool[i]);
+        table_p = data(*table), past_p = data(*past), fresh_p = fresh ? data(*fresh) : nullptr;
+        code = code_of(type);
+        bits = n == 2 ? 16 : n == 4 ? 8 : 4;
+    }
+    explicit operator bool() const { return bits != 0; }
+    int group() const { return bits == 4 ? (int)(dim / groups) : 0; }
+    // rows [B, H, S, dim] of the cache's type (S > 0), in order or as a view whose values lie together
+    const at::Tensor *rows_of(PyObject *o, bool ordered) const {
+        if (!THPVariable_CheckExact(o)) return nullptr;
+        const at::Tensor &t = THPVariable_Unpack(o);
+        if (!t.defined() || !t.has_storage() || !t.is_cuda() || t.layout() != at::kStrided || t.get_device() != c10::hip::current_device() || t.is_neg() || t.dim() != 4) return nullptr;
+        if (t.size(0) != B || t.size(3) != dim || t.size(2) < 1 || t.size(1) < 1 || !fits_int(t.size(2)) || !fits_int(t.size(1)) || t.scalar_type() != type) return nullptr;
+        return (ordered ? t.is_contiguous() : t.stride(3) == 1) ? &t : nullptr;
+    }
+};
+
+// (q or None, k, v, cos, sin, pools, table, past_lens, new_lens or None, positions or None, out or None) -> the rotated q (None is "not taken", so a call without q goes
+// the long way)
+PyObject *rope_append_paged(PyObject *, PyObject *const *args, Py_ssize_t n) {
+    if (n != 11 || args[9] != Py_None || args[10] != Py_None) return none();
+    return guarded([&]() -> PyObject * {
+        const Paged c(args[5], args[6], args[7], args[8]);
+        if (!c) return none();
+        const at::Tensor *x[3] = {c.rows_of(args[0], false), c.rows_of(args[1], false), c.rows_of(args[2], false)}, *cs = here(args[3]), *sn = here(args[4]);
+        if (!x[0] || !x[1] || !x[2] || !cs || !sn) return none();
+        const int64_t S = x[0]->size(2);
+        if (x[1]->size(1) != c.heads || x[2]->size(1) != c.heads || x[1]->size(2) != S || x[2]->size(2) != S || cs->dim() != 2 || cs->sizes() != sn->sizes() || cs->size(1) != c.dim ||
+            !fits_int(cs->size(0)) || cs->scalar_type() != c.type || sn->scalar_type() != c.type)
+            return none();
+        int64_t strides[9];
+        for (int i = 0; i < 3; i++)
+            for (int d = 0; d < 3; d++) strides[3 * i + d] = x[i]->size(d) > 1 ? x[i]->stride(d) : 0;
+        const at::Tensor out = make(x[0]->sizes(), *x[0], c.type);
+        void *o = data(out), *q = data(*x[0]), *k = data(*x[1]), *v = data(*x[2]), *ct = data(*cs), *st = data(*sn);
+        const mynn_stream stream = current_stream();
+        const int rc = without_gil([&] {
+            return g_rope_append_paged(o, q, k, v, strides, ct, st, (int)cs->size(0), nullptr, c.p[0], c.p[1], c.p[2], c.p[3], (uint8_t *)c.p[4], (uint8_t *)c.p[5],
+                                       (const int32_t *)c.table_p, (int)c.n_pages, (int)c.pages, (int)c.rows, (const int32_t *)c.past_p, (const int32_t *)c.fresh_p, (int)c.B, (int)S,
+                                       (int)x[0]->size(1), (int)c.heads, (int)c.dim, c.code, c.bits, c.group(), stream);
+        });
+        return rc ? failed(rc) : THPVariable_Wrap(out);
+    });
+}
+
+// (pools, table, first_rows, n, n_rows or None) -> (k, v)
+PyObject *kv_rows_paged(PyObject *, PyObject *const *args, Py_ssize_t n) {
+    if (n != 5 || !PyLong_CheckExact(args[3])) return none();
+    return guarded([&]() -> PyObject * {
+        const Paged c(args[0], args[1], args[2], args[4]);
+        const int64_t S = PyLong_AsLongLong(args[3]);
+        if (PyErr_Occurred()) PyErr_Clear();
+        if (!c || S < 1 || !fits_int(S)) return none();
+        const at::Tensor k = make({c.B, c.heads, S, c.dim}, *c.pool[0], c.type), v = make({c.B, c.heads, S, c.dim}, *c.pool[0], c.type);
+        void *kp = data(k), *vp = data(v);
+        const mynn_stream stream = current_stream();
+        const int rc = without_gil([&] {
+            return g_kv_rows_paged(kp, vp, c.p[0], c.p[1], c.p[2], c.p[3], (const uint8_t *)c.p[4], (const uint8_t *)c.p[5], (const int32_t *)c.table_p, (int)c.n_pages, (int)c.pages,
+                                   (int)c.rows, (const int32_t *)c.past_p, (const int32_t *)c.fresh_p, (int)c.B, (int)S, (int)c.heads, (int)c.dim, c.code, c.bits, c.group(), stream);
+        });
+        if (rc) return failed(rc);
+        PyObject *tuple = PyTuple_New(2);
+        if (!tuple) return nullptr;
+        PyTuple_SET_ITEM(tuple, 0, THPVariable_Wrap(k));
+        PyTuple_SET_ITEM(tuple, 1, THPVariable_Wrap(v));
+        return tuple;
+    });
+}
+
+// (q, pools, table, scale, past_lens, new_lens or None, is_causal, workspace or None, out or None) -> out; a workspace has the counters in front, in whole 256 bytes
+PyObject *attention_paged_int4(PyObject *, PyObject *const *args, Py_ssize_t n) {
+    if (n != 9 || !PyFloat_CheckExact(args[3]) || !PyBool_Check(args[6]) || args[8] != Py_None) return none();
+    return guarded([&]() -> PyObject * {
+        const Paged c(args[1], args[2], args[4], args[5]);
+        if (!c || c.bits != 4) return none();
+        const at::Tensor *q = c.rows_of(args[0], true), *kept = nullptr;
+        if (!q || (args[7] != Py_None && (!(kept = here(args[7])) || kept->scalar_type() != at::kByte))) return none();
+        const int64_t Hq = q->size(1), S = q->size(2);
+        const size_t need = g_kv4_bytes((int)c.B, (int)S, (int)c.pages, (int)c.rows, (int)Hq, (int)c.heads, (int)c.dim);
+        const size_t front = kept ? (4 * (size_t)(c.B * c.heads) + 255) / 256 * 256 : 0;
+        if (kept && (size_t)kept->numel() < front + need) return none();
+        const at::Tensor out = make(q->sizes(), *q, c.type), own = kept || !need ? at::Tensor() : make({(int64_t)need}, *q, at::kByte);
+        void *o = data(out), *qp = data(*q);
+        char *ws = kept ? (char *)data(*kept) : own.defined() ? (char *)data(own) : nullptr;
+        const float scale = (float)PyFloat_AS_DOUBLE(args[3]);
+        const int causal = args[6] == Py_True;
+        const mynn_stream stream = current_stream();
+        const int rc = without_gil([&] {
+            return g_attention_paged_int4(o, qp, (const uint8_t *)c.p[0], (const uint8_t *)c.p[1], c.p[2], c.p[3], (const uint8_t *)c.p[4], (const uint8_t *)c.p[5],
+                                          (const int32_t *)c.table_p, (int)c.n_pages, (int)c.pages, (int)c.rows, scale, causal, (int)c.B, (int)S, (const int32_t *)c.past_p,
+                                          (const int32_t *)c.fresh_p, (int)Hq, (int)c.heads, (int)c.dim, c.code, c.group(), ws ? ws + front : nullptr, need,
+                                          kept ? (int32_t *)ws : nullptr, stream);
+        });
+        return rc ? failed(rc) : THPVariable_Wrap(out);
+    });
+}
+
 // the addresses of a call's arguments, or false with an exception set
 bool addresses(PyObject *const *args, int count, void **p) {
     for (int i = 0; i < count; i++) {
@@ -368,10 +502,26 @@ PyObject *bind_int4(PyObject *, PyObject *const *args, Py_ssize_t n) {
     Py_RETURN_NONE;
 }
 
+// (addresses of the calls over paged caches)
+PyObject *bind_paged(PyObject *, PyObject *const *args, Py_ssize_t n) {
+    if (n != 4) {
+        PyErr_SetString(PyExc_TypeError, "bind_paged: four arguments");
+        return nullptr;
+    }
+    void *p[4];
+    if (!addresses(args, 4, p)) return nullptr;
+    g_rope_append_paged = (decltype(g_rope_append_paged))p[0];
+    g_kv_rows_paged = (decltype(g_kv_rows_paged))p[1];
+    g_kv4_bytes = (decltype(g_kv4_bytes))p[2];
+    g_attention_paged_int4 = (decltype(g_attention_paged_int4))p[3];
+    Py_RETURN_NONE;
+}
+
 #define MYNN_METHOD(f) {#f, (PyCFunction)(void (*)(void))f, METH_FASTCALL, nullptr}
 PyMethodDef g_methods[] = {MYNN_METHOD(bind), MYNN_METHOD(dequant_matmul), MYNN_METHOD(quantized_matmul), MYNN_METHOD(dynamic_quantize_linear), MYNN_METHOD(attention),
                            MYNN_METHOD(bind_int4), MYNN_METHOD(dequant_matmul_int4), MYNN_METHOD(quantized_matmul_int4), MYNN_METHOD(add_rms_norm),
-                           MYNN_METHOD(add_rms_norm_quantize), MYNN_METHOD(dequantize_linear),
+                           MYNN_METHOD(add_rms_norm_quantize), MYNN_METHOD(dequantize_linear), MYNN_METHOD(bind_paged), MYNN_METHOD(rope_append_paged),
+                           MYNN_METHOD(kv_rows_paged), MYNN_METHOD(attention_paged_int4),
                            {nullptr, nullptr, 0, nullptr}};
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_host_ops", nullptr, -1, g_methods, nullptr, nullptr, nullptr, nullptr};
 
