@@ -4,8 +4,8 @@
 // Both keep the codes exact: (code - zero) is a whole number of -15 .. 15, an fp16 operand of the matrix cores in either product, whatever T is; a key's
 // scale meets its score, a value's scale its weight, in 32 bits.  Queries enter as fp16 times a power of two of their row (T = bf16 has fewer bits and more
 // range).  Weights enter the second product as fp16 numbers p * vs: the reference M of the online softmax is chosen so that they fit,
-//   M = max over the keys of (s + max(e - 14, -100)),   2^e the scale's power of two, s the score in units of log2,
-// so that p = 2^(s - M) <= 2^100 and p * vs < 2^14, with the largest near it.  A value row with a large scale and no weight takes nothing from the others then, and
+//   M = max over the keys of (s + log2 |vs|) - 14,   s the score in units of log2 (|vs| of less than 2^-86 counts as that),
+// so that p = 2^(s - M) <= 2^100 and p * vs < 2^14.1, with the largest near it.  A value row with a large scale and no weight takes nothing from the others then, and
 // no unit is left to be taken out: numerator and denominator have the same M.
 #pragma once
 #include "int4_codes.h"
@@ -38,8 +38,14 @@ __device__ __forceinline__ U4 kv4_pairs(uint32_t w, const h2_t *off, uint32_t ni
 __device__ __forceinline__ h2_t kv4_low(uint32_t zz) { return __builtin_bit_cast(h2_t, (zz & 0x000F000Fu) | 0xE400E400u); }
 __device__ __forceinline__ h2_t kv4_high(uint32_t zz) { return __builtin_bit_cast(h2_t, ((zz << 4) & 0x00F000F0u) | 0xD400D400u); }
 
-// the key's share in the reference: max(e - 14, -100)
-__device__ __forceinline__ float kv4_lift(float vs) { return fmaxf((float)(__builtin_amdgcn_frexp_expf(vs) - 14), -100.f); }
+// The scale's part in the reference, from its bits: exponent and mantissa of T as one number are log2 of it, less than 0.09 too little (subnormal numbers of fp16: too much),
+// in steps of 2^-(bits of the mantissa) from kKv4Zero on.  |vs| of 2^-86 and less counts as 2^-86, so that p <= 2^100.
+template <typename T> constexpr float kKv4Step = std::is_same<T, f16_t>::value ? 0x1p-10f : 0x1p-7f;
+template <typename T> constexpr float kKv4Zero = std::is_same<T, f16_t>::value ? 15.f + 14.f : 127.f + 14.f;  // (what the reference is less than M: 2^14 on top)
+template <typename T> __device__ __forceinline__ uint32_t kv4_bits(uint32_t w, int hi) {
+    const uint32_t x = __builtin_amdgcn_ubfe(w, hi ? 16 : 0, 15);
+    return std::is_same<T, f16_t>::value ? x : max(x, (127u - 86u) << 7);
+}
 
 template <typename T> __device__ __forceinline__ float kv4_half(uint32_t w, int hi) {  // one of two packed values of T
     const uint16_t b = (uint16_t)(hi ? w >> 16 : w & 0xFFFFu);
@@ -54,42 +60,60 @@ template <int UNIT> struct Kv4Share {
     int quota, total;  // units of a workgroup, units in all
     int first;         // this workgroup's first unit
     int b, before;     // the sequence that has it, and the units of the sequences in front
-    __device__ static int units(const PagedKv &c, int b, int S) {
-        const PagedSeq s(c, b, S);
-        return max(1, (s.len + UNIT - 1) / UNIT);
-    }
-    // inclusive sum over the lanes
-    __device__ static int running(int v, int lane) {
-#pragma unroll
-        for (int d = 1; d < 64; d *= 2) {
-            const int o = __shfl_up(v, d, 64);
-            if (lane >= d) v += o;
+    int past, fresh, from;  // lengths of the sequences from .. from + 63, a lane each
+    __device__ static int share_of(const Kv4Args &a, int total) { return (total + a.grid - 1) / a.grid; }
+    __device__ static int units(const PagedSeq &s) { return max(1, (s.len + UNIT - 1) / UNIT); }
+    __device__ void lengths(const Kv4Args &a, int b0, int lane) {
+        from = b0;
+        past = 0, fresh = a.Sq;
+        if (b0 + lane < a.B) {
+            past = a.c.past[b0 + lane];
+            if (a.c.fresh) fresh = a.c.fresh[b0 + lane];
         }
+    }
+    __device__ PagedSeq seq(const Kv4Args &a, int b, int lane) {
+        if (b - from >= 64) lengths(a, b, lane);
+        return PagedSeq(a.c, __builtin_amdgcn_readlane(past, b - from), __builtin_amdgcn_readlane(fresh, b - from), a.Sq);
+    }
+    // inclusive sum over the lanes: inside rows of 16, then over the rows
+    __device__ static int running(int v) {
+        v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false);
+        v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false);
+        v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false);
+        v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false);
+        v += __builtin_amdgcn_update_dpp(0, v, kDppBcast15, 0xA, 0xF, false);
+        v += __builtin_amdgcn_update_dpp(0, v, kDppBcast31, 0xC, 0xF, false);
         return v;
     }
+    // ... of the units of the sequences that `lengths` has
+    __device__ int run(const Kv4Args &a, int lane) { return running(from + lane < a.B ? units(PagedSeq(a.c, past, fresh, a.Sq)) : 0); }
     __device__ Kv4Share(const Kv4Args &a, int wg, int lane) {
         const int H = a.c.Hkv;
-        int run = 0, sum = 0;
+        int sum = 0, r = 0;
         for (int b0 = 0; b0 < a.B; b0 += 64) {
-            run = running(b0 + lane < a.B ? units(a.c, b0 + lane, a.Sq) : 0, lane);
-            sum += __builtin_amdgcn_readlane(run, 63);
+            lengths(a, b0, lane);
+            r = run(a, lane);
+            sum += __builtin_amdgcn_readlane(r, 63);
         }
         total = sum * H;
-        quota = (total + a.grid - 1) / a.grid;
+        quota = share_of(a, total);
         first = wg * quota;
         b = before = 0;
         if (first >= total) return;
         int front = 0;
         for (int b0 = 0;; b0 += 64) {
-            if (a.B > 64) run = running(b0 + lane < a.B ? units(a.c, b0 + lane, a.Sq) : 0, lane);
-            const uint64_t past = __builtin_amdgcn_ballot_w64((front + run) * H > first);
+            if (a.B > 64) {
+                lengths(a, b0, lane);
+                r = run(a, lane);
+            }
+            const uint64_t past = __builtin_amdgcn_ballot_w64((front + r) * H > first);
             if (past) {
                 const int l = __builtin_ctzll(past);
                 b = b0 + l;
-                before = (front + (l ? __builtin_amdgcn_readlane(run, l - 1) : 0)) * H;
+                before = (front + (l ? __builtin_amdgcn_readlane(r, l - 1) : 0)) * H;
                 return;
             }
-            front += __builtin_amdgcn_readlane(run, 63);
+            front += __builtin_amdgcn_readlane(r, 63);
         }
     }
 };

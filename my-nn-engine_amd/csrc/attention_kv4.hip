@@ -7,8 +7,6 @@ namespace mynn {
 int paged_kv_check(const char *who, const PagedKv &c, int page_rows, int kv_bits, int group, int D);
 int paged_shift(int page_rows);
 
-template <int N> using Int = std::integral_constant<int, N>;
-
 static int kv4_cus() {
     static int cus = 0;
     if (!cus) {
@@ -22,25 +20,19 @@ static int kv4_cus() {
     return cus;
 }
 static bool kv4_few_rows(int Hq, int Hkv, int Sq) { return (long)(Hq / Hkv) * Sq <= 16; }
+// How often the rows are put side by side: as 16 columns have room for them.  (Four groups of columns a row: twice at the most, the tile of 64 keys does not fit the registers.)
+static int kv4_fold(long rows, int groups) { return rows <= 4 && groups < 4 ? 4 : rows <= 8 ? 2 : 1; }
+static int kv4_unit(int fold) { return fold == 4 ? kKv4Stride<4> : kKv4Stride<1>; }
 // workgroups of the form for few rows: as many as run at once, no more than there can be units
-static int kv4_stream_grid(int B, int Hkv, long rows) {
-    const long units = (long)B * Hkv * ((rows + kKv4Unit - 1) / kKv4Unit), most = 2l * kv4_cus();
+static int kv4_stream_grid(int B, int Hkv, int unit, long rows) {
+    // Two a CU; where that makes more than 32 parts of a (sequence, kv head), fewer: their join is on one CU (one sequence of 32768 keys, 8 kv heads of 128: with 64 parts each
+    // 24 us, with 32 20).
+    const long pairs = (long)B * Hkv, units = pairs * ((rows + unit - 1) / unit), two = 2l * kv4_cus();
+    const long most = 32 * pairs >= two ? two : 32 * pairs > two / 4 ? 32 * pairs : two / 4;
     return (int)(units < most ? units : most);
 }
 
-template <typename T, int D, int NG> static int kv4_stream_go(const Kv4Args &a, hipStream_t s) {
-    const int R = a.Hq / a.c.Hkv * a.Sq, tile = 32 * (D / 2 + 16), wave = tile > R * D * 4 ? tile : R * D * 4;
-    MYNN_LAUNCH((attn_kv4_stream_kernel<T, D, NG>), dim3(a.grid), dim3(kKv4Waves * 64), kKv4Waves * (wave + 128), s, a);
-    if (const int rc = launch_status("attn_kv4_stream_kernel")) return rc;
-    if (a.grid == a.B * a.c.Hkv && a.c.pages_per_seq << a.c.page_shift <= kKv4Unit) return 0;  // (a unit each: nothing is shared)
-    MYNN_LAUNCH((attn_kv4_join_kernel<T, D>), dim3(a.B * a.c.Hkv), dim3(256), 0, s, a);
-    return launch_status("attn_kv4_join_kernel");
-}
-
-// Rows of a workgroup of the form for many rows, and the ranges that its keys come in where blocks of rows leave the device idle.
-struct Kv4TilePlan {
-    int rows, blocks, ranges;
-};
+// Ranges of keys where blocks of rows leave the device idle.
 static Kv4TilePlan kv4_tile_plan(int B, int Sq, int Hq, int Hkv, long rows) {
     const long R = (long)(Hq / Hkv) * Sq;
     Kv4TilePlan p;
@@ -49,24 +41,6 @@ static Kv4TilePlan kv4_tile_plan(int B, int Sq, int Hq, int Hkv, long rows) {
     const long wgs = (long)B * Hkv * p.blocks, most = (rows + 255) / 256, want = 2l * kv4_cus() / wgs;
     p.ranges = (int)(want < 1 ? 1 : want > most ? most : want);
     return p;
-}
-
-template <typename T, int D, int NG, int QW, int KW> static int kv4_tile_launch(const Kv4Args &a, const Kv4TilePlan &p, hipStream_t s) {
-    using Block = Kv4Block<D, NG, QW, KW, 64>;
-    static bool set = false;
-    if (!set && Block::LDS > 64 * 1024) {
-        MYNN_HIP(hipFuncSetAttribute((const void *)attn_kv4_tile_kernel<T, D, NG, QW, KW, 64>, hipFuncAttributeMaxDynamicSharedMemorySize, Block::LDS));
-        set = true;
-    }
-    MYNN_LAUNCH((attn_kv4_tile_kernel<T, D, NG, QW, KW, 64>), dim3(a.B * a.c.Hkv, p.blocks, p.ranges), dim3(Block::THREADS), Block::LDS, s, a);
-    return launch_status("attn_kv4_tile_kernel");
-}
-template <typename T, int D, int NG> static int kv4_tile_go(const Kv4Args &a, const Kv4TilePlan &p, hipStream_t s) {
-    const int rc = p.rows == 64 ? kv4_tile_launch<T, D, NG, 2, 2>(a, p, s) : kv4_tile_launch<T, D, NG, 4, 1>(a, p, s);
-    if (rc || p.ranges == 1) return rc;
-    const size_t threads = (size_t)a.B * a.Hq * a.Sq * (D / 4);
-    MYNN_LAUNCH((attn_kv4_ranges_kernel<T, D>), dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, s, a, p.ranges, p.rows);
-    return launch_status("attn_kv4_ranges_kernel");
 }
 
 }  // namespace mynn
@@ -80,7 +54,8 @@ extern "C" size_t mynn_attention_paged_int4_workspace_bytes(int B, int Sq, int p
         const int ranges = kv4_tile_plan(B, Sq, num_q_heads, num_kv_heads, (long)pages_per_seq * page_rows).ranges;
         return ranges == 1 ? 0 : (size_t)ranges * B * num_kv_heads * R * (head_dim + 4) * sizeof(float);
     }
-    return 2 * (size_t)kv4_stream_grid(B, num_kv_heads, (long)pages_per_seq * page_rows) * R * (head_dim + 4) * sizeof(float);
+    // (the smaller unit makes more workgroups: enough for either)
+    return 2 * (size_t)kv4_stream_grid(B, num_kv_heads, kv4_unit(1), (long)pages_per_seq * page_rows) * R * (head_dim + 4) * sizeof(float);
 }
 
 extern "C" int mynn_attention_paged_int4(void *out, const void *Q, const uint8_t *k_pool, const uint8_t *v_pool, const void *k_scale_pool, const void *v_scale_pool,
@@ -95,6 +70,7 @@ extern "C" int mynn_attention_paged_int4(void *out, const void *Q, const uint8_t
                n_pages, pages_per_seq, 0, num_kv_heads},
               out, Q, scale, is_causal, B, Sq, num_q_heads, nullptr, nullptr, nullptr, 0};
     if (const int rc = paged_kv_check(who, a.c, page_rows, 4, group, head_dim)) return rc;
+    MYNN_REQUIRE(dtype == MYNN_F16 || dtype == MYNN_BF16, MYNN_ERR_UNSUPPORTED, "%s: dtype %d: a 16-bit float type", who, dtype);
     a.c.page_shift = paged_shift(page_rows);
     MYNN_REQUIRE((long)num_q_heads * Sq < 1l << 30 && (long)B * num_kv_heads < 1l << 30, MYNN_ERR_UNSUPPORTED, "%s: B=%d Sq=%d heads %d", who, B, Sq, num_q_heads);
     const long rows = (long)pages_per_seq * page_rows;
@@ -103,22 +79,16 @@ extern "C" int mynn_attention_paged_int4(void *out, const void *Q, const uint8_t
                  need);
     const size_t R = (size_t)(num_q_heads / num_kv_heads) * Sq;
     a.part_o = (float *)workspace;
-    auto pick = [&](auto &&go) {
-        return dispatch_dtype16(dtype, [&](auto *t) {
-            if (head_dim == 64) return group == 64 ? go(t, Int<64>{}, Int<1>{}) : go(t, Int<64>{}, Int<2>{});
-            return group == 128 ? go(t, Int<128>{}, Int<1>{}) : group == 64 ? go(t, Int<128>{}, Int<2>{}) : go(t, Int<128>{}, Int<4>{});
-        });
-    };
     if (kv4_few_rows(num_q_heads, num_kv_heads, Sq)) {
-        MYNN_REQUIRE((long)B * num_kv_heads * ((rows + kKv4Unit - 1) / kKv4Unit) < 1l << 30, MYNN_ERR_UNSUPPORTED, "%s: %d sequences of %d heads of %ld rows", who, B, num_kv_heads,
-                     rows);
-        a.grid = kv4_stream_grid(B, num_kv_heads, rows);
+        const int fold = kv4_fold((long)R, head_dim / group), unit = kv4_unit(fold);
+        MYNN_REQUIRE((long)B * num_kv_heads * ((rows + unit - 1) / unit) < 1l << 30, MYNN_ERR_UNSUPPORTED, "%s: %d sequences of %d heads of %ld rows", who, B, num_kv_heads, rows);
+        a.grid = kv4_stream_grid(B, num_kv_heads, unit, rows);
         a.part_ml = a.part_o + 2 * (size_t)a.grid * R * head_dim;
         a.counters = counters;
-        return pick([&](auto *t, auto d, auto n) { return kv4_stream_go<std::remove_pointer_t<decltype(t)>, decltype(d)::value, decltype(n)::value>(a, as_stream(s)); });
+        return dtype == MYNN_F16 ? kv4_stream_go<f16_t>(a, head_dim, group, fold, as_stream(s)) : kv4_stream_go<bf16_t>(a, head_dim, group, fold, as_stream(s));
     }
     const Kv4TilePlan plan = kv4_tile_plan(B, Sq, num_q_heads, num_kv_heads, rows);
     MYNN_REQUIRE(plan.blocks <= 65535 && plan.ranges <= 65535, MYNN_ERR_UNSUPPORTED, "%s: Sq=%d heads %d/%d", who, Sq, num_q_heads, num_kv_heads);
     a.part_ml = a.part_o + (size_t)plan.ranges * B * num_kv_heads * R * head_dim;
-    return pick([&](auto *t, auto d, auto n) { return kv4_tile_go<std::remove_pointer_t<decltype(t)>, decltype(d)::value, decltype(n)::value>(a, plan, as_stream(s)); });
+    return dtype == MYNN_F16 ? kv4_tile_go<f16_t>(a, head_dim, group, plan, as_stream(s)) : kv4_tile_go<bf16_t>(a, head_dim, group, plan, as_stream(s));
 }

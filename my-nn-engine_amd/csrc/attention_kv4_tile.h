@@ -43,20 +43,26 @@ template <typename T, int D, int NG, int QW, int KW, int KEYS> __global__ __laun
     const int ntiles = (bound_of(row0 + B::ROWS - 1) + KEYS - 1) / KEYS;
     const int t0 = (int)((long)ntiles * blockIdx.z / nz), t1 = (int)((long)ntiles * (blockIdx.z + 1) / nz);
     const int row = row0 + 32 * wave + col, row_c = min(row, valid - 1);
-    const int bound = bound_of(row), wave_first = bound_of(row0 + 32 * wave), wave_last = row0 + 32 * wave < valid ? bound_of(row0 + 32 * wave + 31) : 0;
+    const int bound = bound_of(row), wave_last = row0 + 32 * wave < valid ? bound_of(row0 + 32 * wave + 31) : 0;
 
     // ---- staging: a thread has a quarter of a row of K and of V, UNITS times
     constexpr int QUARTERS = B::THREADS / 4;
     const int quarter = tid & 3, sg = quarter * NG / 4;
     const int psh = a.c.page_shift, pmask = (1 << psh) - 1;
     int pages = -1, pages_at = -(1 << 30);
+    bool all_there = true;
+    for (int p = (t0 * KEYS) >> psh; p <= (t1 * KEYS - 1) >> psh; p += 64) {
+        int x = 0;
+        if (p + lane < a.c.pages_per_seq && (p + lane) << psh < seq.len) x = a.c.table[(size_t)b * a.c.pages_per_seq + p + lane];
+        all_there = all_there && __builtin_amdgcn_ballot_w64((unsigned)x >= (unsigned)a.c.n_pages) == 0;
+    }
     struct Raw {
         uint32_t k[DW], v[DW];
         T ks, vs;
         uint8_t kz, vz;
         int there;
     } raw[B::UNITS];
-    auto load = [&](int t) {
+    auto load = [&](int t) __attribute__((always_inline)) {
 #pragma unroll
         for (int u = 0; u < B::UNITS; u++) {
             Raw &x = raw[u];
@@ -81,7 +87,7 @@ template <typename T, int D, int NG, int QW, int KW, int KEYS> __global__ __laun
     auto k_swz = [](int r) { return D == 128 ? r & 15 : (r >> 1) & 7; };
     auto v_swz = [](int r) { return D == 128 ? (r & 3) * 5 : (((r >> 1) ^ r) & 1) << 2; };
     Int4Pairs pairs;
-    auto store = [&](char *stage) {
+    auto store = [&](char *stage) __attribute__((always_inline)) {
         float *ksc = (float *)(stage + 2 * B::TILEB), *vsc = ksc + NG * KEYS, *lift = vsc + NG * KEYS;
         int *there = (int *)(lift + KEYS);
 #pragma unroll
@@ -99,8 +105,8 @@ template <typename T, int D, int NG, int QW, int KW, int KEYS> __global__ __laun
                 ksc[sg * KEYS + r] = Elem<T>::ld(&x.ks, 0);
                 vsc[sg * KEYS + r] = vs;
             }
-            const float big = group_max<4>(fabsf(vs));
-            if (quarter == 0) lift[r] = kv4_lift(big);
+            const float bits = group_max<4>((float)kv4_bits<T>(__builtin_bit_cast(uint16_t, x.vs), 0));
+            if (quarter == 0) lift[r] = bits * kKv4Step<T>;
             if (lane == 0) there[r >> 4] = x.there;
         }
     };
@@ -145,7 +151,7 @@ template <typename T, int D, int NG, int QW, int KW, int KEYS> __global__ __laun
         for (int t2 = 0; t2 < DT; t2++) vrow[t2] = r * ROWB + (((4 * t2 + 2 * ((lane >> 4) & 1) + ((i & 3) >> 1)) ^ v_swz(r)) << 4) + 8 * (i & 1);
     }
 
-    auto tile = [&](const char *stage, int key0, auto masked) {
+    auto tile = [&](const char *stage, int key0, auto masked) __attribute__((always_inline)) {
         constexpr bool MASKED = decltype(masked)::value;
         const int off = kg * 32 * NH;  // this wave's keys of the tile
         const char *kt = stage + off * ROWB, *vt = kt + B::TILEB;
@@ -176,12 +182,12 @@ template <typename T, int D, int NG, int QW, int KW, int KEYS> __global__ __laun
             if (MASKED) {
                 seen[hf] = 0;
                 const int room = bound - key0 - 32 * hf - 4 * g;
+                const uint32_t pages = (there[2 * hf] ? 0xFFu : 0u) | (there[2 * hf + 1] ? 0xFF00u : 0u);
 #pragma unroll
-                for (int e = 0; e < 16; e++) {
-                    const bool in = 8 * (e >> 2) + (e & 3) < room && there[2 * hf + (e >> 3)];
-                    seen[hf] |= (uint32_t)in << e;
-                    if (!in) s[hf][e] = -INFINITY;
-                }
+                for (int e = 0; e < 16; e++) seen[hf] |= (uint32_t)(8 * (e >> 2) + (e & 3) < room) << e;
+                seen[hf] &= pages;
+#pragma unroll
+                for (int e = 0; e < 16; e++) s[hf][e] = seen[hf] >> e & 1 ? s[hf][e] : -INFINITY;
             }
 #pragma unroll
             for (int e4 = 0; e4 < 4; e4++) {
@@ -204,7 +210,7 @@ template <typename T, int D, int NG, int QW, int KW, int KEYS> __global__ __laun
 #pragma unroll
                 for (int e = 0; e < 16; e++) o[t2][e] *= corr;
         }
-        const float ref = M == -INFINITY ? 0.f : M;
+        const float ref = M == -INFINITY ? 0.f : M - kKv4Zero<T>;
         float lt = 0.f;
 #pragma unroll
         for (int hf = 0; hf < NH; hf++)
@@ -240,19 +246,23 @@ template <typename T, int D, int NG, int QW, int KW, int KEYS> __global__ __laun
             }
     };
 
-    for (int t = t0, stage = 0; t < t1; t++, stage ^= 1) {
+    int t = t0, stage = 0;
+    auto next = [&]() __attribute__((always_inline)) {
         char *here = sm + stage * B::STAGE;
         store(here);  // (tile t - 2, which lay here, is behind the last barrier for every wave)
         if (t + 1 < t1) load(t + 1);
         __syncthreads();
+        stage ^= 1;
+        return here;
+    };
+    // the tiles that all rows of the workgroup see in full, then those with hidden keys.  (Loops of their own: with both kinds of tile in one, the results were copied from
+    // where one leaves them to where the other expects them.)
+    const int full = min(t1, seq.bound(row0 / G, a.causal) / KEYS);
+    for (; t < full && all_there; t++) tile(next(), 0, std::false_type{});
+    for (; t < t1; t++) {
+        const char *here = next();
         const int key0 = t * KEYS + kg * 32 * NH;
-        if (key0 >= wave_last) continue;
-        const int *there = (const int *)(here + 2 * B::TILEB + B::SCALES) + kg * 2 * NH;
-        int all = 1;
-#pragma unroll
-        for (int x = 0; x < 2 * NH; x++) all &= there[x];
-        if (key0 + 32 * NH <= wave_first && __builtin_amdgcn_readfirstlane(all)) tile(here, key0, std::false_type{});
-        else tile(here, key0, std::true_type{});
+        if (key0 < wave_last) tile(here, key0, std::true_type{});
     }
 
     l = xor32_sum(l);
@@ -330,5 +340,12 @@ template <typename T, int D> __global__ __launch_bounds__(256) void attn_kv4_ran
     if (r >= valid) x = uint2{0u, 0u};
     *(uint2 *)((T *)a.out + (((size_t)b * a.Hq + h * G + r % G) * a.Sq + r / G) * D + d) = x;
 }
+
+// Rows of a workgroup, blocks of rows of a kv head, and the ranges that their keys come in.
+struct Kv4TilePlan {
+    int rows, blocks, ranges;
+};
+// by type, a translation unit each (attention_kv4_go.h)
+template <typename T> int kv4_tile_go(const Kv4Args &a, int D, int group, const Kv4TilePlan &p, hipStream_t s);
 
 }  // namespace mynn

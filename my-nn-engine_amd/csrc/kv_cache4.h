@@ -19,10 +19,11 @@ struct PagedKv {
 // A sequence: rows [0, past) were there before, [past, len) are new.  (An int holds every sum below: a past that no cache could have is cut off.)
 struct PagedSeq {
     int past, fresh, len, cap;
-    __device__ PagedSeq(const PagedKv &c, int b, int S) {
+    __device__ PagedSeq(const PagedKv &c, int b, int S) : PagedSeq(c, c.past[b], c.fresh ? c.fresh[b] : S, S) {}
+    __device__ PagedSeq(const PagedKv &c, int past_len, int new_len, int S) {
         cap = c.pages_per_seq << c.page_shift;
-        past = min(max(c.past[b], -S), cap);
-        fresh = c.fresh ? min(max(c.fresh[b], 0), S) : S;
+        past = min(max(past_len, -S), cap);
+        fresh = min(max(new_len, 0), S);
         len = fresh ? min(max(past + fresh, 0), cap) : 0;
     }
     // keys that query row i sees
