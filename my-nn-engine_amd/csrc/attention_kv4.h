@@ -22,7 +22,9 @@ struct Kv4Args {
     int causal, B, Sq, Hq;
     float *part_o, *part_ml;  // parts of rows that several workgroups share
     int32_t *counters;        // [B * Hkv], zero between calls, or null: joined by a second launch
-    int grid;                 // workgroups
+    int grid;                 // workgroups of the form for few rows, those that run at once of the form for many
+    int blocks, ranges;       // the form for many rows: blocks of rows of a kv head, the most ranges that their keys come in
+    int *length;              // and how long a range is, as the first workgroup found it
 };
 
 // code - zero of a dword's eight, as Int4Pairs has them, each pair with zero points of its own (pairs (0,4), (1,5), (2,6), (3,7): off[0 .. 3])
@@ -38,10 +40,12 @@ __device__ __forceinline__ U4 kv4_pairs(uint32_t w, const h2_t *off, uint32_t ni
 __device__ __forceinline__ h2_t kv4_low(uint32_t zz) { return __builtin_bit_cast(h2_t, (zz & 0x000F000Fu) | 0xE400E400u); }
 __device__ __forceinline__ h2_t kv4_high(uint32_t zz) { return __builtin_bit_cast(h2_t, ((zz << 4) & 0x00F000F0u) | 0xD400D400u); }
 
+// The reference may lag 2^4 behind: moving it moves every sum, and a row meets a new maximum every few keys for long.  (2^14 on top of the largest weight then is 2^10.)
+constexpr float kKv4Lag = 4.f;
 // The scale's part in the reference, from its bits: exponent and mantissa of T as one number are log2 of it, less than 0.09 too little (subnormal numbers of fp16: too much),
 // in steps of 2^-(bits of the mantissa) from kKv4Zero on.  |vs| of 2^-86 and less counts as 2^-86, so that p <= 2^100.
 template <typename T> constexpr float kKv4Step = std::is_same<T, f16_t>::value ? 0x1p-10f : 0x1p-7f;
-template <typename T> constexpr float kKv4Zero = std::is_same<T, f16_t>::value ? 15.f + 14.f : 127.f + 14.f;  // (what the reference is less than M: 2^14 on top)
+template <typename T> constexpr float kKv4Zero = std::is_same<T, f16_t>::value ? 15.f + 14.f : 127.f + 14.f;  // (what is taken off M: 2^14 on top)
 template <typename T> __device__ __forceinline__ uint32_t kv4_bits(uint32_t w, int hi) {
     const uint32_t x = __builtin_amdgcn_ubfe(w, hi ? 16 : 0, 15);
     return std::is_same<T, f16_t>::value ? x : max(x, (127u - 86u) << 7);

@@ -32,14 +32,14 @@ static int kv4_stream_grid(int B, int Hkv, int unit, long rows) {
     return (int)(units < most ? units : most);
 }
 
-// Ranges of keys where blocks of rows leave the device idle.
+// Up to as many ranges of keys as make four workgroups a CU where blocks of rows leave the device idle (two run at once; how many a block has is found by Kv4Ranges).
 static Kv4TilePlan kv4_tile_plan(int B, int Sq, int Hq, int Hkv, long rows) {
     const long R = (long)(Hq / Hkv) * Sq;
     Kv4TilePlan p;
     p.rows = R <= 64 ? 64 : 128;
     p.blocks = (int)((R + p.rows - 1) / p.rows);
-    const long wgs = (long)B * Hkv * p.blocks, most = (rows + 255) / 256, want = 2l * kv4_cus() / wgs;
-    p.ranges = (int)(want < 1 ? 1 : want > most ? most : want);
+    const long wgs = (long)B * Hkv * p.blocks, most = (rows + 127) / 128, want = 4l * kv4_cus() / wgs;
+    p.ranges = (int)(want < 2 ? 1 : want > most ? most : want);
     return p;
 }
 
@@ -68,7 +68,7 @@ extern "C" int mynn_attention_paged_int4(void *out, const void *Q, const uint8_t
                  num_q_heads, num_kv_heads);
     Kv4Args a{{(void *)k_pool, (void *)v_pool, (void *)k_scale_pool, (void *)v_scale_pool, (uint8_t *)k_zero_pool, (uint8_t *)v_zero_pool, page_table, past_lens, new_lens,
                n_pages, pages_per_seq, 0, num_kv_heads},
-              out, Q, scale, is_causal, B, Sq, num_q_heads, nullptr, nullptr, nullptr, 0};
+              out, Q, scale, is_causal, B, Sq, num_q_heads, nullptr, nullptr, nullptr, 0, 0, 0, nullptr};
     if (const int rc = paged_kv_check(who, a.c, page_rows, 4, group, head_dim)) return rc;
     MYNN_REQUIRE(dtype == MYNN_F16 || dtype == MYNN_BF16, MYNN_ERR_UNSUPPORTED, "%s: dtype %d: a 16-bit float type", who, dtype);
     a.c.page_shift = paged_shift(page_rows);
@@ -88,7 +88,12 @@ extern "C" int mynn_attention_paged_int4(void *out, const void *Q, const uint8_t
         return dtype == MYNN_F16 ? kv4_stream_go<f16_t>(a, head_dim, group, fold, as_stream(s)) : kv4_stream_go<bf16_t>(a, head_dim, group, fold, as_stream(s));
     }
     const Kv4TilePlan plan = kv4_tile_plan(B, Sq, num_q_heads, num_kv_heads, rows);
-    MYNN_REQUIRE(plan.blocks <= 65535 && plan.ranges <= 65535, MYNN_ERR_UNSUPPORTED, "%s: Sq=%d heads %d/%d", who, Sq, num_q_heads, num_kv_heads);
-    a.part_ml = a.part_o + (size_t)plan.ranges * B * num_kv_heads * R * head_dim;
+    MYNN_REQUIRE((long)B * num_kv_heads * plan.blocks * plan.ranges < 1l << 24, MYNN_ERR_UNSUPPORTED, "%s: B=%d Sq=%d heads %d/%d", who, B, Sq, num_q_heads, num_kv_heads);
+    a.grid = 2 * kv4_cus();
+    a.blocks = plan.blocks;
+    a.ranges = plan.ranges;
+    const size_t lines = (size_t)plan.ranges * B * num_kv_heads * R;
+    a.part_ml = a.part_o + lines * head_dim;
+    a.length = (int *)(a.part_ml + lines * 2);
     return dtype == MYNN_F16 ? kv4_tile_go<f16_t>(a, head_dim, group, plan, as_stream(s)) : kv4_tile_go<bf16_t>(a, head_dim, group, plan, as_stream(s));
 }

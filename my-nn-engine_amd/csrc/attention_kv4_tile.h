@@ -14,7 +14,8 @@
 namespace mynn {
 
 template <int D, int NG, int QW, int KW, int KEYS> struct Kv4Block {
-    static constexpr int ROWB = D * 2, TILEB = KEYS * ROWB, THREADS = QW * KW * 64, ROWS = QW * 32, NH = KEYS / 32 / KW, UNITS = KEYS * 4 / THREADS;
+    static constexpr int ROWB = D * 2, TILEB = KEYS * ROWB, THREADS = QW * KW * 64, ROWS = QW * 32, NH = KEYS / 32 / KW;
+    static constexpr int UNITS = KEYS * 4 / THREADS;  // a thread stages a quarter of a row, of K and of V
     static constexpr int SCALES = (2 * NG + 1) * KEYS * 4, FLAGS = KEYS / 16 * 4;
     static constexpr int STAGE = 2 * TILEB + SCALES + FLAGS;
     static constexpr int WORDS = D / 2 + 2;  // of a lane's result: reference, sum, O^T
@@ -23,29 +24,66 @@ template <int D, int NG, int QW, int KW, int KEYS> struct Kv4Block {
     static_assert(NH >= 1 && UNITS >= 1 && STAGE % 16 == 0, "whole 32s of keys a wave, whole quarter rows a thread");
 };
 
+// Keys of a range in tiles: ranges of about the same length in all blocks of the call, so many that the workgroups all run at once.  (The lengths are known on the device alone;
+// a wave adds them up, 64 sequences at a time.)
+__device__ inline int kv4_range_length(const Kv4Args &a, int rows, int keys, int lane) {
+    const int G = a.Hq / a.c.Hkv;
+    float sum = 0.f;
+    for (int b0 = 0; b0 < a.B; b0 += 64) {
+        float x = 0.f;
+        if (b0 + lane < a.B) {
+            const PagedSeq s(a.c, b0 + lane, a.Sq);
+            const int middle = s.fresh ? s.bound(s.fresh / 2, a.causal) : 0;
+            x = (float)((s.fresh * G + rows - 1) / rows) * (float)((middle + keys - 1) / keys);
+        }
+        sum += wave_sum(x);
+    }
+    return __builtin_amdgcn_readfirstlane(max(2, (int)ceilf(sum * (float)a.c.Hkv / (0.875f * (float)a.grid))));
+}
+__device__ __forceinline__ int kv4_ranges(int tiles, int length, int most) { return min(max((tiles + length - 1) / length, 1), most); }
+
 template <typename T, int D, int NG, int QW, int KW, int KEYS> __global__ __launch_bounds__(QW *KW * 64, 2) void attn_kv4_tile_kernel(Kv4Args a) {
     using B = Kv4Block<D, NG, QW, KW, KEYS>;
     constexpr int KS = D / 16, DT = D / 32, NH = B::NH, DW = D / 32, ROWB = B::ROWB, KPG = KS / NG, TPG = DT / NG;
     extern __shared__ __align__(16) char sm[];
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), wave = w % QW, kg = w / QW, col = lane & 31, g = lane >> 5;
     const int G = a.Hq / a.c.Hkv, R = G * a.Sq;
-    const int b = blockIdx.x / a.c.Hkv, h = blockIdx.x % a.c.Hkv, nz = gridDim.z;
-    const int row0 = ((int)gridDim.y - 1 - (int)blockIdx.y) * B::ROWS;  // (the rows with the most keys are dispatched first)
+    // kv heads next to each other (XCDs take turns: one works on as few heads as it goes), blocks of rows with the most keys first.
+    const int i0 = blockIdx.x, i1 = i0 / a.c.Hkv, h = i0 - i1 * a.c.Hkv;
+    int b, block, range = 0;
+    if (a.c.fresh || a.ranges > 1) {
+        // Sequences outermost.  Inside the blocks those of a short one, which end at once, take every other place on the shader engines: 2 pieces of prompts, 512 rows and 79,
+        // 91 us instead of 76, 8 of up to 1024 rows 284 instead of 202 (227 with the sequences taking turns).
+        const int i2 = i1 / a.blocks;
+        block = i1 - i2 * a.blocks, b = i2 / a.ranges, range = i2 - b * a.ranges;
+    } else {
+        // All blocks have rows: sequences inside the blocks, taking turns, and the heaviest of all go first (4 x 2048 rows, four times as many workgroups as run at once, 220 us;
+        // outermost 230).
+        block = i1 / a.B, b = (i1 - block * a.B + block / 2) % a.B;
+    }
+    const int row0 = (a.blocks - 1 - block) * B::ROWS;
+    int length = 0;
+    if (a.ranges > 1) {
+        length = kv4_range_length(a, B::ROWS, KEYS, lane);
+        if (i0 == 0 && tid == 0) *a.length = length;
+    }
     const PagedSeq seq(a.c, b, a.Sq);
     const int valid = seq.fresh * G;  // rows behind it are zeros
     auto out_row = [&](int r) { return (T *)a.out + (((size_t)b * a.Hq + h * G + r % G) * a.Sq + r / G) * D; };
     if (row0 >= valid) {
-        if (blockIdx.z == 0)
+        if (range == 0)
             for (int x = tid; x < min(B::ROWS, R - row0) * (D / 8); x += B::THREADS) *(U4 *)(out_row(row0 + x / (D / 8)) + x % (D / 8) * 8) = U4{0u, 0u, 0u, 0u};
         return;
     }
     auto bound_of = [&](int r) { return seq.bound(min(r, valid - 1) / G, a.causal); };
     const int ntiles = (bound_of(row0 + B::ROWS - 1) + KEYS - 1) / KEYS;
-    const int t0 = (int)((long)ntiles * blockIdx.z / nz), t1 = (int)((long)ntiles * (blockIdx.z + 1) / nz);
+    const int nz = a.ranges > 1 ? kv4_ranges(ntiles, length, a.ranges) : 1;
+    if (range >= nz) return;
+    const int t0 = (int)((long)ntiles * range / nz), t1 = (int)((long)ntiles * (range + 1) / nz);
     const int row = row0 + 32 * wave + col, row_c = min(row, valid - 1);
     const int bound = bound_of(row), wave_last = row0 + 32 * wave < valid ? bound_of(row0 + 32 * wave + 31) : 0;
 
-    // ---- staging: a thread has a quarter of a row of K and of V, UNITS times
+    // ---- staging
     constexpr int QUARTERS = B::THREADS / 4;
     const int quarter = tid & 3, sg = quarter * NG / 4;
     const int psh = a.c.page_shift, pmask = (1 << psh) - 1;
@@ -57,15 +95,14 @@ template <typename T, int D, int NG, int QW, int KW, int KEYS> __global__ __laun
         all_there = all_there && __builtin_amdgcn_ballot_w64((unsigned)x >= (unsigned)a.c.n_pages) == 0;
     }
     struct Raw {
-        uint32_t k[DW], v[DW];
-        T ks, vs;
-        uint8_t kz, vz;
-        int there;
-    } raw[B::UNITS];
+        uint32_t codes[DW];
+        T scale;
+        uint8_t zero;
+    } raw[B::UNITS][2];  // keys, values
+    int raw_there[B::UNITS];
     auto load = [&](int t) __attribute__((always_inline)) {
 #pragma unroll
         for (int u = 0; u < B::UNITS; u++) {
-            Raw &x = raw[u];
             // (a wave's 16 rows lie in one page)
             const int first = t * KEYS + u * QUARTERS + 16 * w, p = first >> psh;
             if (p - pages_at >= 64 || p < pages_at) {
@@ -74,40 +111,43 @@ template <typename T, int D, int NG, int QW, int KW, int KEYS> __global__ __laun
                 if ((unsigned)pages >= (unsigned)a.c.n_pages) pages = -1;
             }
             const int page = __builtin_amdgcn_readlane(pages, p - pages_at);
-            x.there = page >= 0;
+            raw_there[u] = page >= 0;
             const size_t r = (((size_t)max(page, 0) * a.c.Hkv + h) << psh) + (size_t)(first & pmask) + (lane >> 2);
-            __builtin_memcpy(&x.k, __builtin_assume_aligned((const uint8_t *)a.c.k + r * (D / 2) + quarter * (D / 8), D / 8), D / 8);
-            __builtin_memcpy(&x.v, __builtin_assume_aligned((const uint8_t *)a.c.v + r * (D / 2) + quarter * (D / 8), D / 8), D / 8);
-            x.ks = ((const T *)a.c.k_scale)[r * NG + sg];
-            x.vs = ((const T *)a.c.v_scale)[r * NG + sg];
-            x.kz = a.c.k_zero[r * NG + sg];
-            x.vz = a.c.v_zero[r * NG + sg];
+#pragma unroll
+            for (int n = 0; n < 2; n++) {
+                Raw &x = raw[u][n];
+                const bool v = n == 1;
+                __builtin_memcpy(&x.codes, __builtin_assume_aligned((const uint8_t *)(v ? a.c.v : a.c.k) + r * (D / 2) + quarter * (D / 8), D / 8), D / 8);
+                x.scale = ((const T *)(v ? a.c.v_scale : a.c.k_scale))[r * NG + sg];
+                x.zero = (v ? a.c.v_zero : a.c.k_zero)[r * NG + sg];
+            }
         }
     };
     auto k_swz = [](int r) { return D == 128 ? r & 15 : (r >> 1) & 7; };
     auto v_swz = [](int r) { return D == 128 ? (r & 3) * 5 : (((r >> 1) ^ r) & 1) << 2; };
     Int4Pairs pairs;
     auto store = [&](char *stage) __attribute__((always_inline)) {
-        float *ksc = (float *)(stage + 2 * B::TILEB), *vsc = ksc + NG * KEYS, *lift = vsc + NG * KEYS;
+        float *scales = (float *)(stage + 2 * B::TILEB), *lift = scales + 2 * NG * KEYS;
         int *there = (int *)(lift + KEYS);
 #pragma unroll
         for (int u = 0; u < B::UNITS; u++) {
-            const Raw &x = raw[u];
             const int r = u * QUARTERS + (tid >> 2);
-            pairs.at(x.kz & 15u);
 #pragma unroll
-            for (int i = 0; i < DW; i++) *(U4 *)(stage + r * ROWB + (((quarter * DW + i) ^ k_swz(r)) << 4)) = pairs(x.k[i]);
-            pairs.at(x.vz & 15u);
+            for (int n = 0; n < 2; n++) {
+                const Raw &x = raw[u][n];
+                const bool v = n == 1;
+                pairs.at(x.zero & 15u);
+                const int swz = v ? v_swz(r) : k_swz(r);
+                char *to = stage + (v ? B::TILEB : 0) + r * ROWB;
 #pragma unroll
-            for (int i = 0; i < DW; i++) *(U4 *)(stage + B::TILEB + r * ROWB + (((quarter * DW + i) ^ v_swz(r)) << 4)) = pairs(x.v[i]);
-            const float vs = Elem<T>::ld(&x.vs, 0);
-            if (quarter % (4 / NG) == 0) {
-                ksc[sg * KEYS + r] = Elem<T>::ld(&x.ks, 0);
-                vsc[sg * KEYS + r] = vs;
+                for (int i = 0; i < DW; i++) *(U4 *)(to + (((quarter * DW + i) ^ swz) << 4)) = pairs(x.codes[i]);
+                if (quarter % (4 / NG) == 0) scales[(v ? NG * KEYS : 0) + sg * KEYS + r] = Elem<T>::ld(&x.scale, 0);
+                if (v) {
+                    const float bits = group_max<4>((float)kv4_bits<T>(__builtin_bit_cast(uint16_t, x.scale), 0));
+                    if (quarter == 0) lift[r] = bits * kKv4Step<T>;
+                }
             }
-            const float bits = group_max<4>((float)kv4_bits<T>(__builtin_bit_cast(uint16_t, x.vs), 0));
-            if (quarter == 0) lift[r] = bits * kKv4Step<T>;
-            if (lane == 0) there[r >> 4] = x.there;
+            if (lane == 0) there[r >> 4] = raw_there[u];
         }
     };
     if (t0 < t1) load(t0);
@@ -200,7 +240,7 @@ template <typename T, int D, int NG, int QW, int KW, int KEYS> __global__ __laun
             }
         }
         top = xor32_max(top);
-        const bool up = top > M;
+        const bool up = top > M + kKv4Lag;
         if (__builtin_amdgcn_ballot_w64(up) != 0) {
             const float mn = up ? top : M, corr = up ? __builtin_amdgcn_exp2f(M - mn) : 1.f;
             M = mn;
@@ -210,7 +250,7 @@ template <typename T, int D, int NG, int QW, int KW, int KEYS> __global__ __laun
 #pragma unroll
                 for (int e = 0; e < 16; e++) o[t2][e] *= corr;
         }
-        const float ref = M == -INFINITY ? 0.f : M - kKv4Zero<T>;
+        const float ref = M == -INFINITY ? 0.f : M - (kKv4Zero<T> - kKv4Lag);
         float lt = 0.f;
 #pragma unroll
         for (int hf = 0; hf < NH; hf++)
@@ -293,8 +333,10 @@ template <typename T, int D, int NG, int QW, int KW, int KEYS> __global__ __laun
                 for (int e = 0; e < 16; e++) o[t2][e] = o[t2][e] * ca + from[(2 + 16 * t2 + e) * 64] * cb;
         }
     }
-    const float inv = nz > 1 ? 1.f : row >= valid || l == 0.f ? 0.f : 1.0f / l;
-    const size_t line = ((size_t)blockIdx.x * R + row) * nz + blockIdx.z;
+    // (The lane's place once more, from the wave: what it is known by at the start would be one register too many over the loops.)
+    const int place = __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0)), row_out = row0 + 32 * wave + (place & 31), gr = place >> 5;
+    const float inv = nz > 1 ? 1.f : row_out >= valid || l == 0.f ? 0.f : 1.0f / l;
+    const size_t line = (((size_t)b * a.c.Hkv + h) * R + row_out) * a.ranges + range;
 #pragma unroll
     for (int t2 = 0; t2 < DT; t2++)
 #pragma unroll
@@ -303,41 +345,60 @@ template <typename T, int D, int NG, int QW, int KW, int KEYS> __global__ __laun
             float x0 = o[t2][4 * e4], x2 = o[t2][4 * e4 + 1], x1 = o[t2][4 * e4 + 2], x3 = o[t2][4 * e4 + 3];
             permlane32_swap(x0, x2);
             permlane32_swap(x1, x3);
-            const int d = 32 * t2 + 8 * e4 + 4 * g;
-            if (row >= R) continue;
+            const int d = 32 * t2 + 8 * e4 + 4 * gr;
+            if (row_out >= R) continue;
             if (nz > 1) *(f4_t *)(a.part_o + line * D + d) = f4_t{x0, x1, x2, x3};
-            else if (row >= valid) *(uint2 *)(out_row(row) + d) = uint2{0u, 0u};
-            else *(uint2 *)(out_row(row) + d) = uint2{pack2<T>(x0 * inv, x1 * inv), pack2<T>(x2 * inv, x3 * inv)};
+            else if (row_out >= valid) *(uint2 *)(out_row(row_out) + d) = uint2{0u, 0u};
+            else *(uint2 *)(out_row(row_out) + d) = uint2{pack2<T>(x0 * inv, x1 * inv), pack2<T>(x2 * inv, x3 * inv)};
         }
-    if (nz > 1 && g == 0 && row < R) *(float2 *)(a.part_ml + line * 2) = float2{M, l};
+    if (nz > 1 && gr == 0 && row_out < R) *(float2 *)(a.part_ml + line * 2) = float2{M, l};
 }
 
-// Joins the ranges of keys of each row.  Rows of a block that has none of the sequence's own are zeros already.
-template <typename T, int D> __global__ __launch_bounds__(256) void attn_kv4_ranges_kernel(Kv4Args a, int nz, int block_rows) {
+// Joins the ranges of keys of each row.  Blocks with one range, or none of the sequence's own rows, are done already.
+template <typename T, int D> __global__ __launch_bounds__(256) void attn_kv4_ranges_kernel(Kv4Args a, int block_rows, int keys) {
     const int G = a.Hq / a.c.Hkv, R = G * a.Sq;
     const size_t at = (size_t)blockIdx.x * 256 + threadIdx.x, line = at / (D / 4);
     const int d = (int)(at % (D / 4)) * 4;
     if (line >= (size_t)a.B * a.c.Hkv * R) return;
-    const int pair = (int)(line / R), r = (int)(line % R), b = pair / a.c.Hkv, h = pair % a.c.Hkv;
+    const int most = a.ranges, pair = (int)(line / R), r = (int)(line % R), b = pair / a.c.Hkv, h = pair % a.c.Hkv;
     const PagedSeq seq(a.c, b, a.Sq);
-    const int valid = seq.fresh * G;
-    if (r / block_rows * block_rows >= valid) return;
-    const float *ml = a.part_ml + line * nz * 2, *po = a.part_o + line * nz * D + d;
-    float mt = -INFINITY;
-    for (int z = 0; z < nz; z++) mt = fmaxf(mt, ml[2 * z]);
-    float lt = 0.f;
+    const int valid = seq.fresh * G, row0 = r / block_rows * block_rows;
+    if (row0 >= valid) return;
+    const int nz = kv4_ranges((seq.bound((min(row0 + block_rows, valid) - 1) / G, a.causal) + keys - 1) / keys, *a.length, most);
+    if (nz == 1) return;
+    const uint64_t *ml = (const uint64_t *)a.part_ml + line * most;
+    const float *po = a.part_o + line * most * D + d;
+    auto lo = [](uint64_t w) { return __builtin_bit_cast(float, (uint32_t)w); };
+    float mt = -INFINITY, lt = 0.f;
     f4_t o = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-    for (int z = 0; z < nz; z++) {
-        const float c = ml[2 * z] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml[2 * z] - mt);
-        const f4_t oz = *(const f4_t *)(po + (size_t)z * D);
-        lt = fmaf(ml[2 * z + 1], c, lt);
+    // four ranges at a time, with a reference of their own
+    for (int z0 = 0; z0 < nz; z0 += 4) {
+        uint64_t w[4];
+        f4_t x[4];
 #pragma unroll
-        for (int e = 0; e < 4; e++) o[e] = fmaf(oz[e], c, o[e]);
+        for (int i = 0; i < 4; i++) {
+            const int z = min(z0 + i, nz - 1);
+            w[i] = ml[z];
+            x[i] = *(const f4_t *)(po + (size_t)z * D);
+        }
+        float mn = mt;
+#pragma unroll
+        for (int i = 0; i < 4; i++) mn = fmaxf(mn, lo(w[i]));
+        const float c0 = mt == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mt - mn);
+        mt = mn;
+        lt *= c0;
+        o *= c0;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const float c = lo(w[i]) == -INFINITY || z0 + i >= nz ? 0.f : __builtin_amdgcn_exp2f(lo(w[i]) - mt);
+            lt = fmaf(lo(w[i] >> 32), c, lt);
+#pragma unroll
+            for (int e = 0; e < 4; e++) o[e] = fmaf(x[i][e], c, o[e]);
+        }
     }
-    const float inv = r >= valid || lt == 0.f ? 0.f : 1.0f / lt;
+    const float inv = 1.0f / lt;
     uint2 x = uint2{pack2<T>(o[0] * inv, o[1] * inv), pack2<T>(o[2] * inv, o[3] * inv)};
-    if (r >= valid) x = uint2{0u, 0u};
+    if (r >= valid || lt == 0.f) x = uint2{0u, 0u};
     *(uint2 *)((T *)a.out + (((size_t)b * a.Hq + h * G + r % G) * a.Sq + r / G) * D + d) = x;
 }
 
