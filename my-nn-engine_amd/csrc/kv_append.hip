@@ -16,7 +16,7 @@ struct AppendArgs {
     long bs[3], hs[3], rs[3];  // their strides in elements: sequence, head, row
     const void *cos_t, *sin_t;
     const int64_t *position;
-    int table_rows, B, S, Hq, slots, per;  // slots * per >= heads
+    int table_rows, B, S, Hq;
 };
 
 template <typename T, bool ALIGNED> __device__ __forceinline__ U4 load8(const T *p) {
@@ -30,17 +30,19 @@ template <typename T> __device__ __forceinline__ U4 pack8(const float *f) {
     return U4{pack2<T>(f[0], f[1]), pack2<T>(f[2], f[3]), pack2<T>(f[4], f[5]), pack2<T>(f[6], f[7])};
 }
 
-// A head of a token is LPH = D/16 lanes': each has 8 dims of the lower half and the 8 that they are rotated with.  A thread has a token and
-// every `slots`-th head of it.
+// A head of a token is LPH = D/16 lanes': each has 8 dims of the lower half and the 8 that they are rotated with.
 template <typename T, int KV, int D, int GROUP, bool ALIGNED> __global__ __launch_bounds__(256) void rope_append_paged_kernel(AppendArgs a) {
     constexpr int LPH = D / 16, HALF = D / 2;
-    const size_t at = (size_t)blockIdx.x * 256 + threadIdx.x;
-    const size_t item = at / LPH;
-    const int u = (int)(at % LPH);
-    const int heads = a.Hq + 2 * a.c.Hkv, first = a.q_out ? 0 : a.Hq;
-    const size_t token = item / a.slots;
-    if (token >= (size_t)a.B * a.S) return;  // (whole heads: the lanes of one meet below)
-    const int b = (int)(token / a.S), i = (int)(token % a.S);
+    // (32 bits, as many as there can be threads: dividing 64 took longer than everything else)
+    const uint32_t at = blockIdx.x * 256u + threadIdx.x, item = at / LPH, u = at % LPH;
+    const uint32_t heads = (a.q_out ? a.Hq : 0) + 2 * a.c.Hkv, token = item / heads;
+    if (token >= (uint32_t)(a.B * a.S)) return;  // (whole heads: the lanes of one meet below)
+    const int head = (int)(item - token * heads) + (a.q_out ? 0 : a.Hq), b = (int)(token / (uint32_t)a.S), i = (int)(token - (uint32_t)b * a.S);
+    const int part = head < a.Hq ? 0 : head < a.Hq + a.c.Hkv ? 1 : 2;
+    const int h = part == 0 ? head : part == 1 ? head - a.Hq : head - a.Hq - a.c.Hkv;
+    // (on its way before it is known whether the token is there)
+    const T *src = (const T *)a.x[part] + (long)b * a.bs[part] + (long)h * a.hs[part] + (long)i * a.rs[part] + 8 * u;
+    U4 lo = load8<T, ALIGNED>(src), hi = load8<T, ALIGNED>(src + HALF);
     const PagedSeq seq(a.c, b, a.S);
     const int row = seq.past + i;
     const int64_t pos = a.position ? a.position[token] : (int64_t)row;
@@ -55,135 +57,131 @@ template <typename T, int KV, int D, int GROUP, bool ALIGNED> __global__ __launc
         widen8<T>(load8<T, ALIGNED>(st), sl);
         widen8<T>(load8<T, ALIGNED>(st + HALF), sh);
     }
-    for (int head = first + (int)(item % a.slots); head < heads; head += a.slots) {
-        const int part = head < a.Hq ? 0 : head < a.Hq + a.c.Hkv ? 1 : 2;
-        const int h = part == 0 ? head : part == 1 ? head - a.Hq : head - a.Hq - a.c.Hkv;
-        T *q_row = part == 0 ? (T *)a.q_out + (((size_t)b * a.Hq + h) * a.S + i) * D + 8 * u : nullptr;
-        if (!there || (part && page < 0)) {
-            if (part == 0) *(U4 *)q_row = *(U4 *)(q_row + HALF) = U4{0u, 0u, 0u, 0u};
-            continue;
+    T *q_row = part == 0 ? (T *)a.q_out + (((size_t)b * a.Hq + h) * a.S + i) * D + 8 * u : nullptr;
+    if (!there || (part && page < 0)) {
+        if (part == 0) *(U4 *)q_row = *(U4 *)(q_row + HALF) = U4{0u, 0u, 0u, 0u};
+        return;
+    }
+    float xl[8], xh[8];
+    if (part < 2) {
+        float ol[8], oh[8];
+        widen8<T>(lo, xl);
+        widen8<T>(hi, xh);
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            ol[e] = xl[e] * cl[e] - xh[e] * sl[e];
+            oh[e] = xh[e] * ch[e] + xl[e] * sh[e];
         }
-        const T *src = (const T *)a.x[part] + (long)b * a.bs[part] + (long)h * a.hs[part] + (long)i * a.rs[part] + 8 * u;
-        U4 lo = load8<T, ALIGNED>(src), hi = load8<T, ALIGNED>(src + HALF);
-        float xl[8], xh[8];
-        if (part < 2) {
-            float ol[8], oh[8];
-            widen8<T>(lo, xl);
-            widen8<T>(hi, xh);
+        lo = pack8<T>(ol);
+        hi = pack8<T>(oh);
+    }
+    if (part == 0) {
+        *(U4 *)q_row = lo;
+        *(U4 *)(q_row + HALF) = hi;
+        return;
+    }
+    const size_t r = paged_row(a.c, page, h, row);
+    void *pool = part == 1 ? a.c.k : a.c.v, *scales = part == 1 ? a.c.k_scale : a.c.v_scale;
+    if constexpr (KV == 16) {
+        T *dst = (T *)pool + r * D + 8 * u;
+        *(U4 *)dst = lo;
+        *(U4 *)(dst + HALF) = hi;
+    } else {
+        widen8<T>(lo, xl);
+        widen8<T>(hi, xh);
+        if constexpr (KV == 8) {
+            float peak = 0.f;
+#pragma unroll
+            for (int e = 0; e < 8; e++) peak = fmaxf(peak, fmaxf(fabsf(xl[e]), fabsf(xh[e])));
+            peak = group_max<LPH>(peak);
+            const float inv = peak == 0.f ? 0.f : 127.0f / peak;
+            auto code = [&](float x) -> uint32_t {
+                const float y = x * inv;
+                const int q = (int)(y + (y >= 0.f ? 0.5f : -0.5f));
+                return (uint32_t)(q < -128 ? -128 : (q > 127 ? 127 : q)) & 0xFFu;
+            };
+            auto four = [&](const float *x) { return code(x[0]) | code(x[1]) << 8 | code(x[2]) << 16 | code(x[3]) << 24; };
+            uint8_t *dst = (uint8_t *)pool + r * D + 8 * u;
+            *(uint2 *)dst = uint2{four(xl), four(xl + 4)};
+            *(uint2 *)(dst + HALF) = uint2{four(xh), four(xh + 4)};
+            if (u == 0) Elem<T>::st((T *)scales, r, peak * (1.0f / 127.0f));
+        } else {
+            // groups: all of the row (both halves of every lane), a half of it (a half of every lane), a quarter (a half of half the lanes)
+            constexpr int GROUPS = D / GROUP;
+            float lo0 = 0.f, hi0 = 0.f, lo1 = 0.f, hi1 = 0.f;
+            float bad0 = 0.f, bad1 = 0.f;  // 0 * x: NaN where x is not finite
 #pragma unroll
             for (int e = 0; e < 8; e++) {
-                ol[e] = xl[e] * cl[e] - xh[e] * sl[e];
-                oh[e] = xh[e] * ch[e] + xl[e] * sh[e];
+                lo0 = fminf(lo0, xl[e]), hi0 = fmaxf(hi0, xl[e]), bad0 += 0.f * xl[e];
+                lo1 = fminf(lo1, xh[e]), hi1 = fmaxf(hi1, xh[e]), bad1 += 0.f * xh[e];
             }
-            lo = pack8<T>(ol);
-            hi = pack8<T>(oh);
-        }
-        if (part == 0) {
-            *(U4 *)q_row = lo;
-            *(U4 *)(q_row + HALF) = hi;
-            continue;
-        }
-        const size_t r = paged_row(a.c, page, h, row);
-        void *pool = part == 1 ? a.c.k : a.c.v, *scales = part == 1 ? a.c.k_scale : a.c.v_scale;
-        if constexpr (KV == 16) {
-            T *dst = (T *)pool + r * D + 8 * u;
-            *(U4 *)dst = lo;
-            *(U4 *)(dst + HALF) = hi;
-        } else {
-            widen8<T>(lo, xl);
-            widen8<T>(hi, xh);
-            if constexpr (KV == 8) {
-                float peak = 0.f;
+            constexpr int LANES = GROUPS == 4 ? LPH / 2 : LPH;
+            lo0 = -group_max<LANES>(-lo0), hi0 = group_max<LANES>(hi0), bad0 = group_sum<LANES>(bad0);
+            lo1 = -group_max<LANES>(-lo1), hi1 = group_max<LANES>(hi1), bad1 = group_sum<LANES>(bad1);
+            if constexpr (GROUPS == 1) lo0 = lo1 = fminf(lo0, lo1), hi0 = hi1 = fmaxf(hi0, hi1), bad0 = bad1 = bad0 + bad1;
+            const Int4Row<T> g0(lo0, hi0, bad0 == 0.f), g1(lo1, hi1, bad1 == 0.f);
+            uint32_t w0 = 0, w1 = 0;
 #pragma unroll
-                for (int e = 0; e < 8; e++) peak = fmaxf(peak, fmaxf(fabsf(xl[e]), fabsf(xh[e])));
-                peak = group_max<LPH>(peak);
-                const float inv = peak == 0.f ? 0.f : 127.0f / peak;
-                auto code = [&](float x) -> uint32_t {
-                    const float y = x * inv;
-                    const int q = (int)(y + (y >= 0.f ? 0.5f : -0.5f));
-                    return (uint32_t)(q < -128 ? -128 : (q > 127 ? 127 : q)) & 0xFFu;
-                };
-                auto four = [&](const float *x) { return code(x[0]) | code(x[1]) << 8 | code(x[2]) << 16 | code(x[3]) << 24; };
-                uint8_t *dst = (uint8_t *)pool + r * D + 8 * u;
-                *(uint2 *)dst = uint2{four(xl), four(xl + 4)};
-                *(uint2 *)(dst + HALF) = uint2{four(xh), four(xh + 4)};
-                if (u == 0) Elem<T>::st((T *)scales, r, peak * (1.0f / 127.0f));
-            } else {
-                // groups: all of the row (both halves of every lane), a half of it (a half of every lane), a quarter (a half of half the lanes)
-                constexpr int GROUPS = D / GROUP;
-                float lo0 = 0.f, hi0 = 0.f, lo1 = 0.f, hi1 = 0.f;
-                float bad0 = 0.f, bad1 = 0.f;  // 0 * x: NaN where x is not finite
-#pragma unroll
-                for (int e = 0; e < 8; e++) {
-                    lo0 = fminf(lo0, xl[e]), hi0 = fmaxf(hi0, xl[e]), bad0 += 0.f * xl[e];
-                    lo1 = fminf(lo1, xh[e]), hi1 = fmaxf(hi1, xh[e]), bad1 += 0.f * xh[e];
-                }
-                constexpr int LANES = GROUPS == 4 ? LPH / 2 : LPH;
-                lo0 = -group_max<LANES>(-lo0), hi0 = group_max<LANES>(hi0), bad0 = group_sum<LANES>(bad0);
-                lo1 = -group_max<LANES>(-lo1), hi1 = group_max<LANES>(hi1), bad1 = group_sum<LANES>(bad1);
-                if constexpr (GROUPS == 1) lo0 = lo1 = fminf(lo0, lo1), hi0 = hi1 = fmaxf(hi0, hi1), bad0 = bad1 = bad0 + bad1;
-                const Int4Row<T> g0(lo0, hi0, bad0 == 0.f), g1(lo1, hi1, bad1 == 0.f);
-                uint32_t w0 = 0, w1 = 0;
-#pragma unroll
-                for (int e = 0; e < 8; e++) w0 |= g0.code(xl[e]) << (4 * e), w1 |= g1.code(xh[e]) << (4 * e);
-                uint8_t *dst = (uint8_t *)pool + r * (D / 2) + 4 * u;
-                *(uint32_t *)dst = w0;
-                *(uint32_t *)(dst + HALF / 2) = w1;
-                if (u % LANES == 0) {
-                    T *sc = (T *)scales + r * GROUPS;
-                    uint8_t *zp = (part == 1 ? a.c.k_zero : a.c.v_zero) + r * GROUPS;
-                    const int g = GROUPS == 4 ? u / LANES : 0;
-                    Elem<T>::st(sc, g, g0.s);
-                    zp[g] = (uint8_t)g0.z;
-                    if constexpr (GROUPS > 1) {
-                        Elem<T>::st(sc, GROUPS / 2 + g, g1.s);
-                        zp[GROUPS / 2 + g] = (uint8_t)g1.z;
-                    }
+            for (int e = 0; e < 8; e++) w0 |= g0.code(xl[e]) << (4 * e), w1 |= g1.code(xh[e]) << (4 * e);
+            uint8_t *dst = (uint8_t *)pool + r * (D / 2) + 4 * u;
+            *(uint32_t *)dst = w0;
+            *(uint32_t *)(dst + HALF / 2) = w1;
+            if (u % LANES == 0) {
+                T *sc = (T *)scales + r * GROUPS;
+                uint8_t *zp = (part == 1 ? a.c.k_zero : a.c.v_zero) + r * GROUPS;
+                const int g = GROUPS == 4 ? u / LANES : 0;
+                Elem<T>::st(sc, g, g0.s);
+                zp[g] = (uint8_t)g0.z;
+                if constexpr (GROUPS > 1) {
+                    Elem<T>::st(sc, GROUPS / 2 + g, g1.s);
+                    zp[GROUPS / 2 + g] = (uint8_t)g1.z;
                 }
             }
         }
     }
 }
 
-// rows first .. first + n - 1 of each sequence as plain rows; a thread has 8 columns
+// rows first .. first + n - 1 of each sequence as plain rows; a thread has 8 columns of k, of v or of both
 template <typename T, int KV> __global__ __launch_bounds__(256) void kv_rows_paged_kernel(PagedKv c, T *k_out, T *v_out, int B, int S, int D, int group) {
-    const int chunks = D / 8;
-    const size_t n = (size_t)B * c.Hkv * S * chunks;
-    size_t at = (size_t)blockIdx.x * 256 + threadIdx.x;
-    const bool second = at >= n;
-    if (second) at -= n;
-    if (at >= n) return;
-    const bool is_v = second || !k_out;
-    T *out = is_v ? v_out : k_out;
-    const int d = (int)(at % chunks) * 8;
-    const size_t line = at / chunks;
-    const int i = (int)(line % S), h = (int)(line / S % c.Hkv), b = (int)(line / S / c.Hkv);
+    const uint32_t at = blockIdx.x * 256u + threadIdx.x, chunks = D / 8, line = at / chunks, pair = line / (uint32_t)S, b = pair / (uint32_t)c.Hkv;
+    if (b >= (uint32_t)B) return;
+    const int d = (int)(at - line * chunks) * 8, i = (int)(line - pair * S), h = (int)(pair - b * c.Hkv);
     const PagedSeq seq(c, b, S);
     const int row = seq.past + i;
     const int page = i < seq.fresh && row >= 0 && row < seq.cap ? paged_page(c, b, row) : -1;
-    U4 y = {0u, 0u, 0u, 0u};
-    if (page >= 0) {
-        const size_t r = paged_row(c, page, h, row);
-        const void *pool = is_v ? c.v : c.k, *scales = is_v ? c.v_scale : c.k_scale;
-        if constexpr (KV == 16) y = *(const U4 *)((const T *)pool + r * D + d);
-        else {
-            float f[8];
-            if constexpr (KV == 8) {
-                const uint2 w = *(const uint2 *)((const int8_t *)pool + r * D + d);
-                const float s = Elem<T>::ld((const T *)scales, r);
+    const size_t r = page >= 0 ? paged_row(c, page, h, row) : 0;
+    T *const out[2] = {k_out, v_out};
+    U4 w[2] = {};
+    float s[2], z[2];
 #pragma unroll
-                for (int e = 0; e < 8; e++) f[e] = (float)(int8_t)((e < 4 ? w.x : w.y) >> (8 * (e & 3)) & 0xFFu) * s;
-            } else {
-                const uint32_t w = *(const uint32_t *)((const uint8_t *)pool + (r * D + d) / 2);
-                const size_t g = r * (D / group) + d / group;
-                const float s = Elem<T>::ld((const T *)scales, g), z = (float)((is_v ? c.v_zero : c.k_zero)[g] & 15);
-#pragma unroll
-                for (int e = 0; e < 8; e++) f[e] = ((float)(w >> (4 * e) & 15u) - z) * s;
-            }
-            y = pack8<T>(f);
+    for (int n = 0; n < 2; n++) {
+        if (!out[n] || page < 0) continue;
+        const void *pool = n ? c.v : c.k, *scales = n ? c.v_scale : c.k_scale;
+        if constexpr (KV == 16) w[n] = *(const U4 *)((const T *)pool + r * D + d);
+        else if constexpr (KV == 8) {
+            const uint2 x = *(const uint2 *)((const int8_t *)pool + r * D + d);
+            w[n].x = x.x, w[n].y = x.y;
+            s[n] = Elem<T>::ld((const T *)scales, r);
+        } else {
+            const size_t g = r * (D / group) + d / group;
+            w[n].x = *(const uint32_t *)((const uint8_t *)pool + (r * D + d) / 2);
+            s[n] = Elem<T>::ld((const T *)scales, g);
+            z[n] = (float)((n ? c.v_zero : c.k_zero)[g] & 15);
         }
     }
-    *(U4 *)(out + line * D + d) = y;
+#pragma unroll
+    for (int n = 0; n < 2; n++) {
+        if (!out[n]) continue;
+        U4 y = w[n];
+        if (KV < 16 && page >= 0) {
+            float f[8];
+#pragma unroll
+            for (int e = 0; e < 8; e++)
+                f[e] = KV == 8 ? (float)(int8_t)((e < 4 ? w[n].x : w[n].y) >> (8 * (e & 3)) & 0xFFu) * s[n] : ((float)(w[n].x >> (4 * e) & 15u) - z[n]) * s[n];
+            y = pack8<T>(f);
+        }
+        *(U4 *)(out[n] + (size_t)line * D + d) = y;
+    }
 }
 
 // what every call over pools asks of them
@@ -228,7 +226,7 @@ extern "C" int mynn_rope_append_paged(void *q_out, const void *q, const void *k,
     MYNN_REQUIRE(B > 0 && S > 0 && num_q_heads > 0 && num_kv_heads > 0 && table_rows > 0, MYNN_ERR_INVALID, "%s: B=%d S=%d heads %d/%d, %d table rows", who, B, S,
                  num_q_heads, num_kv_heads, table_rows);
     AppendArgs a{{k_pool, v_pool, k_scale_pool, v_scale_pool, k_zero_pool, v_zero_pool, page_table, past_lens, new_lens, n_pages, pages_per_seq, 0, num_kv_heads},
-                 q_out, {q, k, v}, {}, {}, {}, cos_t, sin_t, position, table_rows, B, S, num_q_heads, 0, 0};
+                 q_out, {q, k, v}, {}, {}, {}, cos_t, sin_t, position, table_rows, B, S, num_q_heads};
     if (const int rc = paged_kv_check(who, a.c, page_rows, kv_bits, group, D)) return rc;
     a.c.page_shift = paged_shift(page_rows);
     MYNN_REQUIRE(num_q_heads <= 65536 && num_kv_heads <= 65536 && S <= 1 << 30, MYNN_ERR_UNSUPPORTED, "%s: S=%d heads %d/%d", who, S, num_q_heads, num_kv_heads);
@@ -239,10 +237,8 @@ extern "C" int mynn_rope_append_paged(void *q_out, const void *q, const void *k,
     }
     MYNN_REQUIRE(!q_out || aligned16(q_out), MYNN_ERR_INVALID, "%s: q_out has to be 16-byte aligned", who);
     const int heads = (q ? num_q_heads : 0) + 2 * num_kv_heads;
-    a.per = 1;
-    a.slots = heads;
-    const size_t threads = (size_t)B * S * a.slots * (D / 16), blocks = (threads + 255) / 256;
-    MYNN_REQUIRE(blocks < 1u << 31, MYNN_ERR_UNSUPPORTED, "%s: %d x %d tokens of %d heads", who, B, S, heads);
+    const size_t blocks = ((size_t)B * S * heads * (D / 16) + 255) / 256;
+    MYNN_REQUIRE(blocks < 1u << 24, MYNN_ERR_UNSUPPORTED, "%s: %d x %d tokens of %d heads", who, B, S, heads);
     return dispatch_dtype16(dtype, [&](auto *t) {
         using T = std::remove_pointer_t<decltype(t)>;
         auto go = [&](auto d) {
@@ -270,8 +266,8 @@ extern "C" int mynn_kv_rows_paged(void *k_out, void *v_out, const void *k_pool, 
     if (const int rc = paged_kv_check(who, c, page_rows, kv_bits, group, head_dim)) return rc;
     c.page_shift = paged_shift(page_rows);
     MYNN_REQUIRE(num_kv_heads <= 65536 && S <= 1 << 30, MYNN_ERR_UNSUPPORTED, "%s: S=%d kv heads %d", who, S, num_kv_heads);
-    const size_t threads = (size_t)B * num_kv_heads * S * (head_dim / 8) * ((k_out != nullptr) + (v_out != nullptr)), blocks = (threads + 255) / 256;
-    MYNN_REQUIRE(blocks < 1u << 31, MYNN_ERR_UNSUPPORTED, "%s: %d x %d rows of %d heads", who, B, S, num_kv_heads);
+    const size_t threads = (size_t)B * num_kv_heads * S * (head_dim / 8), blocks = (threads + 255) / 256;
+    MYNN_REQUIRE(blocks < 1u << 24, MYNN_ERR_UNSUPPORTED, "%s: %d x %d rows of %d heads", who, B, S, num_kv_heads);
     return dispatch_dtype16(dtype, [&](auto *t) {
         using T = std::remove_pointer_t<decltype(t)>;
         const dim3 grid((unsigned)blocks);
