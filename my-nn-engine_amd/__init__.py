@@ -757,18 +757,17 @@ def kv_rows_paged(pools, table, first_rows, n, n_rows=None):
     return k, v
 
 
+PAGED_INT4_COUNTER_BYTES = 4 * 512  # MYNN_PAGED_INT4_COUNTERS
+
+
 def attention_paged_int4_workspace(q, pools, table):
-    """Memory for attention_paged_int4 on operands like these, to be kept from call to call (one for calls that may overlap each): its first words
-    are counters, zero here and zero again behind every call."""
+    """Memory for attention_paged_int4 on operands like these, and on others that need no more, to be kept from call to call (one each for calls that
+    may overlap): its first words are counters, zero here and zero again behind every call."""
     B, Hq, Sq, D = q.shape
     pages = table.pages_per_seq if isinstance(table, KvPages) else table.shape[1]
     Hkv, rows = pools[0].shape[1:3]
     need = lib().mynn_attention_paged_int4_workspace_bytes(B, Sq, pages, rows, Hq, Hkv, D)
-    return _t().zeros((_counter_bytes(B, Hkv) + need,), dtype=_torch.uint8, device=q.device)
-
-
-def _counter_bytes(B, Hkv):
-    return (4 * B * Hkv + 255) // 256 * 256
+    return _t().zeros((PAGED_INT4_COUNTER_BYTES + need,), dtype=_torch.uint8, device=q.device)
 
 
 def attention_paged_int4(q, pools, table, scale, past_lens, new_lens=None, is_causal=True, workspace=None, out=None):
@@ -794,7 +793,7 @@ def attention_paged_int4(q, pools, table, scale, past_lens, new_lens=None, is_ca
     if workspace is None:
         workspace = q.new_empty((need,), dtype=_torch.uint8) if need else None
     else:
-        at = _counter_bytes(c.batch, c.heads)
+        at = PAGED_INT4_COUNTER_BYTES
         if workspace.dtype != _torch.uint8 or workspace.numel() < at + need:
             raise MynnError("%s: a workspace of %d bytes, %d needed" % (name, workspace.numel(), at + need))
         counters = _ptr(workspace)

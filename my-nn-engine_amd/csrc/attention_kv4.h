@@ -21,7 +21,7 @@ struct Kv4Args {
     float scale;
     int causal, B, Sq, Hq;
     float *part_o, *part_ml;  // parts of rows that several workgroups share
-    int32_t *counters;        // [B * Hkv], zero between calls, or null: joined by a second launch
+    int32_t *counters;        // one for each workgroup, zero between calls, or null: joined by a second launch
     int grid;                 // workgroups of the form for few rows, those that run at once of the form for many
     int blocks, ranges;       // the form for many rows: blocks of rows of a kv head, the most ranges that their keys come in
     int *length;              // and how long a range is, as the first workgroup found it

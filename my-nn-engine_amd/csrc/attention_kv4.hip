@@ -1,4 +1,6 @@
 // Attention over a paged cache held in 4 bits, for sequences of different lengths.
+#include <algorithm>
+
 #include "attention_kv4_stream.h"
 #include "attention_kv4_tile.h"
 
@@ -23,11 +25,11 @@ static bool kv4_few_rows(int Hq, int Hkv, int Sq) { return (long)(Hq / Hkv) * Sq
 // How often the rows are put side by side: as 16 columns have room for them.  (Four groups of columns a row: twice at the most, the tile of 64 keys does not fit the registers.)
 static int kv4_fold(long rows, int groups) { return rows <= 4 && groups < 4 ? 4 : rows <= 8 ? 2 : 1; }
 static int kv4_unit(int fold) { return fold == 4 ? kKv4Stride<4> : kKv4Stride<1>; }
-// workgroups of the form for few rows: as many as run at once, no more than there can be units
+// workgroups of the form for few rows: as many as run at once, no more than there can be units, or than there are counters
 static int kv4_stream_grid(int B, int Hkv, int unit, long rows) {
     // Two a CU; where that makes more than 32 parts of a (sequence, kv head), fewer: their join is on one CU (one sequence of 32768 keys, 8 kv heads of 128: with 64 parts each
     // 24 us, with 32 20).
-    const long pairs = (long)B * Hkv, units = pairs * ((rows + unit - 1) / unit), two = 2l * kv4_cus();
+    const long pairs = (long)B * Hkv, units = pairs * ((rows + unit - 1) / unit), two = std::min(2l * kv4_cus(), (long)MYNN_PAGED_INT4_COUNTERS);
     const long most = 32 * pairs >= two ? two : 32 * pairs > two / 4 ? 32 * pairs : two / 4;
     return (int)(units < most ? units : most);
 }
@@ -78,6 +80,7 @@ extern "C" int mynn_attention_paged_int4(void *out, const void *Q, const uint8_t
     MYNN_REQUIRE(need == 0 || (workspace && aligned16(workspace) && workspace_bytes >= need), MYNN_ERR_INVALID, "%s: %zu bytes of workspace, %zu needed", who, workspace_bytes,
                  need);
     const size_t R = (size_t)(num_q_heads / num_kv_heads) * Sq;
+    MYNN_REQUIRE((uintptr_t)counters % 4 == 0, MYNN_ERR_INVALID, "%s: unaligned counters", who);
     a.part_o = (float *)workspace;
     if (kv4_few_rows(num_q_heads, num_kv_heads, Sq)) {
         const int fold = kv4_fold((long)R, head_dim / group), unit = kv4_unit(fold);

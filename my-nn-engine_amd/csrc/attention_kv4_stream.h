@@ -490,7 +490,8 @@ template <typename T, int D, int NG, int FOLD> __global__ __launch_bounds__(kKv4
         const int w1 = tid ? tail.w1 : front.w1, n = w1 - (tid ? tail.w0 : front.w0);
         int before = -1;
         if (w1 >= 0) {
-            int32_t *counter = a.counters + (size_t)(tid ? tail.b : front.b) * a.c.Hkv + (tid ? tail.h : front.h);
+            // (the one of the first workgroup that has a part: no other (sequence, kv head) that is shared begins there, for this one goes on behind it)
+            int32_t *counter = a.counters + (tid ? tail.w0 : front.w0);
             before = __hip_atomic_fetch_add(counter, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
             if (before == n) __hip_atomic_store(counter, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);  // ready for the next call
         }

@@ -427,7 +427,7 @@ PyObject *kv_rows_paged(PyObject *, PyObject *const *args, Py_ssize_t n) {
     });
 }
 
-// (q, pools, table, scale, past_lens, new_lens or None, is_causal, workspace or None, out or None) -> out; a workspace has the counters in front, in whole 256 bytes
+// (q, pools, table, scale, past_lens, new_lens or None, is_causal, workspace or None, out or None) -> out; a workspace has the counters in front
 PyObject *attention_paged_int4(PyObject *, PyObject *const *args, Py_ssize_t n) {
     if (n != 9 || !PyFloat_CheckExact(args[3]) || !PyBool_Check(args[6]) || args[8] != Py_None) return none();
     return guarded([&]() -> PyObject * {
@@ -437,7 +437,7 @@ PyObject *attention_paged_int4(PyObject *, PyObject *const *args, Py_ssize_t n) 
         if (!q || (args[7] != Py_None && (!(kept = here(args[7])) || kept->scalar_type() != at::kByte))) return none();
         const int64_t Hq = q->size(1), S = q->size(2);
         const size_t need = g_kv4_bytes((int)c.B, (int)S, (int)c.pages, (int)c.rows, (int)Hq, (int)c.heads, (int)c.dim);
-        const size_t front = kept ? (4 * (size_t)(c.B * c.heads) + 255) / 256 * 256 : 0;
+        const size_t front = kept ? 4 * MYNN_PAGED_INT4_COUNTERS : 0;
         if (kept && (size_t)kept->numel() < front + need) return none();
         const at::Tensor out = make(q->sizes(), *q, c.type), own = kept || !need ? at::Tensor() : make({(int64_t)need}, *q, at::kByte);
         void *o = data(out), *qp = data(*q);

@@ -126,13 +126,15 @@ def attention(q, pools, table, scale, past, new, causal, weight_error):
     What is absolute: a weight times its value's scale is an fp16 number in units that make the largest of them 2^13 or more (so off by
     2^-25 where it is small: 2^-38 of the largest, times a code of at most 15), or, where the scales next to the largest weight are
     below 2^-86, units of 2^-100 of that weight (2^-125); a weight below the smallest 32-bit number, in the same units, is lost
-    (2^-140 times the largest scale, times the value)."""
+    (2^-140 times the largest scale, times the value).  More than 16 rows a kv head: their reference may lag 2^4 behind the largest, which
+    then is 2^9 or more in the units of fp16 and all of these are 16 times as large."""
     B, Hq, S, D = q.shape
     Hkv = pools[0].shape[1]
     G, P = Hq // Hkv, pools[0].shape[2]
     out = torch.zeros(q.shape, dtype=torch.float64, device=q.device)
     slack = torch.zeros_like(out)
     half = 2.0 ** -24
+    lag = 1.0 if G * S <= 16 else 16.0
     for b in range(B):
         n = S if new is None else min(max(int(new[b]), 0), S)
         length = min(max(int(past[b]) + n, 0), table.shape[1] * pools[0].shape[2]) if n else 0
@@ -151,7 +153,7 @@ def attention(q, pools, table, scale, past, new, causal, weight_error):
                 size = (torch.mm(x.abs(), kk.abs().t().contiguous()) * abs(scale)).amax(-1, keepdim=True)
                 p = torch.softmax(s, -1)
                 vs = pools[3][table[b][at // P].long().clamp(0, pools[3].shape[0] - 1), h, at % P].double().amax(-1)[seen] if len(pools) == 6 else vv.abs().amax(-1)
-                small = kk.shape[0] * (15 * 2.0 ** -38 * (p * vs).amax(-1, keepdim=True) + 2.0 ** -120 + 2.0 ** -138 * vs.max() * vv.abs().max())
+                small = lag * kk.shape[0] * (15 * 2.0 ** -38 * (p * vs).amax(-1, keepdim=True) + 2.0 ** -120 + 2.0 ** -138 * vs.max() * vv.abs().max())
                 out[b, h * G:(h + 1) * G, i] = torch.mm(p, vv)
                 weight = (D + 8) * half * size + 4 * half * s.abs().amax(-1, keepdim=True) + 2.0 ** -22 + weight_error + (kk.shape[0] + 64) * half
                 slack[b, h * G:(h + 1) * G, i] = 2 * weight * torch.mm(p, vv.abs()) + small

@@ -276,3 +276,111 @@ def test_generation_prompt_then_tokens(mynn, dtype, D, group):
         past += new if step == 0 else 1
     pages.close()
     pool.close()
+
+
+@pytest.mark.parametrize("D,group", [(64, 32), (128, 128), (128, 64), (128, 32)])
+@pytest.mark.parametrize("G,S", [(4, 1), (5, 1), (1, 5), (2, 4), (9, 1), (3, 3), (8, 2), (17, 1), (1, 16), (1, 17), (16, 4), (13, 5), (2, 64), (43, 3)])
+def test_rows_of_a_kv_head_around_the_tiles(mynn, D, group, G, S):
+    """4, 8, 16, 64 and 128 rows are a tile's: as many, and one more"""
+    past = [0, 129, 511]
+    pools, table = cache(3, 2, D, 64, group, torch.float16, [p + S for p in past], seed=30 + S)
+    check(mynn, queries(3, 2 * G, S, D, torch.float16), pools, table, past, new=[S, max(S - 1, 1), S])
+
+
+@pytest.mark.parametrize("S", [30, 130])
+@pytest.mark.parametrize("causal", [True, False])
+def test_ranges_of_keys_of_ragged_prompts(mynn, S, causal):
+    """few blocks of rows over many keys: their ranges are on workgroups of their own, as many as a sequence's length asks for"""
+    past = [5000, 0, 700, 63, 2600]
+    pools, table = cache(5, 1, 128, 128, 128, torch.bfloat16, [p + S for p in past], seed=31)
+    q = queries(5, 4, S, 128, torch.bfloat16)
+    check(mynn, q, pools, table, past, new=[S, S, 1, 0, S - 1], causal=causal)
+    check(mynn, q, pools, table, past, causal=causal)
+    one = [t[:1].contiguous() for t in (q, table)]
+    check(mynn, one[0], pools, one[1], past[:1], causal=causal)
+
+
+def test_many_parts_of_one_sequence(mynn):
+    """more than 64 of them in a join"""
+    pools, table = cache(1, 1, 64, 256, 64, torch.float16, [60001], seed=32)
+    for Hq in (4, 7, 16):
+        check(mynn, queries(1, Hq, 1, 64, torch.float16), pools, table, [60000])
+
+
+def test_one_workspace_for_calls_of_every_shape(mynn):
+    """kept from the call that needs most of it, in any order, rows few and many; one that is too small is refused"""
+    past = [4000, 900, 17, 0, 300, 2222]
+    pools, table = cache(6, 4, 128, 64, 64, torch.float16, [p + 40 for p in past], seed=33)
+    calls = []
+    for B, S in ((1, 1), (6, 1), (2, 1), (1, 4), (6, 2), (3, 40), (1, 40), (6, 1), (6, 40)):
+        q, lens = queries(B, 16, S, 128, torch.float16, seed=B + S), torch.tensor(past[:B], dtype=torch.int32, device="cuda")
+        calls.append((q, pools, table[:B].contiguous(), 0.1, lens))
+    spaces = [mynn.attention_paged_int4_workspace(*c[:3]) for c in calls]
+    ws = max(spaces, key=lambda t: t.numel())
+    want = [mynn.attention_paged_int4(*c) for c in calls]
+    for turn in range(3):
+        for n in torch.randperm(len(calls), generator=torch.Generator().manual_seed(turn)).tolist():
+            assert same_bits(mynn.attention_paged_int4(*calls[n], workspace=ws), want[n]), (turn, n)
+    assert not ws[:mynn.PAGED_INT4_COUNTER_BYTES].any()
+    for bad in (ws[:mynn.PAGED_INT4_COUNTER_BYTES], ws[:spaces[1].numel() - 1], ws.float()):
+        with pytest.raises(mynn.MynnError):
+            mynn.attention_paged_int4(*calls[1], workspace=bad)
+    with pytest.raises(mynn.MynnError):
+        mynn.attention_paged_int4(*calls[1], workspace=ws[1:])
+
+
+def test_two_captured_calls_share_a_workspace(mynn):
+    """of different shapes, replayed in turn with eager calls between them"""
+    past = [3000, 100, 1500]
+    pools, table = cache(3, 2, 128, 64, 128, torch.bfloat16, [p + 60 for p in past], seed=34)
+    calls = []
+    for B, S in ((3, 1), (1, 1), (3, 24)):
+        calls.append((queries(B, 8, S, 128, torch.bfloat16, seed=S + B), pools, table[:B].contiguous(), 0.1, torch.tensor(past[:B], dtype=torch.int32, device="cuda")))
+    ws = max((mynn.attention_paged_int4_workspace(*c[:3]) for c in calls), key=lambda t: t.numel())
+    outs = [torch.empty_like(c[0]) for c in calls]
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        for c, o in zip(calls, outs):
+            mynn.attention_paged_int4(*c, workspace=ws, out=o)
+    torch.cuda.synchronize()
+    graphs = []
+    for c, o in zip(calls, outs):
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1], stream=stream):
+            mynn.attention_paged_int4(*c, workspace=ws, out=o)
+    for turn in range(4):
+        for n in ((0, 1, 2), (2, 1, 0), (1, 0, 2), (0, 2, 1))[turn]:
+            outs[n].zero_()
+            graphs[n].replay()
+            torch.cuda.synchronize()
+            assert same_bits(outs[n], mynn.attention_paged_int4(*calls[n])), (turn, n)
+        for c in calls:
+            c[4].add_(7)
+
+
+def test_pools_of_more_than_32_bits_of_bytes(mynn):
+    """pages at the end of pools whose codes, scales and zero points lie past 2^32 bytes of the first: appended, read back, attended to, the same bits as in small pools"""
+    Hq, Hkv, D, P, S = 8, 2, 128, 256, 40
+    n_pages = (1 << 32) // (Hkv * P * D // 2) + 8
+    group = 32
+    lead = (n_pages, Hkv, P)
+    big = [torch.empty(lead + (D // 2,), dtype=torch.uint8, device="cuda") for _ in range(2)]
+    big += [torch.empty(lead + (D // group,), dtype=t, device="cuda") for t in (torch.float16, torch.float16, torch.uint8, torch.uint8)]
+    pages = [n_pages - 1, 3, n_pages - 5, n_pages - 2, 0, n_pages - 3]
+    small = [torch.empty((6,) + t.shape[1:], dtype=t.dtype, device="cuda") for t in big]
+    g = torch.Generator().manual_seed(35)
+    cos, sin = tables(1024, D, torch.float16)
+    where = [torch.tensor(x, dtype=torch.int32, device="cuda").view(2, 3) for x in (pages, list(range(6)))]
+    past = torch.tensor([0, 0], dtype=torch.int32, device="cuda")
+    for step in range(4):
+        n = (300, S, 1, 5)[step]
+        rows = torch.randn(2, n, (Hq + 2 * Hkv) * D, generator=g).to(torch.float16).cuda().view(2, n, -1, D).transpose(1, 2)
+        got = []
+        for pools, table in zip((big, small), where):
+            q = mynn.rope_append_paged(rows[:, :Hq], rows[:, Hq:Hq + Hkv], rows[:, Hq + Hkv:], cos, sin, pools, table, past)
+            got.append((q, mynn.attention_paged_int4(q, pools, table, 0.1, past), *mynn.kv_rows_paged(pools, table, past, n)))
+        for a, b in zip(*got):
+            assert same_bits(a, b), step
+        past += n
+    check(mynn, got[1][0], small, where[1], (past - n).tolist())

@@ -48,6 +48,9 @@ def test_common_refusals(call, kw):
     (append, dict(rows=0), -1), (append, dict(bits=5), -1), (append, dict(q_out=P16 + 2), -1), (append, dict(B=1 << 20, S=1 << 20), -2),
     (rows, dict(k=None, v=None), -1), (rows, dict(v=P16 + 4), -1), (rows, dict(bits=3), -1), (rows, dict(B=1 << 20, S=1 << 20), -2),
     (attend, dict(q=None), -1), (attend, dict(out=P16 + 8), -1), (attend, dict(Hq=3, Hkv=2), -1), (attend, dict(Hq=1 << 15, S=1 << 20), -2),
+    (attend, dict(pages=64, ws=None), -1), (attend, dict(pages=64, ws_bytes=64), -1), (attend, dict(pages=64, ws=P16 + 8), -1), (attend, dict(counters=P16 + 2), -1),
+    (attend, dict(pages=64, S=64, ws=None), -1), (attend, dict(B=1 << 24, S=64), -2), (attend, dict(B=1 << 28, pages=1 << 20), -2), (append, dict(B=1 << 24, S=64), -2),
+    (rows, dict(B=1 << 24, S=64), -2),
 ], ids=str)
 def test_refusals_of_each(call, kw, code):
     assert call(**kw) == code and mynn.lib().mynn_last_error()
@@ -90,3 +93,16 @@ def test_four_bit_buffers_of_a_pool_ask_for_groups_that_divide_a_row():
         with pytest.raises(mynn.MynnError):
             pool.buffers(1, 1, 64, torch.float16, **kw)
     pool.close()
+
+
+def test_workspaces_ask_for_what_a_call_needs():
+    size = mynn.lib().mynn_attention_paged_int4_workspace_bytes
+    assert size(0, 1, 8, 32, 8, 2, 64) == 0 and size(1, 1, 8, 32, 1, 2, 64) == 0
+    for S in (1, 4, 5, 64, 500):
+        last = 0
+        for pages in (1, 8, 64, 512):
+            need = size(2, S, pages, 64, 8, 2, 128)
+            assert last <= need < 256 << 20  # (more keys, more parts; they end with the device's compute units)
+            last = need
+    header = open(mynn.CSRC + "/../../include/mynn_hip.h").read()
+    assert "#define MYNN_PAGED_INT4_COUNTERS %d" % (mynn.PAGED_INT4_COUNTER_BYTES // 4) in header
