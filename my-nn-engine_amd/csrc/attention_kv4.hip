@@ -34,15 +34,27 @@ static int kv4_stream_grid(int B, int Hkv, int unit, long rows) {
     return (int)(units < most ? units : most);
 }
 
-// Up to as many ranges of keys as make four workgroups a CU where blocks of rows leave the device idle (two run at once; how many a block has is found by Kv4Ranges).
+// Rows of a workgroup, and up to how many ranges of keys its rows' keys come in (two workgroups a CU run at once; Kv4TilePlan::ranges makes twice that at the most, how many
+// of them a block takes is found on the device).  R: rows of a kv head, rows: of a sequence's cache.
 static Kv4TilePlan kv4_tile_plan(int B, int Sq, int Hq, int Hkv, long rows) {
-    const long R = (long)(Hq / Hkv) * Sq;
-    Kv4TilePlan p;
-    p.rows = R <= 64 ? 64 : 128;
-    p.blocks = (int)((R + p.rows - 1) / p.rows);
-    const long wgs = (long)B * Hkv * p.blocks, most = (rows + 127) / 128, want = 4l * kv4_cus() / wgs;
-    p.ranges = (int)(want < 2 ? 1 : want > most ? most : want);
-    return p;
+    const long R = (long)(Hq / Hkv) * Sq, pairs = (long)B * Hkv, cus = kv4_cus();
+    auto plan = [&](int block, bool split) {
+        Kv4TilePlan p;
+        p.rows = block;
+        p.blocks = (int)((R + block - 1) / block);
+        const long most = (rows + 127) / 128, want = split ? 4 * cus / (pairs * p.blocks) : 1;
+        p.ranges = (int)(want < 2 ? 1 : want > most ? most : want);
+        return p;
+    };
+    // Blocks of 128 rows turn codes into operands for the most rows: where they fill the device (32 / 8 heads of 128, groups of 128: one prompt of 4096 rows 236 us, blocks of
+    // 64 286; one of 2048 83 and 88), and, in ranges, where both rows and keys are many (512 tokens behind 3000 rows 65, blocks of 64 in ranges 71, whole 82).
+    if (pairs * ((R + 127) / 128) >= 2 * cus) return plan(128, false);
+    if (R >= 1024 && rows >= 2048) return plan(128, true);
+    // Blocks of 64 leave two waves to a block of 32 rows, half of each tile's keys each, and a tile takes 1.6 us where it took 2.3: one prompt of 1200 rows 38 us, in blocks of
+    // 128 57.  Ranges cost a launch more, 5 us and up: they pay for few blocks of 512 keys and more (4 x 40 tokens behind 2000 rows 32 us, whole 49; one prompt of 300 rows 20, whole
+    // 16), of more than one for each CU only behind many keys (32 x 5 tokens behind 4000 rows 76, whole 91; 8 x 64 behind 1000 rows 39, whole 33).
+    const long wgs = pairs * ((R + 63) / 64);
+    return plan(64, wgs < cus ? rows >= 512 : wgs < 2 * cus && rows >= 2048);
 }
 
 }  // namespace mynn

@@ -52,10 +52,11 @@ template <typename T, int D, int NG, int QW, int KW, int KEYS> __global__ __laun
     const int i0 = blockIdx.x, i1 = i0 / a.c.Hkv, h = i0 - i1 * a.c.Hkv;
     int b, block, range = 0;
     if (a.c.fresh || a.ranges > 1) {
-        // Sequences outermost.  Inside the blocks those of a short one, which end at once, take every other place on the shader engines: 2 pieces of prompts, 512 rows and 79,
-        // 91 us instead of 76, 8 of up to 1024 rows 284 instead of 202 (227 with the sequences taking turns).
+        // Then sequences, ranges outermost.  Workgroups go to the shader engines in turn, and those that end at once should not have every other turn: 2 pieces of prompts, 512
+        // rows and 79, took 91 us for 76 with the sequences inside the blocks, 8 of up to 1024 rows 284 for 202 (227 with the sequences taking turns), and 32 x 5 rows over 4000
+        // keys, 2 ranges of 4 there, 124 for 71 with the ranges inside.
         const int i2 = i1 / a.blocks;
-        block = i1 - i2 * a.blocks, b = i2 / a.ranges, range = i2 - b * a.ranges;
+        block = i1 - i2 * a.blocks, range = i2 / a.B, b = i2 - range * a.B;
     } else {
         // All blocks have rows: sequences inside the blocks, taking turns, and the heaviest of all go first (4 x 2048 rows, four times as many workgroups as run at once, 220 us;
         // outermost 230).
