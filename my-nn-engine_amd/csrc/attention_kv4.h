@@ -57,6 +57,21 @@ template <typename T> __device__ __forceinline__ float kv4_half(uint32_t w, int 
     return Elem<T>::ld(&v, 0);
 }
 
+// Two numbers as fp16, and what is left of them: hi + lo of a pair are 22 bits.  `minus` is -1, from kv4_minus: then a rest is one instruction, which reads either half of hi;
+// of what it knows to be -1 the compiler makes a conversion and a subtraction.
+__device__ __forceinline__ float kv4_minus() {
+    float x = -1.f;
+    asm volatile("" : "+s"(x));
+    return x;
+}
+__device__ __forceinline__ uint32_t kv4_take(float &x, float &y, float minus) {
+    const uint32_t w = cvt2<f16_t>(x, y);
+    const h2_t hi = __builtin_bit_cast(h2_t, w);
+    x = fmaf((float)hi[0], minus, x);
+    y = fmaf((float)hi[1], minus, y);
+    return w;
+}
+
 // Which of a launch's workgroups have which keys.  The keys of a (sequence, kv head) come in units of UNIT; a sequence has at least one.  All units in a
 // row, by sequence, head and place, are dealt out in equal runs, so that workgroups have the same to do whatever the lengths are: lens are read on the
 // device, the launch is the same for all of them.  Every wave finds the run for itself (64 sequences at a time, a lane each).

@@ -126,6 +126,7 @@ template <typename T, int D, int NG, int FOLD> __global__ __launch_bounds__(kKv4
     const int stop = min(unit + quota, total);
     Kv4Parts front{0, 0, 0, 0, -1, 0}, tail{0, 0, 0, 0, -1, 0};  // what this workgroup has parts of
     Int4Pairs pairs;
+    const float minus = kv4_minus();
     const int psh = a.c.page_shift, pmask = (1 << psh) - 1;
     const int fold = col / COLS, row = col % COLS < R ? col % COLS : 0;  // this lane's row, and which of the folds has it
 
@@ -343,8 +344,8 @@ template <typename T, int D, int NG, int FOLD> __global__ __launch_bounds__(kKv4
                         for (int e = 0; e < 4; e++) y[e] = sv[s][e] * vs[s][g][e];
 #pragma unroll
                         for (int part = 0; part < 2; part++) {
-                            w[s][part][0] = take_part<f16_t>(y[0], y[1]);
-                            w[s][part][1] = take_part<f16_t>(y[2], y[3]);
+                            w[s][part][0] = kv4_take(y[0], y[1], minus);
+                            w[s][part][1] = kv4_take(y[2], y[3], minus);
                         }
                     }
 #pragma unroll

@@ -5,7 +5,7 @@
 // -> (code - zero) in fp16 -> LDS, once for all rows of the workgroup: two stages, one barrier a tile.
 //   S^T = K . Q^T      per group of columns; a key's scale meets the group's sum
 //   softmax            a lane has ONE row and half of the keys of each 32; the reference with the value scales in it (attention_kv4.h)
-//   O^T += V^T . P^T   p * vs rounded to fp16 once; P stays in registers (the D layout of S^T is the B layout of P^T with the keys in the order 4g+0..3, 8+4g+0..3), V^T
+//   O^T += V^T . P^T   p * vs as one fp16 number (T = bf16) or two; P stays in registers (the D layout of S^T is the B layout of P^T with the keys in the order 4g+0..3, 8+4g+0..3), V^T
 //                      comes from the row-major tile by transposing reads
 // Codes leave a dword in the order of kv4_pairs, so columns lie in that order inside every 8: queries are put in the same order when they are read, results back when stored.
 #pragma once
@@ -45,6 +45,9 @@ __device__ __forceinline__ int kv4_ranges(int tiles, int length, int most) { ret
 template <typename T, int D, int NG, int QW, int KW, int KEYS> __global__ __launch_bounds__(QW *KW * 64, 2) void attn_kv4_tile_kernel(Kv4Args a) {
     using B = Kv4Block<D, NG, QW, KW, KEYS>;
     constexpr int KS = D / 16, DT = D / 32, NH = B::NH, DW = D / 32, ROWB = B::ROWB, KPG = KS / NG, TPG = DT / NG;
+    // p * vs for the second product: results in bf16 have 8 bits, and its rounding to fp16, 11, does not show; those in fp16 would be off by half as much again (their own
+    // rounding and this one, of the same size), so there it is two numbers of 11 bits.
+    constexpr int PARTS = std::is_same<T, f16_t>::value ? 2 : 1;
     extern __shared__ __align__(16) char sm[];
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), wave = w % QW, kg = w / QW, col = lane & 31, g = lane >> 5;
     const int G = a.Hq / a.c.Hkv, R = G * a.Sq;
@@ -126,6 +129,7 @@ template <typename T, int D, int NG, int QW, int KW, int KEYS> __global__ __laun
     };
     auto k_swz = [](int r) { return D == 128 ? r & 15 : (r >> 1) & 7; };
     auto v_swz = [](int r) { return D == 128 ? (r & 3) * 5 : (((r >> 1) ^ r) & 1) << 2; };
+    const float minus = kv4_minus();
     Int4Pairs pairs;
     auto store = [&](char *stage) __attribute__((always_inline)) {
         float *scales = (float *)(stage + 2 * B::TILEB), *lift = scales + 2 * NG * KEYS;
@@ -277,12 +281,16 @@ template <typename T, int D, int NG, int QW, int KW, int KEYS> __global__ __laun
                         p[4 * e4 + e] = MASKED ? (seen[st >> 1] >> (e0 + 4 * e4 + e) & 1 ? x * f[e] : 0.f) : x * f[e];
                     }
                 }
-                const U4 pf = U4{cvt2<f16_t>(p[0], p[1]), cvt2<f16_t>(p[2], p[3]), cvt2<f16_t>(p[4], p[5]), cvt2<f16_t>(p[6], p[7])};
+                U4 pf[PARTS];
+#pragma unroll
+                for (int part = 0; part < PARTS; part++)
+                    pf[part] = U4{kv4_take(p[0], p[1], minus), kv4_take(p[2], p[3], minus), kv4_take(p[4], p[5], minus), kv4_take(p[6], p[7], minus)};
 #pragma unroll
                 for (int t2 = gr * TPG; t2 < (gr + 1) * TPG; t2++) {
                     const char *vr = vt + vrow[t2] + 16 * st * ROWB;
                     const uint2 lo = lds_read_tr16(vr), hi = lds_read_tr16(vr + 8 * ROWB);
-                    o[t2] = Mfma<f16_t>::run(U4{lo.x, lo.y, hi.x, hi.y}, pf, o[t2]);
+#pragma unroll
+                    for (int part = 0; part < PARTS; part++) o[t2] = Mfma<f16_t>::run(U4{lo.x, lo.y, hi.x, hi.y}, pf[part], o[t2]);
                 }
             }
     };
