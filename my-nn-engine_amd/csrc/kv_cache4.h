@@ -43,16 +43,21 @@ __device__ inline size_t paged_row(const PagedKv &c, int page, int h, int r) {
 // The 4-bit form of a group of columns with least value lo <= 0 and largest hi >= 0 (zero among them: a value of zero stays zero):
 //   s = T(hi/15 - lo/15), z = round(-lo/s), code = round(x/s) + z in 0 .. 15, which stands for s * (code - z)
 // -- mynn_quantize_int4_groups for a row.  A group with a value that is not finite stands for NaN.
+// A division of 32 bits for each value is most of the append's work.  x and s are of T, with at most 11 bits, so x/s is a half or 2^-12 and more away from it, and a product with
+// 1/s, off by 2^-18 at |x/s| < 32, rounds like the quotient where 2^-15 goes on top of the half: 4 x 2048 tokens, 16 heads of 128 quantised, 42.9 -> 39.0 us.
 template <typename T> struct Int4Row {
-    float s, z;
+    float s, z, up, r;  // r = 1 / (s up): up keeps it from overflow where s is one of the least numbers of bf16
     __device__ Int4Row(float lo, float hi, bool finite) {
         s = Elem<T>::rnd(hi / 15.0f - lo / 15.0f);
         if (s == 0.f) s = 1.f;
         z = fminf(roundf(-lo / s), 15.f);
         if (!finite) s = __builtin_nanf(""), z = 0.f;
+        up = !std::is_same<T, f16_t>::value && s < 0x1p-64f ? 0x1p64f : 1.f;
+        r = 1.0f / (s * up);
     }
     __device__ uint32_t code(float x) const {
-        const float c = fminf(fmaxf(roundf(x / s) + z, 0.f), 15.f);
+        if (!std::is_same<T, f16_t>::value) x *= up;
+        const float y = x * r, c = fminf(fmaxf(copysignf(truncf(fabsf(y) + (0.5f + 0x1p-15f)), y) + z, 0.f), 15.f);
         return c == c ? (uint32_t)c : 0u;
     }
 };

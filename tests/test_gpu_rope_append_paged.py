@@ -256,3 +256,39 @@ def test_pages_of_a_session_and_uniform_lengths_meet_the_other_paged_operators(m
     ref.assert_close(out, want, slack)
     pages.close()
     pool.close()
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("group", [128, 64, 32])
+def test_values_halfway_between_two_codes(mynn, dtype, group):
+    """rows whose scale is known (15 of it between least and largest) and whose values are its halves, and the type's next numbers on either side of them: scales of few
+    bits, whose halves the type holds, and of all, of every magnitude down to its least numbers"""
+    D, P = 128, 32
+    info = torch.finfo(dtype)
+    bits = 10 if dtype == torch.float16 else 7
+    least, most = (-24, 11) if dtype == torch.float16 else (-133, 120)
+    scales = [2.0 ** e * m for e in list(range(least, least + 14)) + list(range(least + 14, most, 5)) for m in (1.0, 1.5, 1.25, 1.75, 1.0 + 2.0 ** -bits, 2.0 - 2.0 ** -bits, 1.0 + 2.0 ** -3)]
+    rows = []
+    for s in scales:
+        s = float(torch.tensor(s, dtype=torch.float64).to(dtype).double())
+        if not 0 < s or 15 * s > info.max:
+            continue
+        for z in (0, 4, 15):
+            n = torch.arange(-z, 16 - z, dtype=torch.float64)
+            x = ((n + 0.5) * s).to(dtype)
+            row = torch.cat((x[:-1], n.mul(s).to(dtype)[-1:], n.mul(s).to(dtype)[:1], torch.zeros(15, dtype=dtype)))
+            up, down = row.clone(), row.clone()
+            for t, step in ((up, 1), (down, -1)):  # (one step of the type away from zero, towards it; not the ends, which make the scale)
+                w = t[:15].view(torch.int16)
+                w += step * (w.bitwise_and(0x7FFF) > 1).to(torch.int16)
+            rows += [torch.cat((row, up, down, row))]
+    S = len(rows)
+    v = torch.stack(rows)[None, None].cuda()
+    k = v.flip(-1).contiguous()
+    cos, sin = torch.ones(S, D, dtype=dtype, device="cuda"), torch.zeros(S, D, dtype=dtype, device="cuda")
+    pages = (S + P - 1) // P
+    pools = ref.make_pools(pages, 1, P, D, dtype, 4, group, "cuda", 3)
+    table = torch.arange(pages, dtype=torch.int32, device="cuda")[None]
+    check(mynn, None, k, v, cos, sin, pools, table, torch.zeros(1, dtype=torch.int32, device="cuda"))
+    codes = torch.stack((pools[1] & 15, pools[1] >> 4), -1).flatten(-2)
+    assert all(int((codes == c).sum()) > S for c in range(16))
