@@ -28,7 +28,7 @@ static int kv4_unit(int fold) { return fold == 4 ? kKv4Stride<4> : kKv4Stride<1>
 // workgroups of the form for few rows: as many as run at once, no more than there can be units, or than there are counters
 static int kv4_stream_grid(int B, int Hkv, int unit, long rows) {
     // Two a CU; where that makes more than 32 parts of a (sequence, kv head), fewer: their join is on one CU (one sequence of 32768 keys, 8 kv heads of 128: with 64 parts each
-    // 24 us, with 32 20).
+    // 24 us, with 32 20, with 16 23).
     const long pairs = (long)B * Hkv, units = pairs * ((rows + unit - 1) / unit), two = std::min(2l * kv4_cus(), (long)MYNN_PAGED_INT4_COUNTERS);
     const long most = 32 * pairs >= two ? two : 32 * pairs > two / 4 ? 32 * pairs : two / 4;
     return (int)(units < most ? units : most);
@@ -46,13 +46,13 @@ static Kv4TilePlan kv4_tile_plan(int B, int Sq, int Hq, int Hkv, long rows) {
         p.ranges = (int)(want < 2 ? 1 : want > most ? most : want);
         return p;
     };
-    // Blocks of 128 rows turn codes into operands for the most rows: where they fill the device (32 / 8 heads of 128, groups of 128: one prompt of 4096 rows 236 us, blocks of
-    // 64 286; one of 2048 83 and 88), and, in ranges, where both rows and keys are many (512 tokens behind 3000 rows 65, blocks of 64 in ranges 71, whole 82).
+    // Blocks of 128 rows turn codes into operands for the most rows: where they fill the device (32 / 8 heads of 128, groups of 128, bf16: one prompt of 4096 rows 228 us, blocks
+    // of 64 278; one of 2048 82 and 88), and, in ranges, where both rows and keys are many (512 tokens behind 3000 rows 65, blocks of 64 in ranges 71, whole 84).
     if (pairs * ((R + 127) / 128) >= 2 * cus) return plan(128, false);
     if (R >= 1024 && rows >= 2048) return plan(128, true);
     // Blocks of 64 leave two waves to a block of 32 rows, half of each tile's keys each, and a tile takes 1.6 us where it took 2.3: one prompt of 1200 rows 38 us, in blocks of
-    // 128 57.  Ranges cost a launch more, 5 us and up: they pay for few blocks of 512 keys and more (4 x 40 tokens behind 2000 rows 32 us, whole 49; one prompt of 300 rows 20, whole
-    // 16), of more than one for each CU only behind many keys (32 x 5 tokens behind 4000 rows 76, whole 91; 8 x 64 behind 1000 rows 39, whole 33).
+    // 128 49, those in ranges 57.  Ranges cost a launch more, 5 us and up: they pay for few blocks of 512 keys and more (4 x 40 tokens behind 2000 rows 30 us, whole 49; one prompt
+    // of 300 rows 19, whole 16), of more than one for each CU only behind many keys (32 x 5 tokens behind 4000 rows 75, whole 92; 8 x 64 behind 1000 rows 36, whole 33).
     const long wgs = pairs * ((R + 63) / 64);
     return plan(64, wgs < cus ? rows >= 512 : wgs < 2 * cus && rows >= 2048);
 }

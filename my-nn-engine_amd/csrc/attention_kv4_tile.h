@@ -7,6 +7,11 @@
 //   softmax            a lane has ONE row and half of the keys of each 32; the reference with the value scales in it (attention_kv4.h)
 //   O^T += V^T . P^T   p * vs as one fp16 number (T = bf16) or two; P stays in registers (the D layout of S^T is the B layout of P^T with the keys in the order 4g+0..3, 8+4g+0..3), V^T
 //                      comes from the row-major tile by transposing reads
+// Vector operations and matrix instructions bound it together (busy 65 and 31 % of the time at 4 x 2048 rows): 350 of the one for 32 of the other in a wave's 64 keys of 32 rows,
+// 100 of them the staging's.  4 prompts of 2048 rows, 32 / 8 heads of 128, groups of 128, bf16: 197 us in a program's calls, 0.70 PFLOP/s (the products alone, at what a large
+// matrix product reaches: 112); fp16, whose second product is two, 4 x 512 rows behind 3000 195 for 166.  Blocks of 256 rows, as eight waves or as four with 64 rows each, share
+// a tile's staging between more rows and hold one workgroup a CU: no faster, and 310 us for 230.  Raised priorities around the products, and reads of their operands
+// ahead in a fixed order, were within 4 % of this, 64 columns and groups of 32 slower.
 // Codes leave a dword in the order of kv4_pairs, so columns lie in that order inside every 8: queries are put in the same order when they are read, results back when stored.
 #pragma once
 #include "attention_kv4.h"

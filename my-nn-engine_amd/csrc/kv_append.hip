@@ -4,6 +4,10 @@
 // Rotation: lo' = lo*cos[p,j] - hi*sin[p,j], hi' = hi*cos[p,j+D/2] + lo*sin[p,j+D/2], separate products, one rounding (as
 // rope_kv_append).  What goes to the cache is the row that a 16-bit cache would hold: as it is, by the rule of
 // quantizing_kvcache_update in 8 bits, by that of Int4Row in 4.
+//
+// Memory bounds both where there are many rows (4 x 2048 tokens, 32 / 8 heads of 128; in brackets the bytes at a copy's 5.1 TB/s): in 16 bits 36.5 us (39), in 8 38.5 (36), in 4 39.0
+// (35), rows read back from 4 bits 11.2 (8.2); a launch and a chain of waits elsewhere (32 tokens into 4 bits 4.4 us, 400 5.8).  A thread with several heads of a token
+// keeps its table rows in registers and was no faster (42 us, 43 then), a wave with 8 tokens of a head 42; a thread that reads back 16 columns instead of 8 11.1.
 #include "kv_cache4.h"
 #include "mfma.h"
 
@@ -30,7 +34,8 @@ template <typename T> __device__ __forceinline__ U4 pack8(const float *f) {
     return U4{pack2<T>(f[0], f[1]), pack2<T>(f[2], f[3]), pack2<T>(f[4], f[5]), pack2<T>(f[6], f[7])};
 }
 
-// A head of a token is LPH = D/16 lanes': each has 8 dims of the lower half and the 8 that they are rotated with.
+// A head of a token is LPH = D/16 lanes', neighbours of each other: each has 8 dims of the lower half and the 8 that they are rotated with, so that nothing is exchanged but a
+// group's extremes.
 template <typename T, int KV, int D, int GROUP, bool ALIGNED> __global__ __launch_bounds__(256) void rope_append_paged_kernel(AppendArgs a) {
     constexpr int LPH = D / 16, HALF = D / 2;
     // (32 bits, as many as there can be threads: dividing 64 took longer than everything else)
