@@ -313,7 +313,7 @@ int mynn_kv_rows_paged(void *k_out, void *v_out, const void *k_pool, const void 
  * several workgroups share are joined inside the launch, without them by a second one; the results are the same bits.  They serve
  * calls of every shape, a workspace those that need no more bytes.  Calls that may overlap need workspaces and counters of
  * their own; nothing global is touched. */
-#define MYNN_PAGED_INT4_COUNTERS 512
+#define MYNN_PAGED_INT4_COUNTERS 2048
 size_t mynn_attention_paged_int4_workspace_bytes(int B, int Sq, int pages_per_seq, int page_rows,
                                                  int num_q_heads, int num_kv_heads, int head_dim);
 int mynn_attention_paged_int4(void *out, const void *Q, const uint8_t *k_pool, const uint8_t *v_pool,

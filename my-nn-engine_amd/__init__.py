@@ -757,7 +757,7 @@ def kv_rows_paged(pools, table, first_rows, n, n_rows=None):
     return k, v
 
 
-PAGED_INT4_COUNTER_BYTES = 4 * 512  # MYNN_PAGED_INT4_COUNTERS
+PAGED_INT4_COUNTER_BYTES = 4 * 2048  # MYNN_PAGED_INT4_COUNTERS
 
 
 def attention_paged_int4_workspace(q, pools, table):

@@ -108,11 +108,22 @@ template <int UNIT> struct Kv4Share {
     __device__ int run(const Kv4Args &a, int lane) { return running(from + lane < a.B ? units(PagedSeq(a.c, past, fresh, a.Sq)) : 0); }
     __device__ Kv4Share(const Kv4Args &a, int wg, int lane) {
         const int H = a.c.Hkv;
-        int sum = 0, r = 0;
-        for (int b0 = 0; b0 < a.B; b0 += 64) {
-            lengths(a, b0, lane);
-            r = run(a, lane);
-            sum += __builtin_amdgcn_readlane(r, 63);
+        lengths(a, 0, lane);
+        int r = run(a, lane), sum = __builtin_amdgcn_readlane(r, 63);
+        if (a.B > 64) {
+            // (four lengths of a lane on their way at a time: each of them is a wait for memory)
+            int mine = 0;
+            for (int b0 = 64 + lane; b0 - lane < a.B; b0 += 256) {
+                int p[4], f[4];
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const int b = min(b0 + 64 * i, a.B - 1);
+                    p[i] = a.c.past[b], f[i] = a.c.fresh ? a.c.fresh[b] : a.Sq;
+                }
+#pragma unroll
+                for (int i = 0; i < 4; i++) mine += b0 + 64 * i < a.B ? units(PagedSeq(a.c, p[i], f[i], a.Sq)) : 0;
+            }
+            sum += __builtin_amdgcn_readlane(running(mine), 63);
         }
         total = sum * H;
         quota = share_of(a, total);
@@ -121,18 +132,18 @@ template <int UNIT> struct Kv4Share {
         if (first >= total) return;
         int front = 0;
         for (int b0 = 0;; b0 += 64) {
-            if (a.B > 64) {
-                lengths(a, b0, lane);
-                r = run(a, lane);
-            }
-            const uint64_t past = __builtin_amdgcn_ballot_w64((front + r) * H > first);
-            if (past) {
-                const int l = __builtin_ctzll(past);
+            const int here_past = past, here_fresh = fresh;
+            if (b0 + 64 < a.B) lengths(a, b0 + 64, lane);  // (on their way meanwhile)
+            const uint64_t behind = __builtin_amdgcn_ballot_w64((front + r) * H > first);
+            if (behind) {
+                const int l = __builtin_ctzll(behind);
                 b = b0 + l;
                 before = (front + (l ? __builtin_amdgcn_readlane(r, l - 1) : 0)) * H;
+                from = b0, past = here_past, fresh = here_fresh;
                 return;
             }
             front += __builtin_amdgcn_readlane(r, 63);
+            r = run(a, lane);
         }
     }
 };

@@ -24,14 +24,21 @@ static int kv4_cus() {
 static bool kv4_few_rows(int Hq, int Hkv, int Sq) { return (long)(Hq / Hkv) * Sq <= 16; }
 // How often the rows are put side by side: as 16 columns have room for them.  (Four groups of columns a row: twice at the most, the tile of 64 keys does not fit the registers.)
 static int kv4_fold(long rows, int groups) { return rows <= 4 && groups < 4 ? 4 : rows <= 8 ? 2 : 1; }
-static int kv4_unit(int fold) { return fold == 4 ? kKv4Stride<4> : kKv4Stride<1>; }
+// Waves that share a (sequence, kv head)'s keys step by step.  Four; one where there is a (sequence, kv head) for each wave, or one for every other and few keys: what a workgroup
+// waits for at its ends -- lengths, pages, the first codes, the others' results -- another's work fills then (32 / 8 heads of 128, one token of 256 sequences of 64 keys 24 us and,
+// one wave each, 13, of 512 47 and 38, of 8192 587 and 568; 128 of 256 17 and 15, of up to 2048 62 and 64; 64 of 512 15 and 20).  More than 8 rows keep four: the join by a single wave would have 16 pairs of columns a lane.
+static int kv4_waves(long pairs, long R, long rows) {
+    const long cus = kv4_cus();
+    return R <= 8 && (pairs >= 8 * cus || (pairs >= 4 * cus && rows <= 512)) ? 1 : 4;
+}
+static int kv4_unit(int fold, int waves) { return waves * (fold == 4 ? kKv4Keys<4> : kKv4Keys<1>); }
 // workgroups of the form for few rows: as many as run at once, no more than there can be units, or than there are counters
-static int kv4_stream_grid(int B, int Hkv, int unit, long rows) {
+static int kv4_stream_grid(long pairs, int unit, int waves, long rows) {
+    const long units = pairs * ((rows + unit - 1) / unit), all = std::min(8l / waves * kv4_cus(), (long)MYNN_PAGED_INT4_COUNTERS);
+    if (waves == 1) return (int)std::min(all, pairs);
     // Two a CU; where that makes more than 32 parts of a (sequence, kv head), fewer: their join is on one CU (one sequence of 32768 keys, 8 kv heads of 128: with 64 parts each
     // 24 us, with 32 20, with 16 23).
-    const long pairs = (long)B * Hkv, units = pairs * ((rows + unit - 1) / unit), two = std::min(2l * kv4_cus(), (long)MYNN_PAGED_INT4_COUNTERS);
-    const long most = 32 * pairs >= two ? two : 32 * pairs > two / 4 ? 32 * pairs : two / 4;
-    return (int)(units < most ? units : most);
+    return (int)std::min(units, std::min(all, std::max(32 * pairs, all / 4)));
 }
 
 // Rows of a workgroup, and up to how many ranges of keys its rows' keys come in (two workgroups a CU run at once; Kv4TilePlan::ranges makes twice that at the most, how many
@@ -69,7 +76,9 @@ extern "C" size_t mynn_attention_paged_int4_workspace_bytes(int B, int Sq, int p
         return ranges == 1 ? 0 : (size_t)ranges * B * num_kv_heads * R * (head_dim + 4) * sizeof(float);
     }
     // (the smaller unit makes more workgroups: enough for either)
-    return 2 * (size_t)kv4_stream_grid(B, num_kv_heads, kv4_unit(1), (long)pages_per_seq * page_rows) * R * (head_dim + 4) * sizeof(float);
+    const long pairs = (long)B * num_kv_heads, rows = (long)pages_per_seq * page_rows;
+    const int waves = kv4_waves(pairs, (long)R, rows);
+    return 2 * (size_t)kv4_stream_grid(pairs, kv4_unit(1, waves), waves, rows) * R * (head_dim + 4) * sizeof(float);
 }
 
 extern "C" int mynn_attention_paged_int4(void *out, const void *Q, const uint8_t *k_pool, const uint8_t *v_pool, const void *k_scale_pool, const void *v_scale_pool,
@@ -95,12 +104,13 @@ extern "C" int mynn_attention_paged_int4(void *out, const void *Q, const uint8_t
     MYNN_REQUIRE((uintptr_t)counters % 4 == 0, MYNN_ERR_INVALID, "%s: unaligned counters", who);
     a.part_o = (float *)workspace;
     if (kv4_few_rows(num_q_heads, num_kv_heads, Sq)) {
-        const int fold = kv4_fold((long)R, head_dim / group), unit = kv4_unit(fold);
-        MYNN_REQUIRE((long)B * num_kv_heads * ((rows + unit - 1) / unit) < 1l << 30, MYNN_ERR_UNSUPPORTED, "%s: %d sequences of %d heads of %ld rows", who, B, num_kv_heads, rows);
-        a.grid = kv4_stream_grid(B, num_kv_heads, unit, rows);
+        const long pairs = (long)B * num_kv_heads;
+        const int fold = kv4_fold((long)R, head_dim / group), waves = kv4_waves(pairs, (long)R, rows), unit = kv4_unit(fold, waves);
+        MYNN_REQUIRE(pairs * ((rows + unit - 1) / unit) < 1l << 30, MYNN_ERR_UNSUPPORTED, "%s: %d sequences of %d heads of %ld rows", who, B, num_kv_heads, rows);
+        a.grid = kv4_stream_grid(pairs, unit, waves, rows);
         a.part_ml = a.part_o + 2 * (size_t)a.grid * R * head_dim;
         a.counters = counters;
-        return dtype == MYNN_F16 ? kv4_stream_go<f16_t>(a, head_dim, group, fold, as_stream(s)) : kv4_stream_go<bf16_t>(a, head_dim, group, fold, as_stream(s));
+        return dtype == MYNN_F16 ? kv4_stream_go<f16_t>(a, head_dim, group, fold, waves, as_stream(s)) : kv4_stream_go<bf16_t>(a, head_dim, group, fold, waves, as_stream(s));
     }
     const Kv4TilePlan plan = kv4_tile_plan(B, Sq, num_q_heads, num_kv_heads, rows);
     MYNN_REQUIRE((long)B * num_kv_heads * plan.blocks * plan.ranges < 1l << 24, MYNN_ERR_UNSUPPORTED, "%s: B=%d Sq=%d heads %d/%d", who, B, Sq, num_q_heads, num_kv_heads);

@@ -11,22 +11,23 @@ template <typename F> inline int kv4_shape(int D, int group, F &&go) {
     return group == 128 ? go(Int<128>{}, Int<1>{}) : group == 64 ? go(Int<128>{}, Int<2>{}) : go(Int<128>{}, Int<4>{});
 }
 
-template <typename T, int D, int NG, int FOLD> int kv4_stream_launch(const Kv4Args &a, hipStream_t s) {
+template <typename T, int D, int NG, int FOLD, int W> int kv4_stream_launch(const Kv4Args &a, hipStream_t s) {
     const int R = a.Hq / a.c.Hkv * a.Sq, tile = kKv4TileBytes<D, FOLD>, wave = tile > R * D * 4 ? tile : R * D * 4;
-    const int lds = kKv4Waves * (wave + 128) + 16, join = 64 * R * 8;
-    MYNN_LAUNCH((attn_kv4_stream_kernel<T, D, NG, FOLD>), dim3(a.grid), dim3(kKv4Waves * 64), lds > join + 16 ? lds : join + 16, s, a);
+    const int lds = W * (wave + 128) + 16, join = 64 * R * 8;
+    MYNN_LAUNCH((attn_kv4_stream_kernel<T, D, NG, FOLD, W>), dim3(a.grid), dim3(W * 64), lds > join + 16 ? lds : join + 16, s, a);
     if (const int rc = launch_status("attn_kv4_stream_kernel")) return rc;
-    if (a.counters || a.c.pages_per_seq << a.c.page_shift <= kKv4Stride<FOLD>) return 0;  // (a unit each: nothing is shared)
-    MYNN_LAUNCH((attn_kv4_join_kernel<T, D, FOLD>), dim3(a.B * a.c.Hkv), dim3(256), 0, s, a);
+    if (a.counters || a.c.pages_per_seq << a.c.page_shift <= W * kKv4Keys<FOLD>) return 0;  // (a unit each: nothing is shared)
+    MYNN_LAUNCH((attn_kv4_join_kernel<T, D, FOLD, W>), dim3(a.B * a.c.Hkv), dim3(256), 0, s, a);
     return launch_status("attn_kv4_join_kernel");
 }
-template <typename T> int kv4_stream_go(const Kv4Args &a, int D, int group, int fold, hipStream_t s) {
+template <typename T> int kv4_stream_go(const Kv4Args &a, int D, int group, int fold, int waves, hipStream_t s) {
     return kv4_shape(D, group, [&](auto d, auto n) {
         constexpr int DD = decltype(d)::value, NG = decltype(n)::value;
         if constexpr (NG < 4) {
-            if (fold == 4) return kv4_stream_launch<T, DD, NG, 4>(a, s);
+            if (fold == 4) return waves == 1 ? kv4_stream_launch<T, DD, NG, 4, 1>(a, s) : kv4_stream_launch<T, DD, NG, 4, 4>(a, s);
         }
-        return fold == 2 ? kv4_stream_launch<T, DD, NG, 2>(a, s) : kv4_stream_launch<T, DD, NG, 1>(a, s);
+        if (fold == 2) return waves == 1 ? kv4_stream_launch<T, DD, NG, 2, 1>(a, s) : kv4_stream_launch<T, DD, NG, 2, 4>(a, s);
+        return kv4_stream_launch<T, DD, NG, 1, 4>(a, s);
     });
 }
 

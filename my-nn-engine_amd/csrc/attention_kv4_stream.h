@@ -22,10 +22,8 @@
 
 namespace mynn {
 
-constexpr int kKv4Waves = 4;
 template <int FOLD> constexpr int kKv4Keys = FOLD == 4 ? 64 : 32;              // of a wave's tile
-template <int FOLD> constexpr int kKv4Stride = kKv4Waves * kKv4Keys<FOLD>;       // of a workgroup's step
-template <int FOLD> using Kv4Run = Kv4Share<kKv4Stride<FOLD>>;
+template <int FOLD, int W> using Kv4Run = Kv4Share<W * kKv4Keys<FOLD>>;         // a workgroup's step: W waves
 template <int D, int FOLD> constexpr int kKv4TileBytes = kKv4Keys<FOLD> * (D / 2 + 16);  // of V codes in LDS
 
 // one wave's loads of a tile, all but the codes of the values
@@ -42,10 +40,10 @@ template <int D, int NG, int FOLD> struct Kv4Tile {
 struct Kv4Parts {
     int b, h, fresh, w0, w1, second;
 };
-// Joins them in their order, all threads of a workgroup of 256, `ml` 64 x 16 pairs in LDS.  AGENT: past this XCD's L2.  Parts are a wait for memory each if they are asked for
+// Joins them in their order, all THREADS of a workgroup, `ml` 64 x 16 pairs in LDS.  AGENT: past this XCD's L2.  Parts are a wait for memory each if they are asked for
 // one by one: references and sums of 64 go through LDS, results come in batches, the first of them with the references.
-template <typename T, int D, int ROWS, bool AGENT> __device__ __forceinline__ void kv4_join(const Kv4Args &a, const Kv4Parts &p, uint64_t *ml, int tid) {
-    constexpr int N = (ROWS * D / 2 + 255) / 256, AH = 32 / N;  // pairs of columns of a thread, parts in flight
+template <typename T, int D, int ROWS, int THREADS, bool AGENT> __device__ __forceinline__ void kv4_join(const Kv4Args &a, const Kv4Parts &p, uint64_t *ml, int tid) {
+    constexpr int N = (ROWS * D / 2 + THREADS - 1) / THREADS, AH = 32 / N;  // pairs of columns of a thread, parts in flight
     const int G = a.Hq / a.c.Hkv, R = G * a.Sq, n = p.w1 - p.w0 + 1;
     auto get = [](const uint64_t *x) { return AGENT ? __hip_atomic_load(x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : *x; };
     auto lo = [](uint64_t w) { return __builtin_bit_cast(float, (uint32_t)w); };
@@ -55,7 +53,7 @@ template <typename T, int D, int ROWS, bool AGENT> __device__ __forceinline__ vo
     int r[N], d[N];
 #pragma unroll
     for (int k = 0; k < N; k++) {
-        const int x = min(tid + 256 * k, R * (D / 2) - 1);
+        const int x = min(tid + THREADS * k, R * (D / 2) - 1);
         r[k] = x / (D / 2), d[k] = x % (D / 2) * 2;
         M[k] = -INFINITY, l[k] = o0[k] = o1[k] = 0.f;
     }
@@ -74,7 +72,7 @@ template <typename T, int D, int ROWS, bool AGENT> __device__ __forceinline__ vo
         };
         fetch(0);
         __syncthreads();  // (of the 64 before)
-        for (int x = tid; x < m * R; x += 256) ml[x] = get((const uint64_t *)a.part_ml + slot(c0 + x / R) + x % R);
+        for (int x = tid; x < m * R; x += THREADS) ml[x] = get((const uint64_t *)a.part_ml + slot(c0 + x / R) + x % R);
         __syncthreads();
 #pragma unroll
         for (int k = 0; k < N; k++) {
@@ -102,7 +100,7 @@ template <typename T, int D, int ROWS, bool AGENT> __device__ __forceinline__ vo
     }
 #pragma unroll
     for (int k = 0; k < N; k++) {
-        if (tid + 256 * k >= R * (D / 2)) break;
+        if (tid + THREADS * k >= R * (D / 2)) break;
         T *out = (T *)a.out + (((size_t)p.b * a.Hq + p.h * G + r[k] % G) * a.Sq + r[k] / G) * D + d[k];
         const float inv = 1.0f / l[k];
         *(uint32_t *)out = l[k] == 0.f || r[k] / G >= p.fresh ? 0u : pack2<T>(o0[k] * inv, o1[k] * inv);
@@ -112,11 +110,11 @@ template <typename T, int D, int ROWS, bool AGENT> __device__ __forceinline__ vo
 constexpr int kDppRor4 = 0x124, kDppRor12 = 0x12C;  // lane i <- i - 4, i + 4, inside each row of 16
 template <int CTRL> __device__ __forceinline__ uint32_t dpp_word(uint32_t v) { return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xF, 0xF, false); }
 
-template <typename T, int D, int NG, int FOLD> __global__ __launch_bounds__(kKv4Waves * 64, 2) void attn_kv4_stream_kernel(Kv4Args a) {
+template <typename T, int D, int NG, int FOLD, int NW> __global__ __launch_bounds__(NW * 64, 2) void attn_kv4_stream_kernel(Kv4Args a) {
     using Tile = Kv4Tile<D, NG, FOLD>;
-    constexpr int NW = kKv4Waves, GROUP = D / NG, KS = D / 32, VROW = D / 2 + 16;  // bytes of a row of V codes in LDS
+    constexpr int GROUP = D / NG, KS = D / 32, VROW = D / 2 + 16;  // bytes of a row of V codes in LDS
     constexpr int MPG = GROUP / 32;                                               // matrix instructions of a group
-    constexpr int KEYS = kKv4Keys<FOLD>, UNIT = kKv4Stride<FOLD>, SUBS = Tile::SUBS, OWN = Tile::OWN, COLS = 16 / FOLD;
+    constexpr int KEYS = kKv4Keys<FOLD>, UNIT = NW * KEYS, SUBS = Tile::SUBS, OWN = Tile::OWN, COLS = 16 / FOLD;
     extern __shared__ __align__(16) char sm[];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 15, j = lane >> 4;
     const int G = a.Hq / a.c.Hkv, R = G * a.Sq;
@@ -126,7 +124,7 @@ template <typename T, int D, int NG, int FOLD> __global__ __launch_bounds__(kKv4
     int *flag = (int *)(l_s + NW * 16);
     auto o_s = [&](int w) { return (float *)(sm + w * wave_bytes); };
 
-    Kv4Run<FOLD> share(a, blockIdx.x, lane);
+    Kv4Run<FOLD, NW> share(a, blockIdx.x, lane);
     const int first = __builtin_amdgcn_readfirstlane(share.first), total = __builtin_amdgcn_readfirstlane(share.total), quota = __builtin_amdgcn_readfirstlane(share.quota);
     int unit = first;
     if (unit >= total) return;
@@ -507,30 +505,30 @@ template <typename T, int D, int NG, int FOLD> __global__ __launch_bounds__(kKv4
     }
     __syncthreads();
     const int n_front = flag[0], n_tail = flag[1];
-    if (n_front >= 0 && n_front == front.w1 - front.w0) kv4_join<T, D, COLS, true>(a, front, (uint64_t *)sm, tid);
-    if (n_tail >= 0 && n_tail == tail.w1 - tail.w0) kv4_join<T, D, COLS, true>(a, tail, (uint64_t *)sm, tid);
+    if (n_front >= 0 && n_front == front.w1 - front.w0) kv4_join<T, D, COLS, NW * 64, true>(a, front, (uint64_t *)sm, tid);
+    if (n_tail >= 0 && n_tail == tail.w1 - tail.w0) kv4_join<T, D, COLS, NW * 64, true>(a, tail, (uint64_t *)sm, tid);
 }
 
 // The same by a launch of its own, a workgroup for each pair of sequence and kv head.
-template <typename T, int D, int FOLD> __global__ __launch_bounds__(256) void attn_kv4_join_kernel(Kv4Args a) {
+template <typename T, int D, int FOLD, int W> __global__ __launch_bounds__(256) void attn_kv4_join_kernel(Kv4Args a) {
     __shared__ uint64_t ml[64 * 16 / FOLD];
     const int lane = threadIdx.x & 63, b = blockIdx.x / a.c.Hkv, h = blockIdx.x % a.c.Hkv;
     // the units in front of the pair's, and how many there are in all
     int front = 0, total = 0;
     for (int b0 = 0; b0 < a.B; b0 += 64) {
-        const int n = b0 + lane < a.B ? Kv4Run<FOLD>::units(PagedSeq(a.c, b0 + lane, a.Sq)) : 0;
+        const int n = b0 + lane < a.B ? Kv4Run<FOLD, W>::units(PagedSeq(a.c, b0 + lane, a.Sq)) : 0;
         total += wave_sum_i32(n);
         front += wave_sum_i32(b0 + lane < b ? n : 0);
     }
     const PagedSeq seq(a.c, b, a.Sq);
-    const int n_units = Kv4Run<FOLD>::units(seq);
-    const int quota = Kv4Run<FOLD>::share_of(a, total * a.c.Hkv);
+    const int n_units = Kv4Run<FOLD, W>::units(seq);
+    const int quota = Kv4Run<FOLD, W>::share_of(a, total * a.c.Hkv);
     const int u0 = front * a.c.Hkv + h * n_units, w0 = u0 / quota;
     const Kv4Parts p{b, h, seq.fresh, w0, (u0 + n_units - 1) / quota, u0 != w0 * quota};
-    if (p.w1 > w0) kv4_join<T, D, 16 / FOLD, false>(a, p, ml, threadIdx.x);
+    if (p.w1 > w0) kv4_join<T, D, 16 / FOLD, 256, false>(a, p, ml, threadIdx.x);
 }
 
 // by type, a translation unit each (attention_kv4_go.h): fold: how often the rows are put side by side
-template <typename T> int kv4_stream_go(const Kv4Args &a, int D, int group, int fold, hipStream_t s);
+template <typename T> int kv4_stream_go(const Kv4Args &a, int D, int group, int fold, int waves, hipStream_t s);
 
 }  // namespace mynn

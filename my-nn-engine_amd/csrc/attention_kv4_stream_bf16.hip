@@ -1,5 +1,5 @@
 #include "attention_kv4_go.h"
 
 namespace mynn {
-template int kv4_stream_go<bf16_t>(const Kv4Args &, int, int, int, hipStream_t);
+template int kv4_stream_go<bf16_t>(const Kv4Args &, int, int, int, int, hipStream_t);
 }

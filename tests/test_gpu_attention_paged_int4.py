@@ -307,6 +307,23 @@ def test_many_parts_of_one_sequence(mynn):
         check(mynn, queries(1, Hq, 1, 64, torch.float16), pools, table, [60000])
 
 
+@pytest.mark.parametrize("dtype,B,Hq,Hkv,D,group,P,most", [
+    (torch.float16, 130, 64, 16, 128, 128, 64, 700),   # 2080 (sequence, kv head)s: a wave each
+    (torch.bfloat16, 300, 32, 8, 64, 32, 32, 300),
+    (torch.bfloat16, 70, 256, 32, 64, 64, 128, 200),   # 8 rows
+    (torch.float16, 260, 8, 8, 128, 32, 256, 900),     # one row, four groups
+    (torch.float16, 64, 16, 16, 128, 64, 64, 511),     # 1024, and caches of 512 rows
+])
+def test_a_wave_for_each_sequence_and_kv_head(mynn, dtype, B, Hq, Hkv, D, group, P, most):
+    g = torch.Generator().manual_seed(B)
+    past = [int(x) for x in torch.randint(0, most, (B,), generator=g)]
+    past[0], past[1], past[-1] = most, 0, 1
+    pools, table = cache(B, Hkv, D, P, group, dtype, [p + 1 for p in past], seed=40)
+    table[B // 2, 0] = -1
+    q = queries(B, Hq, 1, D, dtype)
+    check(mynn, q, pools, table, past, new=[int(i % 7 != 3) for i in range(B)])
+
+
 def test_one_workspace_for_calls_of_every_shape(mynn):
     """kept from the call that needs most of it, in any order, rows few and many; one that is too small is refused"""
     past = [4000, 900, 17, 0, 300, 2222]
