@@ -24,12 +24,12 @@ static int kv4_cus() {
 static bool kv4_few_rows(int Hq, int Hkv, int Sq) { return (long)(Hq / Hkv) * Sq <= 16; }
 // How often the rows are put side by side: as 16 columns have room for them.  (Four groups of columns a row: twice at the most, the tile of 64 keys does not fit the registers.)
 static int kv4_fold(long rows, int groups) { return rows <= 4 && groups < 4 ? 4 : rows <= 8 ? 2 : 1; }
-// Waves that share a (sequence, kv head)'s keys step by step.  Four; one where there is a (sequence, kv head) for each wave, or one for every other and few keys: what a workgroup
+// Waves that share a (sequence, kv head)'s keys step by step.  Four; one where there is a (sequence, kv head) for each wave, or fewer and few keys: what a workgroup
 // waits for at its ends -- lengths, pages, the first codes, the others' results -- another's work fills then (32 / 8 heads of 128, one token of 256 sequences of 64 keys 24 us and,
-// one wave each, 13, of 512 47 and 38, of 8192 587 and 568; 128 of 256 17 and 15, of up to 2048 62 and 64; 64 of 512 15 and 20).  More than 8 rows keep four: the join by a single wave would have 16 pairs of columns a lane.
+// one wave each, 13, of 512 47 and 38, of 8192 587 and 568; 128 of 256 17 and 15, of up to 2048 62 and 64; 64 of 128 10.4 and 8.8, of 256 11 and 13).  More than 8 rows keep four: the join by a single wave would have 16 pairs of columns a lane.
 static int kv4_waves(long pairs, long R, long rows) {
     const long cus = kv4_cus();
-    return R <= 8 && (pairs >= 8 * cus || (pairs >= 4 * cus && rows <= 512)) ? 1 : 4;
+    return R <= 8 && (pairs >= 8 * cus || (pairs >= 4 * cus && rows <= 512) || (pairs >= 2 * cus && rows <= 128)) ? 1 : 4;
 }
 static int kv4_unit(int fold, int waves) { return waves * (fold == 4 ? kKv4Keys<4> : kKv4Keys<1>); }
 // workgroups of the form for few rows: as many as run at once, no more than there can be units, or than there are counters

@@ -313,6 +313,7 @@ def test_many_parts_of_one_sequence(mynn):
     (torch.bfloat16, 70, 256, 32, 64, 64, 128, 200),   # 8 rows
     (torch.float16, 260, 8, 8, 128, 32, 256, 900),     # one row, four groups
     (torch.float16, 64, 16, 16, 128, 64, 64, 511),     # 1024, and caches of 512 rows
+    (torch.bfloat16, 64, 32, 8, 128, 128, 32, 127),    # 512, and caches of 128
 ])
 def test_a_wave_for_each_sequence_and_kv_head(mynn, dtype, B, Hq, Hkv, D, group, P, most):
     g = torch.Generator().manual_seed(B)
