@@ -402,3 +402,58 @@ def test_pools_of_more_than_32_bits_of_bytes(mynn):
             assert same_bits(a, b), step
         past += n
     check(mynn, got[1][0], small, where[1], (past - n).tolist())
+
+
+@pytest.mark.parametrize("S", [1, 33])
+def test_sequences_that_share_pages(mynn, S):
+    """a prompt's pages in the tables of several sequences"""
+    past = [200, 170, 128]
+    pools, table = cache(3, 2, 64, 32, 64, torch.bfloat16, [p + S for p in past], seed=41)
+    table[1:, :4] = table[0, :4]
+    check(mynn, queries(3, 16, S, 64, torch.bfloat16), pools, table, past)
+
+
+def test_calls_from_two_threads(mynn):
+    """each on a stream of its own, appends into pages of its own and attention behind them"""
+    import threading
+
+    Hq, Hkv, D, P, steps = 8, 2, 128, 32, 12
+    cos, sin = tables(64, D, torch.float16)
+    state = []
+    for n in range(2):
+        pools, table = cache(2, Hkv, D, P, 128, torch.float16, [64, 64], seed=50 + n)
+        rows = torch.randn(steps, 2, 1, (Hq + 2 * Hkv) * D, generator=torch.Generator().manual_seed(n)).half().cuda()
+        ws = mynn.attention_paged_int4_workspace(torch.empty(2, Hq, 1, D, dtype=torch.float16, device="cuda"), pools, table)
+        state.append((pools, table, rows.view(steps, 2, 1, -1, D).transpose(2, 3), ws))
+
+    def run(n, out):
+        pools, table, rows, ws = state[n]
+        pools = [p.clone() for p in pools]
+        past = torch.tensor([3, 20], dtype=torch.int32, device="cuda")
+        for i in range(steps):
+            q = mynn.rope_append_paged(rows[i][:, :Hq], rows[i][:, Hq:Hq + Hkv], rows[i][:, Hq + Hkv:], cos, sin, pools, table, past)
+            out.append(mynn.attention_paged_int4(q, pools, table, 0.1, past, workspace=ws))
+            past = past + 1
+
+    want = [[], []]
+    for n in range(2):
+        run(n, want[n])
+    torch.cuda.synchronize()
+    got, bad = [[], []], []
+
+    def thread(n):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                run(n, got[n])
+                torch.cuda.current_stream().synchronize()
+        except Exception as e:  # (shown below: an exception in a thread ends only that)
+            bad.append(e)
+
+    threads = [threading.Thread(target=thread, args=(n,)) for n in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join(60)
+    assert not bad
+    for n in range(2):
+        assert len(got[n]) == steps and all(same_bits(a, b) for a, b in zip(got[n], want[n]))
