@@ -278,7 +278,8 @@ int mynn_kv_pages_destroy(mynn_kv_pages *pages);
  * MYNN_F16 or MYNN_BF16.  page_table: device int32 [B, pages_per_seq]; a page number outside [0, n_pages) (an unmapped page is
  * -1) is a page that is not there.  past_lens: device int32 [B], the rows of each sequence in the cache before this step;
  * new_lens: device int32 [B] or NULL, how many of the call's S tokens are the sequence's own (0 .. S; NULL: all): token i
- * of sequence b is cache row past_lens[b] + i.  Both are read on the device: a captured call follows them.
+ * of sequence b is cache row past_lens[b] + i.  Both are read on the device, more than once in a call, which nothing may change
+ * while it runs: a captured call follows them.
  *
  * RoPE of q and k (as mynn_rope), and k and v to the cache: in 16 bits as they are, in 8 by the rule of
  * mynn_quantizing_kvcache_update, in 4 by that of mynn_quantize_int4_groups (of the row in dtype; a group with a value that is

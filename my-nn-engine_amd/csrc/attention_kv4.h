@@ -131,7 +131,7 @@ template <int UNIT> struct Kv4Share {
         b = before = 0;
         if (first >= total) return;
         int front = 0;
-        for (int b0 = 0;; b0 += 64) {
+        for (int b0 = 0; b0 < a.B; b0 += 64) {
             const int here_past = past, here_fresh = fresh;
             if (b0 + 64 < a.B) lengths(a, b0 + 64, lane);  // (on their way meanwhile)
             const uint64_t behind = __builtin_amdgcn_ballot_w64((front + r) * H > first);
@@ -145,6 +145,7 @@ template <int UNIT> struct Kv4Share {
             front += __builtin_amdgcn_readlane(r, 63);
             r = run(a, lane);
         }
+        first = total;  // (lengths that change under the call, which no program may do: nothing to do, and an end)
     }
 };
 

@@ -415,6 +415,7 @@ template <typename T, int D, int NG, int FOLD, int NW> __global__ __launch_bound
         const int done_b = b, done_h = h, done_fresh = seq.fresh, u0 = unit - at, units = n_units, end = min(n_units, at + stop - unit);
         const bool whole = at == 0 && end == n_units, second = unit != first;  // (a workgroup has two parts at the most: in its first place and in another)
         unit += end - at;
+        if (h + 1 == a.c.Hkv && b + 1 == a.B) unit = max(unit, stop);  // (the last there is, whatever the lengths were when they were added up)
         if (unit < stop) {
             at = 0;
             if (++h == a.c.Hkv) {
