@@ -53,15 +53,20 @@ static Kv4TilePlan kv4_tile_plan(int B, int Sq, int Hq, int Hkv, long rows) {
         p.ranges = (int)(want < 2 ? 1 : want > most ? most : want);
         return p;
     };
+    // Up to 32 rows, drafts to be checked: four waves on one block of 32, which shares its tiles of 128 keys between them (32 x 5 tokens behind 4000 rows 66 us, as half of a block of
+    // 64 85; 64 x 5 behind 1000 38 and 66; 8 x 6 behind 4000 31 and 34).  Not where both the (sequence, kv head)s and their keys are few: a tile of 128 is a long wait then
+    // (4 x 8 behind 500 18 and 16; 16 x 6 behind 800 23 both).
+    if (R <= 32 && (pairs >= cus || rows >= 2048)) return plan(32, pairs < 2 * cus && rows >= 2048);
     // Blocks of 128 rows turn codes into operands for the most rows: where they fill the device (32 / 8 heads of 128, groups of 128, bf16: one prompt of 4096 rows 228 us, blocks
     // of 64 278; one of 2048 82 and 88), and, in ranges, where both rows and keys are many (512 tokens behind 3000 rows 65, blocks of 64 in ranges 71, whole 84).
     if (pairs * ((R + 127) / 128) >= 2 * cus) return plan(128, false);
     if (R >= 1024 && rows >= 2048) return plan(128, true);
     // Blocks of 64 leave two waves to a block of 32 rows, half of each tile's keys each, and a tile takes 1.6 us where it took 2.3: one prompt of 1200 rows 38 us, in blocks of
     // 128 49, those in ranges 57.  Ranges cost a launch more, 5 us and up: they pay for few blocks of 512 keys and more (4 x 40 tokens behind 2000 rows 30 us, whole 49; one prompt
-    // of 300 rows 19, whole 16), of more than one for each CU only behind many keys (32 x 5 tokens behind 4000 rows 75, whole 92; 8 x 64 behind 1000 rows 36, whole 33).
+    // of 300 rows 19, whole 16), of one for each CU only behind many keys (8 x 64 tokens behind 3000 rows 65, whole 75, behind 1000 36
+    // and 33; 8 x 100 behind 2100, 448 blocks, 89 and 77).
     const long wgs = pairs * ((R + 63) / 64);
-    return plan(64, wgs < cus ? rows >= 512 : wgs < 2 * cus && rows >= 2048);
+    return plan(64, wgs < cus ? rows >= 512 : 2 * wgs < 3 * cus && rows >= 2048);
 }
 
 }  // namespace mynn

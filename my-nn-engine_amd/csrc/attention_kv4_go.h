@@ -31,23 +31,23 @@ template <typename T> int kv4_stream_go(const Kv4Args &a, int D, int group, int 
     });
 }
 
-template <typename T, int D, int NG, int QW, int KW> static int kv4_tile_launch(const Kv4Args &a, const Kv4TilePlan &p, hipStream_t s) {
-    using Block = Kv4Block<D, NG, QW, KW, 64>;
+template <typename T, int D, int NG, int QW, int KW, int KEYS> static int kv4_tile_launch(const Kv4Args &a, const Kv4TilePlan &p, hipStream_t s) {
+    using Block = Kv4Block<D, NG, QW, KW, KEYS>;
     static bool set = false;
     if (!set && Block::LDS > 64 * 1024) {
-        MYNN_HIP(hipFuncSetAttribute((const void *)attn_kv4_tile_kernel<T, D, NG, QW, KW, 64>, hipFuncAttributeMaxDynamicSharedMemorySize, Block::LDS));
+        MYNN_HIP(hipFuncSetAttribute((const void *)attn_kv4_tile_kernel<T, D, NG, QW, KW, KEYS>, hipFuncAttributeMaxDynamicSharedMemorySize, Block::LDS));
         set = true;
     }
-    MYNN_LAUNCH((attn_kv4_tile_kernel<T, D, NG, QW, KW, 64>), dim3((unsigned)(a.B * a.c.Hkv * p.blocks * p.ranges)), dim3(Block::THREADS), Block::LDS, s, a);
+    MYNN_LAUNCH((attn_kv4_tile_kernel<T, D, NG, QW, KW, KEYS>), dim3((unsigned)(a.B * a.c.Hkv * p.blocks * p.ranges)), dim3(Block::THREADS), Block::LDS, s, a);
     return launch_status("attn_kv4_tile_kernel");
 }
 template <typename T> int kv4_tile_go(const Kv4Args &a, int D, int group, const Kv4TilePlan &p, hipStream_t s) {
     return kv4_shape(D, group, [&](auto d, auto n) {
         constexpr int DD = decltype(d)::value, NG = decltype(n)::value;
-        const int rc = p.rows == 64 ? kv4_tile_launch<T, DD, NG, 2, 2>(a, p, s) : kv4_tile_launch<T, DD, NG, 4, 1>(a, p, s);
+        const int rc = p.rows == 32 ? kv4_tile_launch<T, DD, NG, 1, 4, 128>(a, p, s) : p.rows == 64 ? kv4_tile_launch<T, DD, NG, 2, 2, 64>(a, p, s) : kv4_tile_launch<T, DD, NG, 4, 1, 64>(a, p, s);
         if (rc || p.ranges == 1) return rc;
         const size_t threads = (size_t)a.B * a.Hq * a.Sq * (DD / 4);
-        MYNN_LAUNCH((attn_kv4_ranges_kernel<T, DD>), dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, s, a, p.rows, 64);
+        MYNN_LAUNCH((attn_kv4_ranges_kernel<T, DD>), dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, s, a, p.rows, p.rows == 32 ? 128 : 64);
         return launch_status("attn_kv4_ranges_kernel");
     });
 }

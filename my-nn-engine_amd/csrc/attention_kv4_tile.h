@@ -2,7 +2,7 @@
 // v_mfma_f32_32x32x16_f16.
 //
 // A workgroup of QW x KW waves has QW blocks of rows and walks their keys in tiles of KEYS, a KW-th of each tile a wave.  Codes travel global -> registers (a tile ahead)
-// -> (code - zero) in fp16 -> LDS, once for all rows of the workgroup: two stages, one barrier a tile.
+// -> (code - zero) in fp16 -> LDS, once for all rows of the workgroup: two stages, one barrier a tile (tiles of 128 keys: one stage, two barriers).
 //   S^T = K . Q^T      per group of columns; a key's scale meets the group's sum
 //   softmax            a lane has ONE row and half of the keys of each 32; the reference with the value scales in it (attention_kv4.h)
 //   O^T += V^T . P^T   p * vs as one fp16 number (T = bf16) or two; P stays in registers (the D layout of S^T is the B layout of P^T with the keys in the order 4g+0..3, 8+4g+0..3), V^T
@@ -25,7 +25,8 @@ template <int D, int NG, int QW, int KW, int KEYS> struct Kv4Block {
     static constexpr int STAGE = 2 * TILEB + SCALES + FLAGS;
     static constexpr int WORDS = D / 2 + 2;  // of a lane's result: reference, sum, O^T
     static constexpr int MERGE = KW > 1 ? QW * KW * 64 * WORDS * 4 : 0;
-    static constexpr int LDS = 2 * STAGE > MERGE ? 2 * STAGE : MERGE;
+    static constexpr int STAGES = KEYS == 64 ? 2 : 1;  // (two workgroups a CU)
+    static constexpr int LDS = STAGES * STAGE > MERGE ? STAGES * STAGE : MERGE;
     static_assert(NH >= 1 && UNITS >= 1 && STAGE % 16 == 0, "whole 32s of keys a wave, whole quarter rows a thread");
 };
 
@@ -303,10 +304,11 @@ template <typename T, int D, int NG, int QW, int KW, int KEYS> __global__ __laun
     int t = t0, stage = 0;
     auto next = [&]() __attribute__((always_inline)) {
         char *here = sm + stage * B::STAGE;
+        if (B::STAGES == 1 && t > t0) __syncthreads();
         store(here);  // (tile t - 2, which lay here, is behind the last barrier for every wave)
         if (t + 1 < t1) load(t + 1);
         __syncthreads();
-        stage ^= 1;
+        if (B::STAGES == 2) stage ^= 1;
         return here;
     };
     // the tiles that all rows of the workgroup see in full, then those with hidden keys.  (Loops of their own: with both kinds of tile in one, the results were copied from
@@ -342,9 +344,11 @@ template <typename T, int D, int NG, int QW, int KW, int KEYS> __global__ __laun
             l = l * ca + from[64] * cb;
             M = mn;
 #pragma unroll
-            for (int t2 = 0; t2 < DT; t2++)
+            for (int t2 = 0; t2 < DT; t2++) {
 #pragma unroll
                 for (int e = 0; e < 16; e++) o[t2][e] = o[t2][e] * ca + from[(2 + 16 * t2 + e) * 64] * cb;
+                asm volatile("" : "+v"(o[t2]));  // (here, and not with the stores: the waves' results of all would have to be kept till then)
+            }
         }
     }
     // (The lane's place once more, from the wave: what it is known by at the start would be one register too many over the loops.)

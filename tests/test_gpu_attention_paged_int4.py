@@ -300,6 +300,23 @@ def test_ranges_of_keys_of_ragged_prompts(mynn, S, causal):
     check(mynn, one[0], pools, one[1], past[:1], causal=causal)
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("D,group", [(64, 64), (64, 32), (128, 128), (128, 64), (128, 32)])
+@pytest.mark.parametrize("B,G,S,longest", [(2, 4, 5, 2300), (2, 8, 4, 2500), (130, 4, 8, 300), (130, 17, 1, 150), (2, 3, 7, 4000)])
+def test_drafts(mynn, dtype, D, group, B, G, S, longest):
+    """17 to 32 rows of a kv head, over long caches and in large batches: tiles of 128 keys; pages that are not there among them"""
+    g = torch.Generator().manual_seed(B + S)
+    past = [int(x) for x in torch.randint(0, longest // 4 if B > 2 else longest, (B,), generator=g)]
+    past[0], past[1] = longest, 100
+    pools, table = cache(B, 2, D, 32 if B > 2 else 128, group, dtype, [p + S for p in past], seed=60 + G)
+    q = queries(B, 2 * G, S, D, dtype)
+    new = [S - i % (S + 1) for i in range(B)]
+    check(mynn, q, pools, table, past, new=new)
+    table[0, 1] = -1
+    check(mynn, q, pools, table, past, new=new, causal=False)
+    check(mynn, q[:2], pools, table[:2].contiguous(), past[:2], twice=False)
+
+
 def test_many_parts_of_one_sequence(mynn):
     """more than 64 of them in a join"""
     pools, table = cache(1, 1, 64, 256, 64, torch.float16, [60001], seed=32)

@@ -19,7 +19,7 @@ def test_no_form_uses_scratch_memory(tmp_path):
         notes = subprocess.check_output([READELF, "--notes", str(tmp_path / "code")], text=True)
         for name, scratch in re.findall(r"\.name:\s+(\S*(?:attn_kv4_|append_paged_kernel)\S*)\n(?:(?!\.name:).)*?\.private_segment_fixed_size:\s+(\d+)", notes, re.S):
             forms[name] = int(scratch)
-    # (two types: five shapes with 3 ways to put rows side by side but one, all but 16 rows by four waves or one, their joins; two tiles and the joins of their ranges; the append's
+    # (two types: five shapes with 3 ways to put rows side by side but one, all but 16 rows by four waves or one, their joins; three tiles and the joins of their ranges; the append's
     # kinds, aligned or not)
-    assert len(forms) >= 2 * (23 + 10 + 10 + 2 + 18)
+    assert len(forms) >= 2 * (23 + 10 + 15 + 2 + 18)
     assert not {k: v for k, v in forms.items() if v}
