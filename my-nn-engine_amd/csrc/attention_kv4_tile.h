@@ -5,7 +5,7 @@
 // -> (code - zero) in fp16 -> LDS, once for all rows of the workgroup: two stages, one barrier a tile (tiles of 128 keys: one stage, two barriers).
 //   S^T = K . Q^T      per group of columns; a key's scale meets the group's sum
 //   softmax            a lane has ONE row and half of the keys of each 32; the reference with the value scales in it (attention_kv4.h)
-//   O^T += V^T . P^T   p * vs as one fp16 number (T = bf16) or two; P stays in registers (the D layout of S^T is the B layout of P^T with the keys in the order 4g+0..3, 8+4g+0..3), V^T
+//   O^T += V^T . P^T   p * vs as two fp16 numbers; P stays in registers (the D layout of S^T is the B layout of P^T with the keys in the order 4g+0..3, 8+4g+0..3), V^T
 //                      comes from the row-major tile by transposing reads
 // Vector operations and matrix instructions bound it together (busy 65 and 31 % of the time at 4 x 2048 rows): 350 of the one for 32 of the other in a wave's 64 keys of 32 rows,
 // 100 of them the staging's.  4 prompts of 2048 rows, 32 / 8 heads of 128, groups of 128, bf16: 197 us in a program's calls, 0.70 PFLOP/s (the products alone, at what a large
@@ -51,9 +51,9 @@ __device__ __forceinline__ int kv4_ranges(int tiles, int length, int most) { ret
 template <typename T, int D, int NG, int QW, int KW, int KEYS> __global__ __launch_bounds__(QW *KW * 64, 2) void attn_kv4_tile_kernel(Kv4Args a) {
     using B = Kv4Block<D, NG, QW, KW, KEYS>;
     constexpr int KS = D / 16, DT = D / 32, NH = B::NH, DW = D / 32, ROWB = B::ROWB, KPG = KS / NG, TPG = DT / NG;
-    // p * vs for the second product: results in bf16 have 8 bits, and its rounding to fp16, 11, does not show; those in fp16 would be off by half as much again (their own
-    // rounding and this one, of the same size), so there it is two numbers of 11 bits.
-    constexpr int PARTS = std::is_same<T, f16_t>::value ? 2 : 1;
+    // p * vs for the second product: two numbers of 11 bits.  (One is off by as much as results in fp16 are rounded.  Results in bf16 hide most of that, and 4 x 2048 rows took
+    // 196 us for 225; but those of many rows then differed by 10^-3 from what few rows, 22 bits all, and 32-bit operations give, 6 10^-5 with two.)
+    constexpr int PARTS = 2;
     extern __shared__ __align__(16) char sm[];
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), wave = w % QW, kg = w / QW, col = lane & 31, g = lane >> 5;
     const int G = a.Hq / a.c.Hkv, R = G * a.Sq;
