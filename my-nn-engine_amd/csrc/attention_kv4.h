@@ -1,9 +1,12 @@
 // Attention over a paged cache held in 4 bits, for sequences of different lengths: what the forms for few rows (attention_kv4_stream.h) and for many
 // (attention_kv4_tile.h) share.
 //
-// Both keep the codes exact: (code - zero) is a whole number of -15 .. 15, an fp16 operand of the matrix cores in either product, whatever T is; a key's
-// scale meets its score, a value's scale its weight, in 32 bits.  Queries enter as fp16 times a power of two of their row (T = bf16 has fewer bits and more
-// range).  Weights enter the second product as fp16 numbers p * vs: the reference M of the online softmax is chosen so that they fit,
+// Both keep the codes exact: (code - zero) is a whole number of -15 .. 15, an operand of the matrix cores in either product, whatever T is; a key's scale
+// meets its score, a value's scale its weight, in 32 bits.
+// Scores: queries enter as fp16 times a power of two of their row (T = bf16 has fewer bits and more range), a key's codes as they lie in their nibble, fp16
+// numbers without a leading one: (code - zero) 2^-24 or, four bits further up, 2^-20.  So the sum over a row's columns is below 4, whatever the queries are, and
+// its product with a scale of bf16 fits 32 bits.
+// Weights enter the second product as fp16 numbers p * vs: the reference M of the online softmax is chosen so that they fit,
 //   M = max over the keys of (s + log2 |vs|) - 14,   s the score in units of log2 (|vs| of less than 2^-86 counts as that),
 // so that p = 2^(s - M) <= 2^100 and p * vs < 2^14.1, with the largest near it.  A value row with a large scale and no weight takes nothing from the others then, and
 // no unit is left to be taken out: numerator and denominator have the same M.
@@ -27,7 +30,41 @@ struct Kv4Args {
     int *length;              // and how long a range is, as the first workgroup found it
 };
 
-// code - zero of a dword's eight, as Int4Pairs has them, each pair with zero points of its own (pairs (0,4), (1,5), (2,6), (3,7): off[0 .. 3])
+// Keys: (code - zero) 2^-24 of a dword's eight in pairs (0, 4), (2, 6), 2^-20 in (1, 5), (3, 7): a nibble under no exponent is such a number, and so is its difference to another.
+struct Kv4Keys {
+    h2_t low, high;
+    __device__ void at(uint32_t z) {
+        low = __builtin_bit_cast(h2_t, 0x80008000u + z * 0x00010001u);
+        high = __builtin_bit_cast(h2_t, 0x80008000u + z * 0x00100010u);
+    }
+    __device__ U4 operator()(uint32_t w) const {
+        auto two = [&](uint32_t n, h2_t off) { return __builtin_bit_cast(uint32_t, __builtin_bit_cast(h2_t, n) + off); };
+        const uint32_t v = w >> 8;
+        return U4{two(w & 0x000F000Fu, low), two(w & 0x00F000F0u, high), two(v & 0x000F000Fu, low), two(v & 0x00F000F0u, high)};
+    }
+};
+// A row's queries for them: eight times 2^e in the same order, e as large as fp16 takes for a row whose largest is `peak` (2^e of it below 2^15; the odd columns have 2^-4
+// of that, which their codes make up for).  Values down to 2^-24 of the largest keep their 11 bits.
+__device__ __forceinline__ int kv4_query_exponent(float peak) { return peak > 0.f ? 15 - __builtin_amdgcn_frexp_expf(peak) : 0; }
+__device__ __forceinline__ U4 kv4_queries(const float *f, int e) {
+    float x[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++) x[i] = __builtin_amdgcn_ldexpf(f[i], e - 4 * (i & 1));
+    return U4{pack2<f16_t>(x[0], x[4]), pack2<f16_t>(x[1], x[5]), pack2<f16_t>(x[2], x[6]), pack2<f16_t>(x[3], x[7])};
+}
+// What makes a score, in units of log2, of a sum of theirs: 2^(24 - e) times the call's scale.  For queries past 2^91 (T = bf16) that could leave the 32-bit numbers: the
+// scores of the lanes in `far` are multiplied with 2^37 then.
+struct Kv4Score {
+    float by;
+    uint64_t far;
+    template <typename T> static __device__ __forceinline__ Kv4Score of(float scale, int e) {
+        const bool past = !std::is_same<T, f16_t>::value && 24 - e > 100;
+        return {__builtin_amdgcn_ldexpf(scale * 1.4426950408889634f, 24 - e - (past ? 37 : 0)), __builtin_amdgcn_ballot_w64(past)};
+    }
+    __device__ __forceinline__ float far_by() const { return __builtin_amdgcn_inverse_ballot_w64(far) ? 0x1p37f : 1.f; }
+};
+
+// Values: code - zero of a dword's eight, as Int4Pairs has them, each pair with zero points of its own (pairs (0,4), (1,5), (2,6), (3,7): off[0 .. 3])
 __device__ __forceinline__ U4 kv4_pairs(uint32_t w, const h2_t *off, uint32_t nibbles0, uint32_t nibbles1) {
     auto two = [&](uint32_t v, uint32_t nibbles, uint32_t exponents, h2_t o) {
         const uint32_t n = (v & nibbles) | exponents;

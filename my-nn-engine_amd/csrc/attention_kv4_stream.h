@@ -131,6 +131,7 @@ template <typename T, int D, int NG, int FOLD, int NW> __global__ __launch_bound
     const int stop = min(unit + quota, total);
     Kv4Parts front{0, 0, 0, 0, -1, 0}, tail{0, 0, 0, 0, -1, 0};  // what this workgroup has parts of
     Int4Pairs pairs;
+    Kv4Keys keys;
     const float minus = kv4_minus();
     const int psh = a.c.page_shift, pmask = (1 << psh) - 1;
     const int fold = col / COLS, row = col % COLS < R ? col % COLS : 0;  // this lane's row, and which of the folds has it
@@ -236,7 +237,7 @@ template <typename T, int D, int NG, int FOLD, int NW> __global__ __launch_bound
         // ---- the rows' queries: B operand, columns 32 m + 8 j .. +7 (D = 64: in the order in which the exchange below leaves them) by pairs
         const int bound = col % COLS < R ? seq.bound(again(row) / G, a.causal) : 0;
         U4 qf[KS];
-        float csc;
+        Kv4Score score;
         {
             float x[KS][8], peak = 0.f;
 #pragma unroll
@@ -245,17 +246,10 @@ template <typename T, int D, int NG, int FOLD, int NW> __global__ __launch_bound
 #pragma unroll
                 for (int e = 0; e < 8; e++) peak = fmaxf(peak, fabsf(x[m][e]));
             }
-            peak = xor32_max(xor16_max(peak));
-            // (2^10 at the most: values down to 2^-24 of a row's largest keep their 11 bits, and sums stay far from the largest 32-bit number)
-            const int e10 = peak > 0.f ? 10 - __builtin_amdgcn_frexp_expf(peak) : 0;
+            const int exponent = kv4_query_exponent(xor32_max(xor16_max(peak)));
 #pragma unroll
-            for (int m = 0; m < KS; m++) {
-#pragma unroll
-                for (int e = 0; e < 8; e++) x[m][e] = __builtin_amdgcn_ldexpf(x[m][e], e10);
-                qf[m] = U4{pack2<f16_t>(x[m][0], x[m][4]), pack2<f16_t>(x[m][1], x[m][5]), pack2<f16_t>(x[m][2], x[m][6]), pack2<f16_t>(x[m][3], x[m][7])};
-                if (col % COLS >= R) qf[m] = U4{0u, 0u, 0u, 0u};
-            }
-            csc = __builtin_amdgcn_ldexpf(a.scale * 1.4426950408889634f, -e10);
+            for (int m = 0; m < KS; m++) qf[m] = col % COLS >= R ? U4{0u, 0u, 0u, 0u} : kv4_queries(x[m], exponent);
+            score = Kv4Score::of<T>(a.scale, exponent);
         }
         f4_t acc[D / 16];
 #pragma unroll
@@ -279,10 +273,10 @@ template <typename T, int D, int NG, int FOLD, int NW> __global__ __launch_bound
                 }
 #pragma unroll
                 for (int g = 0; g < NG; g++) {
-                    pairs.at(t.kz[s] >> (8 * g) & 15u);
+                    keys.at(t.kz[s] >> (8 * g) & 15u);
                     f4_t y = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                    for (int m = 0; m < MPG; m++) y = mfma16(pairs(d[g * MPG + m]), qf[g * MPG + m], y);
+                    for (int m = 0; m < MPG; m++) y = mfma16(keys(d[g * MPG + m]), qf[g * MPG + m], y);
 #pragma unroll
                     for (int e = 0; e < 4; e++) {
                         if constexpr (FOLD == 1) x[s][g][e] = y[e];
@@ -294,6 +288,7 @@ template <typename T, int D, int NG, int FOLD, int NW> __global__ __launch_bound
             // keys that the row does not see have no weight, and what lies in their scales does not count.  (Tiles that every row sees in full go the same way: a
             // path of their own would save 3 selections a score, 12 of 480 operations in a tile of 64 keys, and holds half as much code again.)
             float sv[OWN][4], vs[OWN][NG][4], top = -INFINITY;
+            const float far = !std::is_same<T, f16_t>::value ? score.far_by() : 1.f;
 #pragma unroll
             for (int s = 0; s < OWN; s++) {
                 const int there = FOLD == 4 && fold >= 2 ? t.there[SUBS / 2 - 1] : t.there[0];
@@ -310,7 +305,7 @@ template <typename T, int D, int NG, int FOLD, int NW> __global__ __launch_bound
                         vs[s][g][e] = e < room ? kv4_half<T>(t.vs[s][n / 2], n & 1) : 0.f;
                         bits = max(bits, kv4_bits<T>(t.vs[s][n / 2], n & 1));
                     }
-                    sv[s][e] = e < room ? y * csc : -INFINITY;
+                    sv[s][e] = e < room ? y * score.by * far : -INFINITY;
                     top = fmaxf(top, fmaf((float)bits, kKv4Step<T>, sv[s][e]));
                 }
             }

@@ -137,6 +137,7 @@ template <typename T, int D, int NG, int QW, int KW, int KEYS> __global__ __laun
     auto v_swz = [](int r) { return D == 128 ? (r & 3) * 5 : (((r >> 1) ^ r) & 1) << 2; };
     const float minus = kv4_minus();
     Int4Pairs pairs;
+    Kv4Keys keys;
     auto store = [&](char *stage) __attribute__((always_inline)) {
         float *scales = (float *)(stage + 2 * B::TILEB), *lift = scales + 2 * NG * KEYS;
         int *there = (int *)(lift + KEYS);
@@ -147,11 +148,12 @@ template <typename T, int D, int NG, int QW, int KW, int KEYS> __global__ __laun
             for (int n = 0; n < 2; n++) {
                 const Raw &x = raw[u][n];
                 const bool v = n == 1;
-                pairs.at(x.zero & 15u);
+                if (v) pairs.at(x.zero & 15u);
+                else keys.at(x.zero & 15u);
                 const int swz = v ? v_swz(r) : k_swz(r);
                 char *to = stage + (v ? B::TILEB : 0) + r * ROWB;
 #pragma unroll
-                for (int i = 0; i < DW; i++) *(U4 *)(to + (((quarter * DW + i) ^ swz) << 4)) = pairs(x.codes[i]);
+                for (int i = 0; i < DW; i++) *(U4 *)(to + (((quarter * DW + i) ^ swz) << 4)) = v ? pairs(x.codes[i]) : keys(x.codes[i]);
                 if (quarter % (4 / NG) == 0) scales[(v ? NG * KEYS : 0) + sg * KEYS + r] = Elem<T>::ld(&x.scale, 0);
                 if (v) {
                     const float bits = group_max<4>((float)kv4_bits<T>(__builtin_bit_cast(uint16_t, x.scale), 0));
@@ -165,7 +167,7 @@ template <typename T, int D, int NG, int QW, int KW, int KEYS> __global__ __laun
 
     // ---- Q^T: B operand, columns 16 ks + 8 g .. +7 in the codes' order, as fp16 times a power of two of the row
     U4 qf[KS];
-    float csc;
+    Kv4Score score;
     {
         const T *q = (const T *)a.q + (((size_t)b * a.Hq + h * G + row_c % G) * a.Sq + row_c / G) * D;
         U4 x[KS];
@@ -177,16 +179,13 @@ template <typename T, int D, int NG, int QW, int KW, int KEYS> __global__ __laun
 #pragma unroll
             for (int e = 0; e < 8; e++) peak = fmaxf(peak, fabsf(f[e]));
         }
-        peak = xor32_max(peak);
-        const int e10 = peak > 0.f ? 10 - __builtin_amdgcn_frexp_expf(peak) : 0;
+        const int exponent = kv4_query_exponent(xor32_max(peak));
 #pragma unroll
         for (int ks = 0; ks < KS; ks++) {
             widen8<T>(x[ks], f);
-#pragma unroll
-            for (int e = 0; e < 8; e++) f[e] = __builtin_amdgcn_ldexpf(f[e], e10);
-            qf[ks] = U4{pack2<f16_t>(f[0], f[4]), pack2<f16_t>(f[1], f[5]), pack2<f16_t>(f[2], f[6]), pack2<f16_t>(f[3], f[7])};
+            qf[ks] = kv4_queries(f, exponent);
         }
-        csc = __builtin_amdgcn_ldexpf(a.scale * 1.4426950408889634f, -e10);
+        score = Kv4Score::of<T>(a.scale, exponent);
     }
     f16x_t o[DT];
 #pragma unroll
@@ -225,6 +224,13 @@ template <typename T, int D, int NG, int QW, int KW, int KEYS> __global__ __laun
                     for (int e = 0; e < 4; e++) s[hf][4 * e4 + e] = gr == 0 ? x[4 * e4 + e] * f[e] : fmaf(x[4 * e4 + e], f[e], s[hf][4 * e4 + e]);
                 }
             }
+        if (!std::is_same<T, f16_t>::value && __builtin_expect(score.far != 0, 0)) {
+            const float f = score.far_by();
+#pragma unroll
+            for (int hf = 0; hf < NH; hf++)
+#pragma unroll
+                for (int e = 0; e < 16; e++) s[hf][e] *= f;
+        }
         float top = -INFINITY;
         uint32_t seen[NH];  // MASKED: a bit for each of the lane's keys of a 32
 #pragma unroll
@@ -245,7 +251,7 @@ template <typename T, int D, int NG, int QW, int KW, int KEYS> __global__ __laun
                 const f4_t f = *(const f4_t *)&lift[32 * hf + 8 * e4 + 4 * g];
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
-                    const float t = fmaf(s[hf][4 * e4 + e], csc, f[e]);
+                    const float t = fmaf(s[hf][4 * e4 + e], score.by, f[e]);
                     top = fmaxf(top, MASKED ? (seen[hf] >> (4 * e4 + e) & 1 ? t : -INFINITY) : t);
                 }
             }
@@ -267,7 +273,7 @@ template <typename T, int D, int NG, int QW, int KW, int KEYS> __global__ __laun
         for (int hf = 0; hf < NH; hf++)
 #pragma unroll
             for (int e = 0; e < 16; e++) {
-                const float p = __builtin_amdgcn_exp2f(fmaf(s[hf][e], csc, -ref));
+                const float p = __builtin_amdgcn_exp2f(fmaf(s[hf][e], score.by, -ref));
                 s[hf][e] = MASKED ? (seen[hf] >> e & 1 ? p : 0.f) : p;
                 lt += s[hf][e];
             }

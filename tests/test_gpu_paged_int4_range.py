@@ -1,0 +1,112 @@
+"""Attention over paged caches of 4 bits whose keys and queries lie at opposite ends of bf16."""
+import pytest
+import torch
+
+import paged_reference as ref
+from test_gpu_attention_paged_int4 import cache, queries
+from test_gpu_rope_append_paged import same_bits
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def mynn():
+    import gpu_util
+
+    return gpu_util.mynn
+
+
+def attention(q, pools, table, scale, past, new, causal=True):
+    """softmax(q k scale) v in 64 bits, and how far a result may be from it before it is rounded to its type, column by column:
+
+    A weight's error relative to itself: a score is a sum of D products of exact operands in 32 bits, scaled in a few more steps, (D + 8) half steps of 2^-24 of the
+    sum of the magnitudes; its exponential's argument is rounded at the size of the largest score, the exponential good to 2^-22; on its way into the second product a
+    weight keeps 20 bits or more; n keys' sums have n half steps, joins a few more.  Numerator and denominator have them both: twice their sum, times sum(p |v|) / sum(p).
+    And absolute: where the second product takes its weights as fp16 numbers, these are in units in which a scale next to the largest weight is 2^4 (few rows) or 1 (more
+    than 16 of a kv head) or more, so a small one is off by 2^-25 of these: 2^-29 or 2^-25 of its own scale times the largest weight.  In bf16 parts: 2^-100 and less of its
+    scale times the largest weight, and below 2^-133 in units of 2^-8 or more, nothing."""
+    B, Hq, S, D = q.shape
+    Hkv, P = pools[0].shape[1], pools[0].shape[2]
+    G, half = Hq // Hkv, 2.0 ** -24
+    tiny = 2.0 ** (-28 if G * S <= 16 else -24)
+    out = torch.zeros(q.shape, dtype=torch.float64, device=q.device)
+    slack = torch.zeros_like(out)
+    for b in range(B):
+        n = S if new is None else new[b]
+        length = past[b] + n
+        (k, there), (v, _) = ref.rows_of(pools, 0, table, b, 0, length), ref.rows_of(pools, 1, table, b, 0, length)
+        at = torch.arange(length, device=q.device)
+        for i in range(n):
+            seen = there & (at < (past[b] + i + 1 if causal else length))
+            for h in range(Hkv):
+                x, kk, vv = q[b, h * G:(h + 1) * G, i].double(), k[h][seen], v[h][seen]
+                s = torch.mm(x, kk.t().contiguous()) * scale
+                size = (torch.mm(x.abs(), kk.abs().t().contiguous()) * abs(scale)).amax(-1, keepdim=True)
+                p = torch.softmax(s, -1)
+                weight = (D + 8) * half * size + 4 * half * s.abs().amax(-1, keepdim=True) + 2.0 ** -22 + 2.0 ** -20 + (kk.shape[0] + 64) * half
+                out[b, h * G:(h + 1) * G, i] = torch.mm(p, vv)
+                slack[b, h * G:(h + 1) * G, i] = 2 * weight * torch.mm(p, vv.abs()) + tiny * p.amax(-1, keepdim=True) * vv.abs().sum(0) + kk.shape[0] * 2.0 ** -120
+    return out, slack
+
+
+def check(mynn, q, pools, table, past, new=None, causal=True, scale=None, bad=None):
+    """bad: which results stand for no number (the 64-bit ones are taken without what makes them so)"""
+    scale = q.shape[-1] ** -0.5 if scale is None else scale
+    dev = lambda x: None if x is None else torch.tensor(x, dtype=torch.int32, device="cuda")
+    ws = mynn.attention_paged_int4_workspace(q, pools, table)
+    got = mynn.attention_paged_int4(q, pools, table, scale, dev(past), dev(new), causal, workspace=ws)
+    again = mynn.attention_paged_int4(q, pools, table, scale, dev(past), dev(new), causal)
+    if bad is None:
+        want, slack = attention(q, pools, table, scale, past, new, causal)
+        assert same_bits(got, again)
+    else:
+        clean = [torch.where(torch.isfinite(p), p, torch.ones_like(p)) if p.is_floating_point() else p for p in pools]
+        want, slack = attention(q, clean, table, scale, past, new, causal)
+        assert torch.equal(torch.isfinite(got), ~bad) and torch.equal(torch.isfinite(again), ~bad)
+        got, again = (torch.where(bad, want.to(q.dtype), x) for x in (got, again))
+        assert same_bits(got, again)
+    ref.assert_close(got, want, slack)
+    return got
+
+
+def put_values(pools, table, side, x, group):
+    """rows [B, n, Hkv, D] in the place of each sequence's first n"""
+    P = pools[0].shape[2]
+    parts = ref.quantize4(x.to(pools[2].dtype), group, pools[2].dtype)
+    r = torch.arange(x.shape[1])
+    for b in range(x.shape[0]):
+        for n, t in enumerate(parts):
+            pools[2 * n + side][table[b].long().cpu()[r // P], :, (r % P)] = t[b].to(pools[0].device)
+
+
+def made(B, Hkv, D, P, group, dtype, n, values, seed, keys=None):
+    """a cache of B sequences of n rows, values (and keys) as given"""
+    pools, table = cache(B, Hkv, D, P, group, dtype, [n] * B, seed=seed)
+    put_values(pools, table, 1, values, group)
+    if keys is not None:
+        put_values(pools, table, 0, keys, group)
+    return pools, table
+
+
+def normal(seed, *shape):
+    return torch.randn(*shape, generator=torch.Generator().manual_seed(seed))
+
+
+# few rows of a kv head, up to 32, and many; heads, groups
+ROWS = [(1, 8), (4, 8), (6, 8), (40, 8)]
+SHAPES = [(64, 64), (64, 32), (128, 128), (128, 64), (128, 32)]
+
+
+@pytest.mark.parametrize("S,Hq", ROWS)
+@pytest.mark.parametrize("D,group", SHAPES)
+@pytest.mark.parametrize("key", [-118, -100, 100, 112, 120])
+@pytest.mark.parametrize("scale", [0.125, -0.125])
+def test_keys_and_queries_at_opposite_ends(mynn, D, group, S, Hq, key, scale):
+    """their products are ordinary scores"""
+    dtype, n = torch.bfloat16, 150 + S
+    k = normal(14, 2, n, 2, D) * 2.0 ** key
+    pools, table = made(2, 2, D, 64, group, dtype, n, normal(15, 2, n, 2, D), 16, keys=k)
+    q = (normal(17, 2, Hq, S, D) * 2.0 ** -key).to(dtype).cuda()
+    q[:, 0] *= 0.001  # (rows of their own sizes, a row of zeros)
+    q[:, 1] = 0.0
+    check(mynn, q, pools, table, [150, 31], new=[S, S], scale=scale)
