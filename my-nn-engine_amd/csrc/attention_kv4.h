@@ -6,10 +6,10 @@
 // Scores: queries enter as fp16 times a power of two of their row (T = bf16 has fewer bits and more range), a key's codes as they lie in their nibble, fp16
 // numbers without a leading one: (code - zero) 2^-24 or, four bits further up, 2^-20.  So the sum over a row's columns is below 4, whatever the queries are, and
 // its product with a scale of bf16 fits 32 bits.
-// Weights enter the second product as fp16 numbers p * vs: the reference M of the online softmax is chosen so that they fit,
-//   M = max over the keys of (s + log2 |vs|) - 14,   s the score in units of log2 (|vs| of less than 2^-86 counts as that),
-// so that p = 2^(s - M) <= 2^100 and p * vs < 2^14.1, with the largest near it.  A value row with a large scale and no weight takes nothing from the others then, and
-// no unit is left to be taken out: numerator and denominator have the same M.
+// Weights: p = 2^(s - M), s the score in units of log2 and M the largest of them so far, enter the second product with the value's scale: w = p * vs.  As fp16, in two
+// parts, where the scales of all values that are seen lie within 11 binades (Kv4Band): in units of a power of two that puts these near the upper end of fp16.  Elsewhere --
+// a group of zeros has the scale 1 and may lie beside values of 2^-60, one group may be 2^40 of the next, stand for NaN -- in three parts of bf16, all 24 bits of w in the
+// range of 32-bit numbers, and the codes as bf16 too.  (One reference for weight and scale, M = max (s + log2 vs), lost such neighbours without a word.)
 #pragma once
 #include "int4_codes.h"
 #include "kv_cache4.h"
@@ -76,18 +76,72 @@ __device__ __forceinline__ U4 kv4_pairs(uint32_t w, const h2_t *off, uint32_t ni
 // -(1024 + z) and -(64 + z) of two zero points (bytes 0 and 2 of zz)
 __device__ __forceinline__ h2_t kv4_low(uint32_t zz) { return __builtin_bit_cast(h2_t, (zz & 0x000F000Fu) | 0xE400E400u); }
 __device__ __forceinline__ h2_t kv4_high(uint32_t zz) { return __builtin_bit_cast(h2_t, ((zz << 4) & 0x00F000F0u) | 0xD400D400u); }
-
-// The reference may lag 2^4 behind: moving it moves every sum, and a row meets a new maximum every few keys for long.  (2^14 on top of the largest weight then is 2^10.)
-constexpr float kKv4Lag = 4.f;
-// The scale's part in the reference, from its bits: exponent and mantissa of T as one number are log2 of it, less than 0.09 too little (subnormal numbers of fp16: too much),
-// in steps of 2^-(bits of the mantissa) from kKv4Zero on.  |vs| of 2^-86 and less counts as 2^-86, so that p <= 2^100.
-template <typename T> constexpr float kKv4Step = std::is_same<T, f16_t>::value ? 0x1p-10f : 0x1p-7f;
-template <typename T> constexpr float kKv4Zero = std::is_same<T, f16_t>::value ? 15.f + 14.f : 127.f + 14.f;  // (what is taken off M: 2^14 on top)
-template <typename T> __device__ __forceinline__ uint32_t kv4_bits(uint32_t w, int hi) {
-    const uint32_t x = __builtin_amdgcn_ubfe(w, hi ? 16 : 0, 15);
-    return std::is_same<T, f16_t>::value ? x : max(x, (127u - 86u) << 7);
+__device__ inline f4_t mfma16_bf16(const U4 &a, const U4 &b, f4_t c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8_t, a), __builtin_bit_cast(b8_t, b), c, 0, 0, 0);
+}
+// whole numbers of fp16 as bf16 (at most 4 bits: the upper half of the 32-bit number)
+__device__ __forceinline__ U4 kv4_as_bf16(const U4 &x) {
+    auto two = [](uint32_t w) {
+        const h2_t h = __builtin_bit_cast(h2_t, w);
+        return __builtin_amdgcn_perm(__builtin_bit_cast(uint32_t, (float)h[1]), __builtin_bit_cast(uint32_t, (float)h[0]), 0x07060302u);
+    };
+    return U4{two(x.x), two(x.y), two(x.z), two(x.w)};
 }
 
+// M may lag 2^4 behind in the form for many rows: moving it moves every sum, and a row meets a new maximum every few keys for long.
+constexpr float kKv4Lag = 4.f;
+
+// Where the scales of the values lie that a wave has seen, one answer for all its rows: `unit` is log2 of what p is multiplied with.  Compared are the upper bits of a scale, sign
+// off; an exponent of the 32-bit number and T's differ by BIAS.
+//   fp16 parts   2^unit puts a scale of the size e at 2^TOP (2^12, or 2^8 where M may lag: scales of 4 e and weights of 2^4 stay below 2^16), the least that is let through,
+//                2^-8 e, at 2^4 or 1: a weight is off by 2^-25 of that unit, next to a scale of its own.  e is 1 at first, then the largest of the last tile that did not fit, of
+//                2^-40 .. 2^24: sums in one unit are finite in any other.
+//   wide         bf16 parts, from the first tile on whose scales do not lie within 9 binades, or lie outside of that, to the end of the keys.  2^unit is 2^40 while all scales are
+//                below 2^61, so that small ones are far from the least 32-bit number, then 2^-8: weights of 2^4 and scales of 2^125 have a finite product with a code.
+//                Such calls take up to twice as long: one token of 64 sequences of 8192 keys, bf16, 112 us and 224, of one of 32768 17.5 and 29, 4 x 2048 rows 234 and 484.
+template <typename T, int TOP> struct Kv4Band {
+    static constexpr int SHIFT = std::is_same<T, f16_t>::value ? 10 : 7, BIAS = std::is_same<T, f16_t>::value ? 112 : 0, EMAX = std::is_same<T, f16_t>::value ? 31 : 255;
+    uint32_t from, last;  // scales whose bits less `from` are above `last` are not let through
+    int unit;
+    bool wide = false;
+    __device__ __forceinline__ Kv4Band() { put(127); }
+    __device__ __forceinline__ void put(int e) {
+        from = (uint32_t)max(e - 8 - BIAS, 1) << SHIFT;
+        last = ((uint32_t)min(e + 3 - BIAS, EMAX) << SHIFT) - from - 1;
+        unit = TOP + 127 - e;
+    }
+    static __device__ __forceinline__ uint32_t bits(uint32_t w, int hi) { return __builtin_amdgcn_ubfe(w, hi ? 16 : 0, 15); }
+    __device__ __forceinline__ uint32_t off(uint32_t b) const { return b - from; }
+    // the exponent of a scale that is not zero, as of a 32-bit number, among the least lo and the largest hi; what is no number has none, and is below all others
+    static __device__ __forceinline__ void among(float scale, int &lo, int &hi) {
+        const int x = (int)(__builtin_bit_cast(uint32_t, scale) >> 23 & 255u), e = x == 255 ? 0 : x;
+        lo = scale == 0.f ? lo : min(lo, e), hi = max(hi, e);
+    }
+    // Scales that are not let through: each lane has the least and the largest exponent of some.
+    __device__ __forceinline__ void settle(int lane_lo, int lane_hi) {
+        typedef unsigned short us2_t __attribute__((ext_vector_type(2)));
+        int x = (255 - lane_lo) | lane_hi << 16;
+        auto join = [&](int y) { x = __builtin_bit_cast(int, __builtin_elementwise_max(__builtin_bit_cast(us2_t, x), __builtin_bit_cast(us2_t, y))); };
+        join(__builtin_amdgcn_update_dpp(0, x, 0x111, 0xF, 0xF, false));
+        join(__builtin_amdgcn_update_dpp(0, x, 0x112, 0xF, 0xF, false));
+        join(__builtin_amdgcn_update_dpp(0, x, 0x114, 0xF, 0xF, false));
+        join(__builtin_amdgcn_update_dpp(0, x, 0x118, 0xF, 0xF, false));
+        join(__builtin_amdgcn_update_dpp(0, x, kDppBcast15, 0xA, 0xF, false));
+        join(__builtin_amdgcn_update_dpp(0, x, kDppBcast31, 0xC, 0xF, false));
+        const int all = __builtin_amdgcn_readlane(x, 63), lo = 255 - (all & 0xFFFF), hi = all >> 16;
+        if (lo > hi) return;  // (zeros)
+        const bool high = hi > 127 + 60 || (wide && unit < 0);
+        wide = wide || lo < 1 + BIAS || hi - lo > 8 || hi < 127 - 40 || hi > 127 + 24;
+        if (!wide) {
+            put(hi);
+            return;
+        }
+        from = 0u, last = high || BIAS ? 0x7FFFu : ((127 + 61) << SHIFT) - 1;
+        unit = high ? -8 : 40;
+    }
+};
+// what sums in units of 2^unit are multiplied with at the end, so that all parts of a row are in the same one (2^-8: a sum of values at the end of bf16 has room)
+__device__ __forceinline__ float kv4_plain(int unit) { return __builtin_amdgcn_ldexpf(1.f, -8 - unit); }
 template <typename T> __device__ __forceinline__ float kv4_half(uint32_t w, int hi) {  // one of two packed values of T
     const uint16_t b = (uint16_t)(hi ? w >> 16 : w & 0xFFFFu);
     const T v = __builtin_bit_cast(T, b);

@@ -251,14 +251,57 @@ template <typename T, int D, int NG, int FOLD, int NW> __global__ __launch_bound
             for (int m = 0; m < KS; m++) qf[m] = col % COLS >= R ? U4{0u, 0u, 0u, 0u} : kv4_queries(x[m], exponent);
             score = Kv4Score::of<T>(a.scale, exponent);
         }
+        Kv4Band<T, 12> band;
+        int unit_of_sums = band.unit;
         f4_t acc[D / 16];
 #pragma unroll
         for (int c = 0; c < D / 16; c++) acc[c] = f4_t{0.f, 0.f, 0.f, 0.f};
         float M = -INFINITY, l = 0.f;
 
-        auto process = [&](Tile &t, int key0) __attribute__((always_inline)) {
+        // Tiles up to the first whose scales do not fit fp16; that one, and what follows, in a loop of its own: with both ways in one, the sums were copied from where one leaves them
+        // to where the other expects them, and a way out of the middle of a tile took 25 registers more than that tile with all its keys hidden does.
+        int fitting = nt;
+        auto room_of = [&](const Tile &t, int key0, int limit, int s) __attribute__((always_inline)) {
+            const int there = FOLD == 4 && fold >= 2 ? t.there[SUBS / 2 - 1] : t.there[0];
+            return (there ? limit : 0) - key0 - 16 * (FOLD == 1 ? s : fold) - 4 * j;
+        };
+        auto value_scale = [&](const Tile &t, int room, int s, int e, int g) __attribute__((always_inline)) {
+            uint32_t w = t.vs[s][(e * NG + g) / 2];
+            if (NG == 4 && FOLD == 1) asm("" : "+v"(w));  // (made again where they are needed: 32 of them kept from the first look at them on took the registers of other things)
+            return e < room ? kv4_half<T>(w, (e * NG + g) & 1) : 0.f;
+        };
+        auto check = [&](Tile &t, int turn, auto in_parts) __attribute__((always_inline)) {
+            constexpr bool WIDE = decltype(in_parts)::value;
+            const int key0 = tile_at(turn);
+            int limit = bound;
+            // ---- the scales of the values that the row sees
+            {
+                uint32_t off = 0;
+#pragma unroll
+                for (int s = 0; s < OWN; s++)
+#pragma unroll
+                    for (int n = 0; n < 4 * NG; n++) off = max(off, n / NG < room_of(t, key0, limit, s) ? band.off(band.bits(t.vs[s][n / 2], n & 1)) : 0u);
+                if (__builtin_expect(__builtin_amdgcn_ballot_w64(off > band.last) != 0, 0)) {
+                    int lo = 255, hi = 0;
+#pragma unroll
+                    for (int s = 0; s < OWN; s++)
+#pragma unroll
+                        for (int n = 0; n < 4 * NG; n++) band.among(value_scale(t, room_of(t, key0, limit, s), s, n / NG, n % NG), lo, hi);
+                    band.settle(lo, hi);
+                    if (!WIDE && band.wide) limit = 0, fitting = turn;
+                }
+            }
+            return limit;
+        };
+        auto process = [&](Tile &t, int turn, int limit, auto in_parts) __attribute__((always_inline)) {
+            constexpr bool WIDE = decltype(in_parts)::value;
+            const int key0 = tile_at(turn);
             // ---- scores: lane = row, keys 16 s + 4 j + e of its own 16s
-            float x[OWN][NG][4];
+            float x[NG][4], sv[OWN][4];
+            auto scaled = [&](const float *y, int s, int g, int e) __attribute__((always_inline)) {
+                const float f = kv4_half<T>(t.ks[s][(e * NG + g) / 2], (e * NG + g) & 1);
+                sv[s][e] = g == 0 ? y[e] * f : fmaf(y[e], f, sv[s][e]);
+            };
 #pragma unroll
             for (int s = 0; s < SUBS; s++) {
                 uint32_t d[KS];
@@ -279,48 +322,48 @@ template <typename T, int D, int NG, int FOLD, int NW> __global__ __launch_bound
                     for (int m = 0; m < MPG; m++) y = mfma16(keys(d[g * MPG + m]), qf[g * MPG + m], y);
 #pragma unroll
                     for (int e = 0; e < 4; e++) {
-                        if constexpr (FOLD == 1) x[s][g][e] = y[e];
-                        else x[0][g][e] = s == 0 || fold == s ? y[e] : x[0][g][e];
+                        x[g][e] = FOLD == 1 || s == 0 || fold == s ? y[e] : x[g][e];
+                        if (FOLD == 1) scaled(x[g], s, g, e);
                     }
                 }
                 __builtin_amdgcn_sched_barrier(0);  // (operands made for all 16s of keys ahead of their products, and for all columns below, take more registers than there are)
             }
             // keys that the row does not see have no weight, and what lies in their scales does not count.  (Tiles that every row sees in full go the same way: a
             // path of their own would save 3 selections a score, 12 of 480 operations in a tile of 64 keys, and holds half as much code again.)
-            float sv[OWN][4], vs[OWN][NG][4], top = -INFINITY;
-            const float far = !std::is_same<T, f16_t>::value ? score.far_by() : 1.f;
+            float top = -INFINITY;
 #pragma unroll
             for (int s = 0; s < OWN; s++) {
-                const int there = FOLD == 4 && fold >= 2 ? t.there[SUBS / 2 - 1] : t.there[0];
-                const int room = (there ? bound : 0) - key0 - 16 * (FOLD == 1 ? s : fold) - 4 * j;
+                const int room = room_of(t, key0, limit, s);
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
-                    float y = 0.f;
-                    uint32_t bits = 0;
 #pragma unroll
-                    for (int g = 0; g < NG; g++) {
-                        const int n = e * NG + g;
-                        const float f = kv4_half<T>(t.ks[s][n / 2], n & 1);
-                        y = g == 0 ? x[s][g][e] * f : fmaf(x[s][g][e], f, y);
-                        vs[s][g][e] = e < room ? kv4_half<T>(t.vs[s][n / 2], n & 1) : 0.f;
-                        bits = max(bits, kv4_bits<T>(t.vs[s][n / 2], n & 1));
-                    }
-                    sv[s][e] = e < room ? y * score.by * far : -INFINITY;
-                    top = fmaxf(top, fmaf((float)bits, kKv4Step<T>, sv[s][e]));
+                    for (int g = 0; g < NG; g++)
+                        if (FOLD > 1) scaled(x[g], s, g, e);
+                    sv[s][e] = e < room ? sv[s][e] * score.by : -INFINITY;
+                    top = fmaxf(top, sv[s][e]);
                 }
+            }
+            if (!std::is_same<T, f16_t>::value && __builtin_expect(score.far != 0, 0)) {
+                const float f = score.far_by();
+                top *= f;
+#pragma unroll
+                for (int s = 0; s < OWN; s++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) sv[s][e] *= f;
             }
             top = xor32_max(xor16_max(top));
             if constexpr (FOLD >= 2) top = fmaxf(top, dpp_get<kDppRor8>(top));
             if constexpr (FOLD == 4) top = fmaxf(top, dpp_get<kDppRor4>(top));
-            const float Mn = fmaxf(M, top), ref = Mn == -INFINITY ? 0.f : Mn - kKv4Zero<T>;
-            const float alpha = Mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(M - Mn);
+            const float Mn = fmaxf(M, top), ref = Mn == -INFINITY ? 0.f : Mn, unit = (float)band.unit;
+            const float alpha = Mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(M - Mn + (float)(band.unit - unit_of_sums));
             M = Mn;
+            unit_of_sums = band.unit;
             float ps = 0.f;
 #pragma unroll
             for (int s = 0; s < OWN; s++)
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
-                    sv[s][e] = __builtin_amdgcn_exp2f(sv[s][e] - ref);
+                    sv[s][e] = __builtin_amdgcn_exp2f(sv[s][e] - ref + unit);  // (in this order: a score may be so large that the unit is nothing to it)
                     ps += sv[s][e];
                 }
             l = fmaf(l, alpha, ps);
@@ -332,79 +375,94 @@ template <typename T, int D, int NG, int FOLD, int NW> __global__ __launch_bound
             // ---- O^T += V^T . P
             const int i = lane & 15, n = i & 7, key = 4 * j + ((n & 1) << 1) + (n >> 2) + ((n & 2) << 3);
             const char *from = mine + key * VROW + (i >> 3) * 8;
+            // a part of the weights of OWN 16s of keys as the operand: of FOLD columns that are one row, each has keys of its own
+            auto operand = [&](const uint32_t (*w)[2], U4 *p) __attribute__((always_inline)) {
+                const uint32_t *w0 = w[0];
+                if constexpr (FOLD == 1) p[0] = U4{w0[0], w0[1], w[OWN - 1][0], w[OWN - 1][1]};
+                else if constexpr (FOLD == 2) p[0] = U4{w0[0], w0[1], dpp_word<kDppRor8>(w0[0]), dpp_word<kDppRor8>(w0[1])};
+                else {
+                    // (columns 0 .. 3 are the ones whose results count: they take the weights of the folds behind them, 4, 8 and 12 lanes up)
+                    p[0] = U4{w0[0], w0[1], dpp_word<kDppRor12>(w0[0]), dpp_word<kDppRor12>(w0[1])};
+                    p[SUBS / 2 - 1] = U4{dpp_word<kDppRor8>(w0[0]), dpp_word<kDppRor8>(w0[1]), dpp_word<kDppRor4>(w0[0]), dpp_word<kDppRor4>(w0[1])};
+                }
+            };
 #pragma unroll
             for (int g = 0; g < NG; g++) {
-                U4 p[SUBS / 2][2];  // of 32 keys: rounded, and the rest
-                {
-                    uint32_t w[OWN][2][2];
+                float y[OWN][4];
 #pragma unroll
-                    for (int s = 0; s < OWN; s++) {
-                        float y[4];
+                for (int s = 0; s < OWN; s++)
 #pragma unroll
-                        for (int e = 0; e < 4; e++) y[e] = sv[s][e] * vs[s][g][e];
+                    for (int e = 0; e < 4; e++) y[s][e] = sv[s][e] * value_scale(t, room_of(t, key0, limit, s), s, e, g);
+                // fp16: rounded, and the rest, side by side.  bf16: one part after the other.
+                constexpr int PARTS = WIDE ? 1 : 2, TURNS = WIDE ? kParts<bf16_t> : 1;
+#pragma unroll 1
+                for (int part0 = 0; part0 < TURNS; part0++) {
+                    U4 p[PARTS][SUBS / 2];
+                    {
+                        uint32_t w[PARTS][OWN][2];
 #pragma unroll
-                        for (int part = 0; part < 2; part++) {
-                            w[s][part][0] = kv4_take(y[0], y[1], minus);
-                            w[s][part][1] = kv4_take(y[2], y[3], minus);
-                        }
+                        for (int s = 0; s < OWN; s++)
+#pragma unroll
+                            for (int part = 0; part < PARTS; part++)
+#pragma unroll
+                                for (int e = 0; e < 2; e++) w[part][s][e] = WIDE ? take_part<bf16_t>(y[s][2 * e], y[s][2 * e + 1]) : kv4_take(y[s][2 * e], y[s][2 * e + 1], minus);
+#pragma unroll
+                        for (int part = 0; part < PARTS; part++) operand(w[part], p[part]);
                     }
 #pragma unroll
-                    for (int part = 0; part < 2; part++) {
-                        const uint32_t *w0 = w[0][part];
-                        if constexpr (FOLD == 1) p[0][part] = U4{w0[0], w0[1], w[OWN - 1][part][0], w[OWN - 1][part][1]};
-                        else if constexpr (FOLD == 2) p[0][part] = U4{w0[0], w0[1], dpp_word<kDppRor8>(w0[0]), dpp_word<kDppRor8>(w0[1])};
-                        else {
-                            // (columns 0 .. 3 are the ones whose results count: they take the weights of the folds behind them, 4, 8 and 12 lanes up)
-                            p[0][part] = U4{w0[0], w0[1], dpp_word<kDppRor12>(w0[0]), dpp_word<kDppRor12>(w0[1])};
-                            p[SUBS / 2 - 1][part] = U4{dpp_word<kDppRor8>(w0[0]), dpp_word<kDppRor8>(w0[1]), dpp_word<kDppRor4>(w0[0]), dpp_word<kDppRor4>(w0[1])};
+                    for (int sp = 0; sp < SUBS / 2; sp++) {
+                        h2_t off[4];
+#pragma unroll
+                        for (int s = 0; s < 2; s++) {
+                            // zero points of keys (4 j, 4 j + 1) and (4 j + 2, 4 j + 3): bytes NG e + g
+                            const uint32_t *z = t.vz[2 * sp + s];
+                            uint32_t z01, z23;
+                            if constexpr (NG == 1) {
+                                z01 = __builtin_amdgcn_perm(0u, z[0], 0x0C010C00u);
+                                z23 = __builtin_amdgcn_perm(0u, z[0], 0x0C030C02u);
+                            } else if constexpr (NG == 2) {
+                                z01 = z[0] >> (8 * g);
+                                z23 = z[1] >> (8 * g);
+                            } else {
+                                const uint32_t sel = 0x0C040C00u + 0x00010001u * g;
+                                z01 = __builtin_amdgcn_perm(z[1], z[0], sel);
+                                z23 = __builtin_amdgcn_perm(z[NG - 1], z[NG - 2], sel);
+                            }
+                            off[2 * s] = kv4_low(z01);
+                            off[2 * s + 1] = kv4_high(z23);
                         }
-                    }
-                }
 #pragma unroll
-                for (int sp = 0; sp < SUBS / 2; sp++) {
-                    h2_t off[4];
+                        for (int c2 = g * MPG; c2 < (g + 1) * MPG; c2++) {
+                            typedef int i2_t __attribute__((ext_vector_type(2)));
+                            const i2_t w = __builtin_amdgcn_ds_read_tr4_b64_v2i32((__attribute__((address_space(3))) i2_t *)(from + 32 * sp * VROW + 16 * c2));
 #pragma unroll
-                    for (int s = 0; s < 2; s++) {
-                        // zero points of keys (4 j, 4 j + 1) and (4 j + 2, 4 j + 3): bytes NG e + g
-                        const uint32_t *z = t.vz[2 * sp + s];
-                        uint32_t z01, z23;
-                        if constexpr (NG == 1) {
-                            z01 = __builtin_amdgcn_perm(0u, z[0], 0x0C010C00u);
-                            z23 = __builtin_amdgcn_perm(0u, z[0], 0x0C030C02u);
-                        } else if constexpr (NG == 2) {
-                            z01 = z[0] >> (8 * g);
-                            z23 = z[1] >> (8 * g);
-                        } else {
-                            const uint32_t sel = 0x0C040C00u + 0x00010001u * g;
-                            z01 = __builtin_amdgcn_perm(z[1], z[0], sel);
-                            z23 = __builtin_amdgcn_perm(z[NG - 1], z[NG - 2], sel);
+                            for (int y = 0; y < 2; y++) {
+                                const U4 codes = kv4_pairs((uint32_t)w[y], off, pairs.nibbles0, pairs.nibbles1);
+#pragma unroll
+                                for (int part = 0; part < PARTS; part++)
+                                    acc[2 * c2 + y] = WIDE ? mfma16_bf16(kv4_as_bf16(codes), p[part][sp], acc[2 * c2 + y]) : mfma16(codes, p[part][sp], acc[2 * c2 + y]);
+                            }
                         }
-                        off[2 * s] = kv4_low(z01);
-                        off[2 * s + 1] = kv4_high(z23);
+                        __builtin_amdgcn_sched_barrier(0);
                     }
-#pragma unroll
-                    for (int c2 = g * MPG; c2 < (g + 1) * MPG; c2++) {
-                        typedef int i2_t __attribute__((ext_vector_type(2)));
-                        const i2_t w = __builtin_amdgcn_ds_read_tr4_b64_v2i32((__attribute__((address_space(3))) i2_t *)(from + 32 * sp * VROW + 16 * c2));
-#pragma unroll
-                        for (int y = 0; y < 2; y++) {
-                            const U4 codes = kv4_pairs((uint32_t)w[y], off, pairs.nibbles0, pairs.nibbles1);
-                            acc[2 * c2 + y] = mfma16(codes, p[sp][0], acc[2 * c2 + y]);
-                            acc[2 * c2 + y] = mfma16(codes, p[sp][1], acc[2 * c2 + y]);
-                        }
-                    }
-                    __builtin_amdgcn_sched_barrier(0);
                 }
             }
         };
-        for (int n = 0; n < nt; n++) {
+        for (int n = 0; n < fitting; n++) {
             // (the next tile's loads have all of this one's work to arrive.  Two sets that take turns, without the copies, left the registers of the sums no
             // place to stay: up to 256 of them and scratch memory for 156 that are alive)
             load(tb, tile_at(n + 1));
             park_values();
             load_values(tb);
-            process(ta, tile_at(n));
+            process(ta, n, check(ta, n, std::false_type{}), std::false_type{});
             ta = tb;
+        }
+        for (int n = fitting; n < nt; n++) {  // (rare: from memory again, a tile at a time)
+            look_up(tile_at(n) >> psh);
+            load(ta, tile_at(n));
+            load_values(ta);
+            park_values();
+            process(ta, n, check(ta, n, std::true_type{}), std::true_type{});
         }
         // ---- the next (sequence, kv head)'s loads before this one's results are put together
         const int done_b = b, done_h = h, done_fresh = seq.fresh, u0 = unit - at, units = n_units, end = min(n_units, at + stop - unit);
@@ -427,13 +485,15 @@ template <typename T, int D, int NG, int FOLD, int NW> __global__ __launch_bound
         l = xor32_sum(xor16_sum(l));
         if constexpr (FOLD >= 2) l += dpp_get<kDppRor8>(l);
         if constexpr (FOLD == 4) l += dpp_get<kDppRor4>(l);
+        const float plain = kv4_plain(unit_of_sums);
+        l *= plain;
         if (me < 16) {
             m_s[wave * 16 + me] = M;
             l_s[wave * 16 + me] = l;
         }
         if ((me & 15) < R) {
 #pragma unroll
-            for (int c = 0; c < D / 16; c++) *(f4_t *)(o_s(wave) + (me & 15) * D + 16 * c + 4 * (me >> 4)) = acc[c];
+            for (int c = 0; c < D / 16; c++) *(f4_t *)(o_s(wave) + (me & 15) * D + 16 * c + 4 * (me >> 4)) = acc[c] * plain;
         }
         __syncthreads();
         const size_t slot = 2 * (size_t)blockIdx.x + second;

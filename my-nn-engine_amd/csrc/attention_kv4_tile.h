@@ -4,8 +4,8 @@
 // A workgroup of QW x KW waves has QW blocks of rows and walks their keys in tiles of KEYS, a KW-th of each tile a wave.  Codes travel global -> registers (a tile ahead)
 // -> (code - zero) in fp16 -> LDS, once for all rows of the workgroup: two stages, one barrier a tile (tiles of 128 keys: one stage, two barriers).
 //   S^T = K . Q^T      per group of columns; a key's scale meets the group's sum
-//   softmax            a lane has ONE row and half of the keys of each 32; the reference with the value scales in it (attention_kv4.h)
-//   O^T += V^T . P^T   p * vs as two fp16 numbers; P stays in registers (the D layout of S^T is the B layout of P^T with the keys in the order 4g+0..3, 8+4g+0..3), V^T
+//   softmax            a lane has ONE row and half of the keys of each 32
+//   O^T += V^T . P^T   p * vs as two fp16 numbers, or three of bf16 (attention_kv4.h); P stays in registers (the D layout of S^T is the B layout of P^T with the keys in the order 4g+0..3, 8+4g+0..3), V^T
 //                      comes from the row-major tile by transposing reads
 // Vector operations and matrix instructions bound it together (busy 65 and 31 % of the time at 4 x 2048 rows): 350 of the one for 32 of the other in a wave's 64 keys of 32 rows,
 // 100 of them the staging's.  4 prompts of 2048 rows, 32 / 8 heads of 128, groups of 128, bf16: 197 us in a program's calls, 0.70 PFLOP/s (the products alone, at what a large
@@ -21,7 +21,7 @@ namespace mynn {
 template <int D, int NG, int QW, int KW, int KEYS> struct Kv4Block {
     static constexpr int ROWB = D * 2, TILEB = KEYS * ROWB, THREADS = QW * KW * 64, ROWS = QW * 32, NH = KEYS / 32 / KW;
     static constexpr int UNITS = KEYS * 4 / THREADS;  // a thread stages a quarter of a row, of K and of V
-    static constexpr int SCALES = (2 * NG + 1) * KEYS * 4, FLAGS = KEYS / 16 * 4;
+    static constexpr int SCALES = 2 * NG * KEYS * 4, FLAGS = KEYS / 16 * 4;
     static constexpr int STAGE = 2 * TILEB + SCALES + FLAGS;
     static constexpr int WORDS = D / 2 + 2;  // of a lane's result: reference, sum, O^T
     static constexpr int MERGE = KW > 1 ? QW * KW * 64 * WORDS * 4 : 0;
@@ -51,7 +51,7 @@ __device__ __forceinline__ int kv4_ranges(int tiles, int length, int most) { ret
 template <typename T, int D, int NG, int QW, int KW, int KEYS> __global__ __launch_bounds__(QW *KW * 64, 2) void attn_kv4_tile_kernel(Kv4Args a) {
     using B = Kv4Block<D, NG, QW, KW, KEYS>;
     constexpr int KS = D / 16, DT = D / 32, NH = B::NH, DW = D / 32, ROWB = B::ROWB, KPG = KS / NG, TPG = DT / NG;
-    // p * vs for the second product: two numbers of 11 bits.  (One is off by as much as results in fp16 are rounded.  Results in bf16 hide most of that, and 4 x 2048 rows took
+    // p * vs for the second product in fp16: two numbers of 11 bits.  (One is off by as much as results in fp16 are rounded.  Results in bf16 hide most of that, and 4 x 2048 rows took
     // 196 us for 225; but those of many rows then differed by 10^-3 from what few rows, 22 bits all, and 32-bit operations give, 6 10^-5 with two.)
     constexpr int PARTS = 2;
     extern __shared__ __align__(16) char sm[];
@@ -138,9 +138,10 @@ template <typename T, int D, int NG, int QW, int KW, int KEYS> __global__ __laun
     const float minus = kv4_minus();
     Int4Pairs pairs;
     Kv4Keys keys;
-    auto store = [&](char *stage) __attribute__((always_inline)) {
-        float *scales = (float *)(stage + 2 * B::TILEB), *lift = scales + 2 * NG * KEYS;
-        int *there = (int *)(lift + KEYS);
+    Kv4Band<T, 8> band;  // (the same in all waves: each settles it from what lies in LDS)
+    auto store = [&](char *stage, int key0) __attribute__((always_inline)) {
+        float *scales = (float *)(stage + 2 * B::TILEB);
+        int *there = (int *)(scales + 2 * NG * KEYS);
 #pragma unroll
         for (int u = 0; u < B::UNITS; u++) {
             const int r = u * QUARTERS + (tid >> 2);
@@ -154,13 +155,13 @@ template <typename T, int D, int NG, int QW, int KW, int KEYS> __global__ __laun
                 char *to = stage + (v ? B::TILEB : 0) + r * ROWB;
 #pragma unroll
                 for (int i = 0; i < DW; i++) *(U4 *)(to + (((quarter * DW + i) ^ swz) << 4)) = v ? pairs(x.codes[i]) : keys(x.codes[i]);
-                if (quarter % (4 / NG) == 0) scales[(v ? NG * KEYS : 0) + sg * KEYS + r] = Elem<T>::ld(&x.scale, 0);
-                if (v) {
-                    const float bits = group_max<4>((float)kv4_bits<T>(__builtin_bit_cast(uint16_t, x.scale), 0));
-                    if (quarter == 0) lift[r] = bits * kKv4Step<T>;
-                }
+                // (values that no row sees have the scale 0)
+                const bool seen = !v || (raw_there[u] && key0 + r < seq.len);
+                if (quarter % (4 / NG) == 0) scales[(v ? NG * KEYS : 0) + sg * KEYS + r] = seen ? Elem<T>::ld(&x.scale, 0) : 0.f;
             }
-            if (lane == 0) there[r >> 4] = raw_there[u];
+            const bool seen = raw_there[u] && key0 + r < seq.len;
+            const uint64_t off = __builtin_amdgcn_ballot_w64(seen && band.off(band.bits(__builtin_bit_cast(uint16_t, raw[u][1].scale), 0)) > band.last);
+            if (lane == 0) there[r >> 4] = raw_there[u] | (off != 0 ? 2 : 0);
         }
     };
     if (t0 < t1) load(t0);
@@ -180,12 +181,16 @@ template <typename T, int D, int NG, int QW, int KW, int KEYS> __global__ __laun
             for (int e = 0; e < 8; e++) peak = fmaxf(peak, fabsf(f[e]));
         }
         const int exponent = kv4_query_exponent(xor32_max(peak));
+        // (a scale below zero turns the queries around: that of the scores is not, and their largest is that of the sums)
+        const float sign = a.scale < 0.f ? -1.f : 1.f;
 #pragma unroll
         for (int ks = 0; ks < KS; ks++) {
             widen8<T>(x[ks], f);
+#pragma unroll
+            for (int e = 0; e < 8; e++) f[e] *= sign;
             qf[ks] = kv4_queries(f, exponent);
         }
-        score = Kv4Score::of<T>(a.scale, exponent);
+        score = Kv4Score::of<T>(fabsf(a.scale), exponent);
     }
     f16x_t o[DT];
 #pragma unroll
@@ -193,6 +198,7 @@ template <typename T, int D, int NG, int QW, int KW, int KEYS> __global__ __laun
 #pragma unroll
         for (int e = 0; e < 16; e++) o[t][e] = 0.f;
     float M = -INFINITY, l = 0.f;
+    int unit_of_sums = band.unit;
     const int krow = col * ROWB + ((g ^ k_swz(col)) << 4);
     int vrow[DT];
     {
@@ -201,17 +207,18 @@ template <typename T, int D, int NG, int QW, int KW, int KEYS> __global__ __laun
         for (int t2 = 0; t2 < DT; t2++) vrow[t2] = r * ROWB + (((4 * t2 + 2 * ((lane >> 4) & 1) + ((i & 3) >> 1)) ^ v_swz(r)) << 4) + 8 * (i & 1);
     }
 
-    auto tile = [&](const char *stage, int key0, auto masked) __attribute__((always_inline)) {
-        constexpr bool MASKED = decltype(masked)::value;
+    auto tile = [&](const char *stage, int key0, auto masked, auto in_parts) __attribute__((always_inline)) {
+        constexpr bool MASKED = decltype(masked)::value, WIDE = decltype(in_parts)::value;
         const int off = kg * 32 * NH;  // this wave's keys of the tile
         const char *kt = stage + off * ROWB, *vt = kt + B::TILEB;
-        const float *ksc = (const float *)(stage + 2 * B::TILEB) + off, *vsc = ksc + NG * KEYS, *lift = vsc + NG * KEYS;
-        const int *there = (const int *)(lift + KEYS - off + off / 16);
+        const float *ksc = (const float *)(stage + 2 * B::TILEB) + off, *vsc = ksc + NG * KEYS;
+        const int *there = (const int *)(vsc + NG * KEYS - off) + off / 16;
         f16x_t s[NH];
 #pragma unroll
         for (int gr = 0; gr < NG; gr++)
 #pragma unroll
             for (int hf = 0; hf < NH; hf++) {
+                if (NG > 1 && (hf == 0 || NG == 4)) __builtin_amdgcn_sched_barrier(0);  // (operands read ahead for several groups take more registers than there are)
                 f16x_t x;
 #pragma unroll
                 for (int e = 0; e < 16; e++) x[e] = 0.f;
@@ -239,7 +246,7 @@ template <typename T, int D, int NG, int QW, int KW, int KEYS> __global__ __laun
             if (MASKED) {
                 seen[hf] = 0;
                 const int room = bound - key0 - 32 * hf - 4 * g;
-                const uint32_t pages = (there[2 * hf] ? 0xFFu : 0u) | (there[2 * hf + 1] ? 0xFF00u : 0u);
+                const uint32_t pages = (there[2 * hf] & 1 ? 0xFFu : 0u) | (there[2 * hf + 1] & 1 ? 0xFF00u : 0u);
 #pragma unroll
                 for (int e = 0; e < 16; e++) seen[hf] |= (uint32_t)(8 * (e >> 2) + (e & 3) < room) << e;
                 seen[hf] &= pages;
@@ -247,33 +254,40 @@ template <typename T, int D, int NG, int QW, int KW, int KEYS> __global__ __laun
                 for (int e = 0; e < 16; e++) s[hf][e] = seen[hf] >> e & 1 ? s[hf][e] : -INFINITY;
             }
 #pragma unroll
-            for (int e4 = 0; e4 < 4; e4++) {
-                const f4_t f = *(const f4_t *)&lift[32 * hf + 8 * e4 + 4 * g];
-#pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    const float t = fmaf(s[hf][4 * e4 + e], score.by, f[e]);
-                    top = fmaxf(top, MASKED ? (seen[hf] >> (4 * e4 + e) & 1 ? t : -INFINITY) : t);
-                }
-            }
+            for (int e = 0; e < 16; e++) top = fmaxf(top, s[hf][e]);
         }
         top = xor32_max(top);
+        top = top == -INFINITY ? top : top * score.by;
         const bool up = top > M + kKv4Lag;
-        if (__builtin_amdgcn_ballot_w64(up) != 0) {
-            const float mn = up ? top : M, corr = up ? __builtin_amdgcn_exp2f(M - mn) : 1.f;
+        if (__builtin_amdgcn_ballot_w64(up) != 0 || band.unit != unit_of_sums) {
+            const float mn = up ? top : M, corr = __builtin_amdgcn_exp2f((up ? M - mn : 0.f) + (float)(band.unit - unit_of_sums));
             M = mn;
+            unit_of_sums = band.unit;
             l *= corr;
 #pragma unroll
             for (int t2 = 0; t2 < DT; t2++)
 #pragma unroll
                 for (int e = 0; e < 16; e++) o[t2][e] *= corr;
         }
-        const float ref = M == -INFINITY ? 0.f : M - (kKv4Zero<T> - kKv4Lag);
+        float by = score.by, ref = M == -INFINITY ? 0.f : M - (float)band.unit;
+        if (__builtin_expect(__builtin_amdgcn_ballot_w64(fabsf(ref) > 0x1p20f) != 0, 0)) {
+            // scores so large that what M's rounding took off it, or the unit next to it, is no small thing (the fused step below has the scores' products whole)
+            const float m = M == -INFINITY ? 0.f : M;
+#pragma unroll
+            for (int hf = 0; hf < NH; hf++)
+#pragma unroll
+                for (int e = 0; e < 16; e++) {
+                    const float x = s[hf][e] * by;
+                    s[hf][e] = x - m;
+                }
+            by = 1.f, ref = -(float)band.unit;
+        }
         float lt = 0.f;
 #pragma unroll
         for (int hf = 0; hf < NH; hf++)
 #pragma unroll
             for (int e = 0; e < 16; e++) {
-                const float p = __builtin_amdgcn_exp2f(fmaf(s[hf][e], score.by, -ref));
+                const float p = __builtin_amdgcn_exp2f(fmaf(s[hf][e], by, -ref));
                 s[hf][e] = MASKED ? (seen[hf] >> e & 1 ? p : 0.f) : p;
                 lt += s[hf][e];
             }
@@ -293,16 +307,30 @@ template <typename T, int D, int NG, int QW, int KW, int KEYS> __global__ __laun
                         p[4 * e4 + e] = MASKED ? (seen[st >> 1] >> (e0 + 4 * e4 + e) & 1 ? x * f[e] : 0.f) : x * f[e];
                     }
                 }
-                U4 pf[PARTS];
-#pragma unroll
-                for (int part = 0; part < PARTS; part++)
-                    pf[part] = U4{kv4_take(p[0], p[1], minus), kv4_take(p[2], p[3], minus), kv4_take(p[4], p[5], minus), kv4_take(p[6], p[7], minus)};
-#pragma unroll
-                for (int t2 = gr * TPG; t2 < (gr + 1) * TPG; t2++) {
+                auto product = [&](int t2, auto &&take) __attribute__((always_inline)) {
                     const char *vr = vt + vrow[t2] + 16 * st * ROWB;
                     const uint2 lo = lds_read_tr16(vr), hi = lds_read_tr16(vr + 8 * ROWB);
+                    take(U4{lo.x, lo.y, hi.x, hi.y});
+                };
+                if constexpr (WIDE) {
+#pragma unroll 1
+                    for (int part = 0; part < kParts<bf16_t>; part++) {
+                        const U4 pf = {take_part<bf16_t>(p[0], p[1]), take_part<bf16_t>(p[2], p[3]), take_part<bf16_t>(p[4], p[5]), take_part<bf16_t>(p[6], p[7])};
 #pragma unroll
-                    for (int part = 0; part < PARTS; part++) o[t2] = Mfma<f16_t>::run(U4{lo.x, lo.y, hi.x, hi.y}, pf[part], o[t2]);
+                        for (int t2 = gr * TPG; t2 < (gr + 1) * TPG; t2++)
+                            product(t2, [&](const U4 &codes) __attribute__((always_inline)) { o[t2] = Mfma<bf16_t>::run(kv4_as_bf16(codes), pf, o[t2]); });
+                    }
+                } else {
+                    U4 pf[PARTS];
+#pragma unroll
+                    for (int part = 0; part < PARTS; part++)
+                        pf[part] = U4{kv4_take(p[0], p[1], minus), kv4_take(p[2], p[3], minus), kv4_take(p[4], p[5], minus), kv4_take(p[6], p[7], minus)};
+#pragma unroll
+                    for (int t2 = gr * TPG; t2 < (gr + 1) * TPG; t2++)
+                        product(t2, [&](const U4 &codes) __attribute__((always_inline)) {
+#pragma unroll
+                            for (int part = 0; part < PARTS; part++) o[t2] = Mfma<f16_t>::run(codes, pf[part], o[t2]);
+                        });
                 }
             }
     };
@@ -311,24 +339,54 @@ template <typename T, int D, int NG, int QW, int KW, int KEYS> __global__ __laun
     auto next = [&]() __attribute__((always_inline)) {
         char *here = sm + stage * B::STAGE;
         if (B::STAGES == 1 && t > t0) __syncthreads();
-        store(here);  // (tile t - 2, which lay here, is behind the last barrier for every wave)
+        store(here, t * KEYS);  // (tile t - 2, which lay here, is behind the last barrier for every wave)
         if (t + 1 < t1) load(t + 1);
         __syncthreads();
+        // scales that the band does not let through, in any of the tile's rows
+        const float *vsc = (const float *)(here + 2 * B::TILEB) + NG * KEYS;
+        int any = 0;
+#pragma unroll
+        for (int i = 0; i < KEYS / 16; i++) any |= ((const int *)(vsc + NG * KEYS))[i];
+        if (__builtin_expect(__builtin_amdgcn_readfirstlane(any) & 2, 0)) {
+            int lo = 255, hi = 0;
+#pragma unroll
+            for (int i = 0; i < NG * KEYS / 64; i++) band.among(vsc[64 * i + lane], lo, hi);
+            band.settle(lo, hi);
+        }
         if (B::STAGES == 2) stage ^= 1;
         return here;
     };
-    // the tiles that all rows of the workgroup see in full, then those with hidden keys.  (Loops of their own: with both kinds of tile in one, the results were copied from
-    // where one leaves them to where the other expects them.)
+    // the tiles that all rows of the workgroup see in full, then those with hidden keys; and all from the first on whose scales do not fit fp16.  (Loops of their own: with two
+    // kinds of tile in one, the results were copied from where one leaves them to where the other expects them.)
     const int full = min(t1, seq.bound(row0 / G, a.causal) / KEYS);
-    for (; t < full && all_there; t++) tile(next(), 0, std::false_type{});
-    for (; t < t1; t++) {
-        const char *here = next();
-        const int key0 = t * KEYS + kg * 32 * NH;
-        if (key0 < wave_last) tile(here, key0, std::true_type{});
+    const char *here = nullptr;
+    auto key_of = [&](int n) { return n * KEYS + kg * 32 * NH; };
+    for (; t < full && all_there; t++) {
+        here = next();
+        if (band.wide) break;
+        tile(here, 0, std::false_type{}, std::false_type{});
+    }
+    for (; t < t1 && !band.wide; t++) {
+        here = next();
+        if (band.wide) break;
+        if (key_of(t) < wave_last) tile(here, key_of(t), std::true_type{}, std::false_type{});
+    }
+    while (t < t1) {
+        if (key_of(t) < wave_last) tile(here, key_of(t), std::true_type{}, std::true_type{});
+        if (++t < t1) here = next();
     }
 
     l = xor32_sum(l);
     if constexpr (KW > 1) {
+        if (unit_of_sums != band.unit) {  // (a wave whose rows do not see the last tiles)
+            const float f = __builtin_amdgcn_ldexpf(1.f, band.unit - unit_of_sums);
+            l *= f;
+#pragma unroll
+            for (int t2 = 0; t2 < DT; t2++)
+#pragma unroll
+                for (int e = 0; e < 16; e++) o[t2][e] *= f;
+            unit_of_sums = band.unit;
+        }
         // the waves that shared a block of rows: the first of them takes the others' results in
         __syncthreads();
         float *to = (float *)sm + (size_t)w * 64 * B::WORDS + lane;
@@ -359,7 +417,8 @@ template <typename T, int D, int NG, int QW, int KW, int KEYS> __global__ __laun
     }
     // (The lane's place once more, from the wave: what it is known by at the start would be one register too many over the loops.)
     const int place = __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0)), row_out = row0 + 32 * wave + (place & 31), gr = place >> 5;
-    const float inv = nz > 1 ? 1.f : row_out >= valid || l == 0.f ? 0.f : 1.0f / l;
+    const float plain = kv4_plain(unit_of_sums);
+    const float inv = nz > 1 ? plain : row_out >= valid || l == 0.f ? 0.f : 1.0f / l;
     const size_t line = (((size_t)b * a.c.Hkv + h) * R + row_out) * a.ranges + range;
 #pragma unroll
     for (int t2 = 0; t2 < DT; t2++)
@@ -371,11 +430,11 @@ template <typename T, int D, int NG, int QW, int KW, int KEYS> __global__ __laun
             permlane32_swap(x1, x3);
             const int d = 32 * t2 + 8 * e4 + 4 * gr;
             if (row_out >= R) continue;
-            if (nz > 1) *(f4_t *)(a.part_o + line * D + d) = f4_t{x0, x1, x2, x3};
+            if (nz > 1) *(f4_t *)(a.part_o + line * D + d) = f4_t{x0 * inv, x1 * inv, x2 * inv, x3 * inv};
             else if (row_out >= valid) *(uint2 *)(out_row(row_out) + d) = uint2{0u, 0u};
             else *(uint2 *)(out_row(row_out) + d) = uint2{pack2<T>(x0 * inv, x1 * inv), pack2<T>(x2 * inv, x3 * inv)};
         }
-    if (nz > 1 && gr == 0 && row_out < R) *(float2 *)(a.part_ml + line * 2) = float2{M, l};
+    if (nz > 1 && gr == 0 && row_out < R) *(float2 *)(a.part_ml + line * 2) = float2{M, l * plain};
 }
 
 // Joins the ranges of keys of each row.  Blocks with one range, or none of the sequence's own rows, are done already.

@@ -1,4 +1,5 @@
-"""Attention over paged caches of 4 bits whose keys and queries lie at opposite ends of bf16."""
+"""Attention over paged caches of 4 bits whose scales reach over their type: groups and rows of zeros (their scale is 1) beside small values, groups of a row far
+from each other, values that stand for no number, scales that change along a sequence, keys and queries at opposite ends of bf16."""
 import pytest
 import torch
 
@@ -98,6 +99,86 @@ SHAPES = [(64, 64), (64, 32), (128, 128), (128, 64), (128, 32)]
 
 
 @pytest.mark.parametrize("S,Hq", ROWS)
+@pytest.mark.parametrize("D,group", [s for s in SHAPES if s[1] < s[0]])
+@pytest.mark.parametrize("dtype,size", [(torch.float16, -10), (torch.bfloat16, -10), (torch.bfloat16, -24), (torch.bfloat16, -36), (torch.bfloat16, -60), (torch.bfloat16, -100)])
+def test_a_group_of_zeros_beside_small_values(mynn, dtype, size, D, group, S, Hq):
+    """columns of a head that are always zero: their groups' scale is 1, by the rule"""
+    v = normal(1, 2, 300 + S, 2, D) * 2.0 ** size
+    v[..., :group] = 0.0
+    pools, table = made(2, 2, D, 64, group, dtype, 300 + S, v, 2)
+    assert bool((pools[3][int(table[0, 0]), :, :, 0] == 1).all())
+    got = check(mynn, queries(2, Hq, S, D, dtype), pools, table, [300, 120], new=[S, S])
+    assert not got[..., :group].any()
+
+
+@pytest.mark.parametrize("S,Hq", ROWS)
+@pytest.mark.parametrize("D,group", SHAPES)
+@pytest.mark.parametrize("dtype,size", [(torch.float16, -10), (torch.bfloat16, -30), (torch.bfloat16, -70), (torch.bfloat16, -110)])
+def test_rows_of_zeros_beside_small_values(mynn, dtype, size, D, group, S, Hq):
+    """a token whose values are zero, at the front, in the middle of a tile and among the last"""
+    v = normal(3, 1, 300 + S, 2, D) * 2.0 ** size
+    v[:, [0, 77, 290]] = 0.0
+    pools, table = made(1, 2, D, 64, group, dtype, 300 + S, v, 4)
+    check(mynn, queries(1, Hq, S, D, dtype), pools, table, [300])
+
+
+@pytest.mark.parametrize("S,Hq", ROWS)
+@pytest.mark.parametrize("D,group", [s for s in SHAPES if s[1] < s[0]])
+@pytest.mark.parametrize("dtype,low,high", [(torch.float16, -8, 8), (torch.float16, -12, 13), (torch.bfloat16, 0, 28), (torch.bfloat16, 0, 36), (torch.bfloat16, -40, 40), (torch.bfloat16, -90, 110)])
+def test_groups_of_a_row_far_from_each_other(mynn, dtype, low, high, D, group, S, Hq):
+    v = normal(5, 2, 200 + S, 1, D)
+    if dtype == torch.float16:
+        v = v.clamp(-3.5, 3.5)
+    v[..., group:2 * group] *= 2.0 ** high
+    v[..., :group] *= 2.0 ** low
+    v[..., 2 * group:] *= 2.0 ** low
+    pools, table = made(2, 1, D, 32, group, dtype, 200 + S, v, 6)
+    check(mynn, queries(2, Hq, S, D, dtype), pools, table, [200, 33], new=[S, S])
+
+
+@pytest.mark.parametrize("S,Hq", ROWS)
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("D,group", SHAPES)
+@pytest.mark.parametrize("scale_of_it", [float("nan"), float("inf")])
+@pytest.mark.parametrize("longest", [150, 3000])
+def test_a_group_of_values_that_stands_for_no_number(mynn, dtype, D, group, S, Hq, scale_of_it, longest):
+    """only its own columns are none, and only for the rows that see it; 3000: sequences that several workgroups share"""
+    if longest > 150 and (group > 64 or scale_of_it != scale_of_it):
+        pytest.skip("one of them")
+    past = [longest, 40]
+    v = normal(7, 2, longest + S, 2, D) * 2.0 ** -9
+    pools, table = made(2, 2, D, 64, group, dtype, longest + S, v, 8)
+    at, g = longest + S // 2, D // group - 1
+    page, r = int(table[0, at // 64]), at % 64
+    pools[3][page, 1, r, g] = scale_of_it
+    pools[1][page, 1, r] = 0x5A
+    pools[5][page, 1, r] = 0  # (codes 5 and 10: an infinite scale stands for infinities)
+    bad = torch.zeros(2, Hq, S, D, dtype=torch.bool, device="cuda")
+    bad[0, Hq // 2:, S // 2:, g * group:] = True
+    check(mynn, queries(2, Hq, S, D, dtype), pools, table, past, new=[S, S], bad=bad)
+
+
+@pytest.mark.parametrize("S,Hq", ROWS)
+@pytest.mark.parametrize("D,group", [(64, 64), (128, 64)])
+@pytest.mark.parametrize("dtype,way", [(torch.float16, (0, 12, -6)), (torch.float16, (-10, 6, 10)), (torch.bfloat16, (0, 20, -20)), (torch.bfloat16, (-50, 0, 30)), (torch.bfloat16, (40, -20, 0)),
+                                       (torch.bfloat16, (-100, -60, -80)), (torch.bfloat16, (-100, 100, 0)), (torch.bfloat16, (90, -90, 3)), (torch.bfloat16, (10, 50, 100))])
+def test_scales_that_change_along_a_sequence(mynn, dtype, way, D, group, S, Hq):
+    """powers of two of its thirds; the keys of the thirds with small values have the larger scores, so that all of them count"""
+    n = 900 + S
+    third = torch.arange(n) * 3 // n
+    v = normal(9, 1, n, 1, D) * (2.0 ** torch.tensor(way, dtype=torch.float64)[third])[None, :, None, None]
+    if dtype == torch.float16:
+        v = v.clamp(-6e4, 6e4)
+    direction = normal(10, D)
+    order = torch.tensor(way).argsort(descending=True).argsort().float()
+    k = 0.3 * normal(11, 1, n, 1, D) + (order[third] * 4.0)[None, :, None, None] * direction / direction.norm()
+    pools, table = made(1, 1, D, 128, group, dtype, n, v, 12, keys=k)
+    q = (direction + 0.2 * normal(13, 1, Hq, S, D)).to(dtype).cuda()
+    check(mynn, q, pools, table, [900], scale=0.5)
+    check(mynn, q, pools, table, [900], scale=0.0)
+
+
+@pytest.mark.parametrize("S,Hq", ROWS)
 @pytest.mark.parametrize("D,group", SHAPES)
 @pytest.mark.parametrize("key", [-118, -100, 100, 112, 120])
 @pytest.mark.parametrize("scale", [0.125, -0.125])
@@ -110,3 +191,19 @@ def test_keys_and_queries_at_opposite_ends(mynn, D, group, S, Hq, key, scale):
     q[:, 0] *= 0.001  # (rows of their own sizes, a row of zeros)
     q[:, 1] = 0.0
     check(mynn, q, pools, table, [150, 31], new=[S, S], scale=scale)
+
+
+@pytest.mark.parametrize("S,Hq", ROWS)
+def test_scores_that_are_very_large(mynn, S, Hq):
+    """keys of 2^100 and queries of about 1: one key has all the weight"""
+    dtype, D, n = torch.bfloat16, 128, 100 + S
+    k = normal(18, 1, n, 1, D).abs() * 2.0 ** 100
+    pools, table = made(1, 1, D, 64, 64, dtype, n, normal(19, 1, n, 1, D), 20, keys=k)
+    q = normal(21, 1, Hq, S, D).abs().to(dtype).cuda()
+    got = mynn.attention_paged_int4(q, pools, table, 0.125, torch.tensor([100], dtype=torch.int32, device="cuda"))
+    (k, _), (v, _) = (ref.rows_of(pools, side, table, 0, 0, n) for side in (0, 1))
+    for i in range(S):
+        s = torch.mm(q[0, :, i].double(), k[0, :101 + i].t().contiguous())
+        top = s.topk(2, -1)
+        clear = top.values[:, 0] > top.values[:, 1] * (1 + 2.0 ** -16)  # (sums of 128 positive products in 32 bits)
+        assert bool(clear.any()) and torch.equal(got[0, clear, i], v[0][top.indices[clear, 0]].to(dtype))
