@@ -649,6 +649,12 @@ def kvcache_update_paged(pool, new_kv, offset, table, page_rows):
     return pool
 
 
+def _ints(name, *sizes):
+    """the library's sizes are ints: what is left of a larger one would be another size"""
+    if max(sizes) >= 1 << 31:
+        raise MynnError("%s: a size past 2^31 among %s" % (name, list(sizes)))
+
+
 class _Paged:
     """The pools of a layer (KvPool.buffers) and a page table (KvPages, or a cuda int32 tensor [B, pages_per_seq]) as the calls for sequences of
     different lengths take them; what does not fit together is refused here."""
@@ -678,11 +684,13 @@ class _Paged:
             if table.pool.page_rows != self.rows or table.pool.n_pages > self.n_pages:
                 raise MynnError("%s: pages of %d rows out of %d, pools of %d pages of %d" % (name, table.pool.page_rows, table.pool.n_pages, self.n_pages, self.rows))
             self.batch, self.pages, self.table = table.batch, table.pages_per_seq, table.table_ptr
+            _ints(name, self.n_pages, self.heads, self.rows, self.dim)
             table = None
         else:
             if table.dim() != 2 or table.dtype != torch.int32:
                 raise MynnError("%s: page table %s %s (int32 [B, pages])" % (name, tuple(table.shape), table.dtype))
             self.batch, self.pages = table.shape
+            _ints(name, self.batch, self.pages, self.n_pages, self.heads, self.rows, self.dim)
             self.table = _ptr(table)
         for what in (past, new):
             if what is not None and (what.dtype != torch.int32 or tuple(what.shape) != (self.batch,)):
@@ -694,7 +702,7 @@ class _Paged:
 
     def rows_of(self, name, x, heads=None):
         """(S) of [B, H, S, D] rows in the cache's type"""
-        if x.dim() != 4 or x.shape[0] != self.batch or x.shape[3] != self.dim or x.dtype != self.dtype or (heads is not None and x.shape[1] != heads) or x.shape[2] >= 1 << 31:
+        if x.dim() != 4 or x.shape[0] != self.batch or x.shape[3] != self.dim or x.dtype != self.dtype or (heads is not None and x.shape[1] != heads) or x.shape[1] >= 1 << 31 or x.shape[2] >= 1 << 31:
             raise MynnError("%s: rows %s %s over a cache of %d sequences, %d heads of %d, %s" % (
                 name, tuple(x.shape), x.dtype, self.batch, self.heads, self.dim, self.dtype))
         return x.shape[2]
@@ -766,6 +774,7 @@ def attention_paged_int4_workspace(q, pools, table):
     B, Hq, Sq, D = q.shape
     pages = table.pages_per_seq if isinstance(table, KvPages) else table.shape[1]
     Hkv, rows = pools[0].shape[1:3]
+    _ints("attention_paged_int4_workspace", B, Sq, pages, rows, Hq, Hkv, D)
     need = lib().mynn_attention_paged_int4_workspace_bytes(B, Sq, pages, rows, Hq, Hkv, D)
     return _t().zeros((PAGED_INT4_COUNTER_BYTES + need,), dtype=_torch.uint8, device=q.device)
 
