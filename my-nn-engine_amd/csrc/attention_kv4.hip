@@ -80,9 +80,10 @@ extern "C" size_t mynn_attention_paged_int4_workspace_bytes(int B, int Sq, int p
         const int ranges = kv4_tile_plan(B, Sq, num_q_heads, num_kv_heads, (long)pages_per_seq * page_rows).ranges;
         return ranges == 1 ? 0 : (size_t)ranges * B * num_kv_heads * R * (head_dim + 4) * sizeof(float);
     }
-    // (the smaller unit makes more workgroups: enough for either)
+    // (the smaller unit makes more workgroups: enough for either.  A cache of one unit is one workgroup's.)
     const long pairs = (long)B * num_kv_heads, rows = (long)pages_per_seq * page_rows;
     const int waves = kv4_waves(pairs, (long)R, rows);
+    if (rows <= kv4_unit(1, waves)) return 0;
     return 2 * (size_t)kv4_stream_grid(pairs, kv4_unit(1, waves), waves, rows) * R * (head_dim + 4) * sizeof(float);
 }
 
