@@ -112,6 +112,12 @@ template <typename T, int TOP> struct Kv4Band {
     }
     static __device__ __forceinline__ uint32_t bits(uint32_t w, int hi) { return __builtin_amdgcn_ubfe(w, hi ? 16 : 0, 15); }
     __device__ __forceinline__ uint32_t off(uint32_t b) const { return b - from; }
+    // the larger of `most` and what off() makes of two scales, in halves
+    typedef unsigned short us2_t __attribute__((ext_vector_type(2)));
+    __device__ __forceinline__ uint32_t off2(uint32_t most, uint32_t w) const {
+        const us2_t x = __builtin_bit_cast(us2_t, w & 0x7FFF7FFFu) - __builtin_bit_cast(us2_t, from * 0x00010001u);
+        return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(us2_t, most), x));
+    }
     // the exponent of a scale that is not zero, as of a 32-bit number, among the least lo and the largest hi; what is no number has none, and is below all others
     static __device__ __forceinline__ void among(float scale, int &lo, int &hi) {
         const int x = (int)(__builtin_bit_cast(uint32_t, scale) >> 23 & 255u), e = x == 255 ? 0 : x;
@@ -119,7 +125,6 @@ template <typename T, int TOP> struct Kv4Band {
     }
     // Scales that are not let through: each lane has the least and the largest exponent of some.
     __device__ __forceinline__ void settle(int lane_lo, int lane_hi) {
-        typedef unsigned short us2_t __attribute__((ext_vector_type(2)));
         int x = (255 - lane_lo) | lane_hi << 16;
         auto join = [&](int y) { x = __builtin_bit_cast(int, __builtin_elementwise_max(__builtin_bit_cast(us2_t, x), __builtin_bit_cast(us2_t, y))); };
         join(__builtin_amdgcn_update_dpp(0, x, 0x111, 0xF, 0xF, false));

@@ -277,10 +277,19 @@ template <typename T, int D, int NG, int FOLD, int NW> __global__ __launch_bound
             // ---- the scales of the values that the row sees
             {
                 uint32_t off = 0;
+                if (__builtin_amdgcn_ballot_w64(col % COLS < R && room_of(t, key0, limit, OWN - 1) < 4) == 0) {  // (all keys: two scales at a time)
+                    uint32_t most = 0;
 #pragma unroll
-                for (int s = 0; s < OWN; s++)
+                    for (int s = 0; s < OWN; s++)
 #pragma unroll
-                    for (int n = 0; n < 4 * NG; n++) off = max(off, n / NG < room_of(t, key0, limit, s) ? band.off(band.bits(t.vs[s][n / 2], n & 1)) : 0u);
+                        for (int n = 0; n < 2 * NG; n++) most = band.off2(most, t.vs[s][n]);
+                    off = max(most & 0xFFFFu, most >> 16);
+                } else {
+#pragma unroll
+                    for (int s = 0; s < OWN; s++)
+#pragma unroll
+                        for (int n = 0; n < 4 * NG; n++) off = max(off, n / NG < room_of(t, key0, limit, s) ? band.off(band.bits(t.vs[s][n / 2], n & 1)) : 0u);
+                }
                 if (__builtin_expect(__builtin_amdgcn_ballot_w64(off > band.last) != 0, 0)) {
                     int lo = 255, hi = 0;
 #pragma unroll
@@ -354,16 +363,24 @@ template <typename T, int D, int NG, int FOLD, int NW> __global__ __launch_bound
             top = xor32_max(xor16_max(top));
             if constexpr (FOLD >= 2) top = fmaxf(top, dpp_get<kDppRor8>(top));
             if constexpr (FOLD == 4) top = fmaxf(top, dpp_get<kDppRor4>(top));
-            const float Mn = fmaxf(M, top), ref = Mn == -INFINITY ? 0.f : Mn, unit = (float)band.unit;
+            const float Mn = fmaxf(M, top), unit = (float)band.unit;
+            float ref = Mn == -INFINITY ? 0.f : Mn - unit;
             const float alpha = Mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(M - Mn + (float)(band.unit - unit_of_sums));
             M = Mn;
             unit_of_sums = band.unit;
+            if (__builtin_expect(__builtin_amdgcn_ballot_w64(fabsf(ref) > 0x1p20f) != 0, 0)) {  // (scores so large that the unit is a small thing next to them: one after the other)
+#pragma unroll
+                for (int s = 0; s < OWN; s++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) sv[s][e] -= Mn == -INFINITY ? 0.f : Mn;
+                ref = -unit;
+            }
             float ps = 0.f;
 #pragma unroll
             for (int s = 0; s < OWN; s++)
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
-                    sv[s][e] = __builtin_amdgcn_exp2f(sv[s][e] - ref + unit);  // (in this order: a score may be so large that the unit is nothing to it)
+                    sv[s][e] = __builtin_amdgcn_exp2f(sv[s][e] - ref);
                     ps += sv[s][e];
                 }
             l = fmaf(l, alpha, ps);
