@@ -287,7 +287,8 @@ int mynn_kv_pages_destroy(mynn_kv_pages *pages);
  * and row of q, of k, of v; a row's values lie together); q_out [B,Hq,S,D] contiguous, 16-byte aligned, and may be q where
  * q lies so.  q and q_out NULL: k and v alone.  cos, sin [table_rows, D]; position: device int64 [B,S], the table row of each token,
  * or NULL for its cache row.  A token whose cache row or table row does not exist, and every token from new_lens on, is not
- * appended and its q_out row is zeros; what the cache holds besides the appended rows stays as it is.  No two rows of a call may be
+ * appended and its q_out row is zeros; one whose page is not there is not appended either, but its q_out row is the rotated q.  What
+ * the cache holds besides the appended rows stays as it is.  No two rows of a call may be
  * the same row of the cache.  k and v must not overlap the pools. */
 int mynn_rope_append_paged(void *q_out, const void *q, const void *k, const void *v, const int64_t *strides,
                            const void *cos_t, const void *sin_t, int table_rows, const int64_t *position,
@@ -305,10 +306,13 @@ int mynn_kv_rows_paged(void *k_out, void *v_out, const void *k_pool, const void 
                        const int32_t *page_table, int n_pages, int pages_per_seq, int page_rows,
                        const int32_t *first_rows, const int32_t *n_rows, int B, int S,
                        int num_kv_heads, int head_dim, int dtype, int kv_bits, int group, mynn_stream s);
-/* Attention over a cache of 4 bits.  Q, out [B,Hq,Sq,D] contiguous, 16-byte aligned; kv head = q head / (Hq/Hkv).  The Sq rows of
+/* Attention over a cache of 4 bits (of 16, and for one token 8, mynn_attention_paged, for sequences of one length; others by way of
+ * mynn_kv_rows_paged).  Q, out [B,Hq,Sq,D] contiguous, 16-byte aligned, out over none of the operands; kv head = q head / (Hq/Hkv).  The Sq rows of
  * a sequence are its newest tokens, which the cache holds already: row i sees the keys [0, past_lens[b] + i + 1) where is_causal,
  * else all past_lens[b] + new_lens[b].  Keys on a page that is not there are left out.  A row that sees no key, and every row
- * from new_lens on, is zeros.
+ * from new_lens on, is zeros.  A group of values that stands for NaN makes its own columns NaN, for the rows that see it.
+ * Which form of the kernels runs goes by pages_per_seq, not by the lengths on the device: a table far wider than the longest sequence
+ * takes the forms for long caches.
  * workspace: mynn_attention_paged_int4_workspace_bytes(...) bytes, 16-byte aligned (0: none needed).  counters: device int32
  * [MYNN_PAGED_INT4_COUNTERS] that are zero, and are zero again behind the call, or NULL: with them the parts of a sequence that
  * several workgroups share are joined inside the launch, without them by a second one; the results are the same bits.  They serve

@@ -711,7 +711,9 @@ class _Paged:
 def rope_append_paged(q, k, v, cos_t, sin_t, pools, table, past_lens, new_lens=None, positions=None, out=None):
     """mynn_rope_append_paged: rotates q [B,Hq,S,D] (None: keys and values alone) and k [B,Hkv,S,D] and appends k, v to the pools (KvPool.buffers) from row
     past_lens[b] (cuda int32 [B]) on; new_lens (cuda int32 [B]): how many of the S tokens are a sequence's own; positions (cuda int64 [B,S]): the
-    table rows, where they are not the cache rows.  q, k, v may be views (of the projection's rows, say) whose last dimension lies together.
+    table rows, where they are not the cache rows.  A token whose page is not there (a page number outside the pool) keeps its rotated q; its k and v are
+    dropped.  KvPages maps the same rows for every sequence of its batch; for sequences whose pages are to be as many as their rows ask for, the table is a tensor of
+    the caller's.  q, k, v may be views (of the projection's rows, say) whose last dimension lies together.
     Returns the rotated q, contiguous (out, where given)."""
     if k.is_cuda:
         done = (_ops or _host_ops()).rope_append_paged(q, k, v, cos_t, sin_t, pools, table, past_lens, new_lens, positions, out)
@@ -782,7 +784,8 @@ def attention_paged_int4_workspace(q, pools, table):
 def attention_paged_int4(q, pools, table, scale, past_lens, new_lens=None, is_causal=True, workspace=None, out=None):
     """mynn_attention_paged_int4: q [B,Hq,Sq,D], the newest tokens of each sequence, over a cache of 4 bits (KvPool.buffers with kv_int4_group) that holds
     their rows already (rope_append_paged with the same past_lens and new_lens).  workspace: attention_paged_int4_workspace(...), kept by
-    the caller; without one the call allocates its own, and takes a launch more where a sequence is shared by several workgroups."""
+    the caller; without one the call allocates its own, and takes a launch more where a sequence is shared by several workgroups.  (Caches of 16 bits, and for
+    one token of 8, are read by attention_paged, whose sequences have one length, others by way of kv_rows_paged.)"""
     if q.is_cuda:
         done = (_ops or _host_ops()).attention_paged_int4(q, pools, table, scale, past_lens, new_lens, is_causal, workspace, out)
         if done is not None:

@@ -98,7 +98,7 @@ constexpr float kKv4Lag = 4.f;
 //                2^-40 .. 2^24: sums in one unit are finite in any other.
 //   wide         bf16 parts, from the first tile on whose scales do not lie within 9 binades, or lie outside of that, to the end of the keys.  2^unit is 2^40 while all scales are
 //                below 2^61, so that small ones are far from the least 32-bit number, then 2^-8: weights of 2^4 and scales of 2^125 have a finite product with a code.
-//                Such calls take up to twice as long: one token of 64 sequences of 8192 keys, bf16, 112 us and 224, of one of 32768 17.5 and 29, 4 x 2048 rows 234 and 484.
+//                Such calls take up to twice as long: one token of 64 sequences of 8192 keys, bf16, 112 us and 225, of one of 32768 18 and 29, 4 x 2048 rows 234 and 485.
 template <typename T, int TOP> struct Kv4Band {
     static constexpr int SHIFT = std::is_same<T, f16_t>::value ? 10 : 7, BIAS = std::is_same<T, f16_t>::value ? 112 : 0, EMAX = std::is_same<T, f16_t>::value ? 31 : 255;
     uint32_t from, last;  // scales whose bits less `from` are above `last` are not let through

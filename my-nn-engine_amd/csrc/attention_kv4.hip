@@ -42,7 +42,9 @@ static int kv4_stream_grid(long pairs, int unit, int waves, long rows) {
 }
 
 // Rows of a workgroup, and up to how many ranges of keys its rows' keys come in (two workgroups a CU run at once; Kv4TilePlan::ranges makes twice that at the most, how many
-// of them a block takes is found on the device).  R: rows of a kv head, rows: of a sequence's cache.
+// of them a block takes is found on the device).  R: rows of a kv head, rows: those of a sequence's pages in the table, which is all that the host knows of lengths (here and in
+// kv4_waves).  The figures are of tables as wide as the longest sequence.  A table far wider than that has calls take the forms for long caches: over 8192 rows prompts of
+// 100 rows 15 us for 12, of 1200 59 for 40, 3 x 333 36 for 19, 8 x 64 tokens behind 1000 rows 39 for 34, 64 sequences of 128 keys 8.8 for 8.3.
 static Kv4TilePlan kv4_tile_plan(int B, int Sq, int Hq, int Hkv, long rows) {
     const long R = (long)(Hq / Hkv) * Sq, pairs = (long)B * Hkv, cus = kv4_cus();
     auto plan = [&](int block, bool split) {
@@ -53,18 +55,18 @@ static Kv4TilePlan kv4_tile_plan(int B, int Sq, int Hq, int Hkv, long rows) {
         p.ranges = (int)(want < 2 ? 1 : want > most ? most : want);
         return p;
     };
-    // Up to 32 rows, drafts to be checked: four waves on one block of 32, which shares its tiles of 128 keys between them (32 x 5 tokens behind 4000 rows 66 us, as half of a block of
-    // 64 85; 64 x 5 behind 1000 38 and 66; 8 x 6 behind 4000 31 and 34).  Not where both the (sequence, kv head)s and their keys are few: a tile of 128 is a long wait then
-    // (4 x 8 behind 500 18 and 16; 16 x 6 behind 800 23 both).
+    // Up to 32 rows, drafts to be checked: four waves on one block of 32, which shares its tiles of 128 keys between them (32 x 5 tokens behind 4000 rows 59 us, as half of a block of
+    // 64 73; 64 x 5 behind 1000 35 and 41; 8 x 6 behind 4000 29 and 31).  What is left of a tile's time is latency: one stage of LDS and two barriers a tile, two workgroups a CU.  Not where both the (sequence, kv head)s and their keys are few: a tile of 128 is a long wait then
+    // (4 x 8 behind 500 18 us and, blocks of 64 in ranges, 15; 16 x 6 behind 800 24 and 23).
     if (R <= 32 && (pairs >= cus || rows >= 2048)) return plan(32, pairs < 2 * cus && rows >= 2048);
-    // Blocks of 128 rows turn codes into operands for the most rows: where they fill the device (32 / 8 heads of 128, groups of 128, bf16: one prompt of 4096 rows 228 us, blocks
-    // of 64 278; one of 2048 82 and 88), and, in ranges, where both rows and keys are many (512 tokens behind 3000 rows 65, blocks of 64 in ranges 71, whole 84).
+    // Blocks of 128 rows turn codes into operands for the most rows: where they fill the device (32 / 8 heads of 128, groups of 128, bf16: one prompt of 4096 rows 240 us, blocks
+    // of 64 270; one of 2048 81 and 86), and, in ranges, where both rows and keys are many (512 tokens behind 3000 rows 67, blocks of 64 in ranges 74, whole 85).
     if (pairs * ((R + 127) / 128) >= 2 * cus) return plan(128, false);
     if (R >= 1024 && rows >= 2048) return plan(128, true);
-    // Blocks of 64 leave two waves to a block of 32 rows, half of each tile's keys each, and a tile takes 1.6 us where it took 2.3: one prompt of 1200 rows 38 us, in blocks of
-    // 128 49, those in ranges 57.  Ranges cost a launch more, 5 us and up: they pay for few blocks of 512 keys and more (4 x 40 tokens behind 2000 rows 30 us, whole 49; one prompt
-    // of 300 rows 19, whole 16), of one for each CU only behind many keys (8 x 64 tokens behind 3000 rows 65, whole 75, behind 1000 36
-    // and 33; 8 x 100 behind 2100, 448 blocks, 89 and 77).
+    // Blocks of 64 leave two waves to a block of 32 rows, half of each tile's keys each, and a tile takes 1.6 us where it took 2.3: one prompt of 1200 rows 39 us, in blocks of
+    // 128 48, those in ranges 58.  Ranges cost a launch more, 5 us and up: they pay for few blocks of 512 keys and more (4 x 40 tokens behind 2000 rows 33 us, whole 53; one prompt
+    // of 300 rows 20, whole 16), of one for each CU only behind many keys (8 x 64 tokens behind 3000 rows 69, whole 77, behind 1000 38
+    // and 33; 8 x 100 behind 2100, 448 blocks, 89 and 76).
     const long wgs = pairs * ((R + 63) / 64);
     return plan(64, wgs < cus ? rows >= 512 : 2 * wgs < 3 * cus && rows >= 2048);
 }

@@ -6,15 +6,15 @@
 //   softmax                   online; a lane has one row (column of the instruction) and 4 keys of each 16
 //   O^T[columns x rows] += V^T . P   V goes to LDS as codes and comes back transposed (ds_read_b64_tr_b4: of 16 rows that its lanes name, a lane receives
 //                             one column); named are a lane group's own 8 keys twice, for 16 columns and the 16 behind them, so that the order of the
-//                             keys is the one in which the scores lie in registers.  p * vs in two fp16 values, rounded and rest: 22 bits.
-// The vector operations bound it (one pass of 32 keys, D = 128: 144 to turn codes into operands, the softmax 180 where every lane has 8 scores).  So where 8 rows or 4 are
+//                             keys is the one in which the scores lie in registers.  p * vs in two fp16 values, rounded and rest: 22 bits (or three of bf16, attention_kv4.h).
+// The vector operations bound it (one pass of 32 keys, D = 128: 144 to turn codes into operands, the softmax and the look at the value scales 230 where every lane has 8 scores).  So where 8 rows or 4 are
 // all there are (FOLD 2, 4), they are the columns twice or four times, and each of these takes the scores of its own 16 keys of 32 or 64: 4 for a lane.  Weights go back with
 // lane rotations.
 //
 // Measured (kernel times; bytes at what a copy reaches, 5.1 TB/s, in brackets): one token of 64 sequences of 8192 keys, 32 / 8 heads of 128, groups of 128 104 us (110: some of
-// it is from the last cache), of 64 121 (115), of 32 165 (125), 2 tokens 119 (110), 4 tokens 133 (111); 128 sequences, 32 / 4 heads of 64 82 (58), groups of 32 97 (62).  Where
-// the bracket is far the vector operations are busy 85 % of the time.  Short calls are a chain of waits -- lengths, page table, codes, a step of 0.65 us or more for each 128 or
-// 256 keys, the join's 7 us --: one sequence of 32768 keys 18 us, 32 of up to 4096 31, 8 x 4 tokens of up to 2000 keys 22.
+// it is from the last cache), of 64 123 (115), of 32 170 (125), 2 tokens 122 (110), 4 tokens 138 (111); 128 sequences, 32 / 4 heads of 64 85 (58), groups of 32 100 (62).  Where
+// the bracket is far the vector operations are busy 80 % of the time and more.  Short calls are a chain of waits -- lengths, page table, codes, a step of 0.65 us or more for each 128 or
+// 256 keys, the join's 7 us --: one sequence of 32768 keys 18.5 us, 32 of up to 4096 32, 8 x 4 tokens of up to 2000 keys 22.5.
 // Units of a workgroup's run are whole steps: smaller ones dealt out better and split more steps, and took longer.  The join inside the launch or in one of its own: 32 sequences of up to
 // 4096 keys 31 us and 27.3 + 4.8, one of 32768 18.5 and 15 + 6.4, 8 x 4 tokens 22 and 14.5 + 6.4, the second launch's start not counted.
 #pragma once

@@ -7,10 +7,10 @@
 //   softmax            a lane has ONE row and half of the keys of each 32
 //   O^T += V^T . P^T   p * vs as two fp16 numbers, or three of bf16 (attention_kv4.h); P stays in registers (the D layout of S^T is the B layout of P^T with the keys in the order 4g+0..3, 8+4g+0..3), V^T
 //                      comes from the row-major tile by transposing reads
-// Vector operations and matrix instructions bound it together (busy 65 and 31 % of the time at 4 x 2048 rows): 350 of the one for 32 of the other in a wave's 64 keys of 32 rows,
-// 100 of them the staging's.  4 prompts of 2048 rows, 32 / 8 heads of 128, groups of 128, bf16: 197 us in a program's calls, 0.70 PFLOP/s (the products alone, at what a large
-// matrix product reaches: 112); fp16, whose second product is two, 4 x 512 rows behind 3000 195 for 166.  Blocks of 256 rows, as eight waves or as four with 64 rows each, share
-// a tile's staging between more rows and hold one workgroup a CU: no faster, and 310 us for 230.  Raised priorities around the products, and reads of their operands
+// Vector operations and matrix instructions bound it together (busy 65 and 42 % of the time at 4 x 2048 rows): 380 of the one for 48 of the other in a wave's 64 keys of 32 rows,
+// 100 of them the staging's.  4 prompts of 2048 rows, 32 / 8 heads of 128, groups of 128, bf16: 234 us in a program's calls, 0.59 PFLOP/s (the products alone, at what a large
+// matrix product reaches: 112; the second of them is done twice); fp16, 4 x 512 rows behind 3000 200.  Blocks of 256 rows, as eight waves or as four with 64 rows each, share
+// a tile's staging between more rows and hold one workgroup a CU: no faster, and 310 us where this took 230.  Raised priorities around the products, and reads of their operands
 // ahead in a fixed order, were within 4 % of this, 64 columns and groups of 32 slower.
 // Codes leave a dword in the order of kv4_pairs, so columns lie in that order inside every 8: queries are put in the same order when they are read, results back when stored.
 #pragma once
@@ -62,13 +62,13 @@ template <typename T, int D, int NG, int QW, int KW, int KEYS> __global__ __laun
     int b, block, range = 0;
     if (a.c.fresh || a.ranges > 1) {
         // Then sequences, ranges outermost.  Workgroups go to the shader engines in turn, and those that end at once should not have every other turn: 2 pieces of prompts, 512
-        // rows and 79, took 91 us for 76 with the sequences inside the blocks, 8 of up to 1024 rows 284 for 202 (227 with the sequences taking turns), and 32 x 5 rows over 4000
-        // keys, 2 ranges of 4 there, 124 for 71 with the ranges inside.
+        // rows and 79, take 95 us, 108 with the sequences inside the blocks (97 with them taking turns), 8 of up to 1024 rows 170, 245 (175), and 32 x 5 rows over 4000 keys, 2 ranges of 4
+        // there, 62, with the ranges inside 104.
         const int i2 = i1 / a.blocks;
         block = i1 - i2 * a.blocks, range = i2 / a.B, b = i2 - range * a.B;
     } else {
-        // All blocks have rows: sequences inside the blocks, taking turns, and the heaviest of all go first (4 x 2048 rows, four times as many workgroups as run at once, 220 us;
-        // outermost 230).
+        // All blocks have rows: sequences inside the blocks, taking turns, and the heaviest of all go first (4 x 2048 rows, four times as many workgroups as run at once, 233 us;
+        // outermost 239).
         block = i1 / a.B, b = (i1 - block * a.B + block / 2) % a.B;
     }
     const int row0 = (a.blocks - 1 - block) * B::ROWS;
