@@ -97,7 +97,8 @@ constexpr float kKv4Lag = 4.f;
 //                2^-8 e, at 2^4 or 1: a weight is off by 2^-25 of that unit, next to a scale of its own.  e is 1 at first, then the largest of the last tile that did not fit, of
 //                2^-40 .. 2^24: sums in one unit are finite in any other.
 //   wide         bf16 parts, from the first tile on whose scales do not lie within 9 binades, or lie outside of that, to the end of the keys.  2^unit is 2^40 while all scales are
-//                below 2^61, so that small ones are far from the least 32-bit number, then 2^-8: weights of 2^4 and scales of 2^125 have a finite product with a code.
+//                below 2^51, so that small ones are far from the least 32-bit number (and sums over 2^28 keys from the largest), then 2^-8: weights of 2^4 and scales of 2^125 have a
+//                finite product with a code.
 //                Such calls take up to twice as long: one token of 64 sequences of 8192 keys, bf16, 112 us and 225, of one of 32768 18 and 29, 4 x 2048 rows 234 and 485.
 template <typename T, int TOP> struct Kv4Band {
     static constexpr int SHIFT = std::is_same<T, f16_t>::value ? 10 : 7, BIAS = std::is_same<T, f16_t>::value ? 112 : 0, EMAX = std::is_same<T, f16_t>::value ? 31 : 255;
@@ -135,13 +136,13 @@ template <typename T, int TOP> struct Kv4Band {
         join(__builtin_amdgcn_update_dpp(0, x, kDppBcast31, 0xC, 0xF, false));
         const int all = __builtin_amdgcn_readlane(x, 63), lo = 255 - (all & 0xFFFF), hi = all >> 16;
         if (lo > hi) return;  // (zeros)
-        const bool high = hi > 127 + 60 || (wide && unit < 0);
+        const bool high = hi > 127 + 50 || (wide && unit < 0);
         wide = wide || lo < 1 + BIAS || hi - lo > 8 || hi < 127 - 40 || hi > 127 + 24;
         if (!wide) {
             put(hi);
             return;
         }
-        from = 0u, last = high || BIAS ? 0x7FFFu : ((127 + 61) << SHIFT) - 1;
+        from = 0u, last = high || BIAS ? 0x7FFFu : ((127 + 51) << SHIFT) - 1;
         unit = high ? -8 : 40;
     }
 };
