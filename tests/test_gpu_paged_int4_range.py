@@ -138,13 +138,10 @@ def test_groups_of_a_row_far_from_each_other(mynn, dtype, low, high, D, group, S
 
 @pytest.mark.parametrize("S,Hq", ROWS)
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
-@pytest.mark.parametrize("D,group", SHAPES)
-@pytest.mark.parametrize("scale_of_it", [float("nan"), float("inf")])
-@pytest.mark.parametrize("longest", [150, 3000])
+@pytest.mark.parametrize("D,group,scale_of_it,longest", [(d, g, s, 150) for d, g in SHAPES for s in (float("nan"), float("inf"))] + [(64, 32, float("nan"), 3000), (128, 64, float("inf"), 3000),
+                                                                                                                                    (128, 32, float("nan"), 3000), (64, 64, float("inf"), 3000)])
 def test_a_group_of_values_that_stands_for_no_number(mynn, dtype, D, group, S, Hq, scale_of_it, longest):
     """only its own columns are none, and only for the rows that see it; 3000: sequences that several workgroups share"""
-    if longest > 150 and (group > 64 or scale_of_it != scale_of_it):
-        pytest.skip("one of them")
     past = [longest, 40]
     v = normal(7, 2, longest + S, 2, D) * 2.0 ** -9
     pools, table = made(2, 2, D, 64, group, dtype, longest + S, v, 8)
@@ -207,3 +204,35 @@ def test_scores_that_are_very_large(mynn, S, Hq):
         top = s.topk(2, -1)
         clear = top.values[:, 0] > top.values[:, 1] * (1 + 2.0 ** -16)  # (sums of 128 positive products in 32 bits)
         assert bool(clear.any()) and torch.equal(got[0, clear, i], v[0][top.indices[clear, 0]].to(dtype))
+
+
+@pytest.mark.parametrize("S,Hq", ROWS)
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_captured_and_replayed_over_scales_that_change(mynn, dtype, S, Hq):
+    """lengths grow past rows of zeros and of values 2^-14 and 2^12 of the others': what fits fp16 at one replay does not at the next"""
+    D, group, n = 128, 64, 1300
+    v = normal(22, 2, n, 2, D)
+    v[:, 400:600] *= 2.0 ** 12
+    v[:, 700:720] = 0.0
+    v[:, 800:1000] *= 2.0 ** -14
+    pools, table = made(2, 2, D, 64, group, dtype, n, v.clamp(-6e4, 6e4), 23)
+    q = queries(2, Hq, S, D, dtype)
+    past, new = torch.tensor([0, 150], dtype=torch.int32, device="cuda"), torch.tensor([S, S], dtype=torch.int32, device="cuda")
+    ws, out, plain = mynn.attention_paged_int4_workspace(q, pools, table), torch.empty_like(q), torch.empty_like(q)
+    calls = lambda: (mynn.attention_paged_int4(q, pools, table, 0.1, past, new, workspace=ws, out=out), mynn.attention_paged_int4(q, pools, table, 0.1, past, new, out=plain))
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        calls()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        calls()
+    for step in range(6):
+        graph.replay()
+        torch.cuda.synchronize()
+        want = mynn.attention_paged_int4(q, pools, table, 0.1, past, new)
+        assert same_bits(out, want) and same_bits(plain, want)
+        exact, slack = attention(q, pools, table, 0.1, past.tolist(), new.tolist())
+        ref.assert_close(out, exact, slack)
+        past += 190
